@@ -32,7 +32,7 @@ int cgv_debug_trace_(cgv_index* h, uint32_t ctx, double* host_us8, uint64_t* sta
     if (host_us8) memcpy(host_us8, c->host_us, sizeof(c->host_us));
     if (stamps && nq) {
         if (c->trace.bytes < (size_t)nq * 64) return fail(CGV_ERR_INVALID_ARG, "no trace recorded (CGV_TRACE unset?)");
-        HIPCHK(hipSetDevice(h->device));
+        HIPCHK(cgv::use_device(h->device));
         HIPCHK(hipMemcpy(stamps, c->trace.p, (size_t)nq * 64, hipMemcpyDeviceToHost));
     }
     return CGV_OK;
@@ -71,7 +71,7 @@ int cgv_debug_fbflags_(cgv_index* h, uint32_t ctx, uint32_t* out, uint32_t nq) {
     if (!h || !out || ctx >= (uint32_t)N_CTX) return fail(CGV_ERR_INVALID_ARG, "bad argument");
     SearchCtx* c = &h->ctx[ctx];
     if (c->fbflag.bytes < (size_t)nq * 4) return fail(CGV_ERR_INVALID_ARG, "no such search");
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     HIPCHK(hipMemcpy(out, c->fbflag.p, (size_t)nq * 4, hipMemcpyDeviceToHost));
     return CGV_OK;
 }
@@ -121,7 +121,7 @@ int cgv_create(uint32_t dim, int metric, int dtype, int device_id, cgv_index** o
     int ndev = cgv_device_count();
     if (ndev == 0) return fail(CGV_ERR_HIP, "no HIP device visible: libcgvec_hip has no CPU fallback");
     if (device_id < 0 || device_id >= ndev) return fail(CGV_ERR_INVALID_ARG, "device_id out of range");
-    HIPCHK(hipSetDevice(device_id));
+    HIPCHK(cgv::use_device(device_id));
     if (int arc = ensure_kernel_attrs(device_id)) return arc;
     cgv_index* h = new cgv_index();
     h->device = device_id;
@@ -173,7 +173,7 @@ int cgv_create(uint32_t dim, int metric, int dtype, int device_id, cgv_index** o
 
 int cgv_destroy(cgv_index* h) {
     if (!h) return CGV_OK;
-    (void)hipSetDevice(h->device);
+    (void)cgv::use_device(h->device);
     (void)hipStreamSynchronize(h->stream);
     if (h->rows) {
         (void)hipFree(h->rows);
@@ -215,7 +215,7 @@ int cgv_reserve(cgv_index* h, uint64_t n_rows) {
     if (!h) return fail(CGV_ERR_INVALID_ARG, "handle is NULL");
     std::unique_lock<std::mutex> lk(h->mu);
     if (int brc = wait_all_idle(h, lk)) return brc;
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     return grow(h, n_rows);
 }
 
@@ -224,7 +224,7 @@ int cgv_add_f32_dev(cgv_index* h, const float* rows_dev, uint64_t n) {
     if (n && !rows_dev) return fail(CGV_ERR_INVALID_ARG, "rows is NULL");
     std::unique_lock<std::mutex> lk(h->mu);
     if (int brc = wait_all_idle(h, lk)) return brc;
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     return atomic_ingest(h, [&] { return add_dev_locked(h, rows_dev, n); });
 }
 
@@ -233,7 +233,7 @@ int cgv_add_f32(cgv_index* h, const float* rows_host, uint64_t n) {
     if (n && !rows_host) return fail(CGV_ERR_INVALID_ARG, "rows is NULL");
     std::unique_lock<std::mutex> lk(h->mu);
     if (int brc = wait_all_idle(h, lk)) return brc;
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     int rc = grow(h, h->n + n);
     if (rc) return rc;
     return atomic_ingest(h, [&]() -> int {
@@ -255,7 +255,7 @@ int cgv_add_f64(cgv_index* h, const double* rows_host, uint64_t n) {
     if (n && !rows_host) return fail(CGV_ERR_INVALID_ARG, "rows is NULL");
     std::unique_lock<std::mutex> lk(h->mu);
     if (int brc = wait_all_idle(h, lk)) return brc;
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     int rc = grow(h, h->n + n);
     if (rc) return rc;
     return atomic_ingest(h, [&]() -> int {
@@ -320,7 +320,7 @@ int cgv_load_mmap(cgv_index* h, const char* path, uint64_t* out_rows) {
 
     std::unique_lock<std::mutex> lk(h->mu);
     if (int brc = wait_all_idle(h, lk)) return brc;
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     int rc = grow(h, h->n + count);
     if (rc) return rc;
     // page cache -> pinned staging -> device, double buffered: the CPU copy of chunk i+1 overlaps the
@@ -394,7 +394,7 @@ int cgv_save_mmap(cgv_index* h, const char* path) {
     std::unique_lock<std::mutex> lk(h->mu);
     if (int brc = wait_all_idle(h, lk)) return brc;
     if (h->n == 0) return CGV_OK;
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     SearchCtx* c = &h->ctx[0];
     hipStream_t s = c->stream;
     if (int orc = order_after_caller(h, c)) return orc;
@@ -445,7 +445,7 @@ int cgv_update_row_f32(cgv_index* h, uint64_t id, const float* row_host) {
         if (e < FP8_EXP_MIN || e > FP8_EXP_MAX)
             return fail(CGV_ERR_INVALID_ARG, "fp8 storage: the row's largest magnitude is outside [2^-48, 2^48]; not applied");
     }
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     int rc;
     if ((rc = h->addstage.ensure((size_t)h->D * 4))) return rc;
     hipStream_t s = h->stream;
@@ -492,7 +492,7 @@ int cgv_search_begin_f32_dev(cgv_index* h, const float* queries_dev, uint32_t nq
     int rc = check_search_args(h, queries_dev, k, out_idx_dev, out_score_dev);
     if (rc) return rc;
     std::unique_lock<std::mutex> lk(h->mu);
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     SearchCtx* c = acquire_ctx(h, lk, /*split=*/true);
     if (!c)
         return fail(CGV_ERR_BUSY, "this thread already holds all " + std::to_string(N_CTX) +
@@ -524,7 +524,7 @@ int cgv_search_end(cgv_index* h, uint64_t ticket) {
         std::lock_guard<std::mutex> lk(h->mu);
         if (!c->busy || c->gen != (uint32_t)(ticket >> 8)) return fail(CGV_ERR_INVALID_ARG, "stale ticket");
     }
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     int rc = search_finish(h, c);
     if (rc) (void)hipStreamSynchronize(c->cur());
     c->on_caller = false;  // (a packed ticket ended here: its provisional records are simply not refreshed)
@@ -557,7 +557,7 @@ int cgv_search_packed_begin_f32_dev(cgv_index* h, const float* queries_dev, uint
     int rc = check_search_args(h, queries_dev, k, rec_out_dev, rec_out_dev);
     if (rc) return rc;
     std::unique_lock<std::mutex> lk(h->mu);
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     SearchCtx* c = acquire_ctx(h, lk, /*split=*/true);
     if (!c)
         return fail(CGV_ERR_BUSY, "this thread already holds all " + std::to_string(N_CTX) +
@@ -611,7 +611,7 @@ int cgv_search_packed_end(cgv_index* h, uint64_t ticket, int* repacked) {
         std::lock_guard<std::mutex> lk(h->mu);
         if (!c->busy || c->gen != (uint32_t)(ticket >> 8) || !c->rec_out) return fail(CGV_ERR_INVALID_ARG, "stale ticket");
     }
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     int rc = search_finish(h, c);
     if (rc == CGV_OK && c->rewrote) {  // the exact scan replaced (some of) the results: final records now
         launch_pack(c->outidx.as<uint64_t>(), c->outscore.as<float>(), c->nq, c->k, c->rec_out, nullptr, 0u, c->cur());
@@ -640,7 +640,7 @@ static int search_host_plain(cgv_index* h, const float* queries_host, uint32_t n
                              float* out_score_host) {
     int rc;
     std::unique_lock<std::mutex> lk(h->mu);
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     SearchCtx* c = acquire_ctx(h, lk);
     if (!c) return fail(CGV_ERR_BUSY, "this thread holds every search context of the handle (cgv_search_begin without cgv_search_end)");
     hipStream_t s = c->stream;
@@ -756,7 +756,7 @@ static void search_coalesced(cgv_index* h, std::vector<CoReq*>& batch, uint32_t 
     }
     if (nq_total == 0) return;
     std::unique_lock<std::mutex> lk(h->mu);
-    if (hipSetDevice(h->device) != hipSuccess) {
+    if (cgv::use_device(h->device) != hipSuccess) {
         (void)hipGetLastError();
         return all_alone();
     }
@@ -877,7 +877,7 @@ int cgv_get_row_f32(cgv_index* h, uint64_t id, float* out_host) {
     if (int brc = wait_all_idle(h, lk)) return brc;
     SearchCtx* c = &h->ctx[0];
     if (id >= h->n) return fail(CGV_ERR_OUT_OF_RANGE, "row id out of range");
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     int rc;
     if ((rc = c->qstage.ensure((size_t)h->D * 4))) return rc;
     hipStream_t s = c->stream;
@@ -923,7 +923,7 @@ int cgv_batch_similarity_f32(cgv_index* h, const float* query_host, int op, uint
     std::unique_lock<std::mutex> lk(h->mu);
     if (int brc = wait_all_idle(h, lk)) return brc;
     SearchCtx* c = &h->ctx[0];
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     const uint64_t n = limit_rows ? std::min<uint64_t>(limit_rows, h->n) : h->n;
     if (n == 0) return CGV_OK;
     hipStream_t s = c->stream;
@@ -956,7 +956,7 @@ static int score_pairs(cgv_index* h, const float* queries_host, uint32_t nq, int
         for (uint64_t i = 0; i < npairs; ++i)
             if (qsel_host[i] >= nq) return fail(CGV_ERR_INVALID_ARG, "pair list: query index out of range");
     std::unique_lock<std::mutex> lk(h->mu);
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     SearchCtx* c = acquire_ctx(h, lk);
     if (!c) return fail(CGV_ERR_BUSY, "this thread holds every search context of the handle");
     hipStream_t s = c->stream;
@@ -1014,7 +1014,7 @@ int cgv_truncate(cgv_index* h, uint64_t n_rows) {
     std::unique_lock<std::mutex> lk(h->mu);
     if (int brc = wait_all_idle(h, lk)) return brc;
     if (n_rows >= h->n) return CGV_OK;
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     // the corpus-wide maxima (largest norm, shadow residuals) stay as they are: over-estimates only widen the
     // error bound of the exactness check, they never invalidate it
     return ingest_rollback(h, IngestSnapshot{n_rows, h->max_norm_c, h->res_rel_c, h->res_abs_c});
@@ -1029,7 +1029,7 @@ int cgv_search_baseline_f32(cgv_index* h, const float* query_host, uint32_t limi
     if (int brc = wait_all_idle(h, lk)) return brc;
     SearchCtx* c = &h->ctx[0];
     if (h->n == 0 || limit == 0) return CGV_OK;  // optimization.rs:382-384
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     hipStream_t s = c->stream;
     if (int orc = order_after_caller(h, c)) return orc;
     int rc;
@@ -1057,7 +1057,7 @@ static int normalize_rows_host(int device_id, float* rows_host, uint64_t n, uint
     if (n == 0 || dim == 0) return CGV_OK;  // simd_ops.rs:190-192
     if (!rows_host) return fail(CGV_ERR_INVALID_ARG, "rows is NULL");
     if (cgv_device_count() == 0) return fail(CGV_ERR_HIP, "no HIP device visible: libcgvec_hip has no CPU fallback");
-    HIPCHK(hipSetDevice(device_id));
+    HIPCHK(cgv::use_device(device_id));
     float* d = nullptr;
     const size_t bytes = (size_t)n * dim * 4;
     HIPCHK(hipMalloc((void**)&d, bytes));
@@ -1086,7 +1086,7 @@ int cgv_merge_topk_dev(int device_id, const uint64_t* idx_dev, const float* scor
     if (nq == 0 || k == 0) return CGV_OK;
     if (!idx_dev || !score_dev || !out_idx_dev || !out_score_dev || g == 0) return fail(CGV_ERR_INVALID_ARG, "bad argument");
     if (g > 64) return fail(CGV_ERR_INVALID_ARG, "more than 64 partial lists per query");
-    HIPCHK(hipSetDevice(device_id));
+    HIPCHK(cgv::use_device(device_id));
     if ((uint64_t)g * k > 4096) {  // beyond the LDS merge: G-way wave merge (any k)
         hipLaunchKernelGGL(merge_topk_wave_kernel, dim3((nq + 3) / 4), dim3(256), 0, (hipStream_t)stream, (const char*)idx_dev,
                            (uint64_t)k * 8, (const char*)score_dev, (uint64_t)k * 4, g, nq, k, out_idx_dev, out_score_dev);
@@ -1125,7 +1125,7 @@ int cgv_free_pinned(void* p) {
 }
 
 void* cgv_host_device_alias(int device_id, const void* host_ptr, size_t bytes) {
-    if (!host_ptr || hipSetDevice(device_id) != hipSuccess) {
+    if (!host_ptr || cgv::use_device(device_id) != hipSuccess) {
         (void)hipGetLastError();
         return nullptr;
     }
@@ -1136,7 +1136,7 @@ int cgv_pack_topk_dev(int device_id, const uint64_t* idx_dev, const float* score
                       uint32_t* out_rec_dev, void* stream) {
     if (nq == 0 || k == 0) return CGV_OK;
     if (!idx_dev || !score_dev || !out_rec_dev) return fail(CGV_ERR_INVALID_ARG, "NULL buffer");
-    HIPCHK(hipSetDevice(device_id));
+    HIPCHK(cgv::use_device(device_id));
     const uint64_t total = (uint64_t)nq * packed_width(k);
     hipLaunchKernelGGL(pack_topk_kernel, dim3((unsigned)std::min<uint64_t>(1024, (total + 255) / 256)), dim3(256), 0,
                        (hipStream_t)stream, idx_dev, score_dev, nq, k, out_rec_dev);
@@ -1149,7 +1149,7 @@ int cgv_merge_packed_flag_dev(int device_id, const uint32_t* rec_dev, uint32_t g
     if (nq == 0 || k == 0) return CGV_OK;
     if (!rec_dev || !out_idx_dev || !out_score_dev || g == 0) return fail(CGV_ERR_INVALID_ARG, "bad argument");
     if (g > 64) return fail(CGV_ERR_INVALID_ARG, "more than 64 partial lists per query");
-    HIPCHK(hipSetDevice(device_id));
+    HIPCHK(cgv::use_device(device_id));
     // pinned HOST result arrays (and redo word) are written in place by the merge kernel (no D2H copies for the caller to enqueue)
     if (void* al = device_alias(out_idx_dev, (size_t)nq * k * 8)) out_idx_dev = (uint64_t*)al;
     if (void* al = device_alias(out_score_dev, (size_t)nq * k * 4)) out_score_dev = (float*)al;
@@ -1194,7 +1194,7 @@ int cgv_use_own_stream(cgv_index* h) {
 
 int cgv_synchronize(cgv_index* h) {
     if (!h) return fail(CGV_ERR_INVALID_ARG, "handle is NULL");
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     HIPCHK(hipStreamSynchronize(h->stream));
     for (SearchCtx& c : h->ctx) HIPCHK(hipStreamSynchronize(c.stream));
     return CGV_OK;
@@ -1243,7 +1243,7 @@ int cgv_debug_coarse_scores_dev(cgv_index* h, const float* queries_dev, uint32_t
     std::unique_lock<std::mutex> lk(h->mu);
     if (int brc = wait_all_idle(h, lk)) return brc;
     SearchCtx* c = &h->ctx[0];
-    HIPCHK(hipSetDevice(h->device));
+    HIPCHK(cgv::use_device(h->device));
     hipStream_t s = c->stream;
     if (int orc = order_after_caller(h, c)) return orc;
     int rc;

@@ -27,6 +27,7 @@
 #include "../../include/cgvec.h"
 #include "coalesce.h"
 #include "common.h"
+#include "use_device.h"
 #include "coarse_launch.h"
 #include "kernels_coarse.h"
 #include "kernels_exact.h"

@@ -20,6 +20,7 @@
 #include <vector>
 
 #include "../../include/cgvec.h"
+#include "use_device.h"
 #include "../../include/cgvec_i8.h"
 
 extern "C" int cgv_set_error_(int code, const char* msg);  // abi.hip (shared thread-local message)
@@ -250,7 +251,7 @@ int cgv_i8_create(uint32_t dim, int device_id, cgv_i8_index** out) {
     int ndev = cgv_device_count();
     if (ndev == 0) return fail(CGV_ERR_HIP, "no HIP device visible: libcgvec_hip has no CPU fallback");
     if (device_id < 0 || device_id >= ndev) return fail(CGV_ERR_INVALID_ARG, "device_id out of range");
-    I8CHK(hipSetDevice(device_id));
+    I8CHK(cgv::use_device(device_id));
     cgv_i8_index* h = new cgv_i8_index();
     h->device = device_id;
     h->dim = dim;
@@ -270,7 +271,7 @@ int cgv_i8_create(uint32_t dim, int device_id, cgv_i8_index** out) {
 
 int cgv_i8_destroy(cgv_i8_index* h) {
     if (!h) return CGV_OK;
-    (void)hipSetDevice(h->device);
+    (void)cgv::use_device(h->device);
     if (h->stream) (void)hipStreamSynchronize(h->stream);
     void* bufs[] = {h->data, h->scores, h->q8, h->stage, h->f_idx, h->f_score, h->f_cnt};
     for (void* p : bufs)
@@ -285,7 +286,7 @@ int cgv_i8_add_u8(cgv_i8_index* h, const uint8_t* data_host, uint64_t n) {
     if (n == 0) return CGV_OK;
     if (!data_host) return fail(CGV_ERR_INVALID_ARG, "data is NULL");
     std::lock_guard<std::mutex> lk(h->mu);
-    I8CHK(hipSetDevice(h->device));
+    I8CHK(cgv::use_device(h->device));
     int rc = grow(h, h->n + n);
     if (rc) return rc;
     I8CHK(hipMemcpyAsync(h->data + h->n * h->dim, data_host, n * h->dim, hipMemcpyHostToDevice, h->stream));
@@ -299,7 +300,7 @@ int cgv_i8_add_f32(cgv_i8_index* h, const float* rows_host, uint64_t n) {
     if (n == 0) return CGV_OK;
     if (!rows_host) return fail(CGV_ERR_INVALID_ARG, "rows is NULL");
     std::lock_guard<std::mutex> lk(h->mu);
-    I8CHK(hipSetDevice(h->device));
+    I8CHK(cgv::use_device(h->device));
     int rc = grow(h, h->n + n);
     if (rc) return rc;
     const uint64_t chunk = std::max<uint64_t>(1, (256ull << 20) / ((uint64_t)h->dim * 4));
@@ -323,7 +324,7 @@ int cgv_i8_get_row_u8(cgv_i8_index* h, uint64_t id, uint8_t* out_host) {
     if (!h || !out_host) return fail(CGV_ERR_INVALID_ARG, "NULL argument");
     std::lock_guard<std::mutex> lk(h->mu);
     if (id >= h->n) return fail(CGV_ERR_OUT_OF_RANGE, "row id out of range");
-    I8CHK(hipSetDevice(h->device));
+    I8CHK(cgv::use_device(h->device));
     I8CHK(hipMemcpyAsync(out_host, h->data + id * h->dim, h->dim, hipMemcpyDeviceToHost, h->stream));
     I8CHK(hipStreamSynchronize(h->stream));
     return CGV_OK;
@@ -333,7 +334,7 @@ int cgv_i8_scores_f32(cgv_i8_index* h, const float* query_host, uint32_t query_l
     if (!h || !query_host || !out_host) return fail(CGV_ERR_INVALID_ARG, "NULL argument");
     std::lock_guard<std::mutex> lk(h->mu);
     if (h->n == 0) return CGV_OK;
-    I8CHK(hipSetDevice(h->device));
+    I8CHK(cgv::use_device(h->device));
     float nq = 0.0f;
     int rc = launch_scores(h, query_host, query_len, &nq);
     if (rc) return rc;
@@ -353,7 +354,7 @@ int cgv_i8_search_optimized(cgv_i8_index* h, const float* query_host, uint32_t q
     const uint64_t limit = std::max<uint64_t>(limit_in, 1);  // optimization.rs:64
     std::lock_guard<std::mutex> lk(h->mu);
     if (h->n == 0) return CGV_OK;  // :71-73
-    I8CHK(hipSetDevice(h->device));
+    I8CHK(cgv::use_device(h->device));
     float nq = 0.0f;
     int rc = launch_scores(h, query_host, query_len, &nq);
     if (rc) return rc;
@@ -414,7 +415,7 @@ int cgv_quantize_u8_f32(int device_id, const float* rows_host, uint64_t n, uint3
     if (n == 0 || dim == 0) return CGV_OK;
     if (!rows_host || !out_host) return fail(CGV_ERR_INVALID_ARG, "NULL buffer");
     if (cgv_device_count() == 0) return fail(CGV_ERR_HIP, "no HIP device visible: libcgvec_hip has no CPU fallback");
-    I8CHK(hipSetDevice(device_id));
+    I8CHK(cgv::use_device(device_id));
     const uint64_t total = n * dim;
     float* din = nullptr;
     uint8_t* dout = nullptr;
@@ -437,7 +438,7 @@ int cgv_quantize_u4_f32(int device_id, const float* rows_host, uint64_t n, uint3
     if (n == 0 || dim == 0) return CGV_OK;
     if (!rows_host || !out_host) return fail(CGV_ERR_INVALID_ARG, "NULL buffer");
     if (cgv_device_count() == 0) return fail(CGV_ERR_HIP, "no HIP device visible: libcgvec_hip has no CPU fallback");
-    I8CHK(hipSetDevice(device_id));
+    I8CHK(cgv::use_device(device_id));
     const uint64_t total = n * dim, obytes = n * ((dim + 1) / 2);
     float* din = nullptr;
     uint8_t* dout = nullptr;

@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "../../include/cgvec.h"
+#include "use_device.h"
 #include "../../include/cgvec_quant.h"
 
 extern "C" int cgv_set_error_(int code, const char* msg);
@@ -227,7 +228,7 @@ int cgv_sq_train_f32(cgv_sq* q, const float* rows_host, uint64_t n) {
     if (n == 0) return fail(CGV_ERR_INVALID_ARG, "Cannot train on empty vector set");  // :356-360
     if (!rows_host) return fail(CGV_ERR_INVALID_ARG, "rows is NULL");
     std::lock_guard<std::mutex> lk(q->mu);
-    QCHK(hipSetDevice(q->device));
+    QCHK(cgv::use_device(q->device));
     DevMem rows, mn, mx;
     QCHK(rows.alloc(n * q->dim * 4));
     QCHK(mn.alloc((size_t)q->dim * 4));
@@ -276,7 +277,7 @@ int cgv_sq_params(cgv_sq* q, float* scales_out, float* biases_out) {
 }
 
 static int sq_run(cgv_sq* q, const void* in_host, size_t in_bytes, void* out_host, size_t out_bytes, uint64_t n, bool enc) {
-    QCHK(hipSetDevice(q->device));
+    QCHK(cgv::use_device(q->device));
     DevMem in, out, sc, bi;
     QCHK(in.alloc(in_bytes));
     QCHK(out.alloc(out_bytes));
@@ -347,7 +348,7 @@ int cgv_pq_train_f32(cgv_pq* q, const float* rows_host, uint64_t n) {
     if (n == 0) return fail(CGV_ERR_INVALID_ARG, "Cannot train on empty vector set");  // :156-160
     if (!rows_host) return fail(CGV_ERR_INVALID_ARG, "rows is NULL");
     std::lock_guard<std::mutex> lk(q->mu);
-    QCHK(hipSetDevice(q->device));
+    QCHK(cgv::use_device(q->device));
     DevMem rows, cent, assign, flag;
     QCHK(rows.alloc(n * q->dim * 4));
     QCHK(cent.alloc(q->cent.size() * 4));
@@ -390,7 +391,7 @@ int cgv_pq_encode_f32(cgv_pq* q, const float* rows_host, uint64_t n, uint8_t* co
     if (!q->trained) return fail(CGV_ERR_INVALID_ARG, "Quantizer not trained");  // :191-193
     if (n == 0) return CGV_OK;
     if (!rows_host || !codes_out) return fail(CGV_ERR_INVALID_ARG, "NULL buffer");
-    QCHK(hipSetDevice(q->device));
+    QCHK(cgv::use_device(q->device));
     DevMem rows, cent, codes;
     QCHK(rows.alloc(n * q->dim * 4));
     QCHK(cent.alloc(q->cent.size() * 4));
@@ -413,7 +414,7 @@ int cgv_pq_decode(cgv_pq* q, const uint8_t* codes_host, uint64_t n, float* out_h
     if (!q->trained) return fail(CGV_ERR_INVALID_ARG, "Quantizer not trained");  // :222-224
     if (n == 0) return CGV_OK;
     if (!codes_host || !out_host) return fail(CGV_ERR_INVALID_ARG, "NULL buffer");
-    QCHK(hipSetDevice(q->device));
+    QCHK(cgv::use_device(q->device));
     DevMem codes, cent, out, bad;
     QCHK(codes.alloc(n * q->m));
     QCHK(cent.alloc(q->cent.size() * 4));

@@ -41,6 +41,7 @@
 #include <vector>
 
 #include "../../include/cgvec.h"
+#include "use_device.h"
 
 extern "C" int cgv_set_error_(int code, const char* msg);  // abi.hip: the library's thread-local error message
 extern "C" int cgv_score_pairs_f32_(cgv_index* h, const float* queries_host, uint32_t nq, int op, const uint32_t* qsel_host,
@@ -240,7 +241,7 @@ constexpr int N_SLOTS = 3;
 constexpr int ABORT_LOCK_MS = 500;
 
 void worker_main(Shard* s) {
-    (void)hipSetDevice(s->device);
+    (void)cgv::use_device(s->device);
     Worker& w = s->w;
     std::unique_lock<std::mutex> lk(w.mu);
     for (;;) {
@@ -287,7 +288,7 @@ struct DeviceGuard {
         }
     }
     ~DeviceGuard() {
-        if (dev >= 0) (void)hipSetDevice(dev);
+        if (dev >= 0) (void)cgv::use_device(dev);
     }
 };
 
@@ -326,7 +327,7 @@ int warm_up_comms(cgv_sharded* s, const Rccl* r) {
     std::vector<void*> src(s->G, nullptr), dst(s->G, nullptr);
     int rc = CGV_OK, e = 0;
     for (uint32_t g = 0; g < s->G && rc == CGV_OK; ++g) {
-        if (hipSetDevice(s->sh[g]->device) != hipSuccess || hipMalloc(&src[g], 64) != hipSuccess ||
+        if (cgv::use_device(s->sh[g]->device) != hipSuccess || hipMalloc(&src[g], 64) != hipSuccess ||
             hipMalloc(&dst[g], (size_t)64 * s->G) != hipSuccess)
             rc = fail(CGV_ERR_HIP, "warm-up buffers of the RCCL exchange");
     }
@@ -338,7 +339,7 @@ int warm_up_comms(cgv_sharded* s, const Rccl* r) {
         if (e != 0) rc = fail(CGV_ERR_HIP, std::string("ncclAllGather (warm-up): ") + r->GetErrorString(e));
     }
     for (uint32_t g = 0; g < s->G; ++g) {
-        if (hipSetDevice(s->sh[g]->device) != hipSuccess) continue;
+        if (cgv::use_device(s->sh[g]->device) != hipSuccess) continue;
         if (rc == CGV_OK && hipStreamSynchronize(s->sh[g]->xs) != hipSuccess) rc = fail(CGV_ERR_HIP, "warm-up collective did not complete");
         if (src[g]) (void)hipFree(src[g]);
         if (dst[g]) (void)hipFree(dst[g]);
@@ -439,7 +440,7 @@ int cgv_sharded_create(uint32_t dim, int metric, int dtype, uint32_t n_devices, 
         for (uint32_t g = 1; g < n_devices; ++g) {
             int can = 0;
             if (hipDeviceCanAccessPeer(&can, s->sh[g]->device, s->sh[0]->device) == hipSuccess && can) {
-                (void)hipSetDevice(s->sh[g]->device);
+                (void)cgv::use_device(s->sh[g]->device);
                 const hipError_t e = hipDeviceEnablePeerAccess(s->sh[0]->device, 0);
                 if (e != hipSuccess) (void)hipGetLastError();  // already enabled / not supported: copies are staged
             }
@@ -477,7 +478,7 @@ int cgv_sharded_destroy(cgv_sharded* s) {
     }
     const Rccl* r = g_rccl.ok() ? &g_rccl : nullptr;
     for (Shard* sh : s->sh) {
-        (void)hipSetDevice(sh->device);
+        (void)cgv::use_device(sh->device);
         if (sh->xs) (void)hipStreamSynchronize(sh->xs);
         if (sh->comm && r && !s->comms_aborted.load()) (void)r->CommDestroy(sh->comm);
         if (sh->ix) (void)cgv_destroy(sh->ix);
@@ -491,7 +492,7 @@ int cgv_sharded_destroy(cgv_sharded* s) {
         if (sh->xs) (void)hipStreamDestroy(sh->xs);
     }
     if (!s->sh.empty()) {
-        (void)hipSetDevice(s->sh[0]->device);
+        (void)cgv::use_device(s->sh[0]->device);
         for (auto& sl : s->slots) {
             sl.moidx.release();
             sl.mosc.release();
@@ -798,16 +799,16 @@ int cgv_sharded_search_begin_f32(cgv_sharded* s, const float* queries_host, uint
         if (sl.pin_q) (void)hipHostFree(sl.pin_q);
         sl.pin_q = nullptr;
         sl.pin_q_bytes = 0;
-        SHIP(hipSetDevice(root->device));
+        SHIP(cgv::use_device(root->device));
         SHIP(hipHostMalloc((void**)&sl.pin_q, qbytes, hipHostMallocPortable));
         sl.pin_q_bytes = qbytes;
     }
     if (!sl.pin_redo) {
-        SHIP(hipSetDevice(root->device));
+        SHIP(cgv::use_device(root->device));
         SHIP(hipHostMalloc((void**)&sl.pin_redo, 64, hipHostMallocPortable | hipHostMallocMapped));
     }
     for (Shard* sh : s->sh) {
-        SHIP(hipSetDevice(sh->device));
+        SHIP(cgv::use_device(sh->device));
         Shard::SlotBufs& b = sh->slot[si];
         int rc;
         if ((rc = b.qdev.ensure(qbytes))) return rc;
@@ -823,7 +824,7 @@ int cgv_sharded_search_begin_f32(cgv_sharded* s, const float* queries_host, uint
         if (!b.done) SHIP(hipEventCreateWithFlags(&b.done, hipEventDisableTiming));
     }
     if (xch) {
-        SHIP(hipSetDevice(root->device));
+        SHIP(cgv::use_device(root->device));
         int rc;
         if ((rc = sl.moidx.ensure((size_t)nq * k * 8))) return rc;
         if ((rc = sl.mosc.ensure((size_t)nq * k * 4))) return rc;
@@ -980,7 +981,7 @@ int cgv_sharded_search_end(cgv_sharded* s, uint64_t ticket) {
         drain_streams(s);
         rerun_by_copy = true;
     }
-    hipError_t he = hipSetDevice(root->device);
+    hipError_t he = cgv::use_device(root->device);
     if (he != hipSuccess) return finish(fail(CGV_ERR_HIP, std::string("hipSetDevice: ") + hipGetErrorString(he)));
     if (!xch) {  // one shard, no exchange: its results go back as they are
         he = hipMemcpyAsync(sl.out_idx, root->slot[si].oidx.p, (size_t)nq * k * 8, hipMemcpyDeviceToHost, root->xs);
@@ -1039,7 +1040,7 @@ int cgv_sharded_search_end(cgv_sharded* s, uint64_t ticket) {
                 rc = fail(CGV_ERR_HIP, msg + " (RCCL communicators aborted; the handle continues with the copy exchange)");
             }
             if (rc) return finish(rc);
-            if (hipSetDevice(root->device) != hipSuccess) return finish(fail(CGV_ERR_HIP, "hipSetDevice(root)"));
+            if (cgv::use_device(root->device) != hipSuccess) return finish(fail(CGV_ERR_HIP, "hipSetDevice(root)"));
             if ((rc = root_round())) return finish(rc);
             if (*sl.pin_redo != 0u) return finish(fail(CGV_ERR_INTERNAL, "records still provisional after the searches ended"));
             if (was_redo) s->redo_batches++;

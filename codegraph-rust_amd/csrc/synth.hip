@@ -17,6 +17,7 @@
 #include <string>
 
 #include "../../include/cgvec.h"
+#include "use_device.h"
 
 extern "C" int cgv_set_error_(int code, const char* msg);  // abi.hip
 
@@ -141,7 +142,7 @@ extern "C" int cgv_synth_rows_f32_dev(int device_id, uint64_t seed, uint64_t row
     if (nrows == 0 || dim == 0) return CGV_OK;
     if (!out_dev) return cgv_set_error_(CGV_ERR_INVALID_ARG, "out is NULL");
     if (cgv_device_count() == 0) return cgv_set_error_(CGV_ERR_HIP, "no HIP device visible: libcgvec_hip has no CPU fallback");
-    hipError_t e = hipSetDevice(device_id);
+    hipError_t e = cgv::use_device(device_id);
     if (e == hipSuccess) {
         hipLaunchKernelGGL(synth_rows_kernel, dim3((unsigned)((nrows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, out_dev, seed, row0,
                            nrows, dim, normalise);
