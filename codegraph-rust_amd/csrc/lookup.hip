@@ -1,0 +1,472 @@
+// lookup.hip - rows of a table by id, scaled, and the table's gradient (include/cgvec_train.h).
+//
+// Gradient: out of n incoming rows every table row r gets the sum of those whose id is r. A thread owns 16 bytes of one table
+// row and adds up its summands, so that each row is written exactly once and no atomics touch a float; for that the positions
+// are sorted by id first (stable, so that a row's summands come in the order of the input).
+//   few ids (<= DIRECT_IDS): a workgroup owns some table rows, looks through all ids itself, and there is one launch;
+//   more: radix sort of (id, position), 11 bits at most a pass; a run's ends are noted per row; rows whose run is longer than
+//   LONG positions are first summed in pieces of LONG by separate waves (a frequent token would otherwise keep one thread busy).
+// Bound by the bytes of the incoming rows and of the whole table gradient.
+#include <type_traits>
+
+#include "../../include/cgvec_train.h"
+#include "ops_common.h"
+
+using namespace cgv_ops;
+
+namespace {
+
+constexpr uint32_t DIRECT_IDS = 512;
+constexpr uint32_t SORT_THREADS = 256, SORT_STEPS = 8, SORT_BLOCK = SORT_THREADS * SORT_STEPS;   // elements of a workgroup
+constexpr uint32_t MAX_DIGIT = 11;
+
+// ---- a vector of a row: V elements, 16 bytes or one element ------------------------------------------------------------------
+template <int DT, int V>
+struct Vec {
+    float v[V];
+    __device__ void zero() {
+        for (int i = 0; i < V; ++i) v[i] = 0.0f;
+    }
+    __device__ void load(const void* p, uint64_t at) {   // at: in elements, a multiple of V
+        if (V == 1) {
+            v[0] = load_elem<DT>(p, at);
+        } else if (DT == cgv::DT_F32) {
+            const float4 t = *(const float4*)((const float*)p + at);
+            v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+        } else {
+            const uint4 t = *(const uint4*)((const uint16_t*)p + at);
+            const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+            for (int i = 0; i < V; ++i) v[i] = half_to_f32<DT>((uint16_t)(w[(i / 2) & 3] >> (16 * (i & 1))));
+        }
+    }
+    __device__ void store(void* p, uint64_t at) const {
+        if (V == 1) {
+            store_elem<DT>(p, at, v[0]);
+        } else if (DT == cgv::DT_F32) {
+            *(float4*)((float*)p + at) = make_float4(v[0], v[1 % V], v[2 % V], v[3 % V]);
+        } else {
+            uint32_t w[4];
+            for (int i = 0; i < 4; ++i)
+                w[i] = f32_to_half<DT>(v[(2 * i) % V]) | (uint32_t)f32_to_half<DT>(v[(2 * i + 1) % V]) << 16;
+            *(uint4*)((uint16_t*)p + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    __device__ void add(const Vec& o) {
+        for (int i = 0; i < V; ++i) v[i] += o.v[i];
+    }
+    __device__ void mul(float s) {
+        for (int i = 0; i < V; ++i) v[i] *= s;
+    }
+};
+
+// ---- forward ----------------------------------------------------------------------------------------------------------------
+// one thread per vector of the output; VPR vectors a row
+template <int DT, int V>
+__global__ __launch_bounds__(256) void lookup_kernel(const void* __restrict__ table, uint64_t n_rows, uint32_t vpr, uint64_t row_stride,
+                                                     const int64_t* __restrict__ ids, uint64_t n_ids, float scale, void* __restrict__ out) {
+    const uint64_t base = (uint64_t)blockIdx.x * 256;
+    const uint64_t row0 = base / vpr;                       // the same for the whole workgroup
+    const uint32_t in = (uint32_t)(base % vpr) + threadIdx.x;
+    const uint64_t row = row0 + in / vpr;
+    if (row >= n_ids) return;
+    const uint32_t col = in % vpr;
+    const int64_t id = ids[row];
+    Vec<DT, V> v;
+    if (id >= 0 && (uint64_t)id < n_rows) {
+        v.load(table, (uint64_t)id * row_stride + (uint64_t)col * V);
+        v.mul(scale);
+    } else {
+        v.zero();
+    }
+    v.store(out, (row * vpr + col) * V);
+}
+
+// ---- gradient, few ids ------------------------------------------------------------------------------------------------------
+template <int DT, int V>
+__global__ __launch_bounds__(256) void grad_direct_kernel(const void* __restrict__ dout, const int64_t* __restrict__ ids, uint32_t n_ids,
+                                                          uint64_t n_rows, uint32_t vpr, uint32_t rows_per_block, float scale,
+                                                          void* __restrict__ dtable) {
+    __shared__ uint32_t mine[DIRECT_IDS], at[DIRECT_IDS];   // the ids that name a row of this workgroup: row - row0, and their place
+    __shared__ uint32_t found;
+    const uint64_t row0 = (uint64_t)blockIdx.x * rows_per_block;
+    const uint32_t rows = (uint32_t)min((uint64_t)rows_per_block, n_rows - row0);
+    if (threadIdx.x < 64) {   // one wave: the list keeps the order of the input
+        uint32_t base = 0;
+        for (uint32_t a = 0; a < n_ids; a += 64) {
+            const uint32_t i = a + threadIdx.x;
+            const int64_t id = i < n_ids ? ids[i] : -1;
+            const bool in = id >= (int64_t)row0 && id < (int64_t)(row0 + rows);
+            const uint64_t m = __ballot(in);
+            if (in) {
+                const uint32_t k = base + __popcll(m & ((1ull << threadIdx.x) - 1));
+                mine[k] = (uint32_t)(id - (int64_t)row0);
+                at[k] = i;
+            }
+            base += __popcll(m);
+        }
+        if (threadIdx.x == 0) found = base;
+    }
+    __syncthreads();
+    const uint32_t nf = found;
+    for (uint32_t t = threadIdx.x; t < rows * vpr; t += 256) {
+        const uint32_t r = t / vpr, col = t % vpr;
+        Vec<DT, V> acc, v;
+        acc.zero();
+        for (uint32_t k = 0; k < nf; ++k)
+            if (mine[k] == r) {
+                v.load(dout, ((uint64_t)at[k] * vpr + col) * V);
+                acc.add(v);
+            }
+        acc.mul(scale);
+        acc.store(dtable, ((row0 + r) * vpr + col) * V);
+    }
+}
+
+// ---- gradient, sorted -------------------------------------------------------------------------------------------------------
+struct SortPass {
+    const int64_t* ids;             // first pass: keys come from here
+    const uint32_t *keys, *pos;     // later passes
+    uint32_t *keys_out, *pos_out;
+    uint32_t *hist, *total;         // [bins][blocks], [bins]
+    uint32_t n, n_rows, blocks, shift, bits;
+    __device__ uint32_t key(uint32_t i) const {
+        if (!ids) return keys[i];
+        const int64_t id = ids[i];
+        return id >= 0 && id < (int64_t)n_rows ? (uint32_t)id : n_rows;   // strangers go behind the last row
+    }
+    __device__ uint32_t digit(uint32_t k) const { return (k >> shift) & ((1u << bits) - 1u); }
+};
+
+// counts of a workgroup's digits; the first pass clears the rows' run ends on the way
+__global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(SortPass p, uint64_t* __restrict__ runs) {
+    __shared__ uint32_t h[1u << MAX_DIGIT];
+    const uint32_t bins = 1u << p.bits;
+    for (uint32_t i = threadIdx.x; i < bins; i += SORT_THREADS) h[i] = 0;
+    __syncthreads();
+    const uint32_t lo = blockIdx.x * SORT_BLOCK;
+    for (uint32_t s = 0; s < SORT_STEPS; ++s) {
+        const uint32_t i = lo + s * SORT_THREADS + threadIdx.x;
+        if (i < p.n) atomicAdd(&h[p.digit(p.key(i))], 1u);
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < bins; i += SORT_THREADS) p.hist[(uint64_t)i * p.blocks + blockIdx.x] = h[i];
+    if (runs)
+        for (uint64_t i = (uint64_t)blockIdx.x * SORT_THREADS + threadIdx.x; i < p.n_rows; i += (uint64_t)gridDim.x * SORT_THREADS) runs[i] = 0;
+}
+
+// one wave per digit: where each workgroup's elements of that digit start among those of the digit
+__global__ __launch_bounds__(256) void sort_scan_kernel(SortPass p) {
+    const uint32_t bin = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (bin >= (1u << p.bits)) return;
+    uint32_t* h = p.hist + (uint64_t)bin * p.blocks;
+    uint32_t carry = 0;
+    for (uint32_t a = 0; a < p.blocks; a += 64) {
+        const uint32_t v = a + lane < p.blocks ? h[a + lane] : 0u;
+        uint32_t s = v;
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t t = __shfl_up(s, o);
+            if ((int)lane >= o) s += t;
+        }
+        if (a + lane < p.blocks) h[a + lane] = carry + s - v;
+        carry += __shfl(s, 63);
+    }
+    if (lane == 0) p.total[bin] = carry;
+}
+
+__global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(SortPass p) {
+    constexpr uint32_t W = SORT_THREADS / 64;
+    __shared__ uint32_t next[W][1u << MAX_DIGIT];     // where the wave's next element of a digit goes
+    __shared__ uint32_t part[SORT_THREADS];
+    const uint32_t bins = 1u << p.bits, tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+    for (uint32_t i = tid; i < W * bins; i += SORT_THREADS) next[i / bins][i % bins] = 0;
+    __syncthreads();
+    const uint32_t lo = blockIdx.x * SORT_BLOCK + w * (SORT_STEPS * 64);
+    uint32_t k[SORT_STEPS];
+#pragma unroll
+    for (uint32_t s = 0; s < SORT_STEPS; ++s) {
+        const uint32_t i = lo + s * 64 + lane;
+        k[s] = i < p.n ? p.key(i) : 0u;
+        if (i < p.n) atomicAdd(&next[w][p.digit(k[s])], 1u);
+    }
+    // totals of the digits -> where each digit starts: every thread sums its stretch, the stretches are scanned
+    const uint32_t per = (bins + SORT_THREADS - 1) / SORT_THREADS, b0 = tid * per;
+    uint32_t sum = 0;
+    for (uint32_t j = 0; j < per; ++j)
+        if (b0 + j < bins) sum += p.total[b0 + j];
+    part[tid] = sum;
+    __syncthreads();
+    for (uint32_t o = 1; o < SORT_THREADS; o <<= 1) {
+        const uint32_t t = tid >= o ? part[tid - o] : 0u;
+        __syncthreads();
+        part[tid] += t;
+        __syncthreads();
+    }
+    uint32_t start = part[tid] - sum;
+    for (uint32_t j = 0; j < per; ++j) {
+        const uint32_t b = b0 + j;
+        if (b >= bins) break;
+        uint32_t at = start + p.hist[(uint64_t)b * p.blocks + blockIdx.x];
+        start += p.total[b];
+        for (uint32_t x = 0; x < W; ++x) {
+            const uint32_t c = next[x][b];
+            next[x][b] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t s = 0; s < SORT_STEPS; ++s) {
+        const uint32_t i = lo + s * 64 + lane;
+        const bool on = i < p.n;
+        const uint32_t d = p.digit(k[s]);
+        uint64_t same = __ballot(on);
+        for (uint32_t b = 0; b < p.bits; ++b) {
+            const bool bit = (d >> b) & 1u;
+            const uint64_t m = __ballot(bit);
+            same &= bit ? m : ~m;
+        }
+        const uint32_t before = __popcll(same & ((1ull << lane) - 1));
+        uint32_t to = 0;
+        if (on) to = ((volatile uint32_t*)next[w])[d] + before;
+        __builtin_amdgcn_wave_barrier();
+        if (on && before == 0) ((volatile uint32_t*)next[w])[d] = to + (uint32_t)__popcll(same);
+        __builtin_amdgcn_wave_barrier();
+        if (on) {
+            p.keys_out[to] = k[s];
+            p.pos_out[to] = p.ids ? i : p.pos[i];
+        }
+    }
+}
+
+// runs[r] = where the positions of row r begin (low word) and end (high word)
+__global__ __launch_bounds__(256) void runs_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t n_rows, uint32_t* __restrict__ runs) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const uint32_t k = keys[i];
+    if (k >= n_rows) return;
+    if (i == 0 || keys[i - 1] != k) runs[2 * (uint64_t)k] = i;
+    if (i + 1 == n || keys[i + 1] != k) runs[2 * (uint64_t)k + 1] = i + 1;
+}
+
+template <int DT, int V>
+__device__ inline void sum_positions(Vec<DT, V>& acc, const void* dout, const uint32_t* pos, uint32_t lo, uint32_t hi, uint32_t vpr, uint32_t col) {
+    uint32_t k = lo;
+    for (; k + 4 <= hi; k += 4) {
+        Vec<DT, V> v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j].load(dout, ((uint64_t)pos[k + j] * vpr + col) * V);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc.add(v[j]);
+    }
+    for (; k < hi; ++k) {
+        Vec<DT, V> v;
+        v.load(dout, ((uint64_t)pos[k] * vpr + col) * V);
+        acc.add(v);
+    }
+}
+
+// piece c of LONG sorted positions: a run longer than LONG crosses an end of every piece it touches, so a piece has at most two
+// such runs - the one of its first position (slot 2 c) and the one of its last (slot 2 c + 1)
+template <int DT, int V>
+__global__ __launch_bounds__(64) void pieces_kernel(const void* __restrict__ dout, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
+                                                    const uint64_t* __restrict__ runs, uint32_t n, uint32_t n_rows, uint32_t longer, uint32_t vpr,
+                                                    float* __restrict__ partial) {
+    const uint32_t c = blockIdx.x, lo = c * longer, hi = min(lo + longer, n);
+    const uint32_t col = blockIdx.y * 64 + threadIdx.x;
+    if (col >= vpr) return;
+    const uint32_t first = keys[lo], last = keys[hi - 1];
+    for (int side = 0; side < 2; ++side) {
+        const uint32_t k = side ? last : first;
+        if (k >= n_rows || (side && last == first)) continue;
+        const uint32_t b = (uint32_t)runs[k], e = (uint32_t)(runs[k] >> 32);
+        if (e - b <= longer) continue;
+        Vec<DT, V> acc;
+        acc.zero();
+        sum_positions<DT, V>(acc, dout, pos, max(lo, b), min(hi, e), vpr, col);
+        for (int i = 0; i < V; ++i) partial[(((uint64_t)c * 2 + side) * vpr + col) * V + i] = acc.v[i];
+    }
+}
+
+template <int DT, int V>
+__global__ __launch_bounds__(256) void grad_rows_kernel(const void* __restrict__ dout, const uint32_t* __restrict__ pos,
+                                                        const uint64_t* __restrict__ runs, uint64_t n_rows, uint32_t longer, uint32_t vpr,
+                                                        const float* __restrict__ partial, float scale, void* __restrict__ dtable) {
+    const uint64_t base = (uint64_t)blockIdx.x * 256;
+    const uint64_t row0 = base / vpr;
+    const uint32_t in = (uint32_t)(base % vpr) + threadIdx.x;
+    const uint64_t row = row0 + in / vpr;
+    if (row >= n_rows) return;
+    const uint32_t col = in % vpr;
+    const uint32_t b = (uint32_t)runs[row], e = (uint32_t)(runs[row] >> 32);
+    Vec<DT, V> acc;
+    acc.zero();
+    if (e - b <= longer) {
+        sum_positions<DT, V>(acc, dout, pos, b, e, vpr, col);
+    } else {
+        for (uint32_t c = b / longer; c <= (e - 1) / longer; ++c) {
+            const uint64_t slot = (uint64_t)c * 2 + (c * longer < b ? 1 : 0);
+            for (int i = 0; i < V; ++i) acc.v[i] += partial[(slot * vpr + col) * V + i];
+        }
+    }
+    acc.mul(scale);
+    acc.store(dtable, (row * vpr + col) * V);
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------
+
+uint64_t up256(uint64_t b) { return (b + 255) / 256 * 256; }
+
+struct GradPlan {
+    uint32_t passes = 0, bits = 0, blocks = 0, longer = 0;
+    uint64_t off_keys[2], off_pos[2], off_hist, off_total, off_runs, off_partial, bytes = 0;
+    GradPlan(uint64_t n, uint64_t n_rows, uint32_t dim) {
+        if (n <= DIRECT_IDS) return;
+        uint32_t need = 1;
+        while (need < 32 && (n_rows >> need)) ++need;      // bits of n_rows itself: the key of ids that name no row
+        passes = (need + MAX_DIGIT - 1) / MAX_DIGIT;
+        bits = (need + passes - 1) / passes;
+        blocks = (uint32_t)((n + SORT_BLOCK - 1) / SORT_BLOCK);
+        // a run is summed by one thread up to `longer` positions, and pieces of a longer one by one thread again: about the root
+        // of n keeps both chains short
+        longer = 32;
+        while ((uint64_t)longer * longer * 4 < n) longer *= 2;
+        const uint64_t pieces = (n + longer - 1) / longer;
+        for (int i = 0; i < 2; ++i) {
+            off_keys[i] = bytes, bytes += up256(n * 4);
+            off_pos[i] = bytes, bytes += up256(n * 4);
+        }
+        off_hist = bytes, bytes += up256(((uint64_t)blocks << bits) * 4);
+        off_total = bytes, bytes += up256(4ull << bits);
+        off_runs = bytes, bytes += up256(n_rows * 8);
+        off_partial = bytes, bytes += up256(pieces * 2 * dim * 4);
+    }
+};
+
+// 16-byte vectors where every row starts on 16 bytes, single elements otherwise
+bool by_vectors(uint32_t dim, int dtype, uint64_t stride, const void* a, const void* b) {
+    const uint32_t es = esize(dtype);
+    return (uint64_t)dim * es % 16 == 0 && stride * es % 16 == 0 && ((uintptr_t)a | (uintptr_t)b) % 16 == 0;
+}
+
+int check_common(int dtype, uint64_t n_rows, uint32_t dim, uint64_t n_ids, float scale) {
+    if (dtype != CGV_DTYPE_F32 && dtype != CGV_DTYPE_BF16 && dtype != CGV_DTYPE_FP16) return fail(CGV_ERR_INVALID_ARG, "dtype must be f32, bf16 or fp16");
+    if (dim == 0 || dim > 8192) return fail(CGV_ERR_INVALID_ARG, "dim must be in 1..=8192");
+    if (n_rows >= (1ull << 31) || n_ids >= (1ull << 31)) return fail(CGV_ERR_INVALID_ARG, "n_rows and n_ids must be below 2^31");
+    if (!(fabsf(scale) < INFINITY)) return fail(CGV_ERR_NONFINITE, "scale is not finite");
+    return CGV_OK;
+}
+
+template <int DT, int V>
+int launch_lookup(const void* table, uint64_t n_rows, uint32_t dim, uint64_t stride, const int64_t* ids, uint64_t n_ids, float scale, void* out,
+                  hipStream_t s) {
+    const uint32_t vpr = dim / V;
+    const uint64_t blocks = (n_ids * vpr + 255) / 256;
+    if (blocks > 0x7fffffffull) return fail(CGV_ERR_INVALID_ARG, "too many elements for one call");
+    hipLaunchKernelGGL((lookup_kernel<DT, V>), dim3((unsigned)blocks), dim3(256), 0, s, table, n_rows, vpr, stride, ids, n_ids, scale, out);
+    OPCHK(hipGetLastError());
+    return CGV_OK;
+}
+
+template <int DT, int V>
+int launch_grad(const void* dout, const int64_t* ids, uint64_t n_ids, uint64_t n_rows, uint32_t dim, float scale, void* dtable, char* ws,
+                const GradPlan& pl, hipStream_t s) {
+    const uint32_t vpr = dim / V;
+    const uint64_t blocks = (n_rows * vpr + 255) / 256;
+    if (blocks > 0x7fffffffull) return fail(CGV_ERR_INVALID_ARG, "too many elements for one call");
+    if (!pl.passes) {
+        const uint32_t rpb = std::max<uint32_t>(1, 1024 / vpr);      // four vectors a thread
+        hipLaunchKernelGGL((grad_direct_kernel<DT, V>), dim3((unsigned)((n_rows + rpb - 1) / rpb)), dim3(256), 0, s, dout, ids, (uint32_t)n_ids, n_rows,
+                           vpr, rpb, scale, dtable);
+        OPCHK(hipGetLastError());
+        return CGV_OK;
+    }
+    uint64_t* runs = (uint64_t*)(ws + pl.off_runs);
+    for (uint32_t i = 0; i < pl.passes; ++i) {
+        SortPass p{};
+        p.ids = i == 0 ? ids : nullptr;
+        p.keys = (const uint32_t*)(ws + pl.off_keys[(i + 1) & 1]);
+        p.pos = (const uint32_t*)(ws + pl.off_pos[(i + 1) & 1]);
+        p.keys_out = (uint32_t*)(ws + pl.off_keys[i & 1]);
+        p.pos_out = (uint32_t*)(ws + pl.off_pos[i & 1]);
+        p.hist = (uint32_t*)(ws + pl.off_hist);
+        p.total = (uint32_t*)(ws + pl.off_total);
+        p.n = (uint32_t)n_ids;
+        p.n_rows = (uint32_t)n_rows;
+        p.blocks = pl.blocks;
+        p.shift = i * pl.bits;
+        p.bits = pl.bits;
+        hipLaunchKernelGGL(sort_count_kernel, dim3(pl.blocks), dim3(SORT_THREADS), 0, s, p, i == 0 ? runs : (uint64_t*)nullptr);
+        OPCHK(hipGetLastError());
+        hipLaunchKernelGGL(sort_scan_kernel, dim3(((1u << pl.bits) + 3) / 4), dim3(256), 0, s, p);
+        OPCHK(hipGetLastError());
+        hipLaunchKernelGGL(sort_scatter_kernel, dim3(pl.blocks), dim3(SORT_THREADS), 0, s, p);
+        OPCHK(hipGetLastError());
+    }
+    const uint32_t last = (pl.passes - 1) & 1;
+    const uint32_t* keys = (const uint32_t*)(ws + pl.off_keys[last]);
+    const uint32_t* pos = (const uint32_t*)(ws + pl.off_pos[last]);
+    float* partial = (float*)(ws + pl.off_partial);
+    const uint32_t n = (uint32_t)n_ids;
+    hipLaunchKernelGGL(runs_kernel, dim3((n + 255) / 256), dim3(256), 0, s, keys, n, (uint32_t)n_rows, (uint32_t*)runs);
+    OPCHK(hipGetLastError());
+    hipLaunchKernelGGL((pieces_kernel<DT, V>), dim3((n + pl.longer - 1) / pl.longer, (vpr + 63) / 64), dim3(64), 0, s, dout, keys, pos,
+                       (const uint64_t*)runs, n, (uint32_t)n_rows, pl.longer, vpr, partial);
+    OPCHK(hipGetLastError());
+    hipLaunchKernelGGL((grad_rows_kernel<DT, V>), dim3((unsigned)blocks), dim3(256), 0, s, dout, pos, (const uint64_t*)runs, n_rows, pl.longer, vpr,
+                       (const float*)partial, scale, dtable);
+    OPCHK(hipGetLastError());
+    return CGV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cgv_lookup_rows_dev(int device_id, const void* table_dev, int dtype, uint64_t n_rows, uint32_t dim, uint64_t row_stride,
+                        const int64_t* ids_dev, uint64_t n_ids, float scale, void* out_dev, void* stream) {
+    return guarded([&]() -> int {
+        int rc = check_common(dtype, n_rows, dim, n_ids, scale);
+        if (rc) return rc;
+        if (row_stride < dim) return fail(CGV_ERR_INVALID_ARG, "row_stride is smaller than dim");
+        if (n_ids == 0) return CGV_OK;
+        if (!ids_dev || !out_dev || (n_rows && !table_dev)) return fail(CGV_ERR_INVALID_ARG, "NULL argument");
+        if ((rc = need_gpu(device_id))) return rc;
+        DeviceScope dev(device_id);
+        OPCHK(dev.enter());
+        const bool vec = by_vectors(dim, dtype, row_stride, table_dev, out_dev);
+        return by_dtype(dtype, [&](auto t) {
+            constexpr int DT = decltype(t)::value, V = DT == cgv::DT_F32 ? 4 : 8;
+            return vec ? launch_lookup<DT, V>(table_dev, n_rows, dim, row_stride, ids_dev, n_ids, scale, out_dev, (hipStream_t)stream)
+                       : launch_lookup<DT, 1>(table_dev, n_rows, dim, row_stride, ids_dev, n_ids, scale, out_dev, (hipStream_t)stream);
+        });
+    });
+}
+
+size_t cgv_lookup_grad_workspace(uint64_t n_ids, uint64_t n_rows, uint32_t dim) {
+    if (n_rows >= (1ull << 31) || n_ids >= (1ull << 31) || dim == 0 || dim > 8192 || n_rows == 0) return 0;
+    return (size_t)GradPlan(n_ids, n_rows, dim).bytes;
+}
+
+int cgv_lookup_grad_dev(int device_id, const void* dout_dev, int dtype, const int64_t* ids_dev, uint64_t n_ids, uint64_t n_rows,
+                        uint32_t dim, float scale, void* dtable_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
+    return guarded([&]() -> int {
+        int rc = check_common(dtype, n_rows, dim, n_ids, scale);
+        if (rc) return rc;
+        if (n_rows == 0) return CGV_OK;
+        if (!dtable_dev || (n_ids && (!dout_dev || !ids_dev))) return fail(CGV_ERR_INVALID_ARG, "NULL argument");
+        const GradPlan pl(n_ids, n_rows, dim);
+        if (workspace_bytes < pl.bytes || (pl.bytes && !workspace_dev)) return fail(CGV_ERR_INVALID_ARG, "the workspace is smaller than cgv_lookup_grad_workspace says");
+        if ((uintptr_t)workspace_dev % 256 && pl.bytes) return fail(CGV_ERR_INVALID_ARG, "the workspace must be aligned to 256 bytes");
+        if ((rc = need_gpu(device_id))) return rc;
+        DeviceScope dev(device_id);
+        OPCHK(dev.enter());
+        const bool vec = by_vectors(dim, dtype, dim, dout_dev, dtable_dev);
+        return by_dtype(dtype, [&](auto t) {
+            constexpr int DT = decltype(t)::value, V = DT == cgv::DT_F32 ? 4 : 8;
+            return vec ? launch_grad<DT, V>(dout_dev, ids_dev, n_ids, n_rows, dim, scale, dtable_dev, (char*)workspace_dev, pl, (hipStream_t)stream)
+                       : launch_grad<DT, 1>(dout_dev, ids_dev, n_ids, n_rows, dim, scale, dtable_dev, (char*)workspace_dev, pl, (hipStream_t)stream);
+        });
+    });
+}
+
+}  // extern "C"

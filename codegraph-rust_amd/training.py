@@ -1,0 +1,118 @@
+"""ctypes binding of include/cgvec_train.h with torch's autograd: rows of a table by id, and the losses that train what an index
+serves. CUDA tensors only (there is no CPU fallback); every call enqueues on torch's current stream of the tensors' device."""
+import ctypes as C
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .cgvec import CGV_ERR_DIM_MISMATCH, CGV_ERR_INVALID_ARG, CgvError, _check, lib as _base_lib
+
+_decl = False
+_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def lib():
+    global _decl
+    L = _base_lib()
+    if not _decl:
+        vp, u32, u64, i32, f32, sz = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int, C.c_float, C.c_size_t
+        L.cgv_lookup_rows_dev.argtypes = [i32, vp, i32, u64, u32, u64, vp, u64, f32, vp, vp]
+        L.cgv_lookup_grad_workspace.argtypes = [u64, u64, u32]
+        L.cgv_lookup_grad_workspace.restype = sz
+        L.cgv_lookup_grad_dev.argtypes = [i32, vp, i32, vp, u64, u64, u32, f32, vp, vp, sz, vp]
+        for n in ("cgv_lookup_rows_dev", "cgv_lookup_grad_dev"):
+            getattr(L, n).restype = i32
+        _decl = True
+    return L
+
+
+def _ptr(t):
+    return C.c_void_p(t.data_ptr() if t is not None else None)
+
+
+def _bad(msg, code=CGV_ERR_INVALID_ARG):
+    return CgvError(code, msg)
+
+
+def _matrix(t, name):
+    """A CUDA matrix of a supported type whose rows are contiguous."""
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        raise _bad(f"{name} must be a CUDA tensor (there is no CPU fallback)")
+    if t.dim() != 2:
+        raise _bad(f"{name} must be a matrix, got shape {tuple(t.shape)}", CGV_ERR_DIM_MISMATCH)
+    if t.dtype not in _CODES:
+        raise _bad(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
+    if not 1 <= t.shape[1] <= 8192:
+        raise _bad(f"{name}: dim must be in 1..=8192, got {t.shape[1]}")
+    if t.shape[0] > 1 and (t.stride(1) != 1 or t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    elif t.shape[0] <= 1:
+        t = t.contiguous()
+    return t
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _ids(t, name, device):
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        raise _bad(f"{name} must be a tensor on {device}")
+    if t.dtype not in (torch.int64, torch.int32):
+        raise _bad(f"{name} must be int64 or int32, not {t.dtype}")
+    return t.detach().to(torch.int64).contiguous()
+
+
+def _stream(device):
+    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _workspace(nbytes, device):
+    return torch.empty((max(int(nbytes), 1),), dtype=torch.uint8, device=device)
+
+
+class _LookupRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, ids, scale):
+        n, d = table.shape
+        out = torch.empty((ids.numel(), d), dtype=table.dtype, device=table.device)
+        _check(lib().cgv_lookup_rows_dev(table.device.index, _ptr(table), _CODES[table.dtype], n, d, _row_stride(table), _ptr(ids),
+                                         ids.numel(), scale, _ptr(out), _stream(table.device)))
+        ctx.save_for_backward(ids)
+        ctx.shape, ctx.dtype, ctx.scale = (n, d), table.dtype, scale
+        return out.view(*ids.shape, d)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        (ids,) = ctx.saved_tensors
+        return lookup_rows_grad(dout, ids, ctx.shape[0], scale=ctx.scale), None, None
+
+
+def lookup_rows(table, ids, scale=1.0):
+    """scale * table[ids], rounded once to the table's type: ids of any shape (int64 / int32) -> ids.shape + (dim,). An id outside
+    [0, n_rows) - the -1 that pads a short search result among them - gives zeros and takes no part in the gradient.
+    Differentiable in `table`; the gradient is dense, in the table's type, each row summed in f32 in a fixed order."""
+    table = _matrix(table, "table")
+    return _LookupRows.apply(table, _ids(ids, "ids", table.device), float(scale))
+
+
+def lookup_rows_grad(dout, ids, n_rows, scale=1.0):
+    """The gradient of lookup_rows in its table: [n_rows, dim] in dout's type, from dout [..., dim] and ids of dout's leading shape."""
+    if not isinstance(dout, torch.Tensor) or dout.device.type != "cuda":
+        raise _bad("dout must be a CUDA tensor (there is no CPU fallback)")
+    if dout.dtype not in _CODES:
+        raise _bad(f"dout must be float32, bfloat16 or float16, not {dout.dtype}")
+    ids = _ids(ids, "ids", dout.device)
+    if dout.dim() < 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
+        raise _bad(f"dout {tuple(dout.shape)} does not fit ids {tuple(ids.shape)}", CGV_ERR_DIM_MISMATCH)
+    if int(n_rows) < 0:
+        raise _bad("n_rows must be >= 0")
+    g = dout.detach().contiguous()
+    d = g.shape[-1]
+    out = torch.empty((int(n_rows), d), dtype=g.dtype, device=g.device)
+    nbytes = lib().cgv_lookup_grad_workspace(ids.numel(), int(n_rows), d)
+    ws = _workspace(nbytes, g.device)
+    _check(lib().cgv_lookup_grad_dev(g.device.index, _ptr(g), _CODES[g.dtype], _ptr(ids), ids.numel(), int(n_rows), d, float(scale),
+                                     _ptr(out), _ptr(ws), ws.numel(), _stream(g.device)))
+    return out
