@@ -12,5 +12,5 @@ from .sharded import ShardedKnn, shard_range  # noqa: F401
 from . import store  # noqa: F401
 from .i8scan import Int8ScanIndex, quantize_u4, quantize_u8  # noqa: F401
 from .q4scan import Int4ScanIndex  # noqa: F401
-from .training import lookup_rows, lookup_rows_grad  # noqa: F401
+from .training import corpus_cross_entropy, corpus_distillation, lookup_rows, lookup_rows_grad  # noqa: F401
 from .quant import ProductQuantizer, ScalarQuantizer  # noqa: F401

@@ -1,0 +1,429 @@
+// kernels_gemm.h - the matrix products behind the softmax losses (softmax.hip): one persistent MFMA kernel, three products, four
+// epilogues. Written from the formulas: with S = c Q R^T, G = dL/dS * c,
+//     scores   M = corpus rows, N = queries,     K = elements   -> running maximum and sum of exp per query, or a piece of G
+//     dQ       M = elements,    N = queries,     K = corpus     -> f32 partial sums, one slot per share of the corpus
+//     dR       M = elements,    N = corpus rows, K = queries    -> rows of the corpus' gradient
+// An operand lies in memory either with K contiguous ("rows") or with M or N contiguous ("columns", TA / TB): R is read by rows
+// for the scores and by columns for dQ, G [query][corpus] by rows for dQ and by columns for dR. Columns are turned into
+// fragments by ds_read_b64_tr_b16: of 16 lanes, lane 4 j + a supplies the elements 4 a .. 4 a + 3 of k-row j and lane i receives
+// element i of the k-rows 0 .. 3.
+//
+// C layout of v_mfma_f32_32x32x16: a lane holds ONE column n = lane & 31 and 16 rows m = (r & 3) + 8 (r >> 2) + 4 (lane >> 5).
+// With queries as N the softmax statistics of a query stay in its lane; four consecutive m are four neighbours in memory of G
+// [query][corpus], dQ and dR.
+//
+// f32 inputs are three bf16 planes x = h + m + l (8 bits each, exact); a product is the six plane products of weight 2^0 .. 2^-16
+// (the three left out are below 2^-24 of it), added from the smallest up in the same f32 accumulators: six passes of bf16 MFMA run
+// at 2.5 / 6 = 0.42 PFLOP/s, the f32 MFMA at 0.16.
+#pragma once
+#include "common.h"
+
+namespace cgv_gemm {
+
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr uint32_t BK = 64;                 // elements of K a stage: 128 bytes of a row
+constexpr int MAX_SEG = 6;
+
+template <int DT>
+__device__ inline f32x16 mma(s16x8 a, s16x8 b, f32x16 c) {
+    if constexpr (DT == cgv::DT_FP16) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+}
+
+// three bf16 planes of an f32, largest first
+__device__ inline void split3(float x, uint16_t (&p)[3]) {
+    p[0] = cgv::f32_to_bf16_rne(x);
+    const float r = x - cgv::bf16_to_f32(p[0]);
+    p[1] = cgv::f32_to_bf16_rne(r);
+    p[2] = cgv::f32_to_bf16_rne(r - cgv::bf16_to_f32(p[1]));
+}
+
+struct Operand {
+    const char* p;          // plane 0, element (0, 0)
+    uint64_t pitch, plane;  // bytes from row to row in memory, from plane to plane
+    uint32_t limit;         // rows form: rows that exist; columns form: elements of a row (a multiple of 8). Beyond: clamped
+};
+
+enum Epilogue { EPI_LSE, EPI_G, EPI_DQ, EPI_DR };
+
+struct Args {
+    Operand a, b;
+    uint32_t nseg, sa[MAX_SEG], sb[MAX_SEG];      // plane pairs
+    uint32_t ksteps, kvalid;                      // stages of 64; k-rows of `a` that exist (columns form)
+    uint32_t tm, tn;                              // tiles of M and N
+    uint32_t splits, blocks;                      // shares of the long axis; workgroups
+    // epilogues
+    float scale2;                                 // LSE, G: scores in units of log 2 = accumulator * scale2
+    uint32_t m_valid, n_valid;                    // rows / columns of the result that exist
+    uint64_t row0;                                // LSE: corpus row of m = 0
+    const uint32_t* anchor;                       // LSE: [n] corpus row left out of the sum, 0xffffffff for none
+    float2* part;                                 // LSE: [splits * WM][part_ld] (maximum, sum)
+    uint32_t part_ld;
+    const float *coef, *lse2;                     // G: [n] factor and log2 of the softmax sum
+    char* out;                                    // G, DR, DQ
+    uint64_t out_pitch, out_plane;                // bytes
+    uint32_t accumulate, vec_out;                 // DQ: add to what is there; DR: 16-byte stores possible
+    const float* unscale;                         // G: [1] factor of the entries; DR: [1] factor of the result
+};
+
+template <int BM_, int BN_, int WM_, int WN_>
+struct Shape {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM_ * WN_, THREADS = 64 * NW;
+    static constexpr int TM = BM / WM, TN = BN / WN, MB = TM / 32, NB = TN / 32;
+    static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
+    static constexpr int XPOSE = 4096;            // per wave: a 32 x 64 piece of 16-bit results on its way out
+    static constexpr int lds_bytes(bool xpose) { return 2 * STAGE + (xpose ? NW * XPOSE : 0); }
+};
+
+// swizzle of the 32-byte segments of k-row k in the columns form: four k-rows of one read lie in different banks
+template <int W>
+__device__ inline uint32_t seg_swz(uint32_t k) {
+    return W >= 128 ? (k & 3u) << 1 : ((k >> 1) & 1u) << 1;
+}
+
+// where a lane's 16-byte pieces of a W-row (or W-column) stage come from
+template <bool T, int W, int NW>
+struct Loader {
+    static constexpr int I = W / 8 / NW;          // 1-KiB instructions of a wave
+    uint32_t voff[I];
+    // first = first row / column of the tile; krows: k-rows that exist from the stage's first on (columns form)
+    __device__ void place(const Operand& o, uint32_t first, int wave, int lane, uint32_t krows) {
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            const uint32_t u = (uint32_t)(wave * I + i);
+            if (!T) {
+                const uint32_t row = u * 8 + (lane >> 3), chunk = (uint32_t)(lane & 7) ^ (row & 7u);
+                voff[i] = (min(first + row, o.limit - 1) - first) * (uint32_t)o.pitch + chunk * 16;
+            } else {
+                constexpr uint32_t RB = W * 2, LPR = RB / 16;           // bytes of a k-row, lanes of one
+                const uint32_t k = u * (1024 / RB) + lane / LPR, c = lane % LPR;
+                const uint32_t seg = (c >> 1) ^ seg_swz<W>(k), col = seg * 16 + (c & 1) * 8;
+                voff[i] = min(k, krows - 1) * (uint32_t)o.pitch + (min(first + col, o.limit - 8) - first) * 2;
+            }
+        }
+    }
+    __device__ void issue(const char* base, uint32_t soff, char* lds, int wave) const {
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(lds + (wave * I + i) * 1024), 16, voff[i], soff, 0, 0);
+    }
+};
+
+// fragment of 32 rows (or columns) starting at `at` of a stage, 16 elements of K from kk * 16
+template <bool T, int W>
+__device__ inline s16x8 fragment(const char* lds, uint32_t at, int kk, int lane) {
+    if (!T) {
+        const uint32_t row = at + (lane & 31);
+        return *(const s16x8*)(lds + row * 128 + (((uint32_t)(kk * 2 + (lane >> 5)) ^ (row & 7u)) << 4));
+    }
+    constexpr uint32_t RB = W * 2;
+    const uint32_t k = (uint32_t)kk * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2);
+    const uint32_t seg = at / 16 + ((lane >> 4) & 1);
+    const char* p = lds + k * RB + ((seg ^ seg_swz<W>(k)) << 5) + (lane & 3) * 8;
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * RB));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// tile `i` of workgroup `id`: consecutive tiles run on one XCD (the hardware deals workgroups to the 8 XCDs in turn)
+__device__ inline uint32_t unit_of(uint32_t id, uint32_t blocks) {
+    const uint32_t x = id & 7u, per = blocks >> 3, extra = blocks & 7u;
+    return x * per + min(x, extra) + (id >> 3);
+}
+
+template <int DT, class S, bool TA, bool TB, int EPI>
+static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
+#if defined(__HIP_DEVICE_COMPILE__)   // the host pass only needs the launch stub
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave % S::WM, wn = wave / S::WM;
+    const uint32_t unit = unit_of(blockIdx.x, g.blocks);
+
+    // ---- this workgroup's tiles: LSE and G keep a query tile and walk the corpus; dR walks (element tile, corpus tile); dQ has one
+    uint32_t mt, nt, k0 = 0, ksteps = g.ksteps, tiles, split = 0;
+    if (EPI == EPI_LSE || EPI == EPI_G) {
+        nt = unit % g.tn;
+        split = unit / g.tn;
+        mt = split;
+        tiles = split < g.tm ? (g.tm - split + g.splits - 1) / g.splits : 0;
+    } else if (EPI == EPI_DQ) {
+        mt = unit % g.tm;
+        nt = unit / g.tm % g.tn;
+        split = unit / (g.tm * g.tn);
+        k0 = (uint32_t)((uint64_t)g.ksteps * split / g.splits);
+        ksteps = (uint32_t)((uint64_t)g.ksteps * (split + 1) / g.splits) - k0;
+        tiles = 1;
+    } else {
+        const uint32_t all = g.tm * g.tn;
+        mt = nt = 0;
+        tiles = unit < all ? (all - unit + g.blocks - 1) / g.blocks : 0;
+    }
+    auto tile_at = [&](uint32_t i) {
+        if (EPI == EPI_LSE || EPI == EPI_G) {
+            mt = split + i * g.splits;
+        } else if (EPI == EPI_DR) {
+            const uint32_t t = unit + i * g.blocks;
+            mt = t % g.tm;
+            nt = t / g.tm;
+        }
+    };
+
+    Loader<TA, S::BM, S::NW> la;
+    Loader<TB, S::BN, S::NW> lb;
+    const char *abase = nullptr, *bbase = nullptr;    // of the tile, plane 0, k = k0
+    auto enter = [&](uint32_t i) {
+        tile_at(i);
+        la.place(g.a, mt * S::BM, wave, lane, 64);
+        lb.place(g.b, nt * S::BN, wave, lane, 64);
+        abase = g.a.p + (TA ? (uint64_t)mt * S::BM * 2 : (uint64_t)mt * S::BM * g.a.pitch);
+        bbase = g.b.p + (TB ? (uint64_t)nt * S::BN * 2 : (uint64_t)nt * S::BN * g.b.pitch);
+    };
+    auto issue = [&](uint32_t seg, uint32_t ks, int buf) {
+        char* l = smem + buf * S::STAGE;
+        const uint64_t k = k0 + ks;
+        if (TA && EPI == EPI_DQ && (k + 1) * BK > g.kvalid) la.place(g.a, mt * S::BM, wave, lane, (uint32_t)(g.kvalid - k * BK));
+        const char* a = abase + g.sa[seg] * g.a.plane;
+        const char* b = bbase + g.sb[seg] * g.b.plane;
+        if (TA) la.issue(a + k * BK * g.a.pitch, 0, l, wave);
+        else la.issue(a, (uint32_t)k * 128, l, wave);
+        if (TB) lb.issue(b + k * BK * g.b.pitch, 0, l + S::A_BYTES, wave);
+        else lb.issue(b, (uint32_t)k * 128, l + S::A_BYTES, wave);
+        if (TA && EPI == EPI_DQ && (k + 1) * BK > g.kvalid) la.place(g.a, mt * S::BM, wave, lane, 64);
+    };
+
+    float run_m[S::NB], run_s[S::NB];                 // LSE: per query of the lane, over the corpus rows of the lane
+    if (EPI == EPI_LSE)
+        for (int nb = 0; nb < S::NB; ++nb) run_m[nb] = -INFINITY, run_s[nb] = 0.0f;
+
+    int buf = 0;
+    if (tiles && ksteps) {
+        enter(0);
+        issue(0, 0, 0);
+    }
+    for (uint32_t i = 0; i < tiles; ++i) {
+        f32x16 acc[S::MB][S::NB];
+#pragma unroll
+        for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+            for (int nb = 0; nb < S::NB; ++nb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[mb][nb][r] = 0.0f;
+        const uint32_t my_mt = mt, my_nt = nt;
+        for (uint32_t seg = 0; seg < g.nseg; ++seg)
+            for (uint32_t ks = 0; ks < ksteps; ++ks) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's part of the stage has landed
+                __builtin_amdgcn_s_barrier();                      // everybody's has, and the other buffer is free
+                asm volatile("" ::: "memory");
+                if (ks + 1 < ksteps) {
+                    issue(seg, ks + 1, buf ^ 1);
+                } else if (seg + 1 < g.nseg) {
+                    issue(seg + 1, 0, buf ^ 1);
+                } else if (i + 1 < tiles) {
+                    enter(i + 1);
+                    issue(0, 0, buf ^ 1);
+                }
+                const char* as = smem + buf * S::STAGE;
+                const char* bs = as + S::A_BYTES;
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    s16x8 fa[S::MB], fb[S::NB];
+#pragma unroll
+                    for (int mb = 0; mb < S::MB; ++mb) fa[mb] = fragment<TA, S::BM>(as, (uint32_t)(wm * S::TM + mb * 32), kk, lane);
+#pragma unroll
+                    for (int nb = 0; nb < S::NB; ++nb) fb[nb] = fragment<TB, S::BN>(bs, (uint32_t)(wn * S::TN + nb * 32), kk, lane);
+#pragma unroll
+                    for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+                        for (int nb = 0; nb < S::NB; ++nb) acc[mb][nb] = mma<DT>(fa[mb], fb[nb], acc[mb][nb]);
+                }
+                buf ^= 1;
+            }
+
+        // ---- epilogue of the tile
+        const uint32_t m0 = my_mt * S::BM + wm * S::TM, n0 = my_nt * S::BN + wn * S::TN;
+        const uint32_t half4 = (uint32_t)(lane >> 5) * 4;
+        if (EPI == EPI_LSE) {
+            const bool edge = m0 + S::TM > g.m_valid;
+#pragma unroll
+            for (int nb = 0; nb < S::NB; ++nb) {
+                const uint32_t q = n0 + nb * 32 + (lane & 31);
+                // corpus row that this query leaves out, as a row of the wave's part of the tile
+                const uint32_t skip = q < g.n_valid ? g.anchor[q] - (uint32_t)(g.row0 + m0) : 0xffffffffu;
+                const bool any = __ballot(skip < (uint32_t)S::TM) != 0;
+                float mx = -INFINITY;
+#pragma unroll
+                for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        float t = acc[mb][nb][r] * g.scale2;
+                        if (edge || any) {
+                            const uint32_t m = mb * 32 + (r & 3) + 8 * (r >> 2) + half4;
+                            if (m == skip || m0 + m >= g.m_valid) t = -INFINITY;
+                        }
+                        acc[mb][nb][r] = t;
+                        mx = fmaxf(mx, t);
+                    }
+                const float nm = fmaxf(run_m[nb], mx), base = nm == -INFINITY ? 0.0f : nm;
+                float s = run_s[nb] * __builtin_amdgcn_exp2f(run_m[nb] - base);
+#pragma unroll
+                for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(acc[mb][nb][r] - base);
+                run_m[nb] = nm;
+                run_s[nb] = s;
+            }
+        } else if (EPI == EPI_G) {
+            char* xp = smem + 2 * S::STAGE + wave * S::XPOSE;
+#pragma unroll
+            for (int nb = 0; nb < S::NB; ++nb) {
+                const uint32_t q = n0 + nb * 32 + (lane & 31);
+                const float c = q < g.n_valid ? g.coef[q] * *g.unscale : 0.0f, l2 = q < g.n_valid ? g.lse2[q] : 0.0f;
+#pragma unroll
+                for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const uint32_t m = m0 + mb * 32 + (r & 3) + 8 * (r >> 2) + half4;
+                        const float v = c * __builtin_amdgcn_exp2f(acc[mb][nb][r] * g.scale2 - l2);
+                        acc[mb][nb][r] = c == 0.0f || m >= g.m_valid ? 0.0f : v;
+                    }
+            }
+            for (uint32_t plane = 0; plane < (DT == cgv::DT_F32 ? 3u : 1u); ++plane)
+#pragma unroll
+                for (int nb = 0; nb < S::NB; ++nb)
+#pragma unroll
+                    for (int mp = 0; mp < S::MB; mp += 2) {      // 64 corpus rows x 32 queries at a time, through the wave's own LDS
+#pragma unroll
+                        for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+                            for (int r4 = 0; r4 < 4; ++r4) {
+                                uint16_t h[4];
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) {
+                                    const float v = acc[mp + mi][nb][r4 * 4 + x];
+                                    if (DT == cgv::DT_FP16) {
+                                        h[x] = cgv::f32_to_f16_rne(v);
+                                    } else {
+                                        h[x] = cgv::f32_to_bf16_rne(v);
+                                        if (DT == cgv::DT_F32) acc[mp + mi][nb][r4 * 4 + x] = v - cgv::bf16_to_f32(h[x]);   // what the next plane holds
+                                    }
+                                }
+                                const uint32_t n = lane & 31, chunk = (uint32_t)(mi * 4 + r4) ^ (n & 7u);
+                                *(uint2*)(xp + n * 128 + chunk * 16 + half4 * 2) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+                            }
+                        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) {
+                            const uint32_t n = p * 8 + (lane >> 3), chunk = (uint32_t)(lane & 7) ^ (n & 7u);
+                            const uint4 v = *(const uint4*)(xp + n * 128 + chunk * 16);
+                            const uint32_t q = n0 + nb * 32 + n;
+                            if (q < g.part_ld)
+                                *(uint4*)(g.out + plane * g.out_plane + q * g.out_pitch + (uint64_t)(m0 + mp * 32) * 2 + (lane & 7) * 16) = v;
+                        }
+                        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                        __builtin_amdgcn_wave_barrier();
+                    }
+        } else if (EPI == EPI_DQ) {
+            float* out = (float*)(g.out + split * g.out_plane);
+#pragma unroll
+            for (int nb = 0; nb < S::NB; ++nb) {
+                const uint32_t q = n0 + nb * 32 + (lane & 31);
+#pragma unroll
+                for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; ++r4) {
+                        const uint32_t m = m0 + mb * 32 + r4 * 8 + half4;
+                        if (q < g.n_valid && m < g.m_valid) {
+                            float4* p = (float4*)(out + (uint64_t)q * g.part_ld + m);
+                            float4 v = make_float4(acc[mb][nb][r4 * 4], acc[mb][nb][r4 * 4 + 1], acc[mb][nb][r4 * 4 + 2], acc[mb][nb][r4 * 4 + 3]);
+                            if (g.accumulate) {
+                                const float4 o = *p;
+                                v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+                            }
+                            *p = v;
+                        }
+                    }
+            }
+        } else {   // EPI_DR
+            const float u = *g.unscale;
+            char* xp = smem + 2 * S::STAGE + wave * S::XPOSE;
+#pragma unroll
+            for (int nb = 0; nb < S::NB; ++nb) {
+                if (DT != cgv::DT_F32 && g.vec_out) {
+#pragma unroll
+                    for (int mp = 0; mp < S::MB; mp += 2) {
+#pragma unroll
+                        for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+                            for (int r4 = 0; r4 < 4; ++r4) {
+                                uint16_t h[4];
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) {
+                                    const float v = acc[mp + mi][nb][r4 * 4 + x] * u;
+                                    h[x] = DT == cgv::DT_FP16 ? cgv::f32_to_f16_rne(v) : cgv::f32_to_bf16_rne(v);
+                                }
+                                const uint32_t n = lane & 31, chunk = (uint32_t)(mi * 4 + r4) ^ (n & 7u);
+                                *(uint2*)(xp + n * 128 + chunk * 16 + half4 * 2) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+                            }
+                        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) {
+                            const uint32_t n = p * 8 + (lane >> 3), chunk = (uint32_t)(lane & 7) ^ (n & 7u);
+                            const uint4 v = *(const uint4*)(xp + n * 128 + chunk * 16);
+                            const uint32_t row = n0 + nb * 32 + n, m = m0 + mp * 32 + (lane & 7) * 8;
+                            if (row < g.n_valid && m < g.m_valid) *(uint4*)(g.out + row * g.out_pitch + m * 2) = v;   // m_valid: a multiple of 8
+                        }
+                        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                        __builtin_amdgcn_wave_barrier();
+                    }
+                } else {
+                    const uint32_t row = n0 + nb * 32 + (lane & 31);
+#pragma unroll
+                    for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+                        for (int r4 = 0; r4 < 4; ++r4) {
+                            const uint32_t m = m0 + mb * 32 + r4 * 8 + half4;
+                            if (row < g.n_valid && m < g.m_valid) {
+                                char* p = g.out + row * g.out_pitch;
+                                float v[4];
+                                for (int x = 0; x < 4; ++x) v[x] = acc[mb][nb][r4 * 4 + x] * u;
+                                if (DT == cgv::DT_F32 && g.vec_out) {
+                                    *(float4*)(p + m * 4) = make_float4(v[0], v[1], v[2], v[3]);
+                                } else {
+                                    for (int x = 0; x < 4; ++x)
+                                        if (m + x < g.m_valid) {
+                                            if (DT == cgv::DT_F32) ((float*)p)[m + x] = v[x];
+                                            else ((uint16_t*)p)[m + x] = DT == cgv::DT_FP16 ? cgv::f32_to_f16_rne(v[x]) : cgv::f32_to_bf16_rne(v[x]);
+                                        }
+                                }
+                            }
+                        }
+                }
+            }
+        }
+    }
+    if (EPI == EPI_LSE) {
+        const uint32_t n0 = nt * S::BN + wn * S::TN;
+#pragma unroll
+        for (int nb = 0; nb < S::NB; ++nb) {
+            const float om = __shfl_xor(run_m[nb], 32), os = __shfl_xor(run_s[nb], 32);
+            const float nm = fmaxf(run_m[nb], om), base = nm == -INFINITY ? 0.0f : nm;
+            const float s = run_s[nb] * __builtin_amdgcn_exp2f(run_m[nb] - base) + os * __builtin_amdgcn_exp2f(om - base);
+            const uint32_t q = n0 + nb * 32 + (lane & 31);
+            if (lane < 32 && q < g.part_ld) g.part[(uint64_t)(split * S::WM + wm) * g.part_ld + q] = make_float2(nm, s);
+        }
+    }
+#endif
+}
+
+}  // namespace cgv_gemm

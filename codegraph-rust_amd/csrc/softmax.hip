@@ -1,0 +1,617 @@
+// softmax.hip - softmax losses of queries against all rows of a corpus and their gradients (include/cgvec_train.h).
+//
+// forward   queries into a padded copy, scores of the listed rows; scores of the whole corpus tile by tile, keeping a maximum and a
+//           sum of exp per query; loss.
+// backward  per piece of the corpus: G = c (exp(s - lse) - p) in 16 bits (three planes for f32), dQ += G R in f32 partial sums,
+//           dR = G^T Q; then dQ's partial sums are added and rounded.
+//
+// Two things keep a small loss and a small gradient exact where exp(s - lse) is close to 1. The heaviest listed row (the anchor) is
+// left out of the sum over the corpus: tail = lse - s_anchor = log(1 + sum of the others' exp(s - s_anchor)) then comes from log1p
+// and not from the difference of two large numbers, and the anchor's 1 - exp(s - lse) is -expm1(-tail). And the listed rows' entries
+// of G, softmax minus weight, are computed in f32 from the saved scores and put into G as differences, before any rounding.
+//
+// fp16: G is scaled by a power of two that brings the largest |dloss * scale| to 2^13 .. 2^14 (softmax values of 1e-9 are then still
+// above the type's smallest step); the products' results are scaled back in f32.
+#include <type_traits>
+
+#include "../../include/cgvec_train.h"
+#include "kernels_gemm.h"
+#include "ops_common.h"
+
+using namespace cgv_ops;
+using namespace cgv_gemm;
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr uint32_t MAX_K = 256, NONE = 0xffffffffu;
+constexpr uint32_t CUS = 256;                                  // workgroups of one per CU that fill the card
+constexpr uint64_t PIECE_BYTES = 128ull << 20;                 // of G and of copied corpus rows: stays in the last-level cache
+
+// ---- weights of a query's list: one wave, entry j at lane j % 64, slot j / 64 ------------------------------------------------
+struct List {
+    uint32_t id[4];       // NONE: weight 0
+    float logp[4], p[4];
+    uint32_t anchor;      // index of the first heaviest entry
+    bool has;
+};
+__device__ inline float wave_max(float v) {
+    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+__device__ inline float wave_sum(float v) {
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+__device__ inline List read_list(const int64_t* ids, const float* ts, uint64_t i, uint32_t k, uint64_t n_rows, float tscale, int lane) {
+    List l;
+    float t[4], mx = -INFINITY;
+    bool any = false;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        const uint32_t j = s * 64 + lane;
+        l.id[s] = NONE;
+        t[s] = -INFINITY;
+        if (j < k) {
+            const int64_t id = ids[i * k + j];
+            const float raw = ts ? ts[i * k + j] : 0.0f;
+            if (id >= 0 && (uint64_t)id < n_rows && raw != -INFINITY) {
+                l.id[s] = (uint32_t)id;
+                t[s] = ts ? raw * tscale : 0.0f;
+                any = true;
+            }
+        }
+        mx = fmaxf(mx, t[s]);
+    }
+    l.has = __ballot(any) != 0;
+    mx = wave_max(mx);
+    float z = 0.0f;
+    uint32_t first = NONE;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        l.p[s] = l.id[s] == NONE ? 0.0f : expf(t[s] - mx);
+        z += l.p[s];
+        const uint64_t eq = __ballot(l.id[s] != NONE && t[s] == mx);
+        if (first == NONE && eq) first = s * 64 + __ffsll((unsigned long long)eq) - 1;
+    }
+    if (first == NONE)
+        for (int s = 0; s < 4; ++s) {       // only NaN scores: any listed row will do, the loss is NaN
+            const uint64_t some = __ballot(l.id[s] != NONE);
+            if (first == NONE && some) first = s * 64 + __ffsll((unsigned long long)some) - 1;
+        }
+    z = wave_sum(z);
+    const float lz = logf(z);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        if (l.id[s] != NONE) {
+            l.p[s] /= z;
+            l.logp[s] = t[s] - mx - lz;
+            if (l.p[s] == 0.0f) l.id[s] = NONE;     // underflow: no weight, and no 0 * inf below
+        } else {
+            l.logp[s] = 0.0f;
+        }
+    }
+    l.anchor = first;
+    return l;
+}
+template <class T>
+__device__ inline T pick(const T (&v)[4], uint32_t j) {     // entry j of the list, for every lane
+    const T x = j < 64 ? v[0] : j < 128 ? v[1] : j < 192 ? v[2] : v[3];
+    return __shfl(x, (int)(j & 63u));
+}
+
+// a row of the padded copy: 16-bit types as they are, f32 as three planes; zeros beyond dim, and altogether if !src
+template <int DT>
+__device__ inline void copy_row(const void* src, uint64_t at, uint32_t dim, uint32_t dp, uint16_t* dst, uint64_t plane, uint32_t t0, uint32_t step) {
+    for (uint32_t e = t0; e < dp; e += step) {
+        if (DT == cgv::DT_F32) {
+            uint16_t p[3] = {0, 0, 0};
+            if (src && e < dim) split3(((const float*)src)[at + e], p);
+            for (int x = 0; x < 3; ++x) dst[x * plane + e] = p[x];
+        } else {
+            dst[e] = src && e < dim ? ((const uint16_t*)src)[at + e] : (uint16_t)0;
+        }
+    }
+}
+
+struct Problem {
+    const void *queries, *rows;
+    uint64_t q_stride, r_stride, n_rows;
+    const int64_t* ids;
+    const float* tscores;
+    float* saved;             // [b][k + 2]: lse, tail, scores of the list
+    uint32_t b, bp, dim, dp, k;
+    float scale, tscale;
+    uint16_t* qws;            // [planes][bp][dp]
+};
+
+template <int DT>
+__global__ __launch_bounds__(256) void forward_prep_kernel(Problem P, uint32_t* __restrict__ anchor) {
+    const uint32_t i = blockIdx.x, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63;
+    const uint64_t plane = (uint64_t)P.bp * P.dp;
+    uint16_t* dst = P.qws + (uint64_t)i * P.dp;
+    if (i >= P.b) {
+        copy_row<DT>(nullptr, 0, P.dim, P.dp, dst, plane, threadIdx.x, 256);
+        if (threadIdx.x == 0) anchor[i] = NONE;
+        return;
+    }
+    const List l = read_list(P.ids, P.tscores, i, P.k, P.n_rows, P.tscale, lane);
+    copy_row<DT>(l.has ? P.queries : nullptr, (uint64_t)i * P.q_stride, P.dim, P.dp, dst, plane, threadIdx.x, 256);
+    float* sv = P.saved + (uint64_t)i * (P.k + 2);
+    for (uint32_t j = wave; j < P.k; j += 4) {
+        const uint32_t id = pick(l.id, j);
+        float s = 0.0f;
+        if (id != NONE) {
+            for (uint32_t e = lane; e < P.dim; e += 64)
+                s = fmaf(load_elem<DT>(P.queries, (uint64_t)i * P.q_stride + e), load_elem<DT>(P.rows, (uint64_t)id * P.r_stride + e), s);
+            s = wave_sum(s) * P.scale;
+        }
+        if (lane == 0) sv[2 + j] = s;
+    }
+    if (threadIdx.x == 0) anchor[i] = NONE;
+    if (l.has && wave == 0) {
+        const uint32_t a = pick(l.id, l.anchor);
+        if (lane == 0) anchor[i] = a;
+    }
+}
+
+// one wave per query: the corpus' partial maxima and sums, the loss
+__global__ __launch_bounds__(256) void loss_kernel(Problem P, const float2* __restrict__ part, uint32_t parts, float* __restrict__ loss) {
+    const uint32_t i = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (i >= P.b) return;
+    const List l = read_list(P.ids, P.tscores, i, P.k, P.n_rows, P.tscale, lane);
+    float* sv = P.saved + (uint64_t)i * (P.k + 2);
+    if (!l.has) {
+        if (lane == 0) loss[i] = 0.0f, sv[0] = 0.0f, sv[1] = 0.0f;
+        return;
+    }
+    float m = -INFINITY, s = 0.0f;
+    for (uint32_t p = lane; p < parts; p += 64) {
+        const float2 v = part[(uint64_t)p * P.bp + i];
+        const float nm = fmaxf(m, v.x), base = nm == -INFINITY ? 0.0f : nm;
+        s = s * exp2f(m - base) + v.y * exp2f(v.x - base);
+        m = nm;
+    }
+    const float top = wave_max(m), base = top == -INFINITY ? 0.0f : top;
+    s = wave_sum(s * exp2f(m - base));
+    const float sa = sv[2 + l.anchor];
+    const float rest = (base - sa * LOG2E) * LN2 + logf(s);        // log of (the others' sum / the anchor's term)
+    const float tail = rest > 30.0f ? rest : log1pf(expf(rest));
+    float sum = 0.0f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+        if (l.id[x] != NONE) sum += l.p[x] * (l.logp[x] + (sa - sv[2 + x * 64 + lane]) + tail);
+    sum = wave_sum(sum);
+    if (lane == 0) {
+        loss[i] = sum;
+        sv[0] = sa + tail;
+        sv[1] = tail;
+    }
+}
+
+// factor and log2 of the softmax sum per query; entries of G on the listed rows; the padded copy of the queries
+template <int DT>
+__global__ __launch_bounds__(256) void backward_prep_kernel(Problem P, const float* __restrict__ dloss, float* __restrict__ coef, float* __restrict__ lse2,
+                                                            uint32_t* __restrict__ has, uint32_t* __restrict__ ent_id, float* __restrict__ ent_val,
+                                                            float* __restrict__ mul) {
+    __shared__ uint32_t ids[MAX_K];
+    __shared__ float ps[MAX_K];
+    const uint32_t i = blockIdx.x, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63;
+    const uint64_t plane = (uint64_t)P.bp * P.dp;
+    uint16_t* dst = P.qws + (uint64_t)i * P.dp;
+    if (i == 0 && threadIdx.x < 2) mul[threadIdx.x] = 1.0f;
+    if (i >= P.b) {
+        copy_row<DT>(nullptr, 0, P.dim, P.dp, dst, plane, threadIdx.x, 256);
+        if (threadIdx.x == 0) coef[i] = 0.0f, lse2[i] = 0.0f, has[i] = 0;
+        return;
+    }
+    const List l = read_list(P.ids, P.tscores, i, P.k, P.n_rows, P.tscale, lane);
+    copy_row<DT>(l.has ? P.queries : nullptr, (uint64_t)i * P.q_stride, P.dim, P.dp, dst, plane, threadIdx.x, 256);
+    const float* sv = P.saved + (uint64_t)i * (P.k + 2);
+    const float c = l.has ? dloss[i] * P.scale : 0.0f;
+    if (threadIdx.x == 0) {
+        coef[i] = c;
+        lse2[i] = l.has ? sv[0] * LOG2E : 0.0f;
+        has[i] = l.has;
+    }
+    if (wave == 0)
+        for (int x = 0; x < 4; ++x) {
+            ids[x * 64 + lane] = l.id[x];
+            ps[x * 64 + lane] = l.p[x];
+        }
+    __syncthreads();
+    if (threadIdx.x >= P.k) return;
+    const uint32_t j = threadIdx.x, id = ids[j];
+    const uint32_t aid = l.has ? ids[l.anchor] : NONE;
+    bool first = id != NONE;
+    float same = 0.0f, other = 0.0f;
+    for (uint32_t x = 0; x < P.k; ++x) {
+        if (ids[x] == id) {
+            if (x < j) first = false;
+            same += ps[x];
+        } else {
+            other += ps[x];
+        }
+    }
+    float v = 0.0f;
+    if (first) v = id == aid ? expm1f(-sv[1]) + other : expf(sv[2 + j] - sv[0]) - same;
+    ent_id[(uint64_t)i * P.k + j] = first ? id : NONE;
+    ent_val[(uint64_t)i * P.k + j] = v * c;
+}
+
+// fp16: the power of two that brings the largest factor to 2^13 .. 2^14, and its inverse
+__global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ coef, uint32_t b, float* __restrict__ mul) {
+    __shared__ float w[16];
+    float mx = 0.0f;
+    for (uint32_t i = threadIdx.x; i < b; i += 1024) {
+        const float a = fabsf(coef[i]);
+        if (a < INFINITY) mx = fmaxf(mx, a);
+    }
+    mx = wave_max(mx);
+    if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = mx;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int x = 1; x < 16; ++x) mx = fmaxf(mx, w[x]);
+        const int e = mx > 0.0f ? min(max(13 - ilogbf(mx), -100), 100) : 0;
+        mul[0] = ldexpf(1.0f, e);
+        mul[1] = ldexpf(1.0f, -e);
+    }
+}
+
+// the listed rows' entries of G for the corpus rows [n0, n0 + c)
+template <int DT>
+__global__ __launch_bounds__(256) void patch_kernel(const uint32_t* __restrict__ ent_id, const float* __restrict__ ent_val, uint64_t total, uint32_t k,
+                                                    uint64_t n0, uint32_t c, const float* __restrict__ mul, uint16_t* __restrict__ G, uint64_t ld,
+                                                    uint64_t plane) {
+    const uint64_t t = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (t >= total) return;
+    const uint32_t id = ent_id[t];
+    if (id == NONE || id < n0 || id - n0 >= c) return;
+    uint16_t* g = G + t / k * ld + (id - n0);
+    const float v = ent_val[t] * mul[0];
+    if (DT == cgv::DT_F32) {
+        uint16_t p[3];
+        split3(v, p);
+        for (int x = 0; x < 3; ++x) g[x * plane] = p[x];
+    } else {
+        g[0] = f32_to_half<DT>(v);
+    }
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void copy_rows_kernel(const void* __restrict__ rows, uint64_t stride, uint64_t n0, uint32_t dim, uint32_t dp,
+                                                        uint64_t plane, uint16_t* __restrict__ dst) {
+    copy_row<DT>(rows, (n0 + blockIdx.x) * stride, dim, dp, dst + (uint64_t)blockIdx.x * dp, plane, threadIdx.x, 256);
+}
+
+// dQ: the shares' partial sums, rounded once
+template <int DT>
+__global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict__ part, uint32_t splits, uint64_t share, uint32_t dim, uint32_t dp,
+                                                        const uint32_t* __restrict__ has, const float* __restrict__ mul, void* __restrict__ dq) {
+    const uint32_t i = blockIdx.x;
+    for (uint32_t e = threadIdx.x; e < dim; e += 256) {
+        float s = 0.0f;
+        for (uint32_t x = 0; x < splits; ++x) s += part[x * share + (uint64_t)i * dp + e];
+        store_elem<DT>(dq, (uint64_t)i * dim + e, has[i] ? s * mul[1] : 0.0f);
+    }
+}
+
+template <int DT>
+__global__ void zero_kernel(void* p, uint64_t total) {
+    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) store_elem<DT>(p, i, 0.0f);
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------
+
+typedef Shape<256, 64, 4, 1> S64;
+typedef Shape<256, 128, 4, 2> S128;
+typedef Shape<256, 256, 2, 4> S256;
+
+uint64_t up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
+
+struct Plan {
+    uint32_t b, bp, dim, dp, k, planes, bn, wm, tn;
+    bool copy;                     // corpus rows go through a padded copy
+    uint64_t n, piece_f, piece_b;  // corpus rows of a piece, forward and backward
+    uint32_t parts_per_piece, dq_splits;
+    Plan(uint64_t b_, uint64_t n_, uint32_t dim_, uint32_t k_, int dtype) : b((uint32_t)b_), dim(dim_), k(k_), n(n_) {
+        bp = (uint32_t)up(std::max<uint64_t>(b_, 1), 64);
+        dp = (uint32_t)up(dim_, 64);
+        planes = dtype == CGV_DTYPE_F32 ? 3 : 1;
+        copy = dtype == CGV_DTYPE_F32 || dp != dim;
+        bn = bp <= 64 ? 64 : bp <= 128 ? 128 : 256;
+        wm = bn == 256 ? S256::WM : S64::WM;
+        tn = (bp + bn - 1) / bn;
+        const uint64_t rows = up(n_, 256);
+        const uint64_t by_copy = copy ? std::max<uint64_t>(256, PIECE_BYTES / ((uint64_t)dp * 2 * planes) / 256 * 256) : rows;
+        const uint64_t by_g = std::max<uint64_t>(256, PIECE_BYTES / ((uint64_t)bp * 2 * planes) / 256 * 256);
+        piece_f = std::min(rows, by_copy);
+        piece_b = std::min(rows, std::min(by_copy, by_g));
+        if (piece_b < rows && piece_b > 256 * CUS / 4) piece_b = piece_b / (256 * CUS / 4) * (256 * CUS / 4);
+        parts_per_piece = std::max<uint32_t>(1, CUS / tn) * wm;
+        const uint32_t dq_tiles = ((dp + 255) / 256) * tn;
+        dq_splits = std::max<uint32_t>(1, std::min<uint32_t>((uint32_t)(piece_b / BK), CUS / dq_tiles));
+    }
+    uint64_t pieces_f() const { return (n + piece_f - 1) / piece_f; }
+    uint64_t q_bytes() const { return up((uint64_t)planes * bp * dp * 2, 256); }
+    uint64_t r_bytes(uint64_t piece) const { return copy ? up((uint64_t)planes * piece * dp * 2, 256) : 0; }
+    // forward workspace
+    uint64_t f_anchor() const { return q_bytes(); }
+    uint64_t f_part() const { return f_anchor() + up((uint64_t)bp * 4, 256); }
+    uint64_t f_rows() const { return f_part() + up(pieces_f() * parts_per_piece * bp * 8, 256); }
+    uint64_t f_bytes() const { return f_rows() + r_bytes(piece_f); }
+    // backward workspace
+    uint64_t b_coef() const { return q_bytes(); }                       // coef, lse2, has: [bp] each; mul: [2]
+    uint64_t b_ent() const { return b_coef() + up((uint64_t)bp * 12 + 8, 256); }
+    uint64_t b_g() const { return b_ent() + up((uint64_t)b * k * 8, 256); }
+    uint64_t b_part() const { return b_g() + up((uint64_t)planes * bp * piece_b * 2, 256); }
+    uint64_t b_rows() const { return b_part() + up((uint64_t)dq_splits * bp * dp * 4, 256); }
+    uint64_t b_bytes() const { return b_rows() + r_bytes(piece_b); }
+};
+
+void set_segments(Args& a, int dtype, bool swap) {
+    if (dtype != CGV_DTYPE_F32) {
+        a.nseg = 1;
+        a.sa[0] = a.sb[0] = 0;
+        return;
+    }
+    static const uint32_t x[6] = {2, 0, 1, 1, 0, 0}, y[6] = {0, 2, 1, 0, 1, 0};   // the smallest products first
+    a.nseg = 6;
+    for (int i = 0; i < 6; ++i) a.sa[i] = swap ? y[i] : x[i], a.sb[i] = swap ? x[i] : y[i];
+}
+
+template <int DT, class S, bool TA, bool TB, int EPI>
+int launch_gemm(const Args& a, hipStream_t s) {
+    constexpr int bytes = S::lds_bytes(EPI == EPI_G || EPI == EPI_DR);
+    if (a.blocks == 0) return CGV_OK;
+    void (*kern)(const Args) = gemm_kernel<DT, S, TA, TB, EPI>;
+    OPCHK(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    hipLaunchKernelGGL(kern, dim3(a.blocks), dim3(S::THREADS), bytes, s, a);
+    OPCHK(hipGetLastError());
+    return CGV_OK;
+}
+template <int DT, bool TA, bool TB, int EPI>
+int launch_by_queries(uint32_t bn, const Args& a, hipStream_t s) {
+    return bn == 64 ? launch_gemm<DT, S64, TA, TB, EPI>(a, s) : bn == 128 ? launch_gemm<DT, S128, TA, TB, EPI>(a, s)
+                                                              : launch_gemm<DT, S256, TA, TB, EPI>(a, s);
+}
+
+// scores of the corpus rows [n0, n0 + c) against all queries
+Args score_args(const Plan& pl, const Problem& P, int dtype, const char* rows, uint64_t pitch, uint64_t plane, uint32_t c) {
+    Args a{};
+    a.a = {rows, pitch, plane, c};
+    a.b = {(const char*)P.qws, (uint64_t)pl.dp * 2, (uint64_t)pl.bp * pl.dp * 2, pl.bp};
+    set_segments(a, dtype, false);
+    a.ksteps = pl.dp / BK;
+    a.kvalid = pl.dp;
+    a.tm = (c + 255) / 256;
+    a.tn = pl.tn;
+    const uint32_t most = std::max<uint32_t>(1, CUS / pl.tn);
+    const uint32_t each = (a.tm + most - 1) / most;
+    a.splits = (a.tm + each - 1) / each;
+    a.blocks = a.tn * a.splits;
+    a.scale2 = P.scale * LOG2E;
+    a.m_valid = c;
+    a.n_valid = pl.b;
+    a.part_ld = pl.bp;
+    return a;
+}
+
+template <int DT>
+int copy_piece(const Plan& pl, const Problem& P, uint64_t n0, uint32_t c, uint64_t plane_elems, char* dst, hipStream_t s) {
+    hipLaunchKernelGGL((copy_rows_kernel<DT>), dim3(c), dim3(256), 0, s, P.rows, P.r_stride, n0, pl.dim, pl.dp, plane_elems, (uint16_t*)dst);
+    OPCHK(hipGetLastError());
+    return CGV_OK;
+}
+
+template <int DT>
+int forward(const Plan& pl, Problem P, int dtype, float* loss, char* ws, hipStream_t s) {
+    P.qws = (uint16_t*)ws;
+    uint32_t* anchor = (uint32_t*)(ws + pl.f_anchor());
+    float2* part = (float2*)(ws + pl.f_part());
+    hipLaunchKernelGGL((forward_prep_kernel<DT>), dim3(pl.bp), dim3(256), 0, s, P, anchor);
+    OPCHK(hipGetLastError());
+    uint32_t parts = 0;
+    for (uint64_t n0 = 0; n0 < pl.n; n0 += pl.piece_f) {
+        const uint32_t c = (uint32_t)std::min<uint64_t>(pl.piece_f, pl.n - n0);
+        const char* rows = (const char*)P.rows + n0 * P.r_stride * 2;
+        uint64_t pitch = P.r_stride * 2, plane = 0;
+        if (pl.copy) {
+            plane = pl.piece_f * pl.dp;
+            const int rc = copy_piece<DT>(pl, P, n0, c, plane, ws + pl.f_rows(), s);
+            if (rc) return rc;
+            rows = ws + pl.f_rows();
+            pitch = (uint64_t)pl.dp * 2;
+            plane *= 2;
+        }
+        Args a = score_args(pl, P, dtype, rows, pitch, plane, c);
+        a.row0 = n0;
+        a.anchor = anchor;
+        a.part = part + (uint64_t)parts * pl.bp;
+        parts += a.splits * pl.wm;
+        const int rc = launch_by_queries<DT, false, false, EPI_LSE>(pl.bn, a, s);
+        if (rc) return rc;
+    }
+    hipLaunchKernelGGL(loss_kernel, dim3((pl.b + 3) / 4), dim3(256), 0, s, P, (const float2*)part, parts, loss);
+    OPCHK(hipGetLastError());
+    return CGV_OK;
+}
+
+template <int DT>
+int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq, void* dr, char* ws, hipStream_t s) {
+    P.qws = (uint16_t*)ws;
+    float* coef = (float*)(ws + pl.b_coef());
+    float* lse2 = coef + pl.bp;
+    uint32_t* has = (uint32_t*)(lse2 + pl.bp);
+    float* mul = (float*)(has + pl.bp);
+    uint32_t* ent_id = (uint32_t*)(ws + pl.b_ent());
+    float* ent_val = (float*)(ent_id + (uint64_t)pl.b * pl.k);
+    char* G = ws + pl.b_g();
+    float* part = (float*)(ws + pl.b_part());
+    const uint64_t g_pitch = pl.piece_b * 2, g_plane = (uint64_t)pl.bp * g_pitch;
+    hipLaunchKernelGGL((backward_prep_kernel<DT>), dim3(pl.bp), dim3(256), 0, s, P, dloss, coef, lse2, has, ent_id, ent_val, mul);
+    OPCHK(hipGetLastError());
+    if (DT == cgv::DT_FP16) {
+        hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1024), 0, s, (const float*)coef, pl.b, mul);
+        OPCHK(hipGetLastError());
+    }
+    for (uint64_t n0 = 0; n0 < pl.n; n0 += pl.piece_b) {
+        const uint32_t c = (uint32_t)std::min<uint64_t>(pl.piece_b, pl.n - n0);
+        const char* rows = (const char*)P.rows + n0 * P.r_stride * 2;
+        uint64_t pitch = P.r_stride * 2, plane = 0;
+        int rc;
+        if (pl.copy) {
+            plane = pl.piece_b * pl.dp;
+            if ((rc = copy_piece<DT>(pl, P, n0, c, plane, ws + pl.b_rows(), s))) return rc;
+            rows = ws + pl.b_rows();
+            pitch = (uint64_t)pl.dp * 2;
+            plane *= 2;
+        }
+        Args a = score_args(pl, P, dtype, rows, pitch, plane, c);
+        a.coef = coef;
+        a.lse2 = lse2;
+        a.unscale = mul;
+        a.out = G;
+        a.out_pitch = g_pitch;
+        a.out_plane = g_plane;
+        if ((rc = launch_by_queries<DT, false, false, EPI_G>(pl.bn, a, s))) return rc;
+        const uint64_t total = (uint64_t)pl.b * pl.k;
+        hipLaunchKernelGGL((patch_kernel<DT>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, (const uint32_t*)ent_id, (const float*)ent_val, total,
+                           pl.k, n0, c, (const float*)mul, (uint16_t*)G, pl.piece_b, g_plane / 2);
+        OPCHK(hipGetLastError());
+        if (dq) {
+            Args d{};
+            d.a = {rows, pitch, plane, pl.dp};
+            d.b = {G, g_pitch, g_plane, pl.bp};
+            set_segments(d, dtype, false);
+            d.ksteps = (c + BK - 1) / BK;
+            d.kvalid = c;
+            d.tm = (pl.dp + 255) / 256;
+            d.tn = pl.tn;
+            d.splits = pl.dq_splits;
+            d.blocks = d.tm * d.tn * d.splits;
+            d.m_valid = pl.dp;
+            d.n_valid = pl.b;
+            d.part_ld = pl.dp;
+            d.out = (char*)part;
+            d.out_plane = (uint64_t)pl.bp * pl.dp * 4;
+            d.accumulate = n0 > 0;
+            if ((rc = launch_by_queries<DT, true, false, EPI_DQ>(pl.bn, d, s))) return rc;
+        }
+        if (dr) {
+            Args d{};
+            d.a = {(const char*)P.qws, (uint64_t)pl.dp * 2, (uint64_t)pl.bp * pl.dp * 2, pl.dp};
+            d.b = {G, g_pitch, g_plane, (uint32_t)pl.piece_b};
+            set_segments(d, dtype, false);
+            d.ksteps = pl.bp / BK;
+            d.kvalid = pl.bp;
+            d.tm = (pl.dim + 255) / 256;
+            d.tn = (c + 255) / 256;
+            d.splits = 1;
+            d.blocks = (uint32_t)std::min<uint64_t>((uint64_t)d.tm * d.tn, CUS);
+            d.m_valid = pl.dim;
+            d.n_valid = c;
+            d.out = (char*)dr + n0 * pl.dim * esize(dtype);
+            d.out_pitch = (uint64_t)pl.dim * esize(dtype);
+            d.vec_out = d.out_pitch % 16 == 0 && (uintptr_t)dr % 16 == 0;
+            d.unscale = mul + 1;
+            if ((rc = launch_gemm<DT, S256, true, true, EPI_DR>(d, s))) return rc;
+        }
+    }
+    if (dq) {
+        hipLaunchKernelGGL((finish_dq_kernel<DT>), dim3(pl.b), dim3(256), 0, s, (const float*)part, pl.dq_splits, (uint64_t)pl.bp * pl.dp, pl.dim, pl.dp,
+                           (const uint32_t*)has, (const float*)mul, dq);
+        OPCHK(hipGetLastError());
+    }
+    return CGV_OK;
+}
+
+bool sizes_ok(uint64_t b, uint64_t n_rows, uint32_t dim, uint32_t k, int dtype) {
+    return b <= (1ull << 24) && n_rows >= 1 && n_rows < (1ull << 31) - 1 && dim >= 1 && dim <= 8192 && k >= 1 && k <= MAX_K &&
+           (dtype == CGV_DTYPE_F32 || dtype == CGV_DTYPE_BF16 || dtype == CGV_DTYPE_FP16);
+}
+
+int check_loss(const void* q, uint64_t qs, const void* r, uint64_t rs, int dtype, uint64_t b, uint64_t n, uint32_t dim, const int64_t* ids, uint32_t k,
+               float scale, float tscale, const void* saved) {
+    if (dtype != CGV_DTYPE_F32 && dtype != CGV_DTYPE_BF16 && dtype != CGV_DTYPE_FP16) return fail(CGV_ERR_INVALID_ARG, "dtype must be f32, bf16 or fp16");
+    if (!sizes_ok(b, n, dim, k, dtype)) return fail(CGV_ERR_INVALID_ARG, "b must be at most 2^24, n_rows in 1..2^31 - 1, dim in 1..=8192, k in 1..=256");
+    if (qs < dim || rs < dim) return fail(CGV_ERR_INVALID_ARG, "a stride is smaller than dim");
+    if (!(fabsf(scale) < INFINITY) || !(fabsf(tscale) < INFINITY)) return fail(CGV_ERR_NONFINITE, "scale is not finite");
+    if (!r || (b && (!q || !ids || !saved))) return fail(CGV_ERR_INVALID_ARG, "NULL argument");
+    if (dtype != CGV_DTYPE_F32 && dim % 64 == 0 && ((uintptr_t)r % 16 || rs % 8 || rs > (1u << 22)))
+        return fail(CGV_ERR_INVALID_ARG, "rows of 16-bit elements with dim a multiple of 64 are read in place: they must start on 16-byte addresses, at "
+                                         "most 2^22 elements apart");
+    return CGV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t cgv_corpus_loss_workspace(uint64_t b, uint64_t n_rows, uint32_t dim, uint32_t k, int dtype) {
+    if (!sizes_ok(b, n_rows, dim, k, dtype) || b == 0) return 0;
+    return (size_t)Plan(b, n_rows, dim, k, dtype).f_bytes();
+}
+
+size_t cgv_corpus_loss_grad_workspace(uint64_t b, uint64_t n_rows, uint32_t dim, uint32_t k, int dtype) {
+    if (!sizes_ok(b, n_rows, dim, k, dtype) || b == 0) return 0;
+    return (size_t)Plan(b, n_rows, dim, k, dtype).b_bytes();
+}
+
+int cgv_corpus_loss_dev(int device_id, const void* queries_dev, uint64_t query_stride, const void* rows_dev, uint64_t row_stride, int dtype, uint64_t b,
+                        uint64_t n_rows, uint32_t dim, const int64_t* ids_dev, const float* teacher_scores_dev, uint32_t k, float scale,
+                        float teacher_scale, float* loss_dev, float* saved_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
+    return guarded([&]() -> int {
+        int rc = check_loss(queries_dev, query_stride, rows_dev, row_stride, dtype, b, n_rows, dim, ids_dev, k, scale, teacher_scale, saved_dev);
+        if (rc) return rc;
+        if (b == 0) return CGV_OK;
+        if (!loss_dev) return fail(CGV_ERR_INVALID_ARG, "NULL argument");
+        const Plan pl(b, n_rows, dim, k, dtype);
+        if (!workspace_dev || workspace_bytes < pl.f_bytes()) return fail(CGV_ERR_INVALID_ARG, "the workspace is smaller than cgv_corpus_loss_workspace says");
+        if ((uintptr_t)workspace_dev % 256) return fail(CGV_ERR_INVALID_ARG, "the workspace must be aligned to 256 bytes");
+        if ((rc = need_gpu(device_id))) return rc;
+        DeviceScope dev(device_id);
+        OPCHK(dev.enter());
+        const Problem P{queries_dev, rows_dev, query_stride, row_stride, n_rows, ids_dev, teacher_scores_dev, saved_dev,
+                        pl.b, pl.bp, dim, pl.dp, k, scale, teacher_scale, nullptr};
+        return by_dtype(dtype, [&](auto t) { return forward<decltype(t)::value>(pl, P, dtype, loss_dev, (char*)workspace_dev, (hipStream_t)stream); });
+    });
+}
+
+int cgv_corpus_loss_grad_dev(int device_id, const void* queries_dev, uint64_t query_stride, const void* rows_dev, uint64_t row_stride, int dtype,
+                             uint64_t b, uint64_t n_rows, uint32_t dim, const int64_t* ids_dev, const float* teacher_scores_dev, uint32_t k,
+                             float scale, float teacher_scale, const float* saved_dev, const float* dloss_dev, void* dqueries_dev, void* drows_dev,
+                             void* workspace_dev, size_t workspace_bytes, void* stream) {
+    return guarded([&]() -> int {
+        int rc = check_loss(queries_dev, query_stride, rows_dev, row_stride, dtype, b, n_rows, dim, ids_dev, k, scale, teacher_scale, saved_dev);
+        if (rc) return rc;
+        if (!dqueries_dev && !drows_dev) return CGV_OK;
+        if (b && !dloss_dev) return fail(CGV_ERR_INVALID_ARG, "NULL argument");
+        const Plan pl(b, n_rows, dim, k, dtype);
+        if (b && (!workspace_dev || workspace_bytes < pl.b_bytes()))
+            return fail(CGV_ERR_INVALID_ARG, "the workspace is smaller than cgv_corpus_loss_grad_workspace says");
+        if (b && (uintptr_t)workspace_dev % 256) return fail(CGV_ERR_INVALID_ARG, "the workspace must be aligned to 256 bytes");
+        if ((rc = need_gpu(device_id))) return rc;
+        DeviceScope dev(device_id);
+        OPCHK(dev.enter());
+        const hipStream_t s = (hipStream_t)stream;
+        const Problem P{queries_dev, rows_dev, query_stride, row_stride, n_rows, ids_dev, teacher_scores_dev, const_cast<float*>(saved_dev),
+                        pl.b, pl.bp, dim, pl.dp, k, scale, teacher_scale, nullptr};
+        return by_dtype(dtype, [&](auto t) -> int {
+            constexpr int DT = decltype(t)::value;
+            if (b == 0) {
+                if (drows_dev) {
+                    hipLaunchKernelGGL((zero_kernel<DT>), dim3(1024), dim3(256), 0, s, drows_dev, n_rows * dim);
+                    OPCHK(hipGetLastError());
+                }
+                return CGV_OK;
+            }
+            return backward<DT>(pl, P, dtype, dloss_dev, dqueries_dev, drows_dev, (char*)workspace_dev, s);
+        });
+    });
+}
+
+}  // extern "C"

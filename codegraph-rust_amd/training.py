@@ -20,7 +20,12 @@ def lib():
         L.cgv_lookup_grad_workspace.argtypes = [u64, u64, u32]
         L.cgv_lookup_grad_workspace.restype = sz
         L.cgv_lookup_grad_dev.argtypes = [i32, vp, i32, vp, u64, u64, u32, f32, vp, vp, sz, vp]
-        for n in ("cgv_lookup_rows_dev", "cgv_lookup_grad_dev"):
+        for n in ("cgv_corpus_loss_workspace", "cgv_corpus_loss_grad_workspace"):
+            getattr(L, n).argtypes = [u64, u64, u32, u32, i32]
+            getattr(L, n).restype = sz
+        L.cgv_corpus_loss_dev.argtypes = [i32, vp, u64, vp, u64, i32, u64, u64, u32, vp, vp, u32, f32, f32, vp, vp, vp, sz, vp]
+        L.cgv_corpus_loss_grad_dev.argtypes = [i32, vp, u64, vp, u64, i32, u64, u64, u32, vp, vp, u32, f32, f32, vp, vp, vp, vp, vp, sz, vp]
+        for n in ("cgv_lookup_rows_dev", "cgv_lookup_grad_dev", "cgv_corpus_loss_dev", "cgv_corpus_loss_grad_dev"):
             getattr(L, n).restype = i32
         _decl = True
     return L
@@ -116,3 +121,78 @@ def lookup_rows_grad(dout, ids, n_rows, scale=1.0):
     _check(lib().cgv_lookup_grad_dev(g.device.index, _ptr(g), _CODES[g.dtype], _ptr(ids), ids.numel(), int(n_rows), d, float(scale),
                                      _ptr(out), _ptr(ws), ws.numel(), _stream(g.device)))
     return out
+
+
+class _CorpusLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, queries, rows, ids, scores, scale, teacher_scale):
+        L = lib()
+        b, d = queries.shape
+        n, k = rows.shape[0], ids.shape[1]
+        code, dev = _CODES[rows.dtype], rows.device
+        loss = torch.empty((b,), dtype=torch.float32, device=dev)
+        saved = torch.empty((b * (k + 2),), dtype=torch.float32, device=dev)
+        ws = _workspace(L.cgv_corpus_loss_workspace(b, n, d, k, code), dev)
+        _check(L.cgv_corpus_loss_dev(dev.index, _ptr(queries), _row_stride(queries), _ptr(rows), _row_stride(rows), code, b, n, d, _ptr(ids),
+                                     _ptr(scores), k, scale, teacher_scale, _ptr(loss), _ptr(saved), _ptr(ws), ws.numel(), _stream(dev)))
+        ctx.save_for_backward(queries, rows, ids, scores, saved)
+        ctx.scales = (scale, teacher_scale)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        L = lib()
+        queries, rows, ids, scores, saved = ctx.saved_tensors
+        b, d = queries.shape
+        n, k = rows.shape[0], ids.shape[1]
+        code, dev = _CODES[rows.dtype], rows.device
+        dq = torch.empty((b, d), dtype=queries.dtype, device=dev) if ctx.needs_input_grad[0] else None
+        dr = torch.empty((n, d), dtype=rows.dtype, device=dev) if ctx.needs_input_grad[1] else None
+        dloss = dloss.contiguous()
+        ws = _workspace(L.cgv_corpus_loss_grad_workspace(b, n, d, k, code), dev)
+        _check(L.cgv_corpus_loss_grad_dev(dev.index, _ptr(queries), _row_stride(queries), _ptr(rows), _row_stride(rows), code, b, n, d, _ptr(ids),
+                                          _ptr(scores), k, *ctx.scales, _ptr(saved), _ptr(dloss), _ptr(dq), _ptr(dr), _ptr(ws), ws.numel(),
+                                          _stream(dev)))
+        return dq, dr, None, None, None, None
+
+
+def _corpus_loss(queries, rows, ids, scores, scale, teacher_scale):
+    queries, rows = _matrix(queries, "queries"), _matrix(rows, "rows")
+    if queries.device != rows.device:
+        raise _bad(f"queries are on {queries.device}, rows on {rows.device}")
+    if queries.dtype != rows.dtype:
+        raise _bad(f"queries are {queries.dtype}, rows {rows.dtype}")
+    if queries.shape[1] != rows.shape[1]:
+        raise _bad(f"query dim {queries.shape[1]} != row dim {rows.shape[1]}", CGV_ERR_DIM_MISMATCH)
+    if rows.shape[0] == 0:
+        raise _bad("rows must not be empty")
+    if rows.dtype != torch.float32 and rows.shape[1] % 64 == 0 and (rows.data_ptr() % 16 or _row_stride(rows) % 8 or _row_stride(rows) > 1 << 22):
+        rows = rows.clone(memory_format=torch.contiguous_format)      # such rows are read in place, 16 bytes at a time
+    return _CorpusLoss.apply(queries, rows, ids, scores, float(scale), float(teacher_scale))
+
+
+def corpus_cross_entropy(queries, rows, targets, scale=1.0):
+    """Softmax cross entropy of queries [b, dim] over ALL rows [n, dim] of a corpus: loss[i] = log(sum over j of
+    exp(scale * <q_i, r_j>)) - scale * <q_i, r_targets[i]>, f32 [b]. A target outside [0, n) (-1) takes the query out: loss 0, no
+    gradient. The b x n scores are never stored. Differentiable in queries and rows; gradients have their types."""
+    targets = _ids(targets, "targets", queries.device if isinstance(queries, torch.Tensor) else None)
+    if targets.dim() != 1 or targets.shape[0] != queries.shape[0]:
+        raise _bad(f"targets {tuple(targets.shape)} do not fit queries {tuple(queries.shape)}", CGV_ERR_DIM_MISMATCH)
+    return _corpus_loss(queries, rows, targets[:, None], None, scale, 1.0)
+
+
+def corpus_distillation(queries, rows, teacher_ids, teacher_scores, scale=1.0, teacher_scale=1.0):
+    """KL divergence, f32 [b], of softmax(scale * queries @ rows.T) over the WHOLE corpus from the teacher's distribution on its
+    list: softmax(teacher_scale * teacher_scores[i]) over the rows teacher_ids[i] ([b, k] each, k <= 256) - the ids and scores
+    that a search returns, its padding (-1, -inf) included: entries with an id outside [0, n) or a score of -inf have no weight, a
+    query without entries no loss and no gradient. Differentiable in queries and rows; teacher_scores get no gradient."""
+    ids = _ids(teacher_ids, "teacher_ids", queries.device if isinstance(queries, torch.Tensor) else None)
+    if not isinstance(teacher_scores, torch.Tensor) or teacher_scores.device != ids.device or not teacher_scores.dtype.is_floating_point:
+        raise _bad(f"teacher_scores must be a floating-point tensor on {ids.device}")
+    if ids.dim() != 2 or ids.shape[0] != queries.shape[0] or ids.shape != teacher_scores.shape:
+        raise _bad(f"teacher_ids {tuple(ids.shape)} and teacher_scores {tuple(teacher_scores.shape)} do not fit queries {tuple(queries.shape)}",
+                   CGV_ERR_DIM_MISMATCH)
+    if not 1 <= ids.shape[1] <= 256:
+        raise _bad(f"teacher lists must have 1..256 entries, got {ids.shape[1]}")
+    return _corpus_loss(queries, rows, ids, teacher_scores.detach().to(torch.float32).contiguous(), scale, teacher_scale)

@@ -33,6 +33,36 @@ size_t cgv_lookup_grad_workspace(uint64_t n_ids, uint64_t n_rows, uint32_t dim);
 int cgv_lookup_grad_dev(int device_id, const void* dout_dev, int dtype, const int64_t* ids_dev, uint64_t n_ids, uint64_t n_rows,
                         uint32_t dim, float scale, void* dtable_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
 
+/* Softmax losses of b queries against ALL n_rows rows of a corpus. With s[i][j] = scale * <queries[i], rows[j]>, lse[i] =
+ * log(sum over j of exp(s[i][j])) and weights p[i][0..k) on the listed rows ids[i][0..k),
+ *     loss[i] = sum over t of p[i][t] * (log p[i][t] - s[i][ids[i][t]] + lse[i])
+ * teacher_scores NULL: the entries with an id in [0, n_rows) share the weight equally; k = 1 is the cross entropy with label ids[i].
+ * Otherwise p[i] = softmax over the entries of teacher_scale * teacher_scores[i], i.e. loss[i] is the divergence KL(p || softmax(s))
+ * of the student's scores from the teacher's on its list - what a search returns goes in as it is: entries whose id is outside
+ * [0, n_rows) or whose score is -Inf have weight 0 (its padding is both). An id may be listed twice: its weights add up.
+ * A query without an entry of positive weight takes no part: loss 0, no gradient, its values are not read into any other result.
+ * NaN or Inf in a query, in a corpus row or in a teacher's score makes the losses they enter NaN (or Inf).
+ *
+ * The b x n_rows scores are never stored: the corpus is scored in tiles and only a running maximum and sum per query are kept; the
+ * gradient scores it again, piece by piece.
+ * queries [b] rows of dim elements, query_stride elements apart; rows likewise; both of type dtype. ids [b][k] int64,
+ * teacher_scores [b][k] f32, loss [b] f32. saved [b * (k + 2)] f32 carries what the gradient needs (the softmax sums, the scores of
+ * the listed rows). b in 0..=2^24, k in 1..=256, n_rows in 1..2^31 - 1, dim in 1..=8192. */
+size_t cgv_corpus_loss_workspace(uint64_t b, uint64_t n_rows, uint32_t dim, uint32_t k, int dtype);
+int cgv_corpus_loss_dev(int device_id, const void* queries_dev, uint64_t query_stride, const void* rows_dev, uint64_t row_stride, int dtype,
+                        uint64_t b, uint64_t n_rows, uint32_t dim, const int64_t* ids_dev, const float* teacher_scores_dev, uint32_t k,
+                        float scale, float teacher_scale, float* loss_dev, float* saved_dev, void* workspace_dev, size_t workspace_bytes,
+                        void* stream);
+
+/* Gradients of sum over i of dloss[i] * loss[i] in the queries and in the corpus rows (either may be NULL: it is not computed), from
+ * the same arguments and the `saved` of the forward call: dqueries [b][dim] and drows [n_rows][dim], contiguous, of type dtype;
+ * every row of them is written. */
+size_t cgv_corpus_loss_grad_workspace(uint64_t b, uint64_t n_rows, uint32_t dim, uint32_t k, int dtype);
+int cgv_corpus_loss_grad_dev(int device_id, const void* queries_dev, uint64_t query_stride, const void* rows_dev, uint64_t row_stride,
+                             int dtype, uint64_t b, uint64_t n_rows, uint32_t dim, const int64_t* ids_dev, const float* teacher_scores_dev,
+                             uint32_t k, float scale, float teacher_scale, const float* saved_dev, const float* dloss_dev,
+                             void* dqueries_dev, void* drows_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
