@@ -99,51 +99,194 @@ __global__ void q4_get_row_kernel(const uint32_t* __restrict__ codes, const uint
     }
 }
 
-// scores of MB queries (from q0): a wave per tile, its lane (c, r) sums the elements c * 8 .. + 7 of every 32 of row r in f32,
-// the four lanes of a row are added at the end. Queries stand in LDS as f32, padded with zeros to whole chunks.
-template <int MB, int QDT, int SDT>
-__global__ __launch_bounds__(256) void q4_scores_kernel(const uint4* __restrict__ codes, const uint16_t* __restrict__ scales,
-                                                        const void* __restrict__ queries, uint64_t n, Layout L, uint32_t m,
-                                                        float* __restrict__ out) {
-    extern __shared__ float xs[];   // [MB][kc * CHUNK]
-    const uint32_t kp = L.kc * CHUNK;
-    for (uint32_t i = threadIdx.x; i < MB * kp; i += 256) {
-        const uint32_t q = i / kp, e = i % kp;
-        const float v = (q < m && e < L.dim) ? load_elem<QDT>(queries, (uint64_t)q * L.dim + e) : 0.0f;
-        xs[i] = fabsf(v) < INFINITY ? v : NAN;
-    }
-    __syncthreads();
-    const uint32_t lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
-    const uint64_t tiles = (n + 15) / 16;
-    for (uint64_t tile = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); tile < tiles; tile += (uint64_t)gridDim.x * 4) {
-        float acc[MB];
-        for (int q = 0; q < MB; ++q) acc[q] = 0.0f;
-        const uint4* cp = codes + L.tile_codes(tile) / 16 + lane;
-        const uint16_t* sp = scales + L.tile_scales(tile) + r * L.gpc;
-        for (uint32_t k = 0; k < L.kc; ++k) {
-            const uint4 v = cp[(uint64_t)k * 64];
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// ---- scores -----------------------------------------------------------------------------------------------------------------
+// One v_mfma_f32_16x16x32_f16 takes 32 columns of a 16-row tile against 16 rows of query data: codes become f16 integers -8..7
+// (exact), so the only roundings are those of the query's parts and of the f32 sums. An f32 query is three f16 parts (11 bits
+// each: all 24), a 16-bit query one. Parts are taken of the query scaled by a power of two to a largest magnitude of
+// 2^14 .. 2^15, so that f16's range does not matter: an element keeps an absolute 2^-39 of the query's largest. A query's rows of the
+// product depend on nothing but itself, so the 13 rows that a single f32 query leaves unused cost nothing and hold anything.
+// A group's products are scaled and added in f32 (its scale differs from row to row of the corpus: one value per lane).
+//
+// Bound by the codes' way from HBM: a wave streams its tiles' chunks with the next ones already in flight. Per 8 codes a lane
+// spends 11 instructions on unpacking, 4 FMAs per 32 columns on scales of group 32.
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+struct ScoreArgs {
+    const uint4* codes;
+    const uint16_t* scales;
+    const void* queries;
+    float* out;
+    uint64_t n;
+    Layout L;
+    uint32_t m;            // queries of this launch
+    int qdt;
+};
+
+__device__ inline float load_query(const void* q, int dt, uint64_t i) {
+    return dt == CGV_DTYPE_F32 ? load_elem<cgv::DT_F32>(q, i) : dt == CGV_DTYPE_BF16 ? load_elem<cgv::DT_BF16>(q, i) : load_elem<cgv::DT_FP16>(q, i);
+}
+
+// eight codes of a dword as f16 integers -8..7: 0x6400 | c is 1024 + c
+__device__ inline f16x8 unpack(uint32_t w) {
+    const f16x2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+    f16x2 p[4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const float s = half_to_f32<SDT>(sp[(uint64_t)k * 16 * L.gpc + (uint32_t)t * 32 / L.group]);
-                float part[MB];
-                for (int q = 0; q < MB; ++q) part[q] = 0.0f;
+    for (int i = 0; i < 4; ++i) p[i] = __builtin_bit_cast(f16x2, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) + off;
+    f16x8 v;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float cv = (float)((int)((w[t] >> (4 * (j >> 1) + 16 * (j & 1))) & 15u) - 8);
+    for (int i = 0; i < 4; ++i) v[2 * i] = p[i][0], v[2 * i + 1] = p[i][1];
+    return v;
+}
+
+template <int GPC>
+struct ScalePiece;   // the scales of one row's groups in a chunk
+template <>
+struct ScalePiece<1> { typedef uint16_t type; };
+template <>
+struct ScalePiece<2> { typedef uint32_t type; };
+template <>
+struct ScalePiece<4> { typedef uint2 type; };
+__device__ inline uint16_t piece_at(uint16_t v, int) { return v; }
+__device__ inline uint16_t piece_at(uint32_t v, int i) { return (uint16_t)(v >> (16 * i)); }
+__device__ inline uint16_t piece_at(uint2 v, int i) { return (uint16_t)((i < 2 ? v.x : v.y) >> (16 * (i & 1))); }
+
+// PARTS f16 parts of a query (3: f32 queries, 4 queries a 16-row operand; 1: 16 queries), MT such operands, NT tiles at a time
+template <int PARTS, int SDT, int GPC, int MT, int NT>
+__global__ __launch_bounds__(256) void q4_scores_kernel(ScoreArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr uint32_t QPT = PARTS == 3 ? 4 : 16;      // queries of an operand
+    typedef typename ScalePiece<GPC>::type SP;
+    const uint32_t lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4, wave = threadIdx.x >> 6;
+    const uint32_t kc = a.L.kc, rows = a.m * PARTS, kp = kc * CHUNK;
+    _Float16* xs = (_Float16*)smem;                    // [kp / 32][rows][32]
+    int* expo = (int*)(smem + (uint64_t)rows * kp * 2);
+
+    // this wave's tiles, and the first chunks on their way before anything else
+    const uint64_t units = ((a.n + 15) / 16 + NT - 1) / NT, waves = (uint64_t)gridDim.x * 4, w = (uint64_t)blockIdx.x * 4 + wave;
+    const uint64_t u0 = units * w / waves, u1 = units * (w + 1) / waves;
+    const uint64_t tiles = (a.n + 15) / 16;
+    struct Chunk {
+        uint4 v[NT];
+        SP s[NT];
+    };
+    uint64_t lu = u0;          // the load side's unit and chunk
+    uint32_t lk = 0;
+    auto load = [&](Chunk& ch) {
+        if (lu < u1) {
 #pragma unroll
-                    for (int q = 0; q < MB; ++q) part[q] = fmaf(xs[q * kp + k * CHUNK + t * 32 + c * 8 + j], cv, part[q]);
-                }
+            for (int t = 0; t < NT; ++t) {
+                const uint64_t tile = min(lu * NT + t, tiles - 1);
+                ch.v[t] = a.codes[(tile * kc + lk) * 64 + lane];
+                ch.s[t] = *(const SP*)(a.scales + ((tile * kc + lk) * 16 + r) * GPC);
+            }
+            if (++lk == kc) lk = 0, ++lu;
+        }
+    };
+    constexpr int DEPTH = 4;
+    Chunk ring[DEPTH];
 #pragma unroll
-                for (int q = 0; q < MB; ++q) acc[q] = fmaf(s, part[q], acc[q]);
+    for (int i = 0; i < DEPTH; ++i) load(ring[i]);
+
+    // queries into LDS: a wave per query
+    for (uint32_t q = wave; q < a.m; q += 4) {
+        const uint64_t base = (uint64_t)q * a.L.dim;
+        float mx = 0.0f;
+        bool bad = false;
+        for (uint32_t e = lane; e < a.L.dim; e += 64) {
+            const float v = fabsf(load_query(a.queries, a.qdt, base + e));
+            bad |= !(v < INFINITY);
+            mx = fmaxf(mx, v);
+        }
+        for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+        bad = __ballot(bad) != 0;
+        const int ex = mx > 0.0f && !bad ? 14 - ilogbf(mx) : 0;
+        if (lane == 0) expo[q] = -ex;
+        for (uint32_t e = lane; e < kp; e += 64) {
+            float v = e < a.L.dim ? ldexpf(load_query(a.queries, a.qdt, base + e), ex) : 0.0f;
+            if (bad) v = NAN;
+            _Float16* x = xs + ((uint64_t)(e / 32) * rows + q * PARTS) * 32 + e % 32;
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+                const _Float16 h = (_Float16)v;
+                x[p * 32] = h;
+                v -= (float)h;
             }
         }
+    }
+    __syncthreads();
+
+    // LDS row of this lane for each operand: row r is part r & 3 of query r >> 2 (three parts), or query r
+    uint32_t xrow[MT];
 #pragma unroll
-        for (int q = 0; q < MB; ++q) {
-            acc[q] += __shfl_xor(acc[q], 16);
-            acc[q] += __shfl_xor(acc[q], 32);
-            const uint64_t row = tile * 16 + r;
-            if (c == 0 && (uint32_t)q < m && row < n) out[(uint64_t)q * n + row] = acc[q];
+    for (int mt = 0; mt < MT; ++mt) {
+        const uint32_t q = mt * QPT + (PARTS == 3 ? r >> 2 : r), p = PARTS == 3 ? min(r & 3u, 2u) : 0u;
+        xrow[mt] = (min(q, a.m - 1) * PARTS + p) * 32 + c * 8;
+    }
+    f32x4 acc[NT][MT];
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto chunk = [&](const Chunk& ch, uint32_t k) {
+        f32x4 d[NT][MT];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const bool starts = t % (4 / GPC) == 0, ends = t % (4 / GPC) == 4 / GPC - 1;
+            f16x8 x[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) x[mt] = *(const f16x8*)(xs + (uint64_t)(k * 4 + t) * rows * 32 + xrow[mt]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const uint32_t w4 = t == 0 ? ch.v[nt].x : t == 1 ? ch.v[nt].y : t == 2 ? ch.v[nt].z : ch.v[nt].w;
+                const f16x8 wv = unpack(w4);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) d[nt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[mt], wv, starts ? zero : d[nt][mt], 0, 0, 0);
+                if (ends) {
+                    const float s = half_to_f32<SDT>(piece_at(ch.s[nt], t / (4 / GPC)));
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[nt][mt][i] = fmaf(s, d[nt][mt][i], acc[nt][mt][i]);
+                }
+            }
+        }
+    };
+    uint32_t k = 0;
+    for (uint64_t u = u0; u < u1;) {
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i) {
+            if (u < u1) {
+                if (k == 0) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) acc[nt][mt] = zero;
+                }
+                chunk(ring[i], k);
+                load(ring[i]);
+                if (++k == kc) {
+                    k = 0;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint64_t row = (u * NT + nt) * 16 + r;
+                        if (row < a.n) {
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) {
+                                if (PARTS == 3) {
+                                    const uint32_t q = mt * 4 + c;
+                                    if (q < a.m) a.out[(uint64_t)q * a.n + row] = ldexpf(acc[nt][mt][2] + acc[nt][mt][1] + acc[nt][mt][0], expo[q]);
+                                } else {
+#pragma unroll
+                                    for (int x = 0; x < 4; ++x) {
+                                        const uint32_t q = mt * 16 + c * 4 + x;
+                                        if (q < a.m) a.out[(uint64_t)q * a.n + row] = ldexpf(acc[nt][mt][x], expo[q]);
+                                    }
+                                }
+                            }
+                        }
+                    }
+                    ++u;
+                }
+            }
         }
     }
 }
@@ -253,34 +396,47 @@ int begin_add(cgv_q4_index* h, uint64_t n) {
     return grow(h, h->n + n, false);
 }
 
-template <int MB, int QDT, int SDT>
-int launch_scores(const cgv_q4_index* h, const void* q, uint32_t m, float* out, hipStream_t s) {
-    const uint64_t tiles = (h->n + 15) / 16;
-    const unsigned blocks = (unsigned)std::min<uint64_t>((tiles + 3) / 4, 2048);
-    hipLaunchKernelGGL((q4_scores_kernel<MB, QDT, SDT>), dim3(blocks), dim3(256), (size_t)MB * h->L.kc * CHUNK * 4, s,
-                       (const uint4*)h->codes, (const uint16_t*)h->scales, q, h->n, h->L, m, out);
+constexpr size_t LDS_MAX = 160 * 1024;
+
+template <int PARTS, int SDT, int GPC, int MT, int NT>
+int launch_scores(const cgv_q4_index* h, const ScoreArgs& a, hipStream_t s) {
+    const size_t lds = (size_t)a.m * PARTS * h->L.kc * CHUNK * 2 + a.m * 4;
+    const uint64_t units = ((h->n + 15) / 16 + NT - 1) / NT;
+    const uint64_t per_cu = std::min<uint64_t>(4, LDS_MAX / lds);     // workgroups of four waves that a CU holds
+    const unsigned blocks = (unsigned)std::min<uint64_t>((units + 3) / 4, 256 * per_cu);
+    void (*kern)(ScoreArgs) = q4_scores_kernel<PARTS, SDT, GPC, MT, NT>;
+    OPCHK(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS_MAX));
+    hipLaunchKernelGGL(kern, dim3(blocks), dim3(256), lds, s, a);
     OPCHK(hipGetLastError());
     return CGV_OK;
 }
 
-template <int QDT, int SDT>
-int scores_typed(const cgv_q4_index* h, const void* q, uint32_t m, float* out, hipStream_t s) {
-    for (uint32_t a = 0; a < m;) {
-        const uint32_t c = std::min<uint32_t>(4, m - a);
-        const char* qa = (const char*)q + (uint64_t)a * h->L.dim * (QDT == cgv::DT_F32 ? 4 : 2);
-        float* oa = out + (uint64_t)a * h->n;
-        const int rc = c == 1 ? launch_scores<1, QDT, SDT>(h, qa, c, oa, s) : launch_scores<4, QDT, SDT>(h, qa, c, oa, s);
-        if (rc) return rc;
-        a += c;
-    }
-    return CGV_OK;
+template <int PARTS, int SDT, int GPC>
+int launch_by_queries(const cgv_q4_index* h, const ScoreArgs& a, hipStream_t s) {
+    constexpr uint32_t QPT = PARTS == 3 ? 4 : 16;
+    return a.m <= QPT ? launch_scores<PARTS, SDT, GPC, 1, 1>(h, a, s) : a.m <= 2 * QPT ? launch_scores<PARTS, SDT, GPC, 2, 2>(h, a, s)
+                                                                                       : launch_scores<PARTS, SDT, GPC, 4, 2>(h, a, s);
+}
+
+template <int PARTS, int SDT>
+int launch_by_group(const cgv_q4_index* h, const ScoreArgs& a, hipStream_t s) {
+    return h->L.gpc == 1 ? launch_by_queries<PARTS, SDT, 1>(h, a, s) : h->L.gpc == 2 ? launch_by_queries<PARTS, SDT, 2>(h, a, s)
+                                                                                     : launch_by_queries<PARTS, SDT, 4>(h, a, s);
 }
 
 int scores_on(const cgv_q4_index* h, const void* q, int qdt, uint32_t m, float* out, hipStream_t s) {
-    return by_dtype(qdt, [&](auto t) {
-        constexpr int Q = decltype(t)::value;
-        return h->sdt == CGV_DTYPE_FP16 ? scores_typed<Q, cgv::DT_FP16>(h, q, m, out, s) : scores_typed<Q, cgv::DT_BF16>(h, q, m, out, s);
-    });
+    const uint32_t parts = qdt == CGV_DTYPE_F32 ? 3 : 1;
+    const size_t per_query = (size_t)parts * h->L.kc * CHUNK * 2 + 4;
+    const uint32_t most = std::min<uint32_t>(parts == 3 ? 16 : 64, (uint32_t)(LDS_MAX / per_query));   // at least 3 (dim 8192, f32)
+    for (uint32_t i = 0; i < m; i += most) {
+        ScoreArgs a{(const uint4*)h->codes, h->scales, (const char*)q + (uint64_t)i * h->L.dim * esize(qdt), out + (uint64_t)i * h->n, h->n, h->L,
+                    std::min(most, m - i), qdt};
+        const bool f16 = h->sdt == CGV_DTYPE_FP16;
+        const int rc = parts == 3 ? (f16 ? launch_by_group<3, cgv::DT_FP16>(h, a, s) : launch_by_group<3, cgv::DT_BF16>(h, a, s))
+                                  : (f16 ? launch_by_group<1, cgv::DT_FP16>(h, a, s) : launch_by_group<1, cgv::DT_BF16>(h, a, s));
+        if (rc) return rc;
+    }
+    return CGV_OK;
 }
 
 }  // namespace
