@@ -191,6 +191,12 @@ def device_count():
     return int(lib().cgv_device_count())
 
 
+def raw_stream(device_index):
+    """The hipStream_t of torch's current stream on a device, as an integer."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
 def _is_torch(x):
     return type(x).__module__.startswith("torch")
 

@@ -7,6 +7,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
 #include <exception>
 #include <new>
 #include <string>
@@ -46,7 +47,7 @@ int guarded(F&& body) {
 }
 
 inline int need_gpu(int device_id) {
-    const int n = cgv_device_count();
+    static const int n = cgv_device_count();   // does not change while a process lives
     if (n == 0) return fail(CGV_ERR_HIP, "no HIP device visible: libcgvec_hip has no CPU fallback");
     if (device_id < 0 || device_id >= n) return fail(CGV_ERR_INVALID_ARG, "device_id out of range");
     return CGV_OK;
@@ -64,6 +65,18 @@ struct DeviceScope {
     hipError_t enter() { return cgv::use_device(device); }
     ~DeviceScope() {
         if (before >= 0 && before != device) (void)hipSetDevice(before);
+    }
+};
+
+// a kernel's limit of dynamic LDS, raised once per device (it is a property of the kernel on a device); one object per kernel
+struct LdsLimit {
+    std::atomic<uint64_t> done{0};
+    hipError_t raise(const void* kernel, int device, int bytes) {
+        const uint64_t bit = 1ull << (device & 63);
+        if (device < 64 && (done.load(std::memory_order_acquire) & bit)) return hipSuccess;
+        const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == hipSuccess && device < 64) done.fetch_or(bit, std::memory_order_release);
+        return e;
     }
 };
 

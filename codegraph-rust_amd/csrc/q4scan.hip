@@ -6,6 +6,8 @@
 // Inside a dword element 2p sits in nibble p and element 2p + 1 in nibble p + 4, so that one shift and one mask give the
 // two elements of a pair in the two halves of a register.
 // The scales of a tile's chunk are [16 rows][128 / group] behind each other.
+#include <limits.h>
+
 #include <mutex>
 #include <type_traits>
 
@@ -100,21 +102,27 @@ __global__ void q4_get_row_kernel(const uint32_t* __restrict__ codes, const uint
 }
 
 // ---- scores -----------------------------------------------------------------------------------------------------------------
-// One v_mfma_f32_16x16x32_f16 takes 32 columns of a 16-row tile against 16 rows of query data: codes become f16 integers -8..7
-// (exact), so the only roundings are those of the query's parts and of the f32 sums. An f32 query is three f16 parts (11 bits
-// each: all 24), a 16-bit query one. Parts are taken of the query scaled by a power of two to a largest magnitude of
-// 2^14 .. 2^15, so that f16's range does not matter: an element keeps an absolute 2^-39 of the query's largest. A query's rows of the
-// product depend on nothing but itself, so the 13 rows that a single f32 query leaves unused cost nothing and hold anything.
-// A group's products are scaled and added in f32 (its scale differs from row to row of the corpus: one value per lane).
+// A matrix instruction takes 32 columns of a 16-row tile (B operand: a lane holds 8 codes of one row) against 16 rows of query
+// data (A operand); rows of the result depend on nothing but their own row of A, so rows that a few queries leave unused cost
+// nothing and hold anything.
+//   f32 queries: fixed point. A query is scaled by a power of two to integers below 2^38 in magnitude (an element keeps 24
+//     bits, or an absolute 2^-39 of the query's largest) and split into five signed bytes; v_mfma_i32_16x16x32_i8 adds byte x code
+//     exactly. A code's byte is 16 (c - 8): two masks and a shift make eight of them. Three queries of five rows an operand.
+//   16-bit queries: one f16 row per query (scaled to 2^14 .. 2^15, so that bf16's range fits), 16 queries an operand;
+//     codes become f16 integers -8..7 by 0x6400 | c = 1024 + c and one packed multiply-add; v_mfma_f32_16x16x32_f16.
+// A group's sum is multiplied by its scale - one value per lane, its row's - and added up in f32.
 //
-// Bound by the codes' way from HBM: a wave streams its tiles' chunks with the next ones already in flight. Per 8 codes a lane
-// spends 11 instructions on unpacking, 4 FMAs per 32 columns on scales of group 32.
+// Bound by the codes' way from HBM, if the vector instructions per KiB stay below its time: a CU's share of 6 TB/s is a KiB per
+// 105 cycles, its four SIMDs spend 4 cycles on a vector instruction: 105 of them per KiB and SIMD is the limit. The same sums
+// with codes turned to f32 and fmaf (8 + 8 instructions for 8 codes) ran at 3.5 TB/s.
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct ScoreArgs {
-    const uint4* codes;
+    const u32x4* codes;
     const uint16_t* scales;
     const void* queries;
     float* out;
@@ -122,23 +130,8 @@ struct ScoreArgs {
     Layout L;
     uint32_t m;            // queries of this launch
     int qdt;
+    const char* image;     // the queries as the kernel wants them in LDS, or NULL: every workgroup makes them itself
 };
-
-__device__ inline float load_query(const void* q, int dt, uint64_t i) {
-    return dt == CGV_DTYPE_F32 ? load_elem<cgv::DT_F32>(q, i) : dt == CGV_DTYPE_BF16 ? load_elem<cgv::DT_BF16>(q, i) : load_elem<cgv::DT_FP16>(q, i);
-}
-
-// eight codes of a dword as f16 integers -8..7: 0x6400 | c is 1024 + c
-__device__ inline f16x8 unpack(uint32_t w) {
-    const f16x2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
-    f16x2 p[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = __builtin_bit_cast(f16x2, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) + off;
-    f16x8 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[2 * i] = p[i][0], v[2 * i + 1] = p[i][1];
-    return v;
-}
 
 template <int GPC>
 struct ScalePiece;   // the scales of one row's groups in a chunk
@@ -152,36 +145,174 @@ __device__ inline uint16_t piece_at(uint16_t v, int) { return v; }
 __device__ inline uint16_t piece_at(uint32_t v, int i) { return (uint16_t)(v >> (16 * i)); }
 __device__ inline uint16_t piece_at(uint2 v, int i) { return (uint16_t)((i < 2 ? v.x : v.y) >> (16 * (i & 1))); }
 
-// PARTS f16 parts of a query (3: f32 queries, 4 queries a 16-row operand; 1: 16 queries), MT such operands, NT tiles at a time
-template <int PARTS, int SDT, int GPC, int MT, int NT>
-__global__ __launch_bounds__(256) void q4_scores_kernel(ScoreArgs a) {
+__device__ inline float load_query(const void* q, int dt, uint64_t i) {
+    return dt == CGV_DTYPE_F32 ? load_elem<cgv::DT_F32>(q, i) : dt == CGV_DTYPE_BF16 ? load_elem<cgv::DT_BF16>(q, i) : load_elem<cgv::DT_FP16>(q, i);
+}
+
+// f32 queries
+struct Fixed {
+    static constexpr uint32_t QPT = 3, ROWS = 5;      // queries of an operand, LDS rows of a query (byte 0 is the lowest)
+    static constexpr uint32_t ROW_BYTES = 32;         // of 32 columns
+    typedef i32x4 Acc;
+    typedef long Frag;
+    static __device__ Frag weights(uint32_t w) {
+        const uint32_t lo = ((w << 4) & 0xf0f0f0f0u) ^ 0x80808080u, hi = (w & 0xf0f0f0f0u) ^ 0x80808080u;   // nibbles 0 2 4 6, 1 3 5 7
+        return (long)((uint64_t)hi << 32 | lo);
+    }
+    static __device__ Acc mma(Frag x, Frag w, Acc c) { return __builtin_amdgcn_mfma_i32_16x16x32_i8(x, w, c, 0, 0, 0); }
+    // operand row r: rows 4 q .. 4 q + 3 are bytes 1 .. 4 of query q, row 12 + q is its byte 0
+    static __device__ uint32_t query_of(uint32_t r) { return r < 12 ? r >> 2 : min(r - 12, 2u); }
+    static __device__ uint32_t part_of(uint32_t r) { return r < 12 ? (r & 3) + 1 : 0u; }
+    static __device__ int unit(float mx) { return mx > 0.0f ? 37 - ilogbf(mx) : 0; }
+    static constexpr int SCORE_SHIFT = -4;             // the codes are 16 times too large
+    static __device__ void stage(char* xs, uint32_t rows, uint32_t q, uint32_t e, float v) {
+        // v is below 2^38: its bits from 2^16 up and its rest are exact integers of 23 and 17 bits
+        const float t = rintf(v * 0x1p-16f);
+        int low = (int)rintf(v - t * 65536.0f), top = (int)t;
+        int d[5];
+        d[0] = (signed char)(low & 255);
+        low = (low - d[0]) >> 8;
+        d[1] = (signed char)(low & 255);
+        top += (low - d[1]) >> 8;
+#pragma unroll
+        for (int p = 2; p < 5; ++p) {
+            d[p] = (signed char)(top & 255);
+            top = (top - d[p]) >> 8;
+        }
+        // element 2 p lies in nibble p, 2 p + 1 in nibble p + 4: their bytes come out in the order 0 4 1 5 2 6 3 7
+        char* x = xs + ((e / 32) * rows + q * ROWS) * ROW_BYTES + (e % 32 & ~7u) + ((0x75316420u >> (4 * (e & 7u))) & 7u);
+#pragma unroll
+        for (int p = 0; p < 5; ++p) x[p * ROW_BYTES] = (char)d[p];
+    }
+    template <int MT>
+    static __device__ void store(const ScoreArgs& a, const f32x4 (&acc)[MT], uint64_t row, uint32_t lane, const int* expo) {
+        const uint32_t r = lane & 15, c = lane >> 4;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const float e0 = __shfl(acc[mt][0], 48 + r), e1 = __shfl(acc[mt][1], 48 + r), e2 = __shfl(acc[mt][2], 48 + r);
+            const float low = c == 0 ? e0 : c == 1 ? e1 : e2;
+            const float v = fmaf(fmaf(fmaf(fmaf(low, 0x1p-8f, acc[mt][0]), 0x1p-8f, acc[mt][1]), 0x1p-8f, acc[mt][2]), 0x1p-8f, acc[mt][3]);
+            const uint32_t q = mt * 3 + c;
+            if (c < 3 && q < a.m && row < a.n) a.out[(uint64_t)q * a.n + row] = expo[q] == INT_MIN ? NAN : ldexpf(v, expo[q] + 32);
+        }
+    }
+};
+
+// bf16 and fp16 queries
+struct Half {
+    static constexpr uint32_t QPT = 16, ROWS = 1, ROW_BYTES = 64;
+    typedef f32x4 Acc;
+    typedef f16x8 Frag;
+    static __device__ Frag weights(uint32_t w) {
+        // 1024 + c from the low four bits of a half, 1024 + 16 c from the next four
+        const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f}, m1032 = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+        const f16x2 x16 = {(_Float16)0.0625f, (_Float16)0.0625f}, m72 = {(_Float16)-72.0f, (_Float16)-72.0f};
+        const uint32_t w8 = w >> 8;
+        f16x2 p[4];
+        p[0] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w & 0x000f000fu) | 0x64006400u), one, m1032);
+        p[1] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w & 0x00f000f0u) | 0x64006400u), x16, m72);
+        p[2] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w8 & 0x000f000fu) | 0x64006400u), one, m1032);
+        p[3] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w8 & 0x00f000f0u) | 0x64006400u), x16, m72);
+        Frag v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[2 * i] = p[i][0], v[2 * i + 1] = p[i][1];
+        return v;
+    }
+    static __device__ Acc mma(Frag x, Frag w, Acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w, c, 0, 0, 0); }
+    static __device__ uint32_t query_of(uint32_t r) { return r; }
+    static __device__ uint32_t part_of(uint32_t) { return 0; }
+    static __device__ int unit(float mx) { return mx > 0.0f ? 14 - ilogbf(mx) : 0; }
+    static constexpr int SCORE_SHIFT = 0;
+    static __device__ void stage(char* xs, uint32_t rows, uint32_t q, uint32_t e, float v) {
+        ((_Float16*)(xs + ((e / 32) * rows + q) * ROW_BYTES))[e % 32] = (_Float16)v;
+    }
+    template <int MT>
+    static __device__ void store(const ScoreArgs& a, const f32x4 (&acc)[MT], uint64_t row, uint32_t lane, const int* expo) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const uint32_t q = mt * 16 + (lane >> 4) * 4 + x;
+                if (q < a.m && row < a.n) a.out[(uint64_t)q * a.n + row] = expo[q] == INT_MIN ? NAN : ldexpf(acc[mt][x], expo[q]);
+            }
+    }
+};
+
+// queries q0 .. q1 - 1 into their places (LDS, or the image of it in memory), by a workgroup: largest magnitudes first (as bits: NaN
+// and Inf win), then the parts. A thread has four elements on their way at a time
+template <class P, uint32_t THREADS>
+__device__ inline void stage_queries(const ScoreArgs& a, uint32_t q0, uint32_t q1, char* xs, uint32_t rows, int* expo, uint32_t* top) {
+    const uint32_t kp = a.L.kc * CHUNK, total = (q1 - q0) * kp;
+    for (uint32_t q = threadIdx.x; q < q1 - q0; q += THREADS) top[q] = 0;
+    __syncthreads();
+    constexpr uint32_t BATCH = 4;
+    for (int pass = 0; pass < 2; ++pass) {
+        for (uint32_t i0 = 0; i0 < total; i0 += THREADS * BATCH) {
+            float v[BATCH];
+#pragma unroll
+            for (uint32_t j = 0; j < BATCH; ++j) {
+                const uint32_t i = i0 + j * THREADS + threadIdx.x, q = i / kp, e = i - q * kp;
+                v[j] = i < total && e < a.L.dim ? load_query(a.queries, a.qdt, (uint64_t)(q0 + q) * a.L.dim + e) : 0.0f;
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < BATCH; ++j) {
+                const uint32_t i = i0 + j * THREADS + threadIdx.x, q = i / kp, e = i - q * kp;   // kp: a multiple of 128, a wave has one query
+                if (i >= total) continue;
+                if (pass == 0) {
+                    uint32_t bits = __float_as_uint(fabsf(v[j]));
+                    for (int o = 32; o; o >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, o));
+                    if ((threadIdx.x & 63) == 0) atomicMax(&top[q], bits);
+                } else {
+                    const uint32_t t = top[q];
+                    const bool bad = t >= 0x7f800000u;
+                    const int ex = bad ? 0 : P::unit(__uint_as_float(t));
+                    P::stage(xs, rows, q0 + q, e, bad ? 0.0f : ldexpf(v[j], ex));
+                    if (e == 0) expo[q0 + q] = bad ? INT_MIN : P::SCORE_SHIFT - ex;
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// a workgroup per query: the image of what the kernel below wants in LDS
+template <class P>
+__global__ __launch_bounds__(256) void q4_image_kernel(ScoreArgs a, char* image) {
+    __shared__ uint32_t top;
+    const uint32_t rows = a.m * P::ROWS;
+    stage_queries<P, 256>(a, blockIdx.x, blockIdx.x + 1, image, rows, (int*)(image + (uint64_t)(a.L.kc * CHUNK / 32) * rows * P::ROW_BYTES), &top);
+}
+
+// MT operands of queries, NT tiles at a time
+template <class P, int SDT, int GPC, int MT, int NT, bool ONCE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void q4_scores_kernel(ScoreArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    constexpr uint32_t QPT = PARTS == 3 ? 4 : 16;      // queries of an operand
     typedef typename ScalePiece<GPC>::type SP;
     const uint32_t lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4, wave = threadIdx.x >> 6;
-    const uint32_t kc = a.L.kc, rows = a.m * PARTS, kp = kc * CHUNK;
-    _Float16* xs = (_Float16*)smem;                    // [kp / 32][rows][32]
-    int* expo = (int*)(smem + (uint64_t)rows * kp * 2);
+    const uint32_t kc = a.L.kc, rows = a.m * P::ROWS, kp = kc * CHUNK;
+    char* xs = smem;                                   // [kp / 32][rows][32 columns]
+    int* expo = (int*)(smem + (uint64_t)(kp / 32) * rows * P::ROW_BYTES);
 
-    // this wave's tiles, and the first chunks on their way before anything else
-    const uint64_t units = ((a.n + 15) / 16 + NT - 1) / NT, waves = (uint64_t)gridDim.x * 4, w = (uint64_t)blockIdx.x * 4 + wave;
-    const uint64_t u0 = units * w / waves, u1 = units * (w + 1) / waves;
-    const uint64_t tiles = (a.n + 15) / 16;
+    // this wave takes every `waves`-th unit of tiles (all waves together read one stretch of the corpus at a time); its first
+    // chunks are on their way before anything else
+    const uint64_t tiles = (a.n + 15) / 16, units = (tiles + NT - 1) / NT;
+    const uint64_t waves = (uint64_t)gridDim.x * WAVES, w = (uint64_t)wave * gridDim.x + blockIdx.x;
     struct Chunk {
-        uint4 v[NT];
+        u32x4 v[NT];
         SP s[NT];
     };
-    uint64_t lu = u0;          // the load side's unit and chunk
+    uint64_t lu = w;           // the load side's unit and chunk
     uint32_t lk = 0;
     auto load = [&](Chunk& ch) {
-        if (lu < u1) {
+        if (lu < units) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const uint64_t tile = min(lu * NT + t, tiles - 1);
-                ch.v[t] = a.codes[(tile * kc + lk) * 64 + lane];
+                const u32x4* src = &a.codes[(tile * kc + lk) * 64 + lane];
+                ch.v[t] = ONCE ? __builtin_nontemporal_load(src) : *src;
                 ch.s[t] = *(const SP*)(a.scales + ((tile * kc + lk) * 16 + r) * GPC);
             }
-            if (++lk == kc) lk = 0, ++lu;
+            if (++lk == kc) lk = 0, lu += waves;
         }
     };
     constexpr int DEPTH = 4;
@@ -189,102 +320,65 @@ __global__ __launch_bounds__(256) void q4_scores_kernel(ScoreArgs a) {
 #pragma unroll
     for (int i = 0; i < DEPTH; ++i) load(ring[i]);
 
-    // queries into LDS: a wave per query
-    for (uint32_t q = wave; q < a.m; q += 4) {
-        const uint64_t base = (uint64_t)q * a.L.dim;
-        float mx = 0.0f;
-        bool bad = false;
-        for (uint32_t e = lane; e < a.L.dim; e += 64) {
-            const float v = fabsf(load_query(a.queries, a.qdt, base + e));
-            bad |= !(v < INFINITY);
-            mx = fmaxf(mx, v);
-        }
-        for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-        bad = __ballot(bad) != 0;
-        const int ex = mx > 0.0f && !bad ? 14 - ilogbf(mx) : 0;
-        if (lane == 0) expo[q] = -ex;
-        for (uint32_t e = lane; e < kp; e += 64) {
-            float v = e < a.L.dim ? ldexpf(load_query(a.queries, a.qdt, base + e), ex) : 0.0f;
-            if (bad) v = NAN;
-            _Float16* x = xs + ((uint64_t)(e / 32) * rows + q * PARTS) * 32 + e % 32;
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p) {
-                const _Float16 h = (_Float16)v;
-                x[p * 32] = h;
-                v -= (float)h;
-            }
-        }
+    if (a.image) {
+        const uint4* src = (const uint4*)a.image;
+        const uint32_t pieces = (kp / 32) * rows * P::ROW_BYTES / 16;
+        for (uint32_t i = threadIdx.x; i < pieces; i += 64 * WAVES) ((uint4*)xs)[i] = src[i];
+        for (uint32_t i = threadIdx.x; i < a.m; i += 64 * WAVES) expo[i] = ((const int*)(src + pieces))[i];
+    } else {
+        stage_queries<P, 64 * WAVES>(a, 0, a.m, xs, rows, expo, (uint32_t*)expo + a.m);
     }
     __syncthreads();
 
-    // LDS row of this lane for each operand: row r is part r & 3 of query r >> 2 (three parts), or query r
-    uint32_t xrow[MT];
+    uint32_t xrow[MT];                                 // this lane's piece of each operand, in bytes from a step's first row
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        const uint32_t q = mt * QPT + (PARTS == 3 ? r >> 2 : r), p = PARTS == 3 ? min(r & 3u, 2u) : 0u;
-        xrow[mt] = (min(q, a.m - 1) * PARTS + p) * 32 + c * 8;
-    }
+    for (int mt = 0; mt < MT; ++mt)
+        xrow[mt] = (min(mt * P::QPT + P::query_of(r), a.m - 1) * P::ROWS + P::part_of(r)) * P::ROW_BYTES + c * (P::ROW_BYTES / 4);
     f32x4 acc[NT][MT];
-    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    const f32x4 fzero = {0.0f, 0.0f, 0.0f, 0.0f};
+    const typename P::Acc zero = {0, 0, 0, 0};
     auto chunk = [&](const Chunk& ch, uint32_t k) {
-        f32x4 d[NT][MT];
+        typename P::Acc d[NT][MT];
+        const char* xk = xs + k * 4 * rows * P::ROW_BYTES;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             const bool starts = t % (4 / GPC) == 0, ends = t % (4 / GPC) == 4 / GPC - 1;
-            f16x8 x[MT];
+            typename P::Frag x[MT];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) x[mt] = *(const f16x8*)(xs + (uint64_t)(k * 4 + t) * rows * 32 + xrow[mt]);
+            for (int mt = 0; mt < MT; ++mt) x[mt] = *(const typename P::Frag*)(xk + t * rows * P::ROW_BYTES + xrow[mt]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const uint32_t w4 = t == 0 ? ch.v[nt].x : t == 1 ? ch.v[nt].y : t == 2 ? ch.v[nt].z : ch.v[nt].w;
-                const f16x8 wv = unpack(w4);
+                const typename P::Frag wv = P::weights(ch.v[nt][t]);
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) d[nt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[mt], wv, starts ? zero : d[nt][mt], 0, 0, 0);
+                for (int mt = 0; mt < MT; ++mt) d[nt][mt] = P::mma(x[mt], wv, starts ? zero : d[nt][mt]);
                 if (ends) {
                     const float s = half_to_f32<SDT>(piece_at(ch.s[nt], t / (4 / GPC)));
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[nt][mt][i] = fmaf(s, d[nt][mt][i], acc[nt][mt][i]);
+                        for (int i = 0; i < 4; ++i) acc[nt][mt][i] = fmaf(s, (float)d[nt][mt][i], acc[nt][mt][i]);
                 }
             }
         }
     };
     uint32_t k = 0;
-    for (uint64_t u = u0; u < u1;) {
+    for (uint64_t u = w; u < units;) {
 #pragma unroll
         for (int i = 0; i < DEPTH; ++i) {
-            if (u < u1) {
+            if (u < units) {
                 if (k == 0) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) acc[nt][mt] = zero;
+                        for (int mt = 0; mt < MT; ++mt) acc[nt][mt] = fzero;
                 }
                 chunk(ring[i], k);
                 load(ring[i]);
                 if (++k == kc) {
                     k = 0;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const uint64_t row = (u * NT + nt) * 16 + r;
-                        if (row < a.n) {
-#pragma unroll
-                            for (int mt = 0; mt < MT; ++mt) {
-                                if (PARTS == 3) {
-                                    const uint32_t q = mt * 4 + c;
-                                    if (q < a.m) a.out[(uint64_t)q * a.n + row] = ldexpf(acc[nt][mt][2] + acc[nt][mt][1] + acc[nt][mt][0], expo[q]);
-                                } else {
-#pragma unroll
-                                    for (int x = 0; x < 4; ++x) {
-                                        const uint32_t q = mt * 16 + c * 4 + x;
-                                        if (q < a.m) a.out[(uint64_t)q * a.n + row] = ldexpf(acc[nt][mt][x], expo[q]);
-                                    }
-                                }
-                            }
-                        }
-                    }
-                    ++u;
+                    for (int nt = 0; nt < NT; ++nt) P::template store<MT>(a, acc[nt], (u * NT + nt) * 16 + r, lane, expo);
+                    u += waves;
                 }
             }
         }
@@ -398,45 +492,80 @@ int begin_add(cgv_q4_index* h, uint64_t n) {
 
 constexpr size_t LDS_MAX = 160 * 1024;
 
-template <int PARTS, int SDT, int GPC, int MT, int NT>
+template <class P>
+size_t query_bytes(const cgv_q4_index* h) { return (size_t)(h->L.kc * CHUNK / 32) * P::ROWS * P::ROW_BYTES + 8; }
+
+template <class P, int SDT, int GPC, int MT, int NT, bool ONCE = false>
 int launch_scores(const cgv_q4_index* h, const ScoreArgs& a, hipStream_t s) {
-    const size_t lds = (size_t)a.m * PARTS * h->L.kc * CHUNK * 2 + a.m * 4;
+    constexpr int WAVES = 8;
+    const size_t lds = a.m * query_bytes<P>(h);
     const uint64_t units = ((h->n + 15) / 16 + NT - 1) / NT;
-    const uint64_t per_cu = std::min<uint64_t>(4, LDS_MAX / lds);     // workgroups of four waves that a CU holds
-    const unsigned blocks = (unsigned)std::min<uint64_t>((units + 3) / 4, 256 * per_cu);
-    void (*kern)(ScoreArgs) = q4_scores_kernel<PARTS, SDT, GPC, MT, NT>;
-    OPCHK(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS_MAX));
-    hipLaunchKernelGGL(kern, dim3(blocks), dim3(256), lds, s, a);
+    const uint64_t per_cu = std::min<uint64_t>(2, LDS_MAX / lds);     // workgroups of a CU
+    const unsigned blocks = (unsigned)std::min<uint64_t>((units + WAVES - 1) / WAVES, 256 * per_cu);
+    void (*kern)(ScoreArgs) = q4_scores_kernel<P, SDT, GPC, MT, NT, ONCE, WAVES>;
+    static LdsLimit limit;
+    OPCHK(limit.raise((const void*)kern, h->device, (int)LDS_MAX));
+    hipLaunchKernelGGL(kern, dim3(blocks), dim3(64 * WAVES), lds, s, a);
     OPCHK(hipGetLastError());
     return CGV_OK;
 }
 
-template <int PARTS, int SDT, int GPC>
+template <class P, int SDT, int GPC>
 int launch_by_queries(const cgv_q4_index* h, const ScoreArgs& a, hipStream_t s) {
-    constexpr uint32_t QPT = PARTS == 3 ? 4 : 16;
-    return a.m <= QPT ? launch_scores<PARTS, SDT, GPC, 1, 1>(h, a, s) : a.m <= 2 * QPT ? launch_scores<PARTS, SDT, GPC, 2, 2>(h, a, s)
-                                                                                       : launch_scores<PARTS, SDT, GPC, 4, 2>(h, a, s);
+    // one operand of queries: two tiles at a time where every wave gets two such pairs, so that there is always one to work on
+    // (one query, 1M x 768: 87 -> 70 us), single tiles below, where the number of waves counts (10 k x 384: 6.0 -> 5.1 us)
+    // Codes that the 256 MiB last-level cache cannot hold until the next call are read past it (1M x 768: 78 -> 69 us), smaller ones
+    // stay there (250 k x 768, the same corpus again: 25 -> 21 us)
+    if (a.m <= P::QPT) {
+        if (h->n < 16ull * 4 * 4096) return launch_scores<P, SDT, GPC, 1, 1>(h, a, s);
+        return h->L.tile_codes((h->n + 15) / 16) > (256ull << 20) ? launch_scores<P, SDT, GPC, 1, 2, true>(h, a, s)
+                                                                   : launch_scores<P, SDT, GPC, 1, 2>(h, a, s);
+    }
+    return a.m <= 2 * P::QPT ? launch_scores<P, SDT, GPC, 2, 2>(h, a, s)
+                                                                                         : launch_scores<P, SDT, GPC, 4, 2>(h, a, s);
 }
 
-template <int PARTS, int SDT>
+template <class P, int SDT>
 int launch_by_group(const cgv_q4_index* h, const ScoreArgs& a, hipStream_t s) {
-    return h->L.gpc == 1 ? launch_by_queries<PARTS, SDT, 1>(h, a, s) : h->L.gpc == 2 ? launch_by_queries<PARTS, SDT, 2>(h, a, s)
-                                                                                     : launch_by_queries<PARTS, SDT, 4>(h, a, s);
+    return h->L.gpc == 1 ? launch_by_queries<P, SDT, 1>(h, a, s) : h->L.gpc == 2 ? launch_by_queries<P, SDT, 2>(h, a, s)
+                                                                                 : launch_by_queries<P, SDT, 4>(h, a, s);
 }
 
-int scores_on(const cgv_q4_index* h, const void* q, int qdt, uint32_t m, float* out, hipStream_t s) {
-    const uint32_t parts = qdt == CGV_DTYPE_F32 ? 3 : 1;
-    const size_t per_query = (size_t)parts * h->L.kc * CHUNK * 2 + 4;
-    const uint32_t most = std::min<uint32_t>(parts == 3 ? 16 : 64, (uint32_t)(LDS_MAX / per_query));   // at least 3 (dim 8192, f32)
+template <class P>
+uint32_t queries_per_launch(const cgv_q4_index* h) { return std::min<uint32_t>(4 * P::QPT, (uint32_t)(LDS_MAX / query_bytes<P>(h))); }   // 3 at least
+
+// one workgroup's way through 8192 elements is about 4 us, hidden behind the first codes; a launch more costs as much
+constexpr uint32_t STAGE_IN_PLACE = 8192;
+
+template <class P>
+size_t image_bytes(const cgv_q4_index* h, uint32_t m) {
+    const uint32_t most = std::min(m, queries_per_launch<P>(h));
+    return (uint64_t)most * h->L.kc * CHUNK <= STAGE_IN_PLACE ? 0 : most * query_bytes<P>(h);
+}
+
+template <class P>
+int scores_by(const cgv_q4_index* h, const void* q, int qdt, uint32_t m, float* out, char* ws, hipStream_t s) {
+    const uint32_t most = queries_per_launch<P>(h);
     for (uint32_t i = 0; i < m; i += most) {
-        ScoreArgs a{(const uint4*)h->codes, h->scales, (const char*)q + (uint64_t)i * h->L.dim * esize(qdt), out + (uint64_t)i * h->n, h->n, h->L,
-                    std::min(most, m - i), qdt};
-        const bool f16 = h->sdt == CGV_DTYPE_FP16;
-        const int rc = parts == 3 ? (f16 ? launch_by_group<3, cgv::DT_FP16>(h, a, s) : launch_by_group<3, cgv::DT_BF16>(h, a, s))
-                                  : (f16 ? launch_by_group<1, cgv::DT_FP16>(h, a, s) : launch_by_group<1, cgv::DT_BF16>(h, a, s));
+        ScoreArgs a{(const u32x4*)h->codes, h->scales, (const char*)q + (uint64_t)i * h->L.dim * esize(qdt), out + (uint64_t)i * h->n, h->n, h->L,
+                    std::min(most, m - i), qdt, nullptr};
+        if ((uint64_t)a.m * h->L.kc * CHUNK > STAGE_IN_PLACE) {
+            hipLaunchKernelGGL((q4_image_kernel<P>), dim3(a.m), dim3(256), 0, s, a, ws);
+            OPCHK(hipGetLastError());
+            a.image = ws;
+        }
+        const int rc = h->sdt == CGV_DTYPE_FP16 ? launch_by_group<P, cgv::DT_FP16>(h, a, s) : launch_by_group<P, cgv::DT_BF16>(h, a, s);
         if (rc) return rc;
     }
     return CGV_OK;
+}
+
+size_t scores_workspace(const cgv_q4_index* h, int qdt, uint32_t m) {
+    return qdt == CGV_DTYPE_F32 ? image_bytes<Fixed>(h, m) : image_bytes<Half>(h, m);
+}
+
+int scores_on(const cgv_q4_index* h, const void* q, int qdt, uint32_t m, float* out, char* ws, hipStream_t s) {
+    return qdt == CGV_DTYPE_F32 ? scores_by<Fixed>(h, q, qdt, m, out, ws, s) : scores_by<Half>(h, q, qdt, m, out, ws, s);
 }
 
 }  // namespace
@@ -620,15 +749,15 @@ int cgv_q4_scores_f32(cgv_q4_index* h, const float* queries_host, uint32_t m, fl
         OPCHK(dev.enter());
         // queries in pieces whose scores fit the staging buffer
         const uint64_t per = std::max<uint64_t>(1, std::min<uint64_t>(m, (512ull << 20) / (h->n * 4)));
-        const size_t qb = ((size_t)per * h->L.dim * 4 + 255) / 256 * 256;
-        int rc = ensure_stage(h, qb + per * h->n * 4);
+        const size_t qb = ((size_t)per * h->L.dim * 4 + 255) / 256 * 256, sb = (per * h->n * 4 + 255) / 256 * 256;
+        int rc = ensure_stage(h, qb + sb + scores_workspace(h, CGV_DTYPE_F32, (uint32_t)per));
         if (rc) return rc;
         float* dq = (float*)h->stage;
         float* ds = (float*)((char*)h->stage + qb);
         for (uint64_t a = 0; a < m; a += per) {
             const uint32_t c = (uint32_t)std::min<uint64_t>(per, m - a);
             OPCHK(hipMemcpyAsync(dq, queries_host + a * h->L.dim, (size_t)c * h->L.dim * 4, hipMemcpyHostToDevice, h->stream));
-            if ((rc = scores_on(h, dq, CGV_DTYPE_F32, c, ds, h->stream))) return rc;
+            if ((rc = scores_on(h, dq, CGV_DTYPE_F32, c, ds, (char*)h->stage + qb + sb, h->stream))) return rc;
             OPCHK(hipMemcpyAsync(out_host + a * h->n, ds, (size_t)c * h->n * 4, hipMemcpyDeviceToHost, h->stream));
             OPCHK(hipStreamSynchronize(h->stream));
         }
@@ -636,7 +765,10 @@ int cgv_q4_scores_f32(cgv_q4_index* h, const float* queries_host, uint32_t m, fl
     });
 }
 
-int cgv_q4_scores_dev(cgv_q4_index* h, const void* queries_dev, int query_dtype, uint32_t m, float* out_dev, void* stream) {
+size_t cgv_q4_scores_workspace(const cgv_q4_index* h, int query_dtype, uint32_t m) { return h && m ? scores_workspace(h, query_dtype, m) : 0; }
+
+int cgv_q4_scores_dev(cgv_q4_index* h, const void* queries_dev, int query_dtype, uint32_t m, float* out_dev, void* workspace_dev,
+                      size_t workspace_bytes, void* stream) {
     return guarded([&]() -> int {
         if (!h) return fail(CGV_ERR_INVALID_ARG, "handle is NULL");
         if (query_dtype != CGV_DTYPE_F32 && query_dtype != CGV_DTYPE_BF16 && query_dtype != CGV_DTYPE_FP16)
@@ -644,9 +776,12 @@ int cgv_q4_scores_dev(cgv_q4_index* h, const void* queries_dev, int query_dtype,
         std::lock_guard<std::mutex> lk(h->mu);
         if (m == 0 || h->n == 0) return CGV_OK;
         if (!queries_dev || !out_dev) return fail(CGV_ERR_INVALID_ARG, "NULL argument");
+        const size_t need = scores_workspace(h, query_dtype, m);
+        if (workspace_bytes < need || (need && !workspace_dev)) return fail(CGV_ERR_INVALID_ARG, "the workspace is smaller than cgv_q4_scores_workspace says");
+        if (need && (uintptr_t)workspace_dev % 256) return fail(CGV_ERR_INVALID_ARG, "the workspace must be aligned to 256 bytes");
         DeviceScope dev(h->device);
         OPCHK(dev.enter());
-        return scores_on(h, queries_dev, query_dtype, m, out_dev, (hipStream_t)stream);
+        return scores_on(h, queries_dev, query_dtype, m, out_dev, (char*)workspace_dev, (hipStream_t)stream);
     });
 }
 

@@ -123,6 +123,7 @@ struct Problem {
     uint32_t b, bp, dim, dp, k;
     float scale, tscale;
     uint16_t* qws;            // [planes][bp][dp]
+    int device;
 };
 
 template <int DT>
@@ -364,19 +365,20 @@ void set_segments(Args& a, int dtype, bool swap) {
 }
 
 template <int DT, class S, bool TA, bool TB, int EPI>
-int launch_gemm(const Args& a, hipStream_t s) {
+int launch_gemm(const Args& a, int device, hipStream_t s) {
     constexpr int bytes = S::lds_bytes(EPI == EPI_G || EPI == EPI_DR);
     if (a.blocks == 0) return CGV_OK;
     void (*kern)(const Args) = gemm_kernel<DT, S, TA, TB, EPI>;
-    OPCHK(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    static LdsLimit limit;
+    OPCHK(limit.raise((const void*)kern, device, bytes));
     hipLaunchKernelGGL(kern, dim3(a.blocks), dim3(S::THREADS), bytes, s, a);
     OPCHK(hipGetLastError());
     return CGV_OK;
 }
 template <int DT, bool TA, bool TB, int EPI>
-int launch_by_queries(uint32_t bn, const Args& a, hipStream_t s) {
-    return bn == 64 ? launch_gemm<DT, S64, TA, TB, EPI>(a, s) : bn == 128 ? launch_gemm<DT, S128, TA, TB, EPI>(a, s)
-                                                              : launch_gemm<DT, S256, TA, TB, EPI>(a, s);
+int launch_by_queries(uint32_t bn, const Args& a, int device, hipStream_t s) {
+    return bn == 64 ? launch_gemm<DT, S64, TA, TB, EPI>(a, device, s) : bn == 128 ? launch_gemm<DT, S128, TA, TB, EPI>(a, device, s)
+                                                              : launch_gemm<DT, S256, TA, TB, EPI>(a, device, s);
 }
 
 // scores of the corpus rows [n0, n0 + c) against all queries
@@ -432,7 +434,7 @@ int forward(const Plan& pl, Problem P, int dtype, float* loss, char* ws, hipStre
         a.anchor = anchor;
         a.part = part + (uint64_t)parts * pl.bp;
         parts += a.splits * pl.wm;
-        const int rc = launch_by_queries<DT, false, false, EPI_LSE>(pl.bn, a, s);
+        const int rc = launch_by_queries<DT, false, false, EPI_LSE>(pl.bn, a, P.device, s);
         if (rc) return rc;
     }
     hipLaunchKernelGGL(loss_kernel, dim3((pl.b + 3) / 4), dim3(256), 0, s, P, (const float2*)part, parts, loss);
@@ -477,7 +479,7 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
         a.out = G;
         a.out_pitch = g_pitch;
         a.out_plane = g_plane;
-        if ((rc = launch_by_queries<DT, false, false, EPI_G>(pl.bn, a, s))) return rc;
+        if ((rc = launch_by_queries<DT, false, false, EPI_G>(pl.bn, a, P.device, s))) return rc;
         const uint64_t total = (uint64_t)pl.b * pl.k;
         hipLaunchKernelGGL((patch_kernel<DT>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, (const uint32_t*)ent_id, (const float*)ent_val, total,
                            pl.k, n0, c, (const float*)mul, (uint16_t*)G, pl.piece_b, g_plane / 2);
@@ -499,7 +501,7 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             d.out = (char*)part;
             d.out_plane = (uint64_t)pl.bp * pl.dp * 4;
             d.accumulate = n0 > 0;
-            if ((rc = launch_by_queries<DT, true, false, EPI_DQ>(pl.bn, d, s))) return rc;
+            if ((rc = launch_by_queries<DT, true, false, EPI_DQ>(pl.bn, d, P.device, s))) return rc;
         }
         if (dr) {
             Args d{};
@@ -518,7 +520,7 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             d.out_pitch = (uint64_t)pl.dim * esize(dtype);
             d.vec_out = d.out_pitch % 16 == 0 && (uintptr_t)dr % 16 == 0;
             d.unscale = mul + 1;
-            if ((rc = launch_gemm<DT, S256, true, true, EPI_DR>(d, s))) return rc;
+            if ((rc = launch_gemm<DT, S256, true, true, EPI_DR>(d, P.device, s))) return rc;
         }
     }
     if (dq) {
@@ -576,7 +578,7 @@ int cgv_corpus_loss_dev(int device_id, const void* queries_dev, uint64_t query_s
         DeviceScope dev(device_id);
         OPCHK(dev.enter());
         const Problem P{queries_dev, rows_dev, query_stride, row_stride, n_rows, ids_dev, teacher_scores_dev, saved_dev,
-                        pl.b, pl.bp, dim, pl.dp, k, scale, teacher_scale, nullptr};
+                        pl.b, pl.bp, dim, pl.dp, k, scale, teacher_scale, nullptr, device_id};
         return by_dtype(dtype, [&](auto t) { return forward<decltype(t)::value>(pl, P, dtype, loss_dev, (char*)workspace_dev, (hipStream_t)stream); });
     });
 }
@@ -599,7 +601,7 @@ int cgv_corpus_loss_grad_dev(int device_id, const void* queries_dev, uint64_t qu
         OPCHK(dev.enter());
         const hipStream_t s = (hipStream_t)stream;
         const Problem P{queries_dev, rows_dev, query_stride, row_stride, n_rows, ids_dev, teacher_scores_dev, const_cast<float*>(saved_dev),
-                        pl.b, pl.bp, dim, pl.dp, k, scale, teacher_scale, nullptr};
+                        pl.b, pl.bp, dim, pl.dp, k, scale, teacher_scale, nullptr, device_id};
         return by_dtype(dtype, [&](auto t) -> int {
             constexpr int DT = decltype(t)::value;
             if (b == 0) {

@@ -3,7 +3,7 @@ import ctypes as C
 
 import numpy as np
 
-from .cgvec import CGV_ERR_DIM_MISMATCH, CGV_ERR_INVALID_ARG, DTYPES, CgvError, _check, _is_torch, lib as _base_lib
+from .cgvec import CGV_ERR_DIM_MISMATCH, CGV_ERR_INVALID_ARG, DTYPES, CgvError, _check, _is_torch, lib as _base_lib, raw_stream
 
 _decl = False
 
@@ -24,7 +24,9 @@ def lib():
         L.cgv_q4_add_codes_dev.argtypes = [vp, vp, vp, u64, vp]
         L.cgv_q4_get_row_f32.argtypes = [vp, u64, vp]
         L.cgv_q4_scores_f32.argtypes = [vp, vp, u32, vp]
-        L.cgv_q4_scores_dev.argtypes = [vp, vp, i32, u32, vp, vp]
+        L.cgv_q4_scores_dev.argtypes = [vp, vp, i32, u32, vp, vp, C.c_size_t, vp]
+        L.cgv_q4_scores_workspace.argtypes = [vp, i32, u32]
+        L.cgv_q4_scores_workspace.restype = C.c_size_t
         for n in ("cgv_q4_create", "cgv_q4_destroy", "cgv_q4_reserve", "cgv_q4_add_f32", "cgv_q4_add_f32_dev", "cgv_q4_add_codes",
                   "cgv_q4_add_codes_dev", "cgv_q4_get_row_f32", "cgv_q4_scores_f32", "cgv_q4_scores_dev"):
             getattr(L, n).restype = i32
@@ -71,8 +73,7 @@ class Int4ScanIndex:
         _check(lib().cgv_q4_reserve(self._h, int(n)))
 
     def _stream(self):
-        import torch
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+        return raw_stream(self.device)
 
     def _on_device(self, t, what):
         if t.device.type != "cuda" or t.device.index != self.device:
@@ -140,13 +141,16 @@ class Int4ScanIndex:
             if code is None:
                 raise CgvError(CGV_ERR_INVALID_ARG, f"queries must be float32, bfloat16 or float16, not {queries.dtype}")
             self._on_device(queries, "queries")
-            q = queries.detach()
-            q = (q[None] if q.dim() == 1 else q).contiguous()
+            one = queries.dim() == 1
+            q = (queries.detach()[None] if one else queries).contiguous()
             if q.dim() != 2 or q.shape[1] != self.dim:
                 raise CgvError(CGV_ERR_DIM_MISMATCH, f"query dim {tuple(queries.shape)} != {self.dim}")
-            out = torch.empty((q.shape[0], len(self)), dtype=torch.float32, device=q.device)
-            _check(lib().cgv_q4_scores_dev(self._h, C.c_void_p(q.data_ptr()), code, q.shape[0], C.c_void_p(out.data_ptr()), self._stream()))
-            return out[0] if queries.dim() == 1 else out
+            L, m = lib(), q.shape[0]
+            out = torch.empty((m, L.cgv_q4_count(self._h)), dtype=torch.float32, device=q.device)
+            nb = L.cgv_q4_scores_workspace(self._h, code, m)
+            ws = torch.empty((nb,), dtype=torch.uint8, device=q.device) if nb else None
+            _check(L.cgv_q4_scores_dev(self._h, q.data_ptr(), code, m, out.data_ptr(), ws.data_ptr() if nb else None, nb, self._stream()))
+            return out[0] if one else out
         if _is_torch(queries):
             queries = queries.detach().float().numpy()
         q = np.ascontiguousarray(queries, dtype=np.float32)

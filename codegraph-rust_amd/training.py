@@ -5,7 +5,7 @@ import ctypes as C
 import torch
 from torch.autograd.function import once_differentiable
 
-from .cgvec import CGV_ERR_DIM_MISMATCH, CGV_ERR_INVALID_ARG, CgvError, _check, lib as _base_lib
+from .cgvec import CGV_ERR_DIM_MISMATCH, CGV_ERR_INVALID_ARG, CgvError, _check, lib as _base_lib, raw_stream as _stream
 
 _decl = False
 _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -32,7 +32,7 @@ def lib():
 
 
 def _ptr(t):
-    return C.c_void_p(t.data_ptr() if t is not None else None)
+    return t.data_ptr() if t is not None else None
 
 
 def _bad(msg, code=CGV_ERR_INVALID_ARG):
@@ -49,9 +49,7 @@ def _matrix(t, name):
         raise _bad(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
     if not 1 <= t.shape[1] <= 8192:
         raise _bad(f"{name}: dim must be in 1..=8192, got {t.shape[1]}")
-    if t.shape[0] > 1 and (t.stride(1) != 1 or t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    elif t.shape[0] <= 1:
+    if not t.is_contiguous() and (t.shape[0] <= 1 or t.stride(1) != 1 or t.stride(0) < t.shape[1]):
         t = t.contiguous()
     return t
 
@@ -65,15 +63,11 @@ def _ids(t, name, device):
         raise _bad(f"{name} must be a tensor on {device}")
     if t.dtype not in (torch.int64, torch.int32):
         raise _bad(f"{name} must be int64 or int32, not {t.dtype}")
-    return t.detach().to(torch.int64).contiguous()
-
-
-def _stream(device):
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return t if t.dtype == torch.int64 and t.is_contiguous() else t.to(torch.int64).contiguous()
 
 
 def _workspace(nbytes, device):
-    return torch.empty((max(int(nbytes), 1),), dtype=torch.uint8, device=device)
+    return torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
 
 
 class _LookupRows(torch.autograd.Function):
@@ -82,7 +76,7 @@ class _LookupRows(torch.autograd.Function):
         n, d = table.shape
         out = torch.empty((ids.numel(), d), dtype=table.dtype, device=table.device)
         _check(lib().cgv_lookup_rows_dev(table.device.index, _ptr(table), _CODES[table.dtype], n, d, _row_stride(table), _ptr(ids),
-                                         ids.numel(), scale, _ptr(out), _stream(table.device)))
+                                         ids.numel(), scale, _ptr(out), _stream(table.device.index)))
         ctx.save_for_backward(ids)
         ctx.shape, ctx.dtype, ctx.scale = (n, d), table.dtype, scale
         return out.view(*ids.shape, d)
@@ -91,7 +85,17 @@ class _LookupRows(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
-        return lookup_rows_grad(dout, ids, ctx.shape[0], scale=ctx.scale), None, None
+        return _lookup_grad(dout.contiguous(), ids, ctx.shape[0], ctx.scale), None, None
+
+
+def _lookup_grad(dout, ids, n, scale):
+    d, k, dev, L = dout.shape[-1], ids.numel(), dout.device, lib()
+    out = torch.empty((n, d), dtype=dout.dtype, device=dev)
+    nbytes = L.cgv_lookup_grad_workspace(k, n, d)
+    ws = _workspace(nbytes, dev)
+    _check(L.cgv_lookup_grad_dev(dev.index, dout.data_ptr(), _CODES[dout.dtype], ids.data_ptr(), k, n, d, scale, out.data_ptr(), _ptr(ws), nbytes,
+                                 _stream(dev.index)))
+    return out
 
 
 def lookup_rows(table, ids, scale=1.0):
@@ -113,14 +117,7 @@ def lookup_rows_grad(dout, ids, n_rows, scale=1.0):
         raise _bad(f"dout {tuple(dout.shape)} does not fit ids {tuple(ids.shape)}", CGV_ERR_DIM_MISMATCH)
     if int(n_rows) < 0:
         raise _bad("n_rows must be >= 0")
-    g = dout.detach().contiguous()
-    d = g.shape[-1]
-    out = torch.empty((int(n_rows), d), dtype=g.dtype, device=g.device)
-    nbytes = lib().cgv_lookup_grad_workspace(ids.numel(), int(n_rows), d)
-    ws = _workspace(nbytes, g.device)
-    _check(lib().cgv_lookup_grad_dev(g.device.index, _ptr(g), _CODES[g.dtype], _ptr(ids), ids.numel(), int(n_rows), d, float(scale),
-                                     _ptr(out), _ptr(ws), ws.numel(), _stream(g.device)))
-    return out
+    return _lookup_grad(dout.detach().contiguous(), ids, int(n_rows), float(scale))
 
 
 class _CorpusLoss(torch.autograd.Function):
@@ -132,9 +129,10 @@ class _CorpusLoss(torch.autograd.Function):
         code, dev = _CODES[rows.dtype], rows.device
         loss = torch.empty((b,), dtype=torch.float32, device=dev)
         saved = torch.empty((b * (k + 2),), dtype=torch.float32, device=dev)
-        ws = _workspace(L.cgv_corpus_loss_workspace(b, n, d, k, code), dev)
+        nbytes = L.cgv_corpus_loss_workspace(b, n, d, k, code)
+        ws = _workspace(nbytes, dev)
         _check(L.cgv_corpus_loss_dev(dev.index, _ptr(queries), _row_stride(queries), _ptr(rows), _row_stride(rows), code, b, n, d, _ptr(ids),
-                                     _ptr(scores), k, scale, teacher_scale, _ptr(loss), _ptr(saved), _ptr(ws), ws.numel(), _stream(dev)))
+                                     _ptr(scores), k, scale, teacher_scale, _ptr(loss), _ptr(saved), _ptr(ws), nbytes, _stream(dev.index)))
         ctx.save_for_backward(queries, rows, ids, scores, saved)
         ctx.scales = (scale, teacher_scale)
         return loss
@@ -150,10 +148,11 @@ class _CorpusLoss(torch.autograd.Function):
         dq = torch.empty((b, d), dtype=queries.dtype, device=dev) if ctx.needs_input_grad[0] else None
         dr = torch.empty((n, d), dtype=rows.dtype, device=dev) if ctx.needs_input_grad[1] else None
         dloss = dloss.contiguous()
-        ws = _workspace(L.cgv_corpus_loss_grad_workspace(b, n, d, k, code), dev)
+        nbytes = L.cgv_corpus_loss_grad_workspace(b, n, d, k, code)
+        ws = _workspace(nbytes, dev)
         _check(L.cgv_corpus_loss_grad_dev(dev.index, _ptr(queries), _row_stride(queries), _ptr(rows), _row_stride(rows), code, b, n, d, _ptr(ids),
-                                          _ptr(scores), k, *ctx.scales, _ptr(saved), _ptr(dloss), _ptr(dq), _ptr(dr), _ptr(ws), ws.numel(),
-                                          _stream(dev)))
+                                          _ptr(scores), k, *ctx.scales, _ptr(saved), _ptr(dloss), _ptr(dq), _ptr(dr), _ptr(ws), nbytes,
+                                          _stream(dev.index)))
         return dq, dr, None, None, None, None
 
 

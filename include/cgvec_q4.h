@@ -51,9 +51,12 @@ int cgv_q4_get_row_f32(cgv_q4_index* h, uint64_t id, float* out_host);
 /* Scores of m queries against all rows: out [m][count] f32. A query with a NaN or Inf gets NaN for every row.
  * _f32: HOST queries [m][dim] and output, returns when done. _dev: DEVICE queries of type query_dtype (CGV_DTYPE_F32 / BF16 /
  * FP16), contiguous [m][dim]; enqueued on `stream`, no synchronisation, nothing allocated. m == 0 or an empty index: nothing is
- * written. */
+ * written. The workspace (DEVICE, cgv_q4_scores_workspace bytes, 0 for one query of ordinary size; aligned to 256) belongs to one
+ * call until its work on the stream is done. */
 int cgv_q4_scores_f32(cgv_q4_index* h, const float* queries_host, uint32_t m, float* out_host);
-int cgv_q4_scores_dev(cgv_q4_index* h, const void* queries_dev, int query_dtype, uint32_t m, float* out_dev, void* stream);
+size_t cgv_q4_scores_workspace(const cgv_q4_index* h, int query_dtype, uint32_t m);
+int cgv_q4_scores_dev(cgv_q4_index* h, const void* queries_dev, int query_dtype, uint32_t m, float* out_dev, void* workspace_dev,
+                      size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
