@@ -16,6 +16,8 @@
 // (the three left out are below 2^-24 of it), added from the smallest up in the same f32 accumulators: six passes of bf16 MFMA run
 // at 2.5 / 6 = 0.42 PFLOP/s, the f32 MFMA at 0.16.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 namespace cgv_gemm {
@@ -57,7 +59,7 @@ enum Epilogue { EPI_LSE, EPI_G, EPI_DQ, EPI_DR };
 struct Args {
     Operand a, b;
     uint32_t nseg, sa[MAX_SEG], sb[MAX_SEG];      // plane pairs
-    uint32_t ksteps, kvalid;                      // stages of 64; k-rows of `a` that exist (columns form)
+    uint32_t ksteps, kvalid;                      // stages of 64; elements of K that `a` holds
     uint32_t tm, tn;                              // tiles of M and N
     uint32_t splits, blocks;                      // shares of the long axis; workgroups
     // epilogues
@@ -67,7 +69,8 @@ struct Args {
     const uint32_t* anchor;                       // LSE: [n] corpus row left out of the sum, 0xffffffff for none
     float2* part;                                 // LSE: [splits * WM][part_ld] (maximum, sum)
     uint32_t part_ld;
-    const float *coef, *lse2;                     // G: [n] factor and log2 of the softmax sum
+    const float* coef;                            // G: [n] factor
+    const float2* lse2;                           // G: [n] log2 of the softmax sum, its f32 and what that leaves
     char* out;                                    // G, DR, DQ
     uint64_t out_pitch, out_plane;                // bytes
     uint32_t accumulate, vec_out;                 // DQ: add to what is there; DR: 16-byte stores possible
@@ -80,8 +83,17 @@ struct Shape {
     static constexpr int TM = BM / WM, TN = BN / WN, MB = TM / 32, NB = TN / 32;
     static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
     static constexpr int XPOSE = 4096;            // per wave: a 32 x 64 piece of 16-bit results on its way out
-    static constexpr int lds_bytes(bool xpose) { return 2 * STAGE + (xpose ? NW * XPOSE : 0); }
+    // stages in LDS: as many as fit, six at most; all but one of them are loading or waiting
+    static constexpr int stages(bool xpose) {
+        const int n = (160 * 1024 - (xpose ? NW * XPOSE : 0)) / STAGE;
+        return n < 6 ? n : 6;
+    }
+    static constexpr int lds_bytes(bool xpose) { return stages(xpose) * STAGE + (xpose ? NW * XPOSE : 0); }
 };
+
+// swizzle of a row's eight 16-byte pieces: 16 consecutive rows put the same piece at 16 different places of the 256 bytes that the
+// 64 banks hold (row & 7 instead repeats after eight: half of the reads' cycles were conflicts)
+__device__ inline uint32_t row_swz(uint32_t row) { return (row >> 1) & 7u; }
 
 // swizzle of the 32-byte segments of k-row k in the columns form: four k-rows of one read lie in different banks
 template <int W>
@@ -94,19 +106,20 @@ template <bool T, int W, int NW>
 struct Loader {
     static constexpr int I = W / 8 / NW;          // 1-KiB instructions of a wave
     uint32_t voff[I];
-    // first = first row / column of the tile; krows: k-rows that exist from the stage's first on (columns form)
-    __device__ void place(const Operand& o, uint32_t first, int wave, int lane, uint32_t krows) {
+    // first = first row / column of the tile; elems: elements of K that exist from the stage's first on, 64 but for the last stage.
+    // Rows form: the missing ones are read as the row's last eight (the other operand holds zeros there); columns form: as the last k-row
+    __device__ void place(const Operand& o, uint32_t first, int wave, int lane, uint32_t elems) {
 #pragma unroll
         for (int i = 0; i < I; ++i) {
             const uint32_t u = (uint32_t)(wave * I + i);
             if (!T) {
-                const uint32_t row = u * 8 + (lane >> 3), chunk = (uint32_t)(lane & 7) ^ (row & 7u);
-                voff[i] = (min(first + row, o.limit - 1) - first) * (uint32_t)o.pitch + chunk * 16;
+                const uint32_t row = u * 8 + (lane >> 3), chunk = (uint32_t)(lane & 7) ^ row_swz(row);
+                voff[i] = (min(first + row, o.limit - 1) - first) * (uint32_t)o.pitch + min(chunk * 8, elems - 8) * 2;
             } else {
                 constexpr uint32_t RB = W * 2, LPR = RB / 16;           // bytes of a k-row, lanes of one
                 const uint32_t k = u * (1024 / RB) + lane / LPR, c = lane % LPR;
                 const uint32_t seg = (c >> 1) ^ seg_swz<W>(k), col = seg * 16 + (c & 1) * 8;
-                voff[i] = min(k, krows - 1) * (uint32_t)o.pitch + (min(first + col, o.limit - 8) - first) * 2;
+                voff[i] = min(k, elems - 1) * (uint32_t)o.pitch + (min(first + col, o.limit - 8) - first) * 2;
             }
         }
     }
@@ -123,7 +136,7 @@ template <bool T, int W>
 __device__ inline s16x8 fragment(const char* lds, uint32_t at, int kk, int lane) {
     if (!T) {
         const uint32_t row = at + (lane & 31);
-        return *(const s16x8*)(lds + row * 128 + (((uint32_t)(kk * 2 + (lane >> 5)) ^ (row & 7u)) << 4));
+        return *(const s16x8*)(lds + row * 128 + (((uint32_t)(kk * 2 + (lane >> 5)) ^ row_swz(lane & 31)) << 4));
     }
     constexpr uint32_t RB = W * 2;
     const uint32_t k = (uint32_t)kk * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2);
@@ -144,6 +157,7 @@ template <int DT, class S, bool TA, bool TB, int EPI>
 static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
 #if defined(__HIP_DEVICE_COMPILE__)   // the host pass only needs the launch stub
     extern __shared__ __attribute__((aligned(1024))) char smem[];
+    constexpr int NST = S::stages(EPI == EPI_G || EPI == EPI_DR);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % S::WM, wn = wave / S::WM;
     const uint32_t unit = unit_of(blockIdx.x, g.blocks);
@@ -182,71 +196,155 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
     const char *abase = nullptr, *bbase = nullptr;    // of the tile, plane 0, k = k0
     auto enter = [&](uint32_t i) {
         tile_at(i);
-        la.place(g.a, mt * S::BM, wave, lane, 64);
         lb.place(g.b, nt * S::BN, wave, lane, 64);
         abase = g.a.p + (TA ? (uint64_t)mt * S::BM * 2 : (uint64_t)mt * S::BM * g.a.pitch);
         bbase = g.b.p + (TB ? (uint64_t)nt * S::BN * 2 : (uint64_t)nt * S::BN * g.b.pitch);
     };
-    auto issue = [&](uint32_t seg, uint32_t ks, int buf) {
-        char* l = smem + buf * S::STAGE;
-        const uint64_t k = k0 + ks;
-        if (TA && EPI == EPI_DQ && (k + 1) * BK > g.kvalid) la.place(g.a, mt * S::BM, wave, lane, (uint32_t)(g.kvalid - k * BK));
-        const char* a = abase + g.sa[seg] * g.a.plane;
-        const char* b = bbase + g.sb[seg] * g.b.plane;
-        if (TA) la.issue(a + k * BK * g.a.pitch, 0, l, wave);
-        else la.issue(a, (uint32_t)k * 128, l, wave);
-        if (TB) lb.issue(b + k * BK * g.b.pitch, 0, l + S::A_BYTES, wave);
-        else lb.issue(b, (uint32_t)k * 128, l + S::A_BYTES, wave);
-        if (TA && EPI == EPI_DQ && (k + 1) * BK > g.kvalid) la.place(g.a, mt * S::BM, wave, lane, 64);
+    // The load side runs ahead of the products, across plane pairs and tiles. prepare() finds out where the next stage comes from: the
+    // next 64 elements of the same run of stages, but for a run's ends. Behind the last stage the last one is loaded again: nobody
+    // reads it, and the number of loads on the way is always the same.
+    uint32_t li = 0, lseg = 0, left = 0;              // tile and plane pair of the next run; stages left in this one
+    const char *pa = nullptr, *pb = nullptr;
+    uint32_t sa = 0, sb = 0;
+    bool clamped = false, part = false;               // the run's last stage is a partial one: is, is still to come
+    const uint64_t step_a = TA ? (uint64_t)BK * g.a.pitch : 0, step_b = TB ? (uint64_t)BK * g.b.pitch : 0;
+    auto advance = [&]() {
+        if (TA) pa += step_a;
+        else sa += BK * 2;
+        if (TB) pb += step_b;
+        else sb += BK * 2;
+    };
+    const uint32_t rest = (uint32_t)(g.kvalid % BK);
+    const bool ends_part = EPI != EPI_DR && rest && (k0 + ksteps) * (uint64_t)BK > g.kvalid;
+    auto new_run = [&]() {
+        if (part) {
+            advance();
+            la.place(g.a, mt * S::BM, wave, lane, rest);
+            clamped = true;
+            part = false;
+            return;
+        }
+        if (li == tiles) return;
+        if (lseg == 0) enter(li);
+        const uint32_t full = ends_part ? ksteps - 1 : ksteps;
+        if (lseg == 0 || clamped) la.place(g.a, mt * S::BM, wave, lane, full ? BK : rest);
+        clamped = full == 0;
+        part = ends_part && full;
+        pa = abase + g.sa[lseg] * g.a.plane + k0 * step_a;
+        pb = bbase + g.sb[lseg] * g.b.plane + k0 * step_b;
+        sa = TA ? 0 : k0 * BK * 2;
+        sb = TB ? 0 : k0 * BK * 2;
+        left = full ? full - 1 : 0;
+        if (++lseg == g.nseg) lseg = 0, ++li;
+    };
+    auto prepare = [&]() {
+        if (left) {
+            --left;
+            advance();
+        } else {
+            new_run();
+        }
+    };
+    auto issue = [&](int slot) {
+        char* l = smem + slot * S::STAGE;
+        la.issue(pa, sa, l, wave);
+        lb.issue(pb, sb, l + S::A_BYTES, wave);
     };
 
     float run_m[S::NB], run_s[S::NB];                 // LSE: per query of the lane, over the corpus rows of the lane
     if (EPI == EPI_LSE)
         for (int nb = 0; nb < S::NB; ++nb) run_m[nb] = -INFINITY, run_s[nb] = 0.0f;
 
-    int buf = 0;
+    s16x8 fa0[S::MB], fb0[S::NB], fa1[S::MB], fb1[S::NB];
+    f32x16 acc[S::MB][S::NB];
+    auto read = [&](s16x8(&fa)[S::MB], s16x8(&fb)[S::NB], int buf, int kk) {
+        const char* as = smem + buf * S::STAGE;
+#pragma unroll
+        for (int nb = 0; nb < S::NB; ++nb) fb[nb] = fragment<TB, S::BN>(as + S::A_BYTES, (uint32_t)(wn * S::TN + nb * 32), kk, lane);
+#pragma unroll
+        for (int mb = 0; mb < S::MB; ++mb) fa[mb] = fragment<TA, S::BM>(as, (uint32_t)(wm * S::TM + mb * 32), kk, lane);
+    };
+    auto products = [&](s16x8(&fa)[S::MB], s16x8(&fb)[S::NB]) {
+#pragma unroll
+        for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+            for (int nb = 0; nb < S::NB; ++nb) acc[mb][nb] = mma<DT>(fa[mb], fb[nb], acc[mb][nb]);
+    };
+    constexpr int WAIT = (NST - 2) * (decltype(la)::I + decltype(lb)::I);   // loads of the stages behind the next one
+    auto stage_ready = [&]() {
+        // this wave's part of the next stage has landed, its reads of this one are done
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(WAIT) : "memory");
+        __builtin_amdgcn_s_barrier();                                 // everybody's: the next stage can be read, this one overwritten
+        asm volatile("" ::: "memory");
+    };
+
+    constexpr int PRODUCTS = S::MB * S::NB, READS = S::MB * (TA ? 2 : 1) + S::NB * (TB ? 2 : 1);
+    // the order of a phase: behind each of the first matrix instructions come a few reads of the next fragments, then the loads
+    auto interleave = [&](int loads) {
+        constexpr int each = PRODUCTS > 2 ? (READS + PRODUCTS - 3) / (PRODUCTS - 2) : READS;
+        const int per = (loads + PRODUCTS - 1) / PRODUCTS;
+#pragma unroll
+        for (int x = 0; x < PRODUCTS; ++x) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, each, 0);
+            if (per == 1) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+            if (per == 2) __builtin_amdgcn_sched_group_barrier(0x010, 2, 0);
+            if (per > 2) __builtin_amdgcn_sched_group_barrier(0x010, 5, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    if (!ksteps) tiles = EPI == EPI_DQ ? tiles : 0;
+    int buf = 0;                                      // slot of the stage at work; the one before it is where the next load goes
     if (tiles && ksteps) {
-        enter(0);
-        issue(0, 0, 0);
+        for (int x = 0; x < NST - 1; ++x) {
+            prepare();
+            issue(x);
+        }
+        prepare();
+        stage_ready();
+        issue(NST - 1);
+        read(fa0, fb0, 0, 0);
     }
+    uint32_t nmt = mt, nnt = nt;
     for (uint32_t i = 0; i < tiles; ++i) {
-        f32x16 acc[S::MB][S::NB];
+        // (mt, nt) belong to the load side, which may already be in the next tile
+        if (EPI == EPI_LSE || EPI == EPI_G) {
+            nmt = split + i * g.splits;
+        } else if (EPI == EPI_DR) {
+            const uint32_t t = unit + i * g.blocks;
+            nmt = t % g.tm;
+            nnt = t / g.tm;
+        }
+        const uint32_t my_mt = nmt, my_nt = nnt, stages = g.nseg * ksteps;
 #pragma unroll
         for (int mb = 0; mb < S::MB; ++mb)
 #pragma unroll
             for (int nb = 0; nb < S::NB; ++nb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[mb][nb][r] = 0.0f;
-        const uint32_t my_mt = mt, my_nt = nt;
-        for (uint32_t seg = 0; seg < g.nseg; ++seg)
-            for (uint32_t ks = 0; ks < ksteps; ++ks) {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's part of the stage has landed
-                __builtin_amdgcn_s_barrier();                      // everybody's has, and the other buffer is free
-                asm volatile("" ::: "memory");
-                if (ks + 1 < ksteps) {
-                    issue(seg, ks + 1, buf ^ 1);
-                } else if (seg + 1 < g.nseg) {
-                    issue(seg + 1, 0, buf ^ 1);
-                } else if (i + 1 < tiles) {
-                    enter(i + 1);
-                    issue(0, 0, buf ^ 1);
-                }
-                const char* as = smem + buf * S::STAGE;
-                const char* bs = as + S::A_BYTES;
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    s16x8 fa[S::MB], fb[S::NB];
-#pragma unroll
-                    for (int mb = 0; mb < S::MB; ++mb) fa[mb] = fragment<TA, S::BM>(as, (uint32_t)(wm * S::TM + mb * 32), kk, lane);
-#pragma unroll
-                    for (int nb = 0; nb < S::NB; ++nb) fb[nb] = fragment<TB, S::BN>(bs, (uint32_t)(wn * S::TN + nb * 32), kk, lane);
-#pragma unroll
-                    for (int mb = 0; mb < S::MB; ++mb)
-#pragma unroll
-                        for (int nb = 0; nb < S::NB; ++nb) acc[mb][nb] = mma<DT>(fa[mb], fb[nb], acc[mb][nb]);
-                }
-                buf ^= 1;
-            }
+        for (uint32_t s = 0; s < stages; ++s) {
+            // fragments of the next 16 elements of K are on their way from LDS while the products of these run; the stage changes
+            // behind the reads of its last 16, whose products stand ready on the other side of the barrier
+            __builtin_amdgcn_sched_barrier(0);
+            read(fa1, fb1, buf, 1);
+            products(fa0, fb0);
+            interleave(0);
+            read(fa0, fb0, buf, 2);
+            products(fa1, fb1);
+            interleave(0);
+            read(fa1, fb1, buf, 3);
+            products(fa0, fb0);
+            interleave(0);
+            prepare();
+            stage_ready();
+            const int next = NST == 2 ? buf ^ 1 : buf + 1 == NST ? 0 : buf + 1;
+            read(fa0, fb0, next, 0);
+            issue(buf);
+            buf = next;
+            products(fa1, fb1);
+            interleave(decltype(la)::I + decltype(lb)::I);
+        }
 
         // ---- epilogue of the tile
         const uint32_t m0 = my_mt * S::BM + wm * S::TM, n0 = my_nt * S::BN + wn * S::TN;
@@ -259,40 +357,61 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
                 // corpus row that this query leaves out, as a row of the wave's part of the tile
                 const uint32_t skip = q < g.n_valid ? g.anchor[q] - (uint32_t)(g.row0 + m0) : 0xffffffffu;
                 const bool any = __ballot(skip < (uint32_t)S::TM) != 0;
-                float mx = -INFINITY;
+                if (edge || any) {                     // rows beyond the corpus, the row left out
+                    float mx = -INFINITY;
 #pragma unroll
-                for (int mb = 0; mb < S::MB; ++mb)
+                    for (int mb = 0; mb < S::MB; ++mb)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        float t = acc[mb][nb][r] * g.scale2;
-                        if (edge || any) {
+                        for (int r = 0; r < 16; ++r) {
                             const uint32_t m = mb * 32 + (r & 3) + 8 * (r >> 2) + half4;
-                            if (m == skip || m0 + m >= g.m_valid) t = -INFINITY;
+                            const float t = m == skip || m0 + m >= g.m_valid ? -INFINITY : acc[mb][nb][r] * g.scale2;
+                            acc[mb][nb][r] = t;
+                            mx = fmaxf(mx, t);
                         }
-                        acc[mb][nb][r] = t;
-                        mx = fmaxf(mx, t);
+                    const float nm = fmaxf(run_m[nb], mx), base = nm == -INFINITY ? 0.0f : nm;
+                    float s = run_s[nb] * __builtin_amdgcn_exp2f(run_m[nb] - base);
+#pragma unroll
+                    for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(acc[mb][nb][r] - base);
+                    run_m[nb] = nm;
+                    run_s[nb] = s;
+                } else {
+                    float ext = acc[0][nb][0];
+                    if (g.scale2 >= 0.0f) {
+#pragma unroll
+                        for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) ext = fmaxf(ext, acc[mb][nb][r]);
+                    } else {
+#pragma unroll
+                        for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) ext = fminf(ext, acc[mb][nb][r]);
                     }
-                const float nm = fmaxf(run_m[nb], mx), base = nm == -INFINITY ? 0.0f : nm;
-                float s = run_s[nb] * __builtin_amdgcn_exp2f(run_m[nb] - base);
+                    const float nm = fmaxf(run_m[nb], ext * g.scale2), base = nm == -INFINITY ? 0.0f : nm;
+                    float s = run_s[nb] * __builtin_amdgcn_exp2f(run_m[nb] - base);
 #pragma unroll
-                for (int mb = 0; mb < S::MB; ++mb)
+                    for (int mb = 0; mb < S::MB; ++mb)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(acc[mb][nb][r] - base);
-                run_m[nb] = nm;
-                run_s[nb] = s;
+                        for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[mb][nb][r], g.scale2, -base));
+                    run_m[nb] = nm;
+                    run_s[nb] = s;
+                }
             }
         } else if (EPI == EPI_G) {
-            char* xp = smem + 2 * S::STAGE + wave * S::XPOSE;
+            char* xp = smem + NST * S::STAGE + wave * S::XPOSE;
 #pragma unroll
             for (int nb = 0; nb < S::NB; ++nb) {
                 const uint32_t q = n0 + nb * 32 + (lane & 31);
-                const float c = q < g.n_valid ? g.coef[q] * *g.unscale : 0.0f, l2 = q < g.n_valid ? g.lse2[q] : 0.0f;
+                const float c = q < g.n_valid ? g.coef[q] * *g.unscale : 0.0f;
+                const float2 l2 = q < g.n_valid ? g.lse2[q] : make_float2(0.0f, 0.0f);
 #pragma unroll
                 for (int mb = 0; mb < S::MB; ++mb)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const uint32_t m = m0 + mb * 32 + (r & 3) + 8 * (r >> 2) + half4;
-                        const float v = c * __builtin_amdgcn_exp2f(acc[mb][nb][r] * g.scale2 - l2);
+                        const float v = c * __builtin_amdgcn_exp2f(fmaf(acc[mb][nb][r], g.scale2, -l2.x) - l2.y);
                         acc[mb][nb][r] = c == 0.0f || m >= g.m_valid ? 0.0f : v;
                     }
             }
@@ -316,14 +435,14 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
                                         if (DT == cgv::DT_F32) acc[mp + mi][nb][r4 * 4 + x] = v - cgv::bf16_to_f32(h[x]);   // what the next plane holds
                                     }
                                 }
-                                const uint32_t n = lane & 31, chunk = (uint32_t)(mi * 4 + r4) ^ (n & 7u);
+                                const uint32_t n = lane & 31, chunk = (uint32_t)(mi * 4 + r4) ^ row_swz(n);
                                 *(uint2*)(xp + n * 128 + chunk * 16 + half4 * 2) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
                             }
                         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                         __builtin_amdgcn_wave_barrier();
 #pragma unroll
                         for (int p = 0; p < 4; ++p) {
-                            const uint32_t n = p * 8 + (lane >> 3), chunk = (uint32_t)(lane & 7) ^ (n & 7u);
+                            const uint32_t n = p * 8 + (lane >> 3), chunk = (uint32_t)(lane & 7) ^ row_swz(n);
                             const uint4 v = *(const uint4*)(xp + n * 128 + chunk * 16);
                             const uint32_t q = n0 + nb * 32 + n;
                             if (q < g.part_ld)
@@ -355,7 +474,7 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
             }
         } else {   // EPI_DR
             const float u = *g.unscale;
-            char* xp = smem + 2 * S::STAGE + wave * S::XPOSE;
+            char* xp = smem + NST * S::STAGE + wave * S::XPOSE;
 #pragma unroll
             for (int nb = 0; nb < S::NB; ++nb) {
                 if (DT != cgv::DT_F32 && g.vec_out) {
@@ -371,14 +490,14 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
                                     const float v = acc[mp + mi][nb][r4 * 4 + x] * u;
                                     h[x] = DT == cgv::DT_FP16 ? cgv::f32_to_f16_rne(v) : cgv::f32_to_bf16_rne(v);
                                 }
-                                const uint32_t n = lane & 31, chunk = (uint32_t)(mi * 4 + r4) ^ (n & 7u);
+                                const uint32_t n = lane & 31, chunk = (uint32_t)(mi * 4 + r4) ^ row_swz(n);
                                 *(uint2*)(xp + n * 128 + chunk * 16 + half4 * 2) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
                             }
                         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                         __builtin_amdgcn_wave_barrier();
 #pragma unroll
                         for (int p = 0; p < 4; ++p) {
-                            const uint32_t n = p * 8 + (lane >> 3), chunk = (uint32_t)(lane & 7) ^ (n & 7u);
+                            const uint32_t n = p * 8 + (lane >> 3), chunk = (uint32_t)(lane & 7) ^ row_swz(n);
                             const uint4 v = *(const uint4*)(xp + n * 128 + chunk * 16);
                             const uint32_t row = n0 + nb * 32 + n, m = m0 + mp * 32 + (lane & 7) * 8;
                             if (row < g.n_valid && m < g.m_valid) *(uint4*)(g.out + row * g.out_pitch + m * 2) = v;   // m_valid: a multiple of 8
@@ -412,6 +531,7 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
             }
         }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in LDS behind the workgroup's end
     if (EPI == EPI_LSE) {
         const uint32_t n0 = nt * S::BN + wn * S::TN;
 #pragma unroll

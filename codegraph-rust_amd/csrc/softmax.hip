@@ -23,7 +23,7 @@ using namespace cgv_gemm;
 
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
 constexpr uint32_t MAX_K = 256, NONE = 0xffffffffu;
 constexpr uint32_t CUS = 256;                                  // workgroups of one per CU that fill the card
 constexpr uint64_t PIECE_BYTES = 128ull << 20;                 // of G and of copied corpus rows: stays in the last-level cache
@@ -31,7 +31,7 @@ constexpr uint64_t PIECE_BYTES = 128ull << 20;                 // of G and of co
 // ---- weights of a query's list: one wave, entry j at lane j % 64, slot j / 64 ------------------------------------------------
 struct List {
     uint32_t id[4];       // NONE: weight 0
-    float logp[4], p[4];
+    double logp[4], p[4];
     uint32_t anchor;      // index of the first heaviest entry
     bool has;
 };
@@ -39,39 +39,43 @@ __device__ inline float wave_max(float v) {
     for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
     return v;
 }
-__device__ inline float wave_sum(float v) {
+template <class T>
+__device__ inline T wave_sum(T v) {
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
 __device__ inline List read_list(const int64_t* ids, const float* ts, uint64_t i, uint32_t k, uint64_t n_rows, float tscale, int lane) {
     List l;
-    float t[4], mx = -INFINITY;
+    float raw[4], mx = -INFINITY;
     bool any = false;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
         const uint32_t j = s * 64 + lane;
         l.id[s] = NONE;
-        t[s] = -INFINITY;
+        raw[s] = -INFINITY;
         if (j < k) {
             const int64_t id = ids[i * k + j];
-            const float raw = ts ? ts[i * k + j] : 0.0f;
-            if (id >= 0 && (uint64_t)id < n_rows && raw != -INFINITY) {
+            const float v = ts ? ts[i * k + j] : 0.0f;
+            if (id >= 0 && (uint64_t)id < n_rows && v != -INFINITY) {
                 l.id[s] = (uint32_t)id;
-                t[s] = ts ? raw * tscale : 0.0f;
+                raw[s] = v;
                 any = true;
             }
         }
-        mx = fmaxf(mx, t[s]);
+        // a negative factor turns the order round; the list's weights are few: 64 bits
+        mx = fmaxf(mx, l.id[s] == NONE ? -INFINITY : tscale < 0.0f ? -raw[s] : raw[s]);
     }
     l.has = __ballot(any) != 0;
     mx = wave_max(mx);
-    float z = 0.0f;
+    const double top = tscale < 0.0f ? -(double)mx : (double)mx;
+    double z = 0.0;
     uint32_t first = NONE;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        l.p[s] = l.id[s] == NONE ? 0.0f : expf(t[s] - mx);
+        l.logp[s] = l.id[s] == NONE ? 0.0 : (raw[s] - top) * (double)(ts ? tscale : 0.0f);
+        l.p[s] = l.id[s] == NONE ? 0.0 : exp(l.logp[s]);
         z += l.p[s];
-        const uint64_t eq = __ballot(l.id[s] != NONE && t[s] == mx);
+        const uint64_t eq = __ballot(l.id[s] != NONE && (double)raw[s] == top);
         if (first == NONE && eq) first = s * 64 + __ffsll((unsigned long long)eq) - 1;
     }
     if (first == NONE)
@@ -80,15 +84,13 @@ __device__ inline List read_list(const int64_t* ids, const float* ts, uint64_t i
             if (first == NONE && some) first = s * 64 + __ffsll((unsigned long long)some) - 1;
         }
     z = wave_sum(z);
-    const float lz = logf(z);
+    const double lz = log(z);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
         if (l.id[s] != NONE) {
             l.p[s] /= z;
-            l.logp[s] = t[s] - mx - lz;
-            if (l.p[s] == 0.0f) l.id[s] = NONE;     // underflow: no weight, and no 0 * inf below
-        } else {
-            l.logp[s] = 0.0f;
+            l.logp[s] -= lz;
+            if (l.p[s] == 0.0) l.id[s] = NONE;      // underflow: no weight, and no 0 * inf below
         }
     }
     l.anchor = first;
@@ -119,7 +121,7 @@ struct Problem {
     uint64_t q_stride, r_stride, n_rows;
     const int64_t* ids;
     const float* tscores;
-    float* saved;             // [b][k + 2]: lse, tail, scores of the list
+    double* saved;            // [b][k + 2]: lse, tail, scores of the list
     uint32_t b, bp, dim, dp, k;
     float scale, tscale;
     uint16_t* qws;            // [planes][bp][dp]
@@ -139,16 +141,24 @@ __global__ __launch_bounds__(256) void forward_prep_kernel(Problem P, uint32_t* 
     }
     const List l = read_list(P.ids, P.tscores, i, P.k, P.n_rows, P.tscale, lane);
     copy_row<DT>(l.has ? P.queries : nullptr, (uint64_t)i * P.q_stride, P.dim, P.dp, dst, plane, threadIdx.x, 256);
-    float* sv = P.saved + (uint64_t)i * (P.k + 2);
-    for (uint32_t j = wave; j < P.k; j += 4) {
-        const uint32_t id = pick(l.id, j);
-        float s = 0.0f;
-        if (id != NONE) {
-            for (uint32_t e = lane; e < P.dim; e += 64)
-                s = fmaf(load_elem<DT>(P.queries, (uint64_t)i * P.q_stride + e), load_elem<DT>(P.rows, (uint64_t)id * P.r_stride + e), s);
-            s = wave_sum(s) * P.scale;
+    // the listed rows' scores in 64 bits - a small loss and its gradient are as exact as the anchor's score -, four rows of a wave at a time
+    double* sv = P.saved + (uint64_t)i * (P.k + 2);
+    for (uint32_t j0 = wave; j0 < P.k; j0 += 16) {
+        uint32_t id[4];
+        double s[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) id[x] = j0 + 4 * x < P.k ? pick(l.id, j0 + 4 * x) : NONE;
+        for (uint32_t e = lane; e < P.dim; e += 64) {
+            const double q = load_elem<DT>(P.queries, (uint64_t)i * P.q_stride + e);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (id[x] != NONE) s[x] = fma(q, (double)load_elem<DT>(P.rows, (uint64_t)id[x] * P.r_stride + e), s[x]);
         }
-        if (lane == 0) sv[2 + j] = s;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const double v = wave_sum(s[x]) * (double)P.scale;
+            if (lane == 0 && j0 + 4 * x < P.k) sv[2 + j0 + 4 * x] = v;
+        }
     }
     if (threadIdx.x == 0) anchor[i] = NONE;
     if (l.has && wave == 0) {
@@ -163,9 +173,9 @@ __global__ __launch_bounds__(256) void loss_kernel(Problem P, const float2* __re
     const int lane = threadIdx.x & 63;
     if (i >= P.b) return;
     const List l = read_list(P.ids, P.tscores, i, P.k, P.n_rows, P.tscale, lane);
-    float* sv = P.saved + (uint64_t)i * (P.k + 2);
+    double* sv = P.saved + (uint64_t)i * (P.k + 2);
     if (!l.has) {
-        if (lane == 0) loss[i] = 0.0f, sv[0] = 0.0f, sv[1] = 0.0f;
+        if (lane == 0) loss[i] = 0.0f, sv[0] = 0.0, sv[1] = 0.0;
         return;
     }
     float m = -INFINITY, s = 0.0f;
@@ -177,16 +187,16 @@ __global__ __launch_bounds__(256) void loss_kernel(Problem P, const float2* __re
     }
     const float top = wave_max(m), base = top == -INFINITY ? 0.0f : top;
     s = wave_sum(s * exp2f(m - base));
-    const float sa = sv[2 + l.anchor];
-    const float rest = (base - sa * LOG2E) * LN2 + logf(s);        // log of (the others' sum / the anchor's term)
-    const float tail = rest > 30.0f ? rest : log1pf(expf(rest));
-    float sum = 0.0f;
+    const double sa = sv[2 + l.anchor];
+    const double rest = (double)base * LN2 - sa + log((double)s);       // log of (the others' sum / the anchor's term)
+    const double tail = rest > 40.0 ? rest : log1p(exp(rest));
+    double sum = 0.0;
 #pragma unroll
     for (int x = 0; x < 4; ++x)
         if (l.id[x] != NONE) sum += l.p[x] * (l.logp[x] + (sa - sv[2 + x * 64 + lane]) + tail);
     sum = wave_sum(sum);
     if (lane == 0) {
-        loss[i] = sum;
+        loss[i] = (float)sum;
         sv[0] = sa + tail;
         sv[1] = tail;
     }
@@ -194,11 +204,11 @@ __global__ __launch_bounds__(256) void loss_kernel(Problem P, const float2* __re
 
 // factor and log2 of the softmax sum per query; entries of G on the listed rows; the padded copy of the queries
 template <int DT>
-__global__ __launch_bounds__(256) void backward_prep_kernel(Problem P, const float* __restrict__ dloss, float* __restrict__ coef, float* __restrict__ lse2,
+__global__ __launch_bounds__(256) void backward_prep_kernel(Problem P, const float* __restrict__ dloss, float* __restrict__ coef, float2* __restrict__ lse2,
                                                             uint32_t* __restrict__ has, uint32_t* __restrict__ ent_id, float* __restrict__ ent_val,
                                                             float* __restrict__ mul) {
     __shared__ uint32_t ids[MAX_K];
-    __shared__ float ps[MAX_K];
+    __shared__ double ps[MAX_K];
     const uint32_t i = blockIdx.x, wave = threadIdx.x >> 6;
     const int lane = threadIdx.x & 63;
     const uint64_t plane = (uint64_t)P.bp * P.dp;
@@ -206,16 +216,17 @@ __global__ __launch_bounds__(256) void backward_prep_kernel(Problem P, const flo
     if (i == 0 && threadIdx.x < 2) mul[threadIdx.x] = 1.0f;
     if (i >= P.b) {
         copy_row<DT>(nullptr, 0, P.dim, P.dp, dst, plane, threadIdx.x, 256);
-        if (threadIdx.x == 0) coef[i] = 0.0f, lse2[i] = 0.0f, has[i] = 0;
+        if (threadIdx.x == 0) coef[i] = 0.0f, lse2[i] = make_float2(0.0f, 0.0f), has[i] = 0;
         return;
     }
     const List l = read_list(P.ids, P.tscores, i, P.k, P.n_rows, P.tscale, lane);
     copy_row<DT>(l.has ? P.queries : nullptr, (uint64_t)i * P.q_stride, P.dim, P.dp, dst, plane, threadIdx.x, 256);
-    const float* sv = P.saved + (uint64_t)i * (P.k + 2);
+    const double* sv = P.saved + (uint64_t)i * (P.k + 2);
     const float c = l.has ? dloss[i] * P.scale : 0.0f;
     if (threadIdx.x == 0) {
         coef[i] = c;
-        lse2[i] = l.has ? sv[0] * LOG2E : 0.0f;
+        const double l2 = l.has ? sv[0] * LOG2E : 0.0;
+        lse2[i] = make_float2((float)l2, (float)(l2 - (double)(float)l2));
         has[i] = l.has;
     }
     if (wave == 0)
@@ -228,7 +239,7 @@ __global__ __launch_bounds__(256) void backward_prep_kernel(Problem P, const flo
     const uint32_t j = threadIdx.x, id = ids[j];
     const uint32_t aid = l.has ? ids[l.anchor] : NONE;
     bool first = id != NONE;
-    float same = 0.0f, other = 0.0f;
+    double same = 0.0, other = 0.0;
     for (uint32_t x = 0; x < P.k; ++x) {
         if (ids[x] == id) {
             if (x < j) first = false;
@@ -237,10 +248,10 @@ __global__ __launch_bounds__(256) void backward_prep_kernel(Problem P, const flo
             other += ps[x];
         }
     }
-    float v = 0.0f;
-    if (first) v = id == aid ? expm1f(-sv[1]) + other : expf(sv[2 + j] - sv[0]) - same;
+    double v = 0.0;
+    if (first) v = id == aid ? expm1(-sv[1]) + other : exp(sv[2 + j] - sv[0]) - same;
     ent_id[(uint64_t)i * P.k + j] = first ? id : NONE;
-    ent_val[(uint64_t)i * P.k + j] = v * c;
+    ent_val[(uint64_t)i * P.k + j] = (float)(v * c);
 }
 
 // fp16: the power of two that brings the largest factor to 2^13 .. 2^14, and its inverse
@@ -282,22 +293,64 @@ __global__ __launch_bounds__(256) void patch_kernel(const uint32_t* __restrict__
     }
 }
 
+// corpus rows [n0, n0 + c) into the padded copy: a thread takes eight elements of a row
 template <int DT>
-__global__ __launch_bounds__(256) void copy_rows_kernel(const void* __restrict__ rows, uint64_t stride, uint64_t n0, uint32_t dim, uint32_t dp,
+__global__ __launch_bounds__(256) void copy_rows_kernel(const void* __restrict__ rows, uint64_t stride, uint64_t n0, uint32_t c, uint32_t dim, uint32_t dp,
                                                         uint64_t plane, uint16_t* __restrict__ dst) {
-    copy_row<DT>(rows, (n0 + blockIdx.x) * stride, dim, dp, dst + (uint64_t)blockIdx.x * dp, plane, threadIdx.x, 256);
+    const uint32_t per = dp / 8;
+    const uint64_t t = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t row = t / per;
+    if (row >= c) return;
+    const uint32_t e = (uint32_t)(t - row * per) * 8;
+    const uint64_t at = (n0 + row) * stride + e;
+    uint16_t* o = dst + row * dp + e;
+    if (DT == cgv::DT_F32) {
+        const float* src = (const float*)rows + at;
+        float v[8];
+        if (e + 8 <= dim && ((uintptr_t)src & 15) == 0) {
+            const float4 x = *(const float4*)src, y = *(const float4*)(src + 4);
+            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+        } else {
+            for (int j = 0; j < 8; ++j) v[j] = e + j < dim ? src[j] : 0.0f;
+        }
+        uint16_t p[8][3];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) split3(v[j], p[j]);
+#pragma unroll
+        for (int x = 0; x < 3; ++x) {
+            uint32_t w[4];
+            for (int j = 0; j < 4; ++j) w[j] = p[2 * j][x] | (uint32_t)p[2 * j + 1][x] << 16;
+            *(uint4*)(o + x * plane) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    } else {
+        const uint16_t* src = (const uint16_t*)rows + at;
+        uint32_t w[4];
+        for (int j = 0; j < 4; ++j)
+            w[j] = (e + 2 * j < dim ? src[2 * j] : 0u) | (uint32_t)(e + 2 * j + 1 < dim ? src[2 * j + 1] : 0u) << 16;
+        *(uint4*)o = make_uint4(w[0], w[1], w[2], w[3]);
+    }
 }
 
-// dQ: the shares' partial sums, rounded once
+// dQ: the shares' partial sums, added in a fixed order and rounded once. 64 threads a stretch of 256 elements, four groups of shares
 template <int DT>
 __global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict__ part, uint32_t splits, uint64_t share, uint32_t dim, uint32_t dp,
                                                         const uint32_t* __restrict__ has, const float* __restrict__ mul, void* __restrict__ dq) {
-    const uint32_t i = blockIdx.x;
-    for (uint32_t e = threadIdx.x; e < dim; e += 256) {
-        float s = 0.0f;
-        for (uint32_t x = 0; x < splits; ++x) s += part[x * share + (uint64_t)i * dp + e];
-        store_elem<DT>(dq, (uint64_t)i * dim + e, has[i] ? s * mul[1] : 0.0f);
-    }
+    __shared__ float4 sum[4][64];
+    const uint32_t i = blockIdx.x, t = threadIdx.x & 63, group = threadIdx.x >> 6, e = blockIdx.y * 256 + t * 4;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (e < dp)
+#pragma unroll 4
+        for (uint32_t x = group; x < splits; x += 4) {
+            const float4 v = *(const float4*)(part + x * share + (uint64_t)i * dp + e);
+            s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+        }
+    sum[group][t] = s;
+    __syncthreads();
+    const uint32_t o = threadIdx.x, at = blockIdx.y * 256 + o;
+    if (at >= dim) return;
+    float v = 0.0f;
+    for (int x = 0; x < 4; ++x) v += ((const float*)sum[x])[o];
+    store_elem<DT>(dq, (uint64_t)i * dim + at, has[i] ? v * mul[1] : 0.0f);
 }
 
 template <int DT>
@@ -307,6 +360,7 @@ __global__ void zero_kernel(void* p, uint64_t total) {
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
 
+typedef Shape<64, 64, 1, 2> S64x64;
 typedef Shape<256, 64, 4, 1> S64;
 typedef Shape<256, 128, 4, 2> S128;
 typedef Shape<256, 256, 2, 4> S256;
@@ -314,7 +368,7 @@ typedef Shape<256, 256, 2, 4> S256;
 uint64_t up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
 struct Plan {
-    uint32_t b, bp, dim, dp, k, planes, bn, wm, tn;
+    uint32_t b, bp, dim, dp, k, planes, bm, bn, wm, tn;   // tiles of the scores: corpus rows, queries; wave rows of a tile; tiles of the batch
     bool copy;                     // corpus rows go through a padded copy
     uint64_t n, piece_f, piece_b;  // corpus rows of a piece, forward and backward
     uint32_t parts_per_piece, dq_splits;
@@ -322,9 +376,14 @@ struct Plan {
         bp = (uint32_t)up(std::max<uint64_t>(b_, 1), 64);
         dp = (uint32_t)up(dim_, 64);
         planes = dtype == CGV_DTYPE_F32 ? 3 : 1;
-        copy = dtype == CGV_DTYPE_F32 || dp != dim;
-        bn = bp <= 64 ? 64 : bp <= 128 ? 128 : 256;
-        wm = bn == 256 ? S256::WM : S64::WM;
+        copy = dtype == CGV_DTYPE_F32 || dim % 8 != 0;
+        // the tile width whose padded batch takes the least time: narrower tiles read LDS more often per product
+        const double t256 = up(bp, 256) / 1.0, t128 = up(bp, 128) / 0.8, t64 = up(bp, 64) / 0.55;
+        bn = t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64;
+        bm = 256;
+        // few tiles: small ones on more CUs, with more stages on the way (32 queries x 10 k x 384, f32: 31 -> us)
+        if ((n_ + 255) / 256 * ((bp + bn - 1) / bn) < CUS / 2) bm = bn = 64;
+        wm = bm == 64 ? S64x64::WM : bn == 256 ? S256::WM : S64::WM;
         tn = (bp + bn - 1) / bn;
         const uint64_t rows = up(n_, 256);
         const uint64_t by_copy = copy ? std::max<uint64_t>(256, PIECE_BYTES / ((uint64_t)dp * 2 * planes) / 256 * 256) : rows;
@@ -333,7 +392,7 @@ struct Plan {
         piece_b = std::min(rows, std::min(by_copy, by_g));
         if (piece_b < rows && piece_b > 256 * CUS / 4) piece_b = piece_b / (256 * CUS / 4) * (256 * CUS / 4);
         parts_per_piece = std::max<uint32_t>(1, CUS / tn) * wm;
-        const uint32_t dq_tiles = ((dp + 255) / 256) * tn;
+        const uint32_t dq_tiles = ((dp + bm - 1) / bm) * tn;
         dq_splits = std::max<uint32_t>(1, std::min<uint32_t>((uint32_t)(piece_b / BK), CUS / dq_tiles));
     }
     uint64_t pieces_f() const { return (n + piece_f - 1) / piece_f; }
@@ -345,8 +404,8 @@ struct Plan {
     uint64_t f_rows() const { return f_part() + up(pieces_f() * parts_per_piece * bp * 8, 256); }
     uint64_t f_bytes() const { return f_rows() + r_bytes(piece_f); }
     // backward workspace
-    uint64_t b_coef() const { return q_bytes(); }                       // coef, lse2, has: [bp] each; mul: [2]
-    uint64_t b_ent() const { return b_coef() + up((uint64_t)bp * 12 + 8, 256); }
+    uint64_t b_coef() const { return q_bytes(); }                       // lse2 (two f32), coef, has: [bp] each; mul: [2]
+    uint64_t b_ent() const { return b_coef() + up((uint64_t)bp * 16 + 8, 256); }
     uint64_t b_g() const { return b_ent() + up((uint64_t)b * k * 8, 256); }
     uint64_t b_part() const { return b_g() + up((uint64_t)planes * bp * piece_b * 2, 256); }
     uint64_t b_rows() const { return b_part() + up((uint64_t)dq_splits * bp * dp * 4, 256); }
@@ -376,7 +435,9 @@ int launch_gemm(const Args& a, int device, hipStream_t s) {
     return CGV_OK;
 }
 template <int DT, bool TA, bool TB, int EPI>
-int launch_by_queries(uint32_t bn, const Args& a, int device, hipStream_t s) {
+int launch_by_queries(const Plan& pl, const Args& a, int device, hipStream_t s) {
+    if (pl.bm == 64) return launch_gemm<DT, S64x64, TA, TB, EPI>(a, device, s);
+    const uint32_t bn = pl.bn;
     return bn == 64 ? launch_gemm<DT, S64, TA, TB, EPI>(a, device, s) : bn == 128 ? launch_gemm<DT, S128, TA, TB, EPI>(a, device, s)
                                                               : launch_gemm<DT, S256, TA, TB, EPI>(a, device, s);
 }
@@ -388,14 +449,14 @@ Args score_args(const Plan& pl, const Problem& P, int dtype, const char* rows, u
     a.b = {(const char*)P.qws, (uint64_t)pl.dp * 2, (uint64_t)pl.bp * pl.dp * 2, pl.bp};
     set_segments(a, dtype, false);
     a.ksteps = pl.dp / BK;
-    a.kvalid = pl.dp;
-    a.tm = (c + 255) / 256;
+    a.kvalid = pl.copy ? pl.dp : pl.dim;
+    a.tm = (c + pl.bm - 1) / pl.bm;
     a.tn = pl.tn;
     const uint32_t most = std::max<uint32_t>(1, CUS / pl.tn);
     const uint32_t each = (a.tm + most - 1) / most;
     a.splits = (a.tm + each - 1) / each;
     a.blocks = a.tn * a.splits;
-    a.scale2 = P.scale * LOG2E;
+    a.scale2 = (float)(P.scale * LOG2E);
     a.m_valid = c;
     a.n_valid = pl.b;
     a.part_ld = pl.bp;
@@ -404,7 +465,7 @@ Args score_args(const Plan& pl, const Problem& P, int dtype, const char* rows, u
 
 template <int DT>
 int copy_piece(const Plan& pl, const Problem& P, uint64_t n0, uint32_t c, uint64_t plane_elems, char* dst, hipStream_t s) {
-    hipLaunchKernelGGL((copy_rows_kernel<DT>), dim3(c), dim3(256), 0, s, P.rows, P.r_stride, n0, pl.dim, pl.dp, plane_elems, (uint16_t*)dst);
+    hipLaunchKernelGGL((copy_rows_kernel<DT>), dim3((unsigned)(((uint64_t)c * (pl.dp / 8) + 255) / 256)), dim3(256), 0, s, P.rows, P.r_stride, n0, c, pl.dim, pl.dp, plane_elems, (uint16_t*)dst);
     OPCHK(hipGetLastError());
     return CGV_OK;
 }
@@ -434,7 +495,7 @@ int forward(const Plan& pl, Problem P, int dtype, float* loss, char* ws, hipStre
         a.anchor = anchor;
         a.part = part + (uint64_t)parts * pl.bp;
         parts += a.splits * pl.wm;
-        const int rc = launch_by_queries<DT, false, false, EPI_LSE>(pl.bn, a, P.device, s);
+        const int rc = launch_by_queries<DT, false, false, EPI_LSE>(pl, a, P.device, s);
         if (rc) return rc;
     }
     hipLaunchKernelGGL(loss_kernel, dim3((pl.b + 3) / 4), dim3(256), 0, s, P, (const float2*)part, parts, loss);
@@ -445,9 +506,9 @@ int forward(const Plan& pl, Problem P, int dtype, float* loss, char* ws, hipStre
 template <int DT>
 int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq, void* dr, char* ws, hipStream_t s) {
     P.qws = (uint16_t*)ws;
-    float* coef = (float*)(ws + pl.b_coef());
-    float* lse2 = coef + pl.bp;
-    uint32_t* has = (uint32_t*)(lse2 + pl.bp);
+    float2* lse2 = (float2*)(ws + pl.b_coef());
+    float* coef = (float*)(lse2 + pl.bp);
+    uint32_t* has = (uint32_t*)(coef + pl.bp);
     float* mul = (float*)(has + pl.bp);
     uint32_t* ent_id = (uint32_t*)(ws + pl.b_ent());
     float* ent_val = (float*)(ent_id + (uint64_t)pl.b * pl.k);
@@ -479,19 +540,19 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
         a.out = G;
         a.out_pitch = g_pitch;
         a.out_plane = g_plane;
-        if ((rc = launch_by_queries<DT, false, false, EPI_G>(pl.bn, a, P.device, s))) return rc;
+        if ((rc = launch_by_queries<DT, false, false, EPI_G>(pl, a, P.device, s))) return rc;
         const uint64_t total = (uint64_t)pl.b * pl.k;
         hipLaunchKernelGGL((patch_kernel<DT>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, (const uint32_t*)ent_id, (const float*)ent_val, total,
                            pl.k, n0, c, (const float*)mul, (uint16_t*)G, pl.piece_b, g_plane / 2);
         OPCHK(hipGetLastError());
         if (dq) {
             Args d{};
-            d.a = {rows, pitch, plane, pl.dp};
+            d.a = {rows, pitch, plane, pl.copy ? pl.dp : pl.dim};
             d.b = {G, g_pitch, g_plane, pl.bp};
             set_segments(d, dtype, false);
             d.ksteps = (c + BK - 1) / BK;
             d.kvalid = c;
-            d.tm = (pl.dp + 255) / 256;
+            d.tm = (pl.dp + pl.bm - 1) / pl.bm;
             d.tn = pl.tn;
             d.splits = pl.dq_splits;
             d.blocks = d.tm * d.tn * d.splits;
@@ -501,7 +562,7 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             d.out = (char*)part;
             d.out_plane = (uint64_t)pl.bp * pl.dp * 4;
             d.accumulate = n0 > 0;
-            if ((rc = launch_by_queries<DT, true, false, EPI_DQ>(pl.bn, d, P.device, s))) return rc;
+            if ((rc = launch_by_queries<DT, true, false, EPI_DQ>(pl, d, P.device, s))) return rc;
         }
         if (dr) {
             Args d{};
@@ -510,21 +571,23 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             set_segments(d, dtype, false);
             d.ksteps = pl.bp / BK;
             d.kvalid = pl.bp;
-            d.tm = (pl.dim + 255) / 256;
-            d.tn = (c + 255) / 256;
+            const bool big = (uint64_t)((pl.dim + 255) / 256) * ((c + 255) / 256) >= CUS / 2;
+            const uint32_t side = big ? 256 : 64;
+            d.tm = (pl.dim + side - 1) / side;
+            d.tn = (c + side - 1) / side;
             d.splits = 1;
-            d.blocks = (uint32_t)std::min<uint64_t>((uint64_t)d.tm * d.tn, CUS);
+            d.blocks = (uint32_t)std::min<uint64_t>((uint64_t)d.tm * d.tn, big ? CUS : 4 * CUS);
             d.m_valid = pl.dim;
             d.n_valid = c;
             d.out = (char*)dr + n0 * pl.dim * esize(dtype);
             d.out_pitch = (uint64_t)pl.dim * esize(dtype);
             d.vec_out = d.out_pitch % 16 == 0 && (uintptr_t)dr % 16 == 0;
             d.unscale = mul + 1;
-            if ((rc = launch_gemm<DT, S256, true, true, EPI_DR>(d, P.device, s))) return rc;
+            if ((rc = big ? launch_gemm<DT, S256, true, true, EPI_DR>(d, P.device, s) : launch_gemm<DT, S64x64, true, true, EPI_DR>(d, P.device, s))) return rc;
         }
     }
     if (dq) {
-        hipLaunchKernelGGL((finish_dq_kernel<DT>), dim3(pl.b), dim3(256), 0, s, (const float*)part, pl.dq_splits, (uint64_t)pl.bp * pl.dp, pl.dim, pl.dp,
+        hipLaunchKernelGGL((finish_dq_kernel<DT>), dim3(pl.b, (pl.dim + 255) / 256), dim3(256), 0, s, (const float*)part, pl.dq_splits, (uint64_t)pl.bp * pl.dp, pl.dim, pl.dp,
                            (const uint32_t*)has, (const float*)mul, dq);
         OPCHK(hipGetLastError());
     }
@@ -543,8 +606,8 @@ int check_loss(const void* q, uint64_t qs, const void* r, uint64_t rs, int dtype
     if (qs < dim || rs < dim) return fail(CGV_ERR_INVALID_ARG, "a stride is smaller than dim");
     if (!(fabsf(scale) < INFINITY) || !(fabsf(tscale) < INFINITY)) return fail(CGV_ERR_NONFINITE, "scale is not finite");
     if (!r || (b && (!q || !ids || !saved))) return fail(CGV_ERR_INVALID_ARG, "NULL argument");
-    if (dtype != CGV_DTYPE_F32 && dim % 64 == 0 && ((uintptr_t)r % 16 || rs % 8 || rs > (1u << 22)))
-        return fail(CGV_ERR_INVALID_ARG, "rows of 16-bit elements with dim a multiple of 64 are read in place: they must start on 16-byte addresses, at "
+    if (dtype != CGV_DTYPE_F32 && dim % 8 == 0 && ((uintptr_t)r % 16 || rs % 8 || rs > (1u << 22)))
+        return fail(CGV_ERR_INVALID_ARG, "rows of 16-bit elements with dim a multiple of 8 are read in place: they must start on 16-byte addresses, at "
                                          "most 2^22 elements apart");
     return CGV_OK;
 }
@@ -565,7 +628,7 @@ size_t cgv_corpus_loss_grad_workspace(uint64_t b, uint64_t n_rows, uint32_t dim,
 
 int cgv_corpus_loss_dev(int device_id, const void* queries_dev, uint64_t query_stride, const void* rows_dev, uint64_t row_stride, int dtype, uint64_t b,
                         uint64_t n_rows, uint32_t dim, const int64_t* ids_dev, const float* teacher_scores_dev, uint32_t k, float scale,
-                        float teacher_scale, float* loss_dev, float* saved_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
+                        float teacher_scale, float* loss_dev, double* saved_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
     return guarded([&]() -> int {
         int rc = check_loss(queries_dev, query_stride, rows_dev, row_stride, dtype, b, n_rows, dim, ids_dev, k, scale, teacher_scale, saved_dev);
         if (rc) return rc;
@@ -585,7 +648,7 @@ int cgv_corpus_loss_dev(int device_id, const void* queries_dev, uint64_t query_s
 
 int cgv_corpus_loss_grad_dev(int device_id, const void* queries_dev, uint64_t query_stride, const void* rows_dev, uint64_t row_stride, int dtype,
                              uint64_t b, uint64_t n_rows, uint32_t dim, const int64_t* ids_dev, const float* teacher_scores_dev, uint32_t k,
-                             float scale, float teacher_scale, const float* saved_dev, const float* dloss_dev, void* dqueries_dev, void* drows_dev,
+                             float scale, float teacher_scale, const double* saved_dev, const float* dloss_dev, void* dqueries_dev, void* drows_dev,
                              void* workspace_dev, size_t workspace_bytes, void* stream) {
     return guarded([&]() -> int {
         int rc = check_loss(queries_dev, query_stride, rows_dev, row_stride, dtype, b, n_rows, dim, ids_dev, k, scale, teacher_scale, saved_dev);
@@ -600,7 +663,7 @@ int cgv_corpus_loss_grad_dev(int device_id, const void* queries_dev, uint64_t qu
         DeviceScope dev(device_id);
         OPCHK(dev.enter());
         const hipStream_t s = (hipStream_t)stream;
-        const Problem P{queries_dev, rows_dev, query_stride, row_stride, n_rows, ids_dev, teacher_scores_dev, const_cast<float*>(saved_dev),
+        const Problem P{queries_dev, rows_dev, query_stride, row_stride, n_rows, ids_dev, teacher_scores_dev, const_cast<double*>(saved_dev),
                         pl.b, pl.bp, dim, pl.dp, k, scale, teacher_scale, nullptr, device_id};
         return by_dtype(dtype, [&](auto t) -> int {
             constexpr int DT = decltype(t)::value;

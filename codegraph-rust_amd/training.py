@@ -128,7 +128,7 @@ class _CorpusLoss(torch.autograd.Function):
         n, k = rows.shape[0], ids.shape[1]
         code, dev = _CODES[rows.dtype], rows.device
         loss = torch.empty((b,), dtype=torch.float32, device=dev)
-        saved = torch.empty((b * (k + 2),), dtype=torch.float32, device=dev)
+        saved = torch.empty((b * (k + 2),), dtype=torch.float64, device=dev)
         nbytes = L.cgv_corpus_loss_workspace(b, n, d, k, code)
         ws = _workspace(nbytes, dev)
         _check(L.cgv_corpus_loss_dev(dev.index, _ptr(queries), _row_stride(queries), _ptr(rows), _row_stride(rows), code, b, n, d, _ptr(ids),
@@ -166,7 +166,7 @@ def _corpus_loss(queries, rows, ids, scores, scale, teacher_scale):
         raise _bad(f"query dim {queries.shape[1]} != row dim {rows.shape[1]}", CGV_ERR_DIM_MISMATCH)
     if rows.shape[0] == 0:
         raise _bad("rows must not be empty")
-    if rows.dtype != torch.float32 and rows.shape[1] % 64 == 0 and (rows.data_ptr() % 16 or _row_stride(rows) % 8 or _row_stride(rows) > 1 << 22):
+    if rows.dtype != torch.float32 and rows.shape[1] % 8 == 0 and (rows.data_ptr() % 16 or _row_stride(rows) % 8 or _row_stride(rows) > 1 << 22):
         rows = rows.clone(memory_format=torch.contiguous_format)      # such rows are read in place, 16 bytes at a time
     return _CorpusLoss.apply(queries, rows, ids, scores, float(scale), float(teacher_scale))
 

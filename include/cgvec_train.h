@@ -46,12 +46,12 @@ int cgv_lookup_grad_dev(int device_id, const void* dout_dev, int dtype, const in
  * The b x n_rows scores are never stored: the corpus is scored in tiles and only a running maximum and sum per query are kept; the
  * gradient scores it again, piece by piece.
  * queries [b] rows of dim elements, query_stride elements apart; rows likewise; both of type dtype. ids [b][k] int64,
- * teacher_scores [b][k] f32, loss [b] f32. saved [b * (k + 2)] f32 carries what the gradient needs (the softmax sums, the scores of
+ * teacher_scores [b][k] f32, loss [b] f32. saved [b * (k + 2)] f64 carries what the gradient needs (the softmax sums, the scores of
  * the listed rows). b in 0..=2^24, k in 1..=256, n_rows in 1..2^31 - 1, dim in 1..=8192. */
 size_t cgv_corpus_loss_workspace(uint64_t b, uint64_t n_rows, uint32_t dim, uint32_t k, int dtype);
 int cgv_corpus_loss_dev(int device_id, const void* queries_dev, uint64_t query_stride, const void* rows_dev, uint64_t row_stride, int dtype,
                         uint64_t b, uint64_t n_rows, uint32_t dim, const int64_t* ids_dev, const float* teacher_scores_dev, uint32_t k,
-                        float scale, float teacher_scale, float* loss_dev, float* saved_dev, void* workspace_dev, size_t workspace_bytes,
+                        float scale, float teacher_scale, float* loss_dev, double* saved_dev, void* workspace_dev, size_t workspace_bytes,
                         void* stream);
 
 /* Gradients of sum over i of dloss[i] * loss[i] in the queries and in the corpus rows (either may be NULL: it is not computed), from
@@ -60,7 +60,7 @@ int cgv_corpus_loss_dev(int device_id, const void* queries_dev, uint64_t query_s
 size_t cgv_corpus_loss_grad_workspace(uint64_t b, uint64_t n_rows, uint32_t dim, uint32_t k, int dtype);
 int cgv_corpus_loss_grad_dev(int device_id, const void* queries_dev, uint64_t query_stride, const void* rows_dev, uint64_t row_stride,
                              int dtype, uint64_t b, uint64_t n_rows, uint32_t dim, const int64_t* ids_dev, const float* teacher_scores_dev,
-                             uint32_t k, float scale, float teacher_scale, const float* saved_dev, const float* dloss_dev,
+                             uint32_t k, float scale, float teacher_scale, const double* saved_dev, const float* dloss_dev,
                              void* dqueries_dev, void* drows_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
