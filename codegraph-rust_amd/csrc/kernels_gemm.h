@@ -147,6 +147,11 @@ __device__ inline s16x8 fragment(const char* lds, uint32_t at, int kk, int lane)
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+__device__ inline const char* uniform(const char* p) {
+    const uint64_t v = (uint64_t)p;
+    return (const char*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
 // tile `i` of workgroup `id`: consecutive tiles run on one XCD (the hardware deals workgroups to the 8 XCDs in turn)
 __device__ inline uint32_t unit_of(uint32_t id, uint32_t blocks) {
     const uint32_t x = id & 7u, per = blocks >> 3, extra = blocks & 7u;
@@ -244,6 +249,12 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
         } else {
             new_run();
         }
+        // all of this is the same for every lane; said here, because the compiler loses sight of it
+        left = __builtin_amdgcn_readfirstlane(left);
+        sa = __builtin_amdgcn_readfirstlane(sa);
+        sb = __builtin_amdgcn_readfirstlane(sb);
+        pa = uniform(pa);
+        pb = uniform(pb);
     };
     auto issue = [&](int slot) {
         char* l = smem + slot * S::STAGE;
@@ -255,7 +266,11 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
     if (EPI == EPI_LSE)
         for (int nb = 0; nb < S::NB; ++nb) run_m[nb] = -INFINITY, run_s[nb] = 0.0f;
 
-    s16x8 fa0[S::MB], fb0[S::NB], fa1[S::MB], fb1[S::NB];
+    // A small wave tile has few products per read: it keeps the fragments of two whole stages and reads the next one while it
+    // multiplies this one; a large one keeps those of two times 16 elements of K
+    constexpr bool SMALL = S::MB * S::NB <= 2;
+    constexpr int SETS = SMALL ? 4 : 1;
+    s16x8 fa0[SETS][S::MB], fb0[SETS][S::NB], fa1[SETS][S::MB], fb1[SETS][S::NB];
     f32x16 acc[S::MB][S::NB];
     auto read = [&](s16x8(&fa)[S::MB], s16x8(&fb)[S::NB], int buf, int kk) {
         const char* as = smem + buf * S::STAGE;
@@ -296,6 +311,23 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
 
     if (!ksteps) tiles = EPI == EPI_DQ ? tiles : 0;
     int buf = 0;                                      // slot of the stage at work; the one before it is where the next load goes
+    auto read_stage = [&](s16x8(&fa)[SETS][S::MB], s16x8(&fb)[SETS][S::NB], int slot) {
+#pragma unroll
+        for (int kk = 0; kk < SETS; ++kk) read(fa[kk], fb[kk], slot, kk);
+    };
+    // small wave tiles: a stage's products while the next stage's fragments are read
+    auto step = [&](s16x8(&ca)[SETS][S::MB], s16x8(&cb)[SETS][S::NB], s16x8(&na)[SETS][S::MB], s16x8(&nb)[SETS][S::NB]) {
+        __builtin_amdgcn_sched_barrier(0);
+        prepare();
+        stage_ready();
+        const int next = buf + 1 == NST ? 0 : buf + 1;
+        read_stage(na, nb, next);
+        issue(buf);
+        buf = next;
+#pragma unroll
+        for (int kk = 0; kk < SETS; ++kk) products(ca[kk], cb[kk]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
     if (tiles && ksteps) {
         for (int x = 0; x < NST - 1; ++x) {
             prepare();
@@ -304,7 +336,7 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
         prepare();
         stage_ready();
         issue(NST - 1);
-        read(fa0, fb0, 0, 0);
+        read_stage(fa0, fb0, 0);
     }
     uint32_t nmt = mt, nnt = nt;
     for (uint32_t i = 0; i < tiles; ++i) {
@@ -323,27 +355,45 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
             for (int nb = 0; nb < S::NB; ++nb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[mb][nb][r] = 0.0f;
-        for (uint32_t s = 0; s < stages; ++s) {
-            // fragments of the next 16 elements of K are on their way from LDS while the products of these run; the stage changes
-            // behind the reads of its last 16, whose products stand ready on the other side of the barrier
-            __builtin_amdgcn_sched_barrier(0);
-            read(fa1, fb1, buf, 1);
-            products(fa0, fb0);
-            interleave(0);
-            read(fa0, fb0, buf, 2);
-            products(fa1, fb1);
-            interleave(0);
-            read(fa1, fb1, buf, 3);
-            products(fa0, fb0);
-            interleave(0);
-            prepare();
-            stage_ready();
-            const int next = NST == 2 ? buf ^ 1 : buf + 1 == NST ? 0 : buf + 1;
-            read(fa0, fb0, next, 0);
-            issue(buf);
-            buf = next;
-            products(fa1, fb1);
-            interleave(decltype(la)::I + decltype(lb)::I);
+        if constexpr (SMALL) {
+            uint32_t s = 0;
+            for (; s + 2 <= stages; s += 2) {
+                step(fa0, fb0, fa1, fb1);
+                step(fa1, fb1, fa0, fb0);
+            }
+            if (s < stages) {
+                step(fa0, fb0, fa1, fb1);
+#pragma unroll
+                for (int kk = 0; kk < SETS; ++kk) {
+#pragma unroll
+                    for (int mb = 0; mb < S::MB; ++mb) fa0[kk][mb] = fa1[kk][mb];
+#pragma unroll
+                    for (int nb = 0; nb < S::NB; ++nb) fb0[kk][nb] = fb1[kk][nb];
+                }
+            }
+        } else {
+            for (uint32_t s = 0; s < stages; ++s) {
+                // fragments of the next 16 elements of K are on their way from LDS while the products of these run; the stage changes
+                // behind the reads of its last 16, whose products stand ready on the other side of the barrier
+                __builtin_amdgcn_sched_barrier(0);
+                read(fa1[0], fb1[0], buf, 1);
+                products(fa0[0], fb0[0]);
+                interleave(0);
+                read(fa0[0], fb0[0], buf, 2);
+                products(fa1[0], fb1[0]);
+                interleave(0);
+                read(fa1[0], fb1[0], buf, 3);
+                products(fa0[0], fb0[0]);
+                interleave(0);
+                prepare();
+                stage_ready();
+                const int next = NST == 2 ? buf ^ 1 : buf + 1 == NST ? 0 : buf + 1;
+                read(fa0[0], fb0[0], next, 0);
+                issue(buf);
+                buf = next;
+                products(fa1[0], fb1[0]);
+                interleave(decltype(la)::I + decltype(lb)::I);
+            }
         }
 
         // ---- epilogue of the tile
@@ -407,19 +457,17 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
                 const float c = q < g.n_valid ? g.coef[q] * *g.unscale : 0.0f;
                 const float2 l2 = q < g.n_valid ? g.lse2[q] : make_float2(0.0f, 0.0f);
 #pragma unroll
-                for (int mb = 0; mb < S::MB; ++mb)
+                for (int mp = 0; mp < S::MB; mp += 2) {      // 64 corpus rows x 32 queries at a time, through the wave's own LDS
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const uint32_t m = m0 + mb * 32 + (r & 3) + 8 * (r >> 2) + half4;
-                        const float v = c * __builtin_amdgcn_exp2f(fmaf(acc[mb][nb][r], g.scale2, -l2.x) - l2.y);
-                        acc[mb][nb][r] = c == 0.0f || m >= g.m_valid ? 0.0f : v;
-                    }
-            }
-            for (uint32_t plane = 0; plane < (DT == cgv::DT_F32 ? 3u : 1u); ++plane)
+                    for (int mi = 0; mi < 2; ++mi)
 #pragma unroll
-                for (int nb = 0; nb < S::NB; ++nb)
+                        for (int r = 0; r < 16; ++r) {
+                            const uint32_t m = m0 + (mp + mi) * 32 + (r & 3) + 8 * (r >> 2) + half4;
+                            const float v = c * __builtin_amdgcn_exp2f(fmaf(acc[mp + mi][nb][r], g.scale2, -l2.x) - l2.y);
+                            acc[mp + mi][nb][r] = c == 0.0f || m >= g.m_valid ? 0.0f : v;
+                        }
 #pragma unroll
-                    for (int mp = 0; mp < S::MB; mp += 2) {      // 64 corpus rows x 32 queries at a time, through the wave's own LDS
+                    for (uint32_t plane = 0; plane < (DT == cgv::DT_F32 ? 3u : 1u); ++plane) {
 #pragma unroll
                         for (int mi = 0; mi < 2; ++mi)
 #pragma unroll
@@ -451,6 +499,8 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
                         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                         __builtin_amdgcn_wave_barrier();
                     }
+                }
+            }
         } else if (EPI == EPI_DQ) {
             float* out = (float*)(g.out + split * g.out_plane);
 #pragma unroll

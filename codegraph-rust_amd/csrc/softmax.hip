@@ -26,7 +26,9 @@ namespace {
 constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
 constexpr uint32_t MAX_K = 256, NONE = 0xffffffffu;
 constexpr uint32_t CUS = 256;                                  // workgroups of one per CU that fill the card
-constexpr uint64_t PIECE_BYTES = 128ull << 20;                 // of G and of copied corpus rows: stays in the last-level cache
+// of G, and of copied corpus rows. Each piece costs a round over dQ's partial sums (1024 x 500 k x 768, gradient: 3.05 ms with 128 MiB, 2.99 with
+// 512, 2.97 with 1024); the corpus' gradient needs some 256 tiles a piece, however many queries there are
+constexpr uint64_t PIECE_BYTES = 512ull << 20, PIECE_ROWS = 16384;
 
 // ---- weights of a query's list: one wave, entry j at lane j % 64, slot j / 64 ------------------------------------------------
 struct List {
@@ -387,7 +389,7 @@ struct Plan {
         tn = (bp + bn - 1) / bn;
         const uint64_t rows = up(n_, 256);
         const uint64_t by_copy = copy ? std::max<uint64_t>(256, PIECE_BYTES / ((uint64_t)dp * 2 * planes) / 256 * 256) : rows;
-        const uint64_t by_g = std::max<uint64_t>(256, PIECE_BYTES / ((uint64_t)bp * 2 * planes) / 256 * 256);
+        const uint64_t by_g = std::max<uint64_t>(PIECE_ROWS, PIECE_BYTES / ((uint64_t)bp * 2 * planes) / 256 * 256);
         piece_f = std::min(rows, by_copy);
         piece_b = std::min(rows, std::min(by_copy, by_g));
         if (piece_b < rows && piece_b > 256 * CUS / 4) piece_b = piece_b / (256 * CUS / 4) * (256 * CUS / 4);
@@ -576,7 +578,7 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             d.tm = (pl.dim + side - 1) / side;
             d.tn = (c + side - 1) / side;
             d.splits = 1;
-            d.blocks = (uint32_t)std::min<uint64_t>((uint64_t)d.tm * d.tn, big ? CUS : 4 * CUS);
+            d.blocks = (uint32_t)std::min<uint64_t>((uint64_t)d.tm * d.tn, CUS);
             d.m_valid = pl.dim;
             d.n_valid = c;
             d.out = (char*)dr + n0 * pl.dim * esize(dtype);
