@@ -17,39 +17,58 @@ using namespace cgv_ops;
 namespace {
 
 constexpr uint32_t DIRECT_IDS = 512;
-constexpr uint32_t SORT_THREADS = 256, SORT_STEPS = 8, SORT_BLOCK = SORT_THREADS * SORT_STEPS;   // elements of a workgroup
+constexpr uint32_t SORT_THREADS = 256, SORT_STEPS = 4, SORT_BLOCK = SORT_THREADS * SORT_STEPS;   // elements of a workgroup
 constexpr uint32_t MAX_DIGIT = 11;
+constexpr uint32_t FLIGHT = 4;
 
-// ---- a vector of a row: V elements, 16 bytes or one element ------------------------------------------------------------------
+// ---- a vector of a row: V elements, 16 bytes where rows are so aligned, else 8, 4 or one element -----------------------------
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <int BYTES>
+struct Words { typedef u32x4 type; };
+template <>
+struct Words<8> { typedef u32x2 type; };
+template <>
+struct Words<4> { typedef uint32_t type; };
+template <>
+struct Words<2> { typedef uint16_t type; };
+__device__ inline uint32_t word(u32x4 v, int i) { return v[i]; }
+__device__ inline uint32_t word(u32x2 v, int i) { return v[i & 1]; }
+__device__ inline uint32_t word(uint32_t v, int) { return v; }
+__device__ inline uint32_t word(uint16_t v, int) { return v; }
+__device__ inline void set_word(u32x4& v, int i, uint32_t x) { v[i] = x; }
+__device__ inline void set_word(u32x2& v, int i, uint32_t x) { v[i & 1] = x; }
+__device__ inline void set_word(uint32_t& v, int, uint32_t x) { v = x; }
+__device__ inline void set_word(uint16_t& v, int, uint32_t x) { v = (uint16_t)x; }
+
 template <int DT, int V>
 struct Vec {
+    static constexpr int ES = DT == cgv::DT_F32 ? 4 : 2, N = V * ES < 4 ? 1 : V * ES / 4;   // words
+    typedef typename Words<V * ES>::type Raw;
     float v[V];
     __device__ void zero() {
         for (int i = 0; i < V; ++i) v[i] = 0.0f;
     }
     __device__ void load(const void* p, uint64_t at) {   // at: in elements, a multiple of V
-        if (V == 1) {
-            v[0] = load_elem<DT>(p, at);
-        } else if (DT == cgv::DT_F32) {
-            const float4 t = *(const float4*)((const float*)p + at);
-            v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
-        } else {
-            const uint4 t = *(const uint4*)((const uint16_t*)p + at);
-            const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-            for (int i = 0; i < V; ++i) v[i] = half_to_f32<DT>((uint16_t)(w[(i / 2) & 3] >> (16 * (i & 1))));
+        const Raw r = *(const Raw*)((const char*)p + at * ES);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if (DT == cgv::DT_F32) v[i] = __uint_as_float(word(r, i));
+            else v[i] = half_to_f32<DT>((uint16_t)(word(r, i / 2) >> (16 * (i & 1))));
         }
     }
+    // ONCE: past the caches
+    template <bool ONCE>
     __device__ void store(void* p, uint64_t at) const {
-        if (V == 1) {
-            store_elem<DT>(p, at, v[0]);
-        } else if (DT == cgv::DT_F32) {
-            *(float4*)((float*)p + at) = make_float4(v[0], v[1 % V], v[2 % V], v[3 % V]);
-        } else {
-            uint32_t w[4];
-            for (int i = 0; i < 4; ++i)
-                w[i] = f32_to_half<DT>(v[(2 * i) % V]) | (uint32_t)f32_to_half<DT>(v[(2 * i + 1) % V]) << 16;
-            *(uint4*)((uint16_t*)p + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        Raw r;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (DT == cgv::DT_F32) set_word(r, i, __float_as_uint(v[i]));
+            else set_word(r, i, f32_to_half<DT>(v[2 * i]) | (V > 1 ? (uint32_t)f32_to_half<DT>(v[(2 * i + 1) % V]) << 16 : 0u));
         }
+        Raw* o = (Raw*)((char*)p + at * ES);
+        if (ONCE) __builtin_nontemporal_store(r, o);
+        else *o = r;
     }
     __device__ void add(const Vec& o) {
         for (int i = 0; i < V; ++i) v[i] += o.v[i];
@@ -61,7 +80,7 @@ struct Vec {
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------
 // one thread per vector of the output; VPR vectors a row
-template <int DT, int V>
+template <int DT, int V, bool ONCE>
 __global__ __launch_bounds__(256) void lookup_kernel(const void* __restrict__ table, uint64_t n_rows, uint32_t vpr, uint64_t row_stride,
                                                      const int64_t* __restrict__ ids, uint64_t n_ids, float scale, void* __restrict__ out) {
     const uint64_t base = (uint64_t)blockIdx.x * 256;
@@ -78,11 +97,11 @@ __global__ __launch_bounds__(256) void lookup_kernel(const void* __restrict__ ta
     } else {
         v.zero();
     }
-    v.store(out, (row * vpr + col) * V);
+    v.template store<ONCE>(out, (row * vpr + col) * V);
 }
 
 // ---- gradient, few ids ------------------------------------------------------------------------------------------------------
-template <int DT, int V>
+template <int DT, int V, bool ONCE>
 __global__ __launch_bounds__(256) void grad_direct_kernel(const void* __restrict__ dout, const int64_t* __restrict__ ids, uint32_t n_ids,
                                                           uint64_t n_rows, uint32_t vpr, uint32_t rows_per_block, float scale,
                                                           void* __restrict__ dtable) {
@@ -118,7 +137,7 @@ __global__ __launch_bounds__(256) void grad_direct_kernel(const void* __restrict
                 acc.add(v);
             }
         acc.mul(scale);
-        acc.store(dtable, ((row0 + r) * vpr + col) * V);
+        acc.template store<ONCE>(dtable, ((row0 + r) * vpr + col) * V);
     }
 }
 
@@ -251,12 +270,12 @@ __global__ __launch_bounds__(256) void runs_kernel(const uint32_t* __restrict__ 
 template <int DT, int V>
 __device__ inline void sum_positions(Vec<DT, V>& acc, const void* dout, const uint32_t* pos, uint32_t lo, uint32_t hi, uint32_t vpr, uint32_t col) {
     uint32_t k = lo;
-    for (; k + 4 <= hi; k += 4) {
-        Vec<DT, V> v[4];
+    for (; k + FLIGHT <= hi; k += FLIGHT) {     // that many rows on their way at a time
+        Vec<DT, V> v[FLIGHT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j].load(dout, ((uint64_t)pos[k + j] * vpr + col) * V);
+        for (uint32_t j = 0; j < FLIGHT; ++j) v[j].load(dout, ((uint64_t)pos[k + j] * vpr + col) * V);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc.add(v[j]);
+        for (uint32_t j = 0; j < FLIGHT; ++j) acc.add(v[j]);
     }
     for (; k < hi; ++k) {
         Vec<DT, V> v;
@@ -287,7 +306,7 @@ __global__ __launch_bounds__(64) void pieces_kernel(const void* __restrict__ dou
     }
 }
 
-template <int DT, int V>
+template <int DT, int V, bool ONCE>
 __global__ __launch_bounds__(256) void grad_rows_kernel(const void* __restrict__ dout, const uint32_t* __restrict__ pos,
                                                         const uint64_t* __restrict__ runs, uint64_t n_rows, uint32_t longer, uint32_t vpr,
                                                         const float* __restrict__ partial, float scale, void* __restrict__ dtable) {
@@ -303,13 +322,30 @@ __global__ __launch_bounds__(256) void grad_rows_kernel(const void* __restrict__
     if (e - b <= longer) {
         sum_positions<DT, V>(acc, dout, pos, b, e, vpr, col);
     } else {
-        for (uint32_t c = b / longer; c <= (e - 1) / longer; ++c) {
-            const uint64_t slot = (uint64_t)c * 2 + (c * longer < b ? 1 : 0);
-            for (int i = 0; i < V; ++i) acc.v[i] += partial[(slot * vpr + col) * V + i];
-        }
+        // the piece in which the run begins has it in slot 1, unless it begins there too; the others in slot 0
+        uint32_t c = b / longer;
+        const uint32_t last = (e - 1) / longer;
+        constexpr int W = V < 4 ? V : 4, H = V / W;        // partial sums are f32: two vectors for eight elements
+        Vec<cgv::DT_F32, W> t[FLIGHT][H];
+        auto add = [&](uint32_t count) {
+#pragma unroll
+            for (uint32_t j = 0; j < FLIGHT; ++j)
+                if (j < count)
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+                        t[j][h].load(partial, (((uint64_t)(c + j) * 2 + ((c + j) * longer < b ? 1 : 0)) * vpr + col) * V + h * W);
+#pragma unroll
+            for (uint32_t j = 0; j < FLIGHT; ++j)
+                if (j < count)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) acc.v[i] += t[j][i / W].v[i % W];
+            c += count;
+        };
+        while (c + FLIGHT <= last + 1) add(FLIGHT);
+        if (c <= last) add(last + 1 - c);
     }
     acc.mul(scale);
-    acc.store(dtable, (row * vpr + col) * V);
+    acc.template store<ONCE>(dtable, (row * vpr + col) * V);
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
@@ -326,10 +362,10 @@ struct GradPlan {
         passes = (need + MAX_DIGIT - 1) / MAX_DIGIT;
         bits = (need + passes - 1) / passes;
         blocks = (uint32_t)((n + SORT_BLOCK - 1) / SORT_BLOCK);
-        // a run is summed by one thread up to `longer` positions, and pieces of a longer one by one thread again: about the root
-        // of n keeps both chains short
+        // a run is summed by one thread up to `longer` positions, and pieces of a longer one by one thread again: an eighth
+        // of the root of n keeps both chains short (100 k ids into 20 k x 1024 fp16: 106 us with half the root, 78 with an eighth)
         longer = 32;
-        while ((uint64_t)longer * longer * 4 < n) longer *= 2;
+        while ((uint64_t)longer * longer * 64 < n) longer *= 2;
         const uint64_t pieces = (n + longer - 1) / longer;
         for (int i = 0; i < 2; ++i) {
             off_keys[i] = bytes, bytes += up256(n * 4);
@@ -342,10 +378,26 @@ struct GradPlan {
     }
 };
 
-// 16-byte vectors where every row starts on 16 bytes, single elements otherwise
-bool by_vectors(uint32_t dim, int dtype, uint64_t stride, const void* a, const void* b) {
+// elements of a vector: the most that 16 bytes hold and every row's start and length allow
+uint32_t vector_elems(uint32_t dim, int dtype, uint64_t stride, const void* a, const void* b) {
     const uint32_t es = esize(dtype);
-    return (uint64_t)dim * es % 16 == 0 && stride * es % 16 == 0 && ((uintptr_t)a | (uintptr_t)b) % 16 == 0;
+    uint32_t v = 16 / es;
+    while (v > 1 && ((uint64_t)dim % v || stride % v || ((uintptr_t)a | (uintptr_t)b) % (v * es))) v /= 2;
+    return v;
+}
+
+// Results larger than this are stored past the caches, which could not hold them for a reader anyway (gradient of 100 k x 768 f32 by 65 536
+// ids: 187 -> 115 us; 200 MB of looked-up rows: 60 -> 44 us)
+constexpr uint64_t ONCE_BYTES = 64ull << 20;
+
+template <class F>
+int by_vector(int dtype, uint32_t v, F&& f) {
+    return by_dtype(dtype, [&](auto t) {
+        if (v == 1) return f(t, std::integral_constant<int, 1>());
+        if (v == 2) return f(t, std::integral_constant<int, 2>());
+        if (decltype(t)::value == cgv::DT_F32 || v == 4) return f(t, std::integral_constant<int, 4>());
+        return f(t, std::integral_constant<int, decltype(t)::value == cgv::DT_F32 ? 4 : 8>());
+    });
 }
 
 int check_common(int dtype, uint64_t n_rows, uint32_t dim, uint64_t n_ids, float scale) {
@@ -362,7 +414,8 @@ int launch_lookup(const void* table, uint64_t n_rows, uint32_t dim, uint64_t str
     const uint32_t vpr = dim / V;
     const uint64_t blocks = (n_ids * vpr + 255) / 256;
     if (blocks > 0x7fffffffull) return fail(CGV_ERR_INVALID_ARG, "too many elements for one call");
-    hipLaunchKernelGGL((lookup_kernel<DT, V>), dim3((unsigned)blocks), dim3(256), 0, s, table, n_rows, vpr, stride, ids, n_ids, scale, out);
+    auto kern = n_ids * dim * (DT == cgv::DT_F32 ? 4 : 2) > ONCE_BYTES ? lookup_kernel<DT, V, true> : lookup_kernel<DT, V, false>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, s, table, n_rows, vpr, stride, ids, n_ids, scale, out);
     OPCHK(hipGetLastError());
     return CGV_OK;
 }
@@ -373,9 +426,11 @@ int launch_grad(const void* dout, const int64_t* ids, uint64_t n_ids, uint64_t n
     const uint32_t vpr = dim / V;
     const uint64_t blocks = (n_rows * vpr + 255) / 256;
     if (blocks > 0x7fffffffull) return fail(CGV_ERR_INVALID_ARG, "too many elements for one call");
+    const bool once = n_rows * dim * (DT == cgv::DT_F32 ? 4 : 2) > ONCE_BYTES;
     if (!pl.passes) {
         const uint32_t rpb = std::max<uint32_t>(1, 1024 / vpr);      // four vectors a thread
-        hipLaunchKernelGGL((grad_direct_kernel<DT, V>), dim3((unsigned)((n_rows + rpb - 1) / rpb)), dim3(256), 0, s, dout, ids, (uint32_t)n_ids, n_rows,
+        auto kern = once ? grad_direct_kernel<DT, V, true> : grad_direct_kernel<DT, V, false>;
+        hipLaunchKernelGGL(kern, dim3((unsigned)((n_rows + rpb - 1) / rpb)), dim3(256), 0, s, dout, ids, (uint32_t)n_ids, n_rows,
                            vpr, rpb, scale, dtable);
         OPCHK(hipGetLastError());
         return CGV_OK;
@@ -412,7 +467,8 @@ int launch_grad(const void* dout, const int64_t* ids, uint64_t n_ids, uint64_t n
     hipLaunchKernelGGL((pieces_kernel<DT, V>), dim3((n + pl.longer - 1) / pl.longer, (vpr + 63) / 64), dim3(64), 0, s, dout, keys, pos,
                        (const uint64_t*)runs, n, (uint32_t)n_rows, pl.longer, vpr, partial);
     OPCHK(hipGetLastError());
-    hipLaunchKernelGGL((grad_rows_kernel<DT, V>), dim3((unsigned)blocks), dim3(256), 0, s, dout, pos, (const uint64_t*)runs, n_rows, pl.longer, vpr,
+    auto kern = once ? grad_rows_kernel<DT, V, true> : grad_rows_kernel<DT, V, false>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, s, dout, pos, (const uint64_t*)runs, n_rows, pl.longer, vpr,
                        (const float*)partial, scale, dtable);
     OPCHK(hipGetLastError());
     return CGV_OK;
@@ -433,11 +489,9 @@ int cgv_lookup_rows_dev(int device_id, const void* table_dev, int dtype, uint64_
         if ((rc = need_gpu(device_id))) return rc;
         DeviceScope dev(device_id);
         OPCHK(dev.enter());
-        const bool vec = by_vectors(dim, dtype, row_stride, table_dev, out_dev);
-        return by_dtype(dtype, [&](auto t) {
-            constexpr int DT = decltype(t)::value, V = DT == cgv::DT_F32 ? 4 : 8;
-            return vec ? launch_lookup<DT, V>(table_dev, n_rows, dim, row_stride, ids_dev, n_ids, scale, out_dev, (hipStream_t)stream)
-                       : launch_lookup<DT, 1>(table_dev, n_rows, dim, row_stride, ids_dev, n_ids, scale, out_dev, (hipStream_t)stream);
+        return by_vector(dtype, vector_elems(dim, dtype, row_stride, table_dev, out_dev), [&](auto t, auto v) {
+            return launch_lookup<decltype(t)::value, decltype(v)::value>(table_dev, n_rows, dim, row_stride, ids_dev, n_ids, scale, out_dev,
+                                                                         (hipStream_t)stream);
         });
     });
 }
@@ -460,11 +514,9 @@ int cgv_lookup_grad_dev(int device_id, const void* dout_dev, int dtype, const in
         if ((rc = need_gpu(device_id))) return rc;
         DeviceScope dev(device_id);
         OPCHK(dev.enter());
-        const bool vec = by_vectors(dim, dtype, dim, dout_dev, dtable_dev);
-        return by_dtype(dtype, [&](auto t) {
-            constexpr int DT = decltype(t)::value, V = DT == cgv::DT_F32 ? 4 : 8;
-            return vec ? launch_grad<DT, V>(dout_dev, ids_dev, n_ids, n_rows, dim, scale, dtable_dev, (char*)workspace_dev, pl, (hipStream_t)stream)
-                       : launch_grad<DT, 1>(dout_dev, ids_dev, n_ids, n_rows, dim, scale, dtable_dev, (char*)workspace_dev, pl, (hipStream_t)stream);
+        return by_vector(dtype, vector_elems(dim, dtype, dim, dout_dev, dtable_dev), [&](auto t, auto v) {
+            return launch_grad<decltype(t)::value, decltype(v)::value>(dout_dev, ids_dev, n_ids, n_rows, dim, scale, dtable_dev, (char*)workspace_dev, pl,
+                                                                       (hipStream_t)stream);
         });
     });
 }

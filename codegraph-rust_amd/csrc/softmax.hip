@@ -118,6 +118,55 @@ __device__ inline void copy_row(const void* src, uint64_t at, uint32_t dim, uint
     }
 }
 
+struct Piece {              // corpus rows [n0, n0 + c) on their way into the padded copy
+    const void* rows;
+    uint64_t stride, n0, plane;
+    uint16_t* dst;
+    uint32_t c, dim, dp;
+};
+// a workgroup of 256 threads, each with eight elements of a row
+template <int DT>
+__device__ inline void copy_piece_block(const Piece& P, uint32_t block) {
+    const void* rows = P.rows;
+    const uint64_t stride = P.stride, n0 = P.n0, plane = P.plane;
+    const uint32_t c = P.c, dim = P.dim, dp = P.dp;
+    uint16_t* dst = P.dst;
+    const uint32_t per = dp / 8;
+    const uint64_t t = (uint64_t)block * 256 + threadIdx.x;
+    const uint64_t row = t / per;
+    if (row >= c) return;
+    const uint32_t e = (uint32_t)(t - row * per) * 8;
+    const uint64_t at = (n0 + row) * stride + e;
+    uint16_t* o = dst + row * dp + e;
+    if (DT == cgv::DT_F32) {
+        const float* src = (const float*)rows + at;
+        float v[8];
+        if (e + 8 <= dim && ((uintptr_t)src & 15) == 0) {
+            const float4 x = *(const float4*)src, y = *(const float4*)(src + 4);
+            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+        } else {
+            for (int j = 0; j < 8; ++j) v[j] = e + j < dim ? src[j] : 0.0f;
+        }
+        uint16_t p[8][3];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) split3(v[j], p[j]);
+#pragma unroll
+        for (int x = 0; x < 3; ++x) {
+            uint32_t w[4];
+            for (int j = 0; j < 4; ++j) w[j] = p[2 * j][x] | (uint32_t)p[2 * j + 1][x] << 16;
+            *(uint4*)(o + x * plane) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    } else {
+        const uint16_t* src = (const uint16_t*)rows + at;
+        uint32_t w[4];
+        for (int j = 0; j < 4; ++j)
+            w[j] = (e + 2 * j < dim ? src[2 * j] : 0u) | (uint32_t)(e + 2 * j + 1 < dim ? src[2 * j + 1] : 0u) << 16;
+        *(uint4*)o = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+template <int DT>
+__global__ __launch_bounds__(256) void copy_rows_kernel(Piece P) { copy_piece_block<DT>(P, blockIdx.x); }
+
 struct Problem {
     const void *queries, *rows;
     uint64_t q_stride, r_stride, n_rows;
@@ -130,8 +179,10 @@ struct Problem {
     int device;
 };
 
+// (the first piece of the corpus is copied by further workgroups of the same launch)
 template <int DT>
-__global__ __launch_bounds__(256) void forward_prep_kernel(Problem P, uint32_t* __restrict__ anchor) {
+__global__ __launch_bounds__(256) void forward_prep_kernel(Problem P, uint32_t* __restrict__ anchor, Piece first) {
+    if (blockIdx.x >= P.bp) return copy_piece_block<DT>(first, blockIdx.x - P.bp);
     const uint32_t i = blockIdx.x, wave = threadIdx.x >> 6;
     const int lane = threadIdx.x & 63;
     const uint64_t plane = (uint64_t)P.bp * P.dp;
@@ -208,7 +259,8 @@ __global__ __launch_bounds__(256) void loss_kernel(Problem P, const float2* __re
 template <int DT>
 __global__ __launch_bounds__(256) void backward_prep_kernel(Problem P, const float* __restrict__ dloss, float* __restrict__ coef, float2* __restrict__ lse2,
                                                             uint32_t* __restrict__ has, uint32_t* __restrict__ ent_id, float* __restrict__ ent_val,
-                                                            float* __restrict__ mul) {
+                                                            float* __restrict__ mul, Piece first_piece) {
+    if (blockIdx.x >= P.bp) return copy_piece_block<DT>(first_piece, blockIdx.x - P.bp);
     __shared__ uint32_t ids[MAX_K];
     __shared__ double ps[MAX_K];
     const uint32_t i = blockIdx.x, wave = threadIdx.x >> 6;
@@ -295,44 +347,6 @@ __global__ __launch_bounds__(256) void patch_kernel(const uint32_t* __restrict__
     }
 }
 
-// corpus rows [n0, n0 + c) into the padded copy: a thread takes eight elements of a row
-template <int DT>
-__global__ __launch_bounds__(256) void copy_rows_kernel(const void* __restrict__ rows, uint64_t stride, uint64_t n0, uint32_t c, uint32_t dim, uint32_t dp,
-                                                        uint64_t plane, uint16_t* __restrict__ dst) {
-    const uint32_t per = dp / 8;
-    const uint64_t t = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    const uint64_t row = t / per;
-    if (row >= c) return;
-    const uint32_t e = (uint32_t)(t - row * per) * 8;
-    const uint64_t at = (n0 + row) * stride + e;
-    uint16_t* o = dst + row * dp + e;
-    if (DT == cgv::DT_F32) {
-        const float* src = (const float*)rows + at;
-        float v[8];
-        if (e + 8 <= dim && ((uintptr_t)src & 15) == 0) {
-            const float4 x = *(const float4*)src, y = *(const float4*)(src + 4);
-            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-        } else {
-            for (int j = 0; j < 8; ++j) v[j] = e + j < dim ? src[j] : 0.0f;
-        }
-        uint16_t p[8][3];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) split3(v[j], p[j]);
-#pragma unroll
-        for (int x = 0; x < 3; ++x) {
-            uint32_t w[4];
-            for (int j = 0; j < 4; ++j) w[j] = p[2 * j][x] | (uint32_t)p[2 * j + 1][x] << 16;
-            *(uint4*)(o + x * plane) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-    } else {
-        const uint16_t* src = (const uint16_t*)rows + at;
-        uint32_t w[4];
-        for (int j = 0; j < 4; ++j)
-            w[j] = (e + 2 * j < dim ? src[2 * j] : 0u) | (uint32_t)(e + 2 * j + 1 < dim ? src[2 * j + 1] : 0u) << 16;
-        *(uint4*)o = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-}
-
 // dQ: the shares' partial sums, added in a fixed order and rounded once. 64 threads a stretch of 256 elements, four groups of shares
 template <int DT>
 __global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict__ part, uint32_t splits, uint64_t share, uint32_t dim, uint32_t dp,
@@ -365,6 +379,7 @@ __global__ void zero_kernel(void* p, uint64_t total) {
 typedef Shape<64, 64, 1, 2> S64x64;
 typedef Shape<256, 64, 4, 1> S64;
 typedef Shape<256, 128, 4, 2> S128;
+typedef Shape<256, 192, 4, 2> S192;
 typedef Shape<256, 256, 2, 4> S256;
 
 uint64_t up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
@@ -380,8 +395,13 @@ struct Plan {
         planes = dtype == CGV_DTYPE_F32 ? 3 : 1;
         copy = dtype == CGV_DTYPE_F32 || dim % 8 != 0;
         // the tile width whose padded batch takes the least time: narrower tiles read LDS more often per product
-        const double t256 = up(bp, 256) / 1.0, t128 = up(bp, 128) / 0.8, t64 = up(bp, 64) / 0.55;
-        bn = t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64;
+        static const uint32_t width[4] = {256, 192, 128, 64};
+        static const double worth[4] = {1.0, 0.94, 0.83, 0.61};      // loss and gradients of 768 queries over 200 k x 768 with each
+        double least = 1e30;
+        for (int i = 0; i < 4; ++i) {
+            const double t = up(bp, width[i]) / worth[i];
+            if (t < least) least = t, bn = width[i];
+        }
         bm = 256;
         // few tiles: small ones on more CUs, with more stages on the way (32 queries x 10 k x 384, f32: 31 -> us)
         if ((n_ + 255) / 256 * ((bp + bn - 1) / bn) < CUS / 2) bm = bn = 64;
@@ -440,6 +460,7 @@ template <int DT, bool TA, bool TB, int EPI>
 int launch_by_queries(const Plan& pl, const Args& a, int device, hipStream_t s) {
     if (pl.bm == 64) return launch_gemm<DT, S64x64, TA, TB, EPI>(a, device, s);
     const uint32_t bn = pl.bn;
+    if (bn == 192) return launch_gemm<DT, S192, TA, TB, EPI>(a, device, s);
     return bn == 64 ? launch_gemm<DT, S64, TA, TB, EPI>(a, device, s) : bn == 128 ? launch_gemm<DT, S128, TA, TB, EPI>(a, device, s)
                                                               : launch_gemm<DT, S256, TA, TB, EPI>(a, device, s);
 }
@@ -465,9 +486,14 @@ Args score_args(const Plan& pl, const Problem& P, int dtype, const char* rows, u
     return a;
 }
 
+Piece piece_of(const Plan& pl, const Problem& P, uint64_t n0, uint64_t most, char* dst) {
+    return {P.rows, P.r_stride, n0, most * pl.dp, (uint16_t*)dst, pl.copy ? (uint32_t)std::min<uint64_t>(most, pl.n - n0) : 0u, pl.dim, pl.dp};
+}
+uint32_t copy_blocks(const Piece& p) { return (uint32_t)(((uint64_t)p.c * (p.dp / 8) + 255) / 256); }
+
 template <int DT>
-int copy_piece(const Plan& pl, const Problem& P, uint64_t n0, uint32_t c, uint64_t plane_elems, char* dst, hipStream_t s) {
-    hipLaunchKernelGGL((copy_rows_kernel<DT>), dim3((unsigned)(((uint64_t)c * (pl.dp / 8) + 255) / 256)), dim3(256), 0, s, P.rows, P.r_stride, n0, c, pl.dim, pl.dp, plane_elems, (uint16_t*)dst);
+int copy_piece(const Piece& p, hipStream_t s) {
+    hipLaunchKernelGGL((copy_rows_kernel<DT>), dim3(copy_blocks(p)), dim3(256), 0, s, p);
     OPCHK(hipGetLastError());
     return CGV_OK;
 }
@@ -477,7 +503,8 @@ int forward(const Plan& pl, Problem P, int dtype, float* loss, char* ws, hipStre
     P.qws = (uint16_t*)ws;
     uint32_t* anchor = (uint32_t*)(ws + pl.f_anchor());
     float2* part = (float2*)(ws + pl.f_part());
-    hipLaunchKernelGGL((forward_prep_kernel<DT>), dim3(pl.bp), dim3(256), 0, s, P, anchor);
+    const Piece first = piece_of(pl, P, 0, pl.piece_f, ws + pl.f_rows());
+    hipLaunchKernelGGL((forward_prep_kernel<DT>), dim3(pl.bp + copy_blocks(first)), dim3(256), 0, s, P, anchor, first);
     OPCHK(hipGetLastError());
     uint32_t parts = 0;
     for (uint64_t n0 = 0; n0 < pl.n; n0 += pl.piece_f) {
@@ -485,12 +512,11 @@ int forward(const Plan& pl, Problem P, int dtype, float* loss, char* ws, hipStre
         const char* rows = (const char*)P.rows + n0 * P.r_stride * 2;
         uint64_t pitch = P.r_stride * 2, plane = 0;
         if (pl.copy) {
-            plane = pl.piece_f * pl.dp;
-            const int rc = copy_piece<DT>(pl, P, n0, c, plane, ws + pl.f_rows(), s);
+            const int rc = n0 ? copy_piece<DT>(piece_of(pl, P, n0, pl.piece_f, ws + pl.f_rows()), s) : CGV_OK;
             if (rc) return rc;
             rows = ws + pl.f_rows();
             pitch = (uint64_t)pl.dp * 2;
-            plane *= 2;
+            plane = pl.piece_f * pitch;
         }
         Args a = score_args(pl, P, dtype, rows, pitch, plane, c);
         a.row0 = n0;
@@ -517,7 +543,8 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
     char* G = ws + pl.b_g();
     float* part = (float*)(ws + pl.b_part());
     const uint64_t g_pitch = pl.piece_b * 2, g_plane = (uint64_t)pl.bp * g_pitch;
-    hipLaunchKernelGGL((backward_prep_kernel<DT>), dim3(pl.bp), dim3(256), 0, s, P, dloss, coef, lse2, has, ent_id, ent_val, mul);
+    const Piece first = piece_of(pl, P, 0, pl.piece_b, ws + pl.b_rows());
+    hipLaunchKernelGGL((backward_prep_kernel<DT>), dim3(pl.bp + copy_blocks(first)), dim3(256), 0, s, P, dloss, coef, lse2, has, ent_id, ent_val, mul, first);
     OPCHK(hipGetLastError());
     if (DT == cgv::DT_FP16) {
         hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1024), 0, s, (const float*)coef, pl.b, mul);
@@ -529,11 +556,10 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
         uint64_t pitch = P.r_stride * 2, plane = 0;
         int rc;
         if (pl.copy) {
-            plane = pl.piece_b * pl.dp;
-            if ((rc = copy_piece<DT>(pl, P, n0, c, plane, ws + pl.b_rows(), s))) return rc;
+            if (n0 && (rc = copy_piece<DT>(piece_of(pl, P, n0, pl.piece_b, ws + pl.b_rows()), s))) return rc;
             rows = ws + pl.b_rows();
             pitch = (uint64_t)pl.dp * 2;
-            plane *= 2;
+            plane = pl.piece_b * pitch;
         }
         Args a = score_args(pl, P, dtype, rows, pitch, plane, c);
         a.coef = coef;

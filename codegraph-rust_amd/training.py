@@ -70,22 +70,27 @@ def _workspace(nbytes, device):
     return torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
 
 
+def _lookup(table, ids, scale):
+    n, d = table.shape
+    dev, k = table.device, ids.numel()
+    out = torch.empty((*ids.shape, d), dtype=table.dtype, device=dev)
+    _check(lib().cgv_lookup_rows_dev(dev.index, table.data_ptr(), _CODES[table.dtype], n, d, _row_stride(table), ids.data_ptr(), k, scale,
+                                     out.data_ptr(), _stream(dev.index)))
+    return out
+
+
 class _LookupRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, ids, scale):
-        n, d = table.shape
-        out = torch.empty((ids.numel(), d), dtype=table.dtype, device=table.device)
-        _check(lib().cgv_lookup_rows_dev(table.device.index, _ptr(table), _CODES[table.dtype], n, d, _row_stride(table), _ptr(ids),
-                                         ids.numel(), scale, _ptr(out), _stream(table.device.index)))
         ctx.save_for_backward(ids)
-        ctx.shape, ctx.dtype, ctx.scale = (n, d), table.dtype, scale
-        return out.view(*ids.shape, d)
+        ctx.n, ctx.scale = table.shape[0], scale
+        return _lookup(table, ids, scale)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
-        return _lookup_grad(dout.contiguous(), ids, ctx.shape[0], ctx.scale), None, None
+        return _lookup_grad(dout.contiguous(), ids, ctx.n, ctx.scale), None, None
 
 
 def _lookup_grad(dout, ids, n, scale):
@@ -103,7 +108,10 @@ def lookup_rows(table, ids, scale=1.0):
     [0, n_rows) - the -1 that pads a short search result among them - gives zeros and takes no part in the gradient.
     Differentiable in `table`; the gradient is dense, in the table's type, each row summed in f32 in a fixed order."""
     table = _matrix(table, "table")
-    return _LookupRows.apply(table, _ids(ids, "ids", table.device), float(scale))
+    ids = _ids(ids, "ids", table.device)
+    if not (table.requires_grad and torch.is_grad_enabled()):
+        return _lookup(table, ids, float(scale))
+    return _LookupRows.apply(table, ids, float(scale))
 
 
 def lookup_rows_grad(dout, ids, n_rows, scale=1.0):
@@ -120,19 +128,24 @@ def lookup_rows_grad(dout, ids, n_rows, scale=1.0):
     return _lookup_grad(dout.detach().contiguous(), ids, int(n_rows), float(scale))
 
 
+def _loss(queries, rows, ids, scores, scale, teacher_scale):
+    L = lib()
+    b, d = queries.shape
+    n, k = rows.shape[0], ids.shape[1]
+    code, dev = _CODES[rows.dtype], rows.device
+    loss = torch.empty((b,), dtype=torch.float32, device=dev)
+    saved = torch.empty((b * (k + 2),), dtype=torch.float64, device=dev)
+    nbytes = L.cgv_corpus_loss_workspace(b, n, d, k, code)
+    ws = _workspace(nbytes, dev)
+    _check(L.cgv_corpus_loss_dev(dev.index, queries.data_ptr(), _row_stride(queries), rows.data_ptr(), _row_stride(rows), code, b, n, d, ids.data_ptr(),
+                                 _ptr(scores), k, scale, teacher_scale, loss.data_ptr(), saved.data_ptr(), _ptr(ws), nbytes, _stream(dev.index)))
+    return loss, saved
+
+
 class _CorpusLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, queries, rows, ids, scores, scale, teacher_scale):
-        L = lib()
-        b, d = queries.shape
-        n, k = rows.shape[0], ids.shape[1]
-        code, dev = _CODES[rows.dtype], rows.device
-        loss = torch.empty((b,), dtype=torch.float32, device=dev)
-        saved = torch.empty((b * (k + 2),), dtype=torch.float64, device=dev)
-        nbytes = L.cgv_corpus_loss_workspace(b, n, d, k, code)
-        ws = _workspace(nbytes, dev)
-        _check(L.cgv_corpus_loss_dev(dev.index, _ptr(queries), _row_stride(queries), _ptr(rows), _row_stride(rows), code, b, n, d, _ptr(ids),
-                                     _ptr(scores), k, scale, teacher_scale, _ptr(loss), _ptr(saved), _ptr(ws), nbytes, _stream(dev.index)))
+        loss, saved = _loss(queries, rows, ids, scores, scale, teacher_scale)
         ctx.save_for_backward(queries, rows, ids, scores, saved)
         ctx.scales = (scale, teacher_scale)
         return loss
@@ -168,6 +181,8 @@ def _corpus_loss(queries, rows, ids, scores, scale, teacher_scale):
         raise _bad("rows must not be empty")
     if rows.dtype != torch.float32 and rows.shape[1] % 8 == 0 and (rows.data_ptr() % 16 or _row_stride(rows) % 8 or _row_stride(rows) > 1 << 22):
         rows = rows.clone(memory_format=torch.contiguous_format)      # such rows are read in place, 16 bytes at a time
+    if not ((queries.requires_grad or rows.requires_grad) and torch.is_grad_enabled()):
+        return _loss(queries, rows, ids, scores, float(scale), float(teacher_scale))[0]
     return _CorpusLoss.apply(queries, rows, ids, scores, float(scale), float(teacher_scale))
 
 
