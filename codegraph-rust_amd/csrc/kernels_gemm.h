@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "ops_common.h"
 
 namespace cgv_gemm {
 
@@ -65,23 +66,28 @@ struct Args {
     // epilogues
     float scale2;                                 // LSE, G: scores in units of log 2 = accumulator * scale2
     uint32_t m_valid, n_valid;                    // rows / columns of the result that exist
-    uint64_t row0;                                // LSE: corpus row of m = 0
+    uint64_t row0;                                // LSE, G: corpus row of m = 0
     const uint32_t* anchor;                       // LSE: [n] corpus row left out of the sum, 0xffffffff for none
     float2* part;                                 // LSE: [splits * WM][part_ld] (maximum, sum)
     uint32_t part_ld;
     const float* coef;                            // G: [n] factor
     const float2* lse2;                           // G: [n] log2 of the softmax sum, its f32 and what that leaves
+    const uint32_t* ent_id;                       // G: [n][ent_k] corpus rows whose entries are given, 0xffffffff for none
+    const float* ent_val;                         // G: [n][ent_k] those entries
+    uint32_t ent_k;
     char* out;                                    // G, DR, DQ
     uint64_t out_pitch, out_plane;                // bytes
     uint32_t accumulate, vec_out;                 // DQ: add to what is there; DR: 16-byte stores possible
     const float* unscale;                         // G: [1] factor of the entries; DR: [1] factor of the result
 };
 
-template <int BM_, int BN_, int WM_, int WN_>
+// PL planes of an operand in a stage: 3 for f32 where tiles are small - each plane is then loaded once and not once per product
+template <int BM_, int BN_, int WM_, int WN_, int PL_ = 1>
 struct Shape {
+    static constexpr int PL = PL_;
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM_ * WN_, THREADS = 64 * NW;
     static constexpr int TM = BM / WM, TN = BN / WN, MB = TM / 32, NB = TN / 32;
-    static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
+    static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, STAGE = PL * (A_BYTES + B_BYTES);
     static constexpr int XPOSE = 4096;            // per wave: a 32 x 64 piece of 16-bit results on its way out
     // stages in LDS: as many as fit, six at most; all but one of them are loading or waiting
     static constexpr int stages(bool xpose) {
@@ -158,14 +164,14 @@ __device__ inline uint32_t unit_of(uint32_t id, uint32_t blocks) {
     return x * per + min(x, extra) + (id >> 3);
 }
 
+#if defined(__HIP_DEVICE_COMPILE__)   // the host pass only needs the launch stubs
 template <int DT, class S, bool TA, bool TB, int EPI>
-static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
-#if defined(__HIP_DEVICE_COMPILE__)   // the host pass only needs the launch stub
+__device__ __forceinline__ void work(const Args& g, uint32_t block) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     constexpr int NST = S::stages(EPI == EPI_G || EPI == EPI_DR);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % S::WM, wn = wave / S::WM;
-    const uint32_t unit = unit_of(blockIdx.x, g.blocks);
+    const uint32_t unit = unit_of(block, g.blocks);
 
     // ---- this workgroup's tiles: LSE and G keep a query tile and walk the corpus; dR walks (element tile, corpus tile); dQ has one
     uint32_t mt, nt, k0 = 0, ksteps = g.ksteps, tiles, split = 0;
@@ -258,8 +264,11 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
     };
     auto issue = [&](int slot) {
         char* l = smem + slot * S::STAGE;
-        la.issue(pa, sa, l, wave);
-        lb.issue(pb, sb, l + S::A_BYTES, wave);
+#pragma unroll
+        for (int p = 0; p < S::PL; ++p) {
+            la.issue(pa + p * g.a.plane, sa, l + p * S::A_BYTES, wave);
+            lb.issue(pb + p * g.b.plane, sb, l + S::PL * S::A_BYTES + p * S::B_BYTES, wave);
+        }
     };
 
     float run_m[S::NB], run_s[S::NB];                 // LSE: per query of the lane, over the corpus rows of the lane
@@ -268,24 +277,40 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
 
     // A small wave tile has few products per read: it keeps the fragments of two whole stages and reads the next one while it
     // multiplies this one; a large one keeps those of two times 16 elements of K
-    constexpr bool SMALL = S::MB * S::NB <= 2;
-    constexpr int SETS = SMALL ? 4 : 1;
-    s16x8 fa0[SETS][S::MB], fb0[SETS][S::NB], fa1[SETS][S::MB], fb1[SETS][S::NB];
-    f32x16 acc[S::MB][S::NB];
-    auto read = [&](s16x8(&fa)[S::MB], s16x8(&fb)[S::NB], int buf, int kk) {
-        const char* as = smem + buf * S::STAGE;
+    constexpr bool SMALL = S::MB * S::NB <= 2 && S::PL == 1;
+    constexpr int SETS = SMALL ? 4 : 1, FA = S::PL * S::MB, FB = S::PL * S::NB;
+    s16x8 fa0[SETS][FA], fb0[SETS][FB], fa1[SETS][FA], fb1[SETS][FB];
+    f32x16 acc[S::MB][S::NB], low[S::PL == 3 ? S::MB : 1][S::PL == 3 ? S::NB : 1];   // three planes: the five small products have their own sum
+    auto read = [&](s16x8(&fa)[FA], s16x8(&fb)[FB], int buf, int kk) {
+        const char *as = smem + buf * S::STAGE, *bs = as + S::PL * S::A_BYTES;
 #pragma unroll
-        for (int nb = 0; nb < S::NB; ++nb) fb[nb] = fragment<TB, S::BN>(as + S::A_BYTES, (uint32_t)(wn * S::TN + nb * 32), kk, lane);
+        for (int p = 0; p < S::PL; ++p) {
 #pragma unroll
-        for (int mb = 0; mb < S::MB; ++mb) fa[mb] = fragment<TA, S::BM>(as, (uint32_t)(wm * S::TM + mb * 32), kk, lane);
+            for (int nb = 0; nb < S::NB; ++nb) fb[p * S::NB + nb] = fragment<TB, S::BN>(bs + p * S::B_BYTES, (uint32_t)(wn * S::TN + nb * 32), kk, lane);
+#pragma unroll
+            for (int mb = 0; mb < S::MB; ++mb) fa[p * S::MB + mb] = fragment<TA, S::BM>(as + p * S::A_BYTES, (uint32_t)(wm * S::TM + mb * 32), kk, lane);
+        }
     };
-    auto products = [&](s16x8(&fa)[S::MB], s16x8(&fb)[S::NB]) {
+    auto products = [&](s16x8(&fa)[FA], s16x8(&fb)[FB]) {
+        if constexpr (S::PL == 3) {
+            constexpr int x[6] = {2, 0, 0, 1, 1, 0}, y[6] = {0, 2, 0, 1, 0, 1};
 #pragma unroll
-        for (int mb = 0; mb < S::MB; ++mb)
+            for (int i = 0; i < 6; ++i)
 #pragma unroll
-            for (int nb = 0; nb < S::NB; ++nb) acc[mb][nb] = mma<DT>(fa[mb], fb[nb], acc[mb][nb]);
+                for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+                    for (int nb = 0; nb < S::NB; ++nb) {
+                        f32x16& c = x[i] + y[i] ? low[mb][nb] : acc[mb][nb];
+                        c = mma<DT>(fa[x[i] * S::MB + mb], fb[y[i] * S::NB + nb], c);
+                    }
+        } else {
+#pragma unroll
+            for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+                for (int nb = 0; nb < S::NB; ++nb) acc[mb][nb] = mma<DT>(fa[mb], fb[nb], acc[mb][nb]);
+        }
     };
-    constexpr int WAIT = (NST - 2) * (decltype(la)::I + decltype(lb)::I);   // loads of the stages behind the next one
+    constexpr int LOADS = S::PL * (decltype(la)::I + decltype(lb)::I), WAIT = (NST - 2) * LOADS;   // of a stage; of the stages behind the next one
     auto stage_ready = [&]() {
         // this wave's part of the next stage has landed, its reads of this one are done
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(WAIT) : "memory");
@@ -293,7 +318,7 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
         asm volatile("" ::: "memory");
     };
 
-    constexpr int PRODUCTS = S::MB * S::NB, READS = S::MB * (TA ? 2 : 1) + S::NB * (TB ? 2 : 1);
+    constexpr int PRODUCTS = S::MB * S::NB * (S::PL == 3 ? 6 : 1), READS = FA * (TA ? 2 : 1) + FB * (TB ? 2 : 1);
     // the order of a phase: behind each of the first matrix instructions come a few reads of the next fragments, then the loads
     auto interleave = [&](int loads) {
         constexpr int each = PRODUCTS > 2 ? (READS + PRODUCTS - 3) / (PRODUCTS - 2) : READS;
@@ -311,12 +336,12 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
 
     if (!ksteps) tiles = EPI == EPI_DQ ? tiles : 0;
     int buf = 0;                                      // slot of the stage at work; the one before it is where the next load goes
-    auto read_stage = [&](s16x8(&fa)[SETS][S::MB], s16x8(&fb)[SETS][S::NB], int slot) {
+    auto read_stage = [&](s16x8(&fa)[SETS][FA], s16x8(&fb)[SETS][FB], int slot) {
 #pragma unroll
         for (int kk = 0; kk < SETS; ++kk) read(fa[kk], fb[kk], slot, kk);
     };
     // small wave tiles: a stage's products while the next stage's fragments are read
-    auto step = [&](s16x8(&ca)[SETS][S::MB], s16x8(&cb)[SETS][S::NB], s16x8(&na)[SETS][S::MB], s16x8(&nb)[SETS][S::NB]) {
+    auto step = [&](s16x8(&ca)[SETS][FA], s16x8(&cb)[SETS][FB], s16x8(&na)[SETS][FA], s16x8(&nb)[SETS][FB]) {
         __builtin_amdgcn_sched_barrier(0);
         prepare();
         stage_ready();
@@ -354,7 +379,10 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
 #pragma unroll
             for (int nb = 0; nb < S::NB; ++nb)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[mb][nb][r] = 0.0f;
+                for (int r = 0; r < 16; ++r) {
+                    acc[mb][nb][r] = 0.0f;
+                    if (S::PL == 3) low[mb][nb][r] = 0.0f;
+                }
         if constexpr (SMALL) {
             uint32_t s = 0;
             for (; s + 2 <= stages; s += 2) {
@@ -392,11 +420,18 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
                 issue(buf);
                 buf = next;
                 products(fa1[0], fb1[0]);
-                interleave(decltype(la)::I + decltype(lb)::I);
+                interleave(LOADS);
+            }
+            if constexpr (S::PL == 3) {
+#pragma unroll
+                for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+                    for (int nb = 0; nb < S::NB; ++nb) acc[mb][nb] += low[mb][nb];
             }
         }
 
         // ---- epilogue of the tile
+        constexpr int PAIR = S::MB < 2 ? 1 : 2, LPR = PAIR * 4, OUT = 64 / LPR;   // G, DR: blocks of 32 that leave together; lanes of a row, rows of an instruction
         const uint32_t m0 = my_mt * S::BM + wm * S::TM, n0 = my_nt * S::BN + wn * S::TN;
         const uint32_t half4 = (uint32_t)(lane >> 5) * 4;
         if (EPI == EPI_LSE) {
@@ -457,9 +492,9 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
                 const float c = q < g.n_valid ? g.coef[q] * *g.unscale : 0.0f;
                 const float2 l2 = q < g.n_valid ? g.lse2[q] : make_float2(0.0f, 0.0f);
 #pragma unroll
-                for (int mp = 0; mp < S::MB; mp += 2) {      // 64 corpus rows x 32 queries at a time, through the wave's own LDS
+                for (int mp = 0; mp < S::MB; mp += PAIR) {      // 64 (32) corpus rows x 32 queries at a time, through the wave's own LDS
 #pragma unroll
-                    for (int mi = 0; mi < 2; ++mi)
+                    for (int mi = 0; mi < PAIR; ++mi)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const uint32_t m = m0 + (mp + mi) * 32 + (r & 3) + 8 * (r >> 2) + half4;
@@ -469,7 +504,7 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
 #pragma unroll
                     for (uint32_t plane = 0; plane < (DT == cgv::DT_F32 ? 3u : 1u); ++plane) {
 #pragma unroll
-                        for (int mi = 0; mi < 2; ++mi)
+                        for (int mi = 0; mi < PAIR; ++mi)
 #pragma unroll
                             for (int r4 = 0; r4 < 4; ++r4) {
                                 uint16_t h[4];
@@ -489,12 +524,12 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
                         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                        for (int p = 0; p < 4; ++p) {
-                            const uint32_t n = p * 8 + (lane >> 3), chunk = (uint32_t)(lane & 7) ^ row_swz(n);
+                        for (int p = 0; p < 32 / OUT; ++p) {
+                            const uint32_t n = p * OUT + lane / LPR, chunk = (uint32_t)(lane % LPR) ^ row_swz(n);
                             const uint4 v = *(const uint4*)(xp + n * 128 + chunk * 16);
                             const uint32_t q = n0 + nb * 32 + n;
                             if (q < g.part_ld)
-                                *(uint4*)(g.out + plane * g.out_plane + q * g.out_pitch + (uint64_t)(m0 + mp * 32) * 2 + (lane & 7) * 16) = v;
+                                *(uint4*)(g.out + plane * g.out_plane + q * g.out_pitch + (uint64_t)(m0 + mp * 32) * 2 + lane % LPR * 16) = v;
                         }
                         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                         __builtin_amdgcn_wave_barrier();
@@ -529,9 +564,9 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
             for (int nb = 0; nb < S::NB; ++nb) {
                 if (DT != cgv::DT_F32 && g.vec_out) {
 #pragma unroll
-                    for (int mp = 0; mp < S::MB; mp += 2) {
+                    for (int mp = 0; mp < S::MB; mp += PAIR) {
 #pragma unroll
-                        for (int mi = 0; mi < 2; ++mi)
+                        for (int mi = 0; mi < PAIR; ++mi)
 #pragma unroll
                             for (int r4 = 0; r4 < 4; ++r4) {
                                 uint16_t h[4];
@@ -546,10 +581,10 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
                         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                        for (int p = 0; p < 4; ++p) {
-                            const uint32_t n = p * 8 + (lane >> 3), chunk = (uint32_t)(lane & 7) ^ row_swz(n);
+                        for (int p = 0; p < 32 / OUT; ++p) {
+                            const uint32_t n = p * OUT + lane / LPR, chunk = (uint32_t)(lane % LPR) ^ row_swz(n);
                             const uint4 v = *(const uint4*)(xp + n * 128 + chunk * 16);
-                            const uint32_t row = n0 + nb * 32 + n, m = m0 + mp * 32 + (lane & 7) * 8;
+                            const uint32_t row = n0 + nb * 32 + n, m = m0 + mp * 32 + lane % LPR * 8;
                             if (row < g.n_valid && m < g.m_valid) *(uint4*)(g.out + row * g.out_pitch + m * 2) = v;   // m_valid: a multiple of 8
                         }
                         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -593,6 +628,50 @@ static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
             if (lane < 32 && q < g.part_ld) g.part[(uint64_t)(split * S::WM + wm) * g.part_ld + q] = make_float2(nm, s);
         }
     }
+    if (EPI == EPI_G) {
+        // the listed rows' entries, computed apart, take the place of what this workgroup has stored for them: every wave's stores are done
+        __syncthreads();
+        const float u = *g.unscale;
+        const uint32_t n0 = nt * S::BN, queries = min((uint32_t)S::BN, g.n_valid - n0);
+        const uint32_t* ids = g.ent_id + (uint64_t)n0 * g.ent_k;
+        const float* vals = g.ent_val + (uint64_t)n0 * g.ent_k;
+        for (uint32_t t0 = threadIdx.x; t0 < queries * g.ent_k; t0 += 8 * S::THREADS) {
+            uint32_t id[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) id[x] = t0 + x * S::THREADS < queries * g.ent_k ? ids[t0 + x * S::THREADS] : 0xffffffffu;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const uint64_t m = (uint64_t)id[x] - g.row0;                // none: beyond every piece; earlier pieces: wraps round
+                if (m >= g.m_valid || (uint32_t)m / S::BM % g.splits != split) continue;
+                const uint32_t t = t0 + x * S::THREADS;
+                uint16_t* o = (uint16_t*)(g.out + (n0 + t / g.ent_k) * g.out_pitch) + m;
+                const float v = vals[t] * u;
+                if (DT == cgv::DT_F32) {
+                    uint16_t p[3];
+                    split3(v, p);
+                    for (int i = 0; i < 3; ++i) o[i * (g.out_plane / 2)] = p[i];
+                } else {
+                    *o = cgv_ops::f32_to_half<DT>(v);
+                }
+            }
+        }
+    }
+}
+#endif
+
+template <int DT, class S, bool TA, bool TB, int EPI>
+static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    work<DT, S, TA, TB, EPI>(g, blockIdx.x);
+#endif
+}
+
+// dQ and dR, which share nothing but their input, in one launch
+template <int DT, class S>
+static __global__ __launch_bounds__(S::THREADS) void gradients_kernel(const Args q, const Args r) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    if (blockIdx.x < q.blocks) work<DT, S, true, false, EPI_DQ>(q, blockIdx.x);
+    else work<DT, S, true, true, EPI_DR>(r, blockIdx.x - q.blocks);
 #endif
 }
 

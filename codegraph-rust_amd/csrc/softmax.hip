@@ -30,7 +30,7 @@ constexpr uint32_t CUS = 256;                                  // workgroups of 
 // 512, 2.97 with 1024); the corpus' gradient needs some 256 tiles a piece, however many queries there are
 constexpr uint64_t PIECE_BYTES = 512ull << 20, PIECE_ROWS = 16384;
 
-// ---- weights of a query's list: one wave, entry j at lane j % 64, slot j / 64 ------------------------------------------------
+// ---- weights of a query's list (WEIGHTS; else only its ids and the anchor): one wave, entry j at lane j % 64, slot j / 64 -----
 struct List {
     uint32_t id[4];       // NONE: weight 0
     double logp[4], p[4];
@@ -46,6 +46,7 @@ __device__ inline T wave_sum(T v) {
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
+template <bool WEIGHTS = true>
 __device__ inline List read_list(const int64_t* ids, const float* ts, uint64_t i, uint32_t k, uint64_t n_rows, float tscale, int lane) {
     List l;
     float raw[4], mx = -INFINITY;
@@ -74,9 +75,11 @@ __device__ inline List read_list(const int64_t* ids, const float* ts, uint64_t i
     uint32_t first = NONE;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        l.logp[s] = l.id[s] == NONE ? 0.0 : (raw[s] - top) * (double)(ts ? tscale : 0.0f);
-        l.p[s] = l.id[s] == NONE ? 0.0 : exp(l.logp[s]);
-        z += l.p[s];
+        if (WEIGHTS) {
+            l.logp[s] = l.id[s] == NONE ? 0.0 : (raw[s] - top) * (double)(ts ? tscale : 0.0f);
+            l.p[s] = l.id[s] == NONE ? 0.0 : exp(l.logp[s]);
+            z += l.p[s];
+        }
         const uint64_t eq = __ballot(l.id[s] != NONE && (double)raw[s] == top);
         if (first == NONE && eq) first = s * 64 + __ffsll((unsigned long long)eq) - 1;
     }
@@ -85,6 +88,8 @@ __device__ inline List read_list(const int64_t* ids, const float* ts, uint64_t i
             const uint64_t some = __ballot(l.id[s] != NONE);
             if (first == NONE && some) first = s * 64 + __ffsll((unsigned long long)some) - 1;
         }
+    l.anchor = first;
+    if (!WEIGHTS) return l;
     z = wave_sum(z);
     const double lz = log(z);
 #pragma unroll
@@ -95,7 +100,6 @@ __device__ inline List read_list(const int64_t* ids, const float* ts, uint64_t i
             if (l.p[s] == 0.0) l.id[s] = NONE;      // underflow: no weight, and no 0 * inf below
         }
     }
-    l.anchor = first;
     return l;
 }
 template <class T>
@@ -182,21 +186,24 @@ struct Problem {
 // (the first piece of the corpus is copied by further workgroups of the same launch)
 template <int DT>
 __global__ __launch_bounds__(256) void forward_prep_kernel(Problem P, uint32_t* __restrict__ anchor, Piece first) {
-    if (blockIdx.x >= P.bp) return copy_piece_block<DT>(first, blockIdx.x - P.bp);
-    const uint32_t i = blockIdx.x, wave = threadIdx.x >> 6;
+    const uint32_t lists = (P.k + 15) / 16;            // workgroups of a query
+    if (blockIdx.x >= P.bp * lists) return copy_piece_block<DT>(first, blockIdx.x - P.bp * lists);
+    const uint32_t i = blockIdx.x / lists, list = blockIdx.x % lists, wave = threadIdx.x >> 6;
     const int lane = threadIdx.x & 63;
     const uint64_t plane = (uint64_t)P.bp * P.dp;
     uint16_t* dst = P.qws + (uint64_t)i * P.dp;
     if (i >= P.b) {
+        if (list) return;
         copy_row<DT>(nullptr, 0, P.dim, P.dp, dst, plane, threadIdx.x, 256);
         if (threadIdx.x == 0) anchor[i] = NONE;
         return;
     }
-    const List l = read_list(P.ids, P.tscores, i, P.k, P.n_rows, P.tscale, lane);
-    copy_row<DT>(l.has ? P.queries : nullptr, (uint64_t)i * P.q_stride, P.dim, P.dp, dst, plane, threadIdx.x, 256);
-    // the listed rows' scores in 64 bits - a small loss and its gradient are as exact as the anchor's score -, four rows of a wave at a time
+    const List l = read_list<false>(P.ids, P.tscores, i, P.k, P.n_rows, P.tscale, lane);
+    if (!list) copy_row<DT>(l.has ? P.queries : nullptr, (uint64_t)i * P.q_stride, P.dim, P.dp, dst, plane, threadIdx.x, 256);
+    // the listed rows' scores in 64 bits - a small loss and its gradient are as exact as the anchor's score -, four rows a wave
     double* sv = P.saved + (uint64_t)i * (P.k + 2);
-    for (uint32_t j0 = wave; j0 < P.k; j0 += 16) {
+    const uint32_t j0 = list * 16 + wave;
+    if (j0 < P.k) {
         uint32_t id[4];
         double s[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
@@ -213,11 +220,9 @@ __global__ __launch_bounds__(256) void forward_prep_kernel(Problem P, uint32_t* 
             if (lane == 0 && j0 + 4 * x < P.k) sv[2 + j0 + 4 * x] = v;
         }
     }
-    if (threadIdx.x == 0) anchor[i] = NONE;
-    if (l.has && wave == 0) {
-        const uint32_t a = pick(l.id, l.anchor);
-        if (lane == 0) anchor[i] = a;
-    }
+    if (list || wave) return;
+    const uint32_t a = l.has ? pick(l.id, l.anchor) : NONE;
+    if (lane == 0) anchor[i] = a;
 }
 
 // one wave per query: the corpus' partial maxima and sums, the loss
@@ -327,26 +332,6 @@ __global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ c
     }
 }
 
-// the listed rows' entries of G for the corpus rows [n0, n0 + c)
-template <int DT>
-__global__ __launch_bounds__(256) void patch_kernel(const uint32_t* __restrict__ ent_id, const float* __restrict__ ent_val, uint64_t total, uint32_t k,
-                                                    uint64_t n0, uint32_t c, const float* __restrict__ mul, uint16_t* __restrict__ G, uint64_t ld,
-                                                    uint64_t plane) {
-    const uint64_t t = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if (t >= total) return;
-    const uint32_t id = ent_id[t];
-    if (id == NONE || id < n0 || id - n0 >= c) return;
-    uint16_t* g = G + t / k * ld + (id - n0);
-    const float v = ent_val[t] * mul[0];
-    if (DT == cgv::DT_F32) {
-        uint16_t p[3];
-        split3(v, p);
-        for (int x = 0; x < 3; ++x) g[x * plane] = p[x];
-    } else {
-        g[0] = f32_to_half<DT>(v);
-    }
-}
-
 // dQ: the shares' partial sums, added in a fixed order and rounded once. 64 threads a stretch of 256 elements, four groups of shares
 template <int DT>
 __global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict__ part, uint32_t splits, uint64_t share, uint32_t dim, uint32_t dp,
@@ -376,7 +361,10 @@ __global__ void zero_kernel(void* p, uint64_t total) {
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
 
-typedef Shape<64, 64, 1, 2> S64x64;
+typedef Shape<64, 64, 2, 2> S64x64;
+typedef Shape<64, 64, 2, 2, 3> S64x64f;      // f32
+template <int DT>
+using Small = std::conditional_t<DT == cgv::DT_F32, S64x64f, S64x64>;
 typedef Shape<256, 64, 4, 1> S64;
 typedef Shape<256, 128, 4, 2> S128;
 typedef Shape<256, 192, 4, 2> S192;
@@ -394,17 +382,20 @@ struct Plan {
         dp = (uint32_t)up(dim_, 64);
         planes = dtype == CGV_DTYPE_F32 ? 3 : 1;
         copy = dtype == CGV_DTYPE_F32 || dim % 8 != 0;
-        // the tile width whose padded batch takes the least time: narrower tiles read LDS more often per product
+        // the tile width whose padded batch takes the least time. Narrower tiles read LDS more often per product: 768 queries over 200 k x 768
+        // (bf16, loss and both gradients) take 1.29 ms with tiles of 256, 1.35 with 192, 1.48 with 128, 1.91 with 64. Against that stands the
+        // padding: 576 queries take 0.99 ms with 192, 1.06 with 256, 1.14 with 128
         static const uint32_t width[4] = {256, 192, 128, 64};
-        static const double worth[4] = {1.0, 0.94, 0.83, 0.61};      // loss and gradients of 768 queries over 200 k x 768 with each
+        static const double worth[4] = {1.0, 0.95, 0.87, 0.68};
         double least = 1e30;
         for (int i = 0; i < 4; ++i) {
             const double t = up(bp, width[i]) / worth[i];
             if (t < least) least = t, bn = width[i];
         }
         bm = 256;
-        // few tiles: small ones on more CUs, with more stages on the way (32 queries x 10 k x 384, f32: 31 -> us)
-        if ((n_ + 255) / 256 * ((bp + bn - 1) / bn) < CUS / 2) bm = bn = 64;
+        // few tiles: small ones on more CUs, with more stages on the way. Loss and gradients of 256 queries x 768 with small and with large tiles,
+        // bf16: 127 and 134 us at 20 k rows, 156 and 148 at 25 k; f32: 317 and 401 us at 20 k, 481 and 512 at 30 k
+        if ((n_ + 255) / 256 * ((bp + bn - 1) / bn) < (planes == 3 ? CUS / 2 : CUS * 3 / 8)) bm = bn = 64;
         wm = bm == 64 ? S64x64::WM : bn == 256 ? S256::WM : S64::WM;
         tn = (bp + bn - 1) / bn;
         const uint64_t rows = up(n_, 256);
@@ -434,15 +425,15 @@ struct Plan {
     uint64_t b_bytes() const { return b_rows() + r_bytes(piece_b); }
 };
 
-void set_segments(Args& a, int dtype, bool swap) {
-    if (dtype != CGV_DTYPE_F32) {
+void set_segments(Args& a, int dtype, bool small) {
+    if (dtype != CGV_DTYPE_F32 || small) {       // small tiles: all planes are in a stage
         a.nseg = 1;
         a.sa[0] = a.sb[0] = 0;
         return;
     }
     static const uint32_t x[6] = {2, 0, 1, 1, 0, 0}, y[6] = {0, 2, 1, 0, 1, 0};   // the smallest products first
     a.nseg = 6;
-    for (int i = 0; i < 6; ++i) a.sa[i] = swap ? y[i] : x[i], a.sb[i] = swap ? x[i] : y[i];
+    for (int i = 0; i < 6; ++i) a.sa[i] = x[i], a.sb[i] = y[i];
 }
 
 template <int DT, class S, bool TA, bool TB, int EPI>
@@ -456,9 +447,20 @@ int launch_gemm(const Args& a, int device, hipStream_t s) {
     OPCHK(hipGetLastError());
     return CGV_OK;
 }
+template <int DT>
+int launch_gradients(const Args& q, const Args& r, int device, hipStream_t s) {
+    typedef Small<DT> S;
+    constexpr int bytes = S::lds_bytes(true);
+    void (*kern)(const Args, const Args) = gradients_kernel<DT, S>;
+    static LdsLimit limit;
+    OPCHK(limit.raise((const void*)kern, device, bytes));
+    hipLaunchKernelGGL(kern, dim3(q.blocks + r.blocks), dim3(S::THREADS), bytes, s, q, r);
+    OPCHK(hipGetLastError());
+    return CGV_OK;
+}
 template <int DT, bool TA, bool TB, int EPI>
 int launch_by_queries(const Plan& pl, const Args& a, int device, hipStream_t s) {
-    if (pl.bm == 64) return launch_gemm<DT, S64x64, TA, TB, EPI>(a, device, s);
+    if (pl.bm == 64) return launch_gemm<DT, Small<DT>, TA, TB, EPI>(a, device, s);
     const uint32_t bn = pl.bn;
     if (bn == 192) return launch_gemm<DT, S192, TA, TB, EPI>(a, device, s);
     return bn == 64 ? launch_gemm<DT, S64, TA, TB, EPI>(a, device, s) : bn == 128 ? launch_gemm<DT, S128, TA, TB, EPI>(a, device, s)
@@ -470,7 +472,7 @@ Args score_args(const Plan& pl, const Problem& P, int dtype, const char* rows, u
     Args a{};
     a.a = {rows, pitch, plane, c};
     a.b = {(const char*)P.qws, (uint64_t)pl.dp * 2, (uint64_t)pl.bp * pl.dp * 2, pl.bp};
-    set_segments(a, dtype, false);
+    set_segments(a, dtype, pl.bm == 64);
     a.ksteps = pl.dp / BK;
     a.kvalid = pl.copy ? pl.dp : pl.dim;
     a.tm = (c + pl.bm - 1) / pl.bm;
@@ -504,7 +506,7 @@ int forward(const Plan& pl, Problem P, int dtype, float* loss, char* ws, hipStre
     uint32_t* anchor = (uint32_t*)(ws + pl.f_anchor());
     float2* part = (float2*)(ws + pl.f_part());
     const Piece first = piece_of(pl, P, 0, pl.piece_f, ws + pl.f_rows());
-    hipLaunchKernelGGL((forward_prep_kernel<DT>), dim3(pl.bp + copy_blocks(first)), dim3(256), 0, s, P, anchor, first);
+    hipLaunchKernelGGL((forward_prep_kernel<DT>), dim3(pl.bp * ((pl.k + 15) / 16) + copy_blocks(first)), dim3(256), 0, s, P, anchor, first);
     OPCHK(hipGetLastError());
     uint32_t parts = 0;
     for (uint64_t n0 = 0; n0 < pl.n; n0 += pl.piece_f) {
@@ -542,6 +544,7 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
     float* ent_val = (float*)(ent_id + (uint64_t)pl.b * pl.k);
     char* G = ws + pl.b_g();
     float* part = (float*)(ws + pl.b_part());
+    const uint32_t splits = pl.dq_splits;
     const uint64_t g_pitch = pl.piece_b * 2, g_plane = (uint64_t)pl.bp * g_pitch;
     const Piece first = piece_of(pl, P, 0, pl.piece_b, ws + pl.b_rows());
     hipLaunchKernelGGL((backward_prep_kernel<DT>), dim3(pl.bp + copy_blocks(first)), dim3(256), 0, s, P, dloss, coef, lse2, has, ent_id, ent_val, mul, first);
@@ -565,24 +568,26 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
         a.coef = coef;
         a.lse2 = lse2;
         a.unscale = mul;
+        a.row0 = n0;
+        a.ent_id = ent_id;
+        a.ent_val = ent_val;
+        a.ent_k = pl.k;
         a.out = G;
         a.out_pitch = g_pitch;
         a.out_plane = g_plane;
         if ((rc = launch_by_queries<DT, false, false, EPI_G>(pl, a, P.device, s))) return rc;
-        const uint64_t total = (uint64_t)pl.b * pl.k;
-        hipLaunchKernelGGL((patch_kernel<DT>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, (const uint32_t*)ent_id, (const float*)ent_val, total,
-                           pl.k, n0, c, (const float*)mul, (uint16_t*)G, pl.piece_b, g_plane / 2);
-        OPCHK(hipGetLastError());
+        // the corpus' gradient: large tiles if they are enough to occupy half the card; in small ones both gradients share a launch
+        const bool big = dr && (uint64_t)((pl.dim + 255) / 256) * ((c + 255) / 256) >= CUS / 2, together = dq && dr && !big && pl.bm == 64;
+        Args d{}, e{};
         if (dq) {
-            Args d{};
             d.a = {rows, pitch, plane, pl.copy ? pl.dp : pl.dim};
             d.b = {G, g_pitch, g_plane, pl.bp};
-            set_segments(d, dtype, false);
+            set_segments(d, dtype, pl.bm == 64);
             d.ksteps = (c + BK - 1) / BK;
             d.kvalid = c;
             d.tm = (pl.dp + pl.bm - 1) / pl.bm;
             d.tn = pl.tn;
-            d.splits = pl.dq_splits;
+            d.splits = splits;
             d.blocks = d.tm * d.tn * d.splits;
             d.m_valid = pl.dp;
             d.n_valid = pl.b;
@@ -590,47 +595,49 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             d.out = (char*)part;
             d.out_plane = (uint64_t)pl.bp * pl.dp * 4;
             d.accumulate = n0 > 0;
-            if ((rc = launch_by_queries<DT, true, false, EPI_DQ>(pl, d, P.device, s))) return rc;
         }
         if (dr) {
-            Args d{};
-            d.a = {(const char*)P.qws, (uint64_t)pl.dp * 2, (uint64_t)pl.bp * pl.dp * 2, pl.dp};
-            d.b = {G, g_pitch, g_plane, (uint32_t)pl.piece_b};
-            set_segments(d, dtype, false);
-            d.ksteps = pl.bp / BK;
-            d.kvalid = pl.bp;
-            const bool big = (uint64_t)((pl.dim + 255) / 256) * ((c + 255) / 256) >= CUS / 2;
+            e.a = {(const char*)P.qws, (uint64_t)pl.dp * 2, (uint64_t)pl.bp * pl.dp * 2, pl.dp};
+            e.b = {G, g_pitch, g_plane, (uint32_t)pl.piece_b};
+            e.ksteps = pl.bp / BK;
+            e.kvalid = pl.bp;
+            set_segments(e, dtype, !big);
             const uint32_t side = big ? 256 : 64;
-            d.tm = (pl.dim + side - 1) / side;
-            d.tn = (c + side - 1) / side;
-            d.splits = 1;
-            d.blocks = (uint32_t)std::min<uint64_t>((uint64_t)d.tm * d.tn, CUS);
-            d.m_valid = pl.dim;
-            d.n_valid = c;
-            d.out = (char*)dr + n0 * pl.dim * esize(dtype);
-            d.out_pitch = (uint64_t)pl.dim * esize(dtype);
-            d.vec_out = d.out_pitch % 16 == 0 && (uintptr_t)dr % 16 == 0;
-            d.unscale = mul + 1;
-            if ((rc = big ? launch_gemm<DT, S256, true, true, EPI_DR>(d, P.device, s) : launch_gemm<DT, S64x64, true, true, EPI_DR>(d, P.device, s))) return rc;
+            e.tm = (pl.dim + side - 1) / side;
+            e.tn = (c + side - 1) / side;
+            e.splits = 1;
+            e.blocks = (uint32_t)std::min<uint64_t>((uint64_t)e.tm * e.tn, CUS);
+            e.m_valid = pl.dim;
+            e.n_valid = c;
+            e.out = (char*)dr + n0 * pl.dim * esize(dtype);
+            e.out_pitch = (uint64_t)pl.dim * esize(dtype);
+            e.vec_out = e.out_pitch % 16 == 0 && (uintptr_t)dr % 16 == 0;
+            e.unscale = mul + 1;
         }
+        if (together) {
+            if ((rc = launch_gradients<DT>(d, e, P.device, s))) return rc;
+            continue;
+        }
+        if (dq && (rc = launch_by_queries<DT, true, false, EPI_DQ>(pl, d, P.device, s))) return rc;
+        if (dr && (rc = big ? launch_gemm<DT, S256, true, true, EPI_DR>(e, P.device, s) : launch_gemm<DT, Small<DT>, true, true, EPI_DR>(e, P.device, s))) return rc;
     }
     if (dq) {
-        hipLaunchKernelGGL((finish_dq_kernel<DT>), dim3(pl.b, (pl.dim + 255) / 256), dim3(256), 0, s, (const float*)part, pl.dq_splits, (uint64_t)pl.bp * pl.dp, pl.dim, pl.dp,
-                           (const uint32_t*)has, (const float*)mul, dq);
+        hipLaunchKernelGGL((finish_dq_kernel<DT>), dim3(pl.b, (pl.dim + 255) / 256), dim3(256), 0, s, (const float*)part, splits, (uint64_t)pl.bp * pl.dp,
+                           pl.dim, pl.dp, (const uint32_t*)has, (const float*)mul, dq);
         OPCHK(hipGetLastError());
     }
     return CGV_OK;
 }
 
 bool sizes_ok(uint64_t b, uint64_t n_rows, uint32_t dim, uint32_t k, int dtype) {
-    return b <= (1ull << 24) && n_rows >= 1 && n_rows < (1ull << 31) - 1 && dim >= 1 && dim <= 8192 && k >= 1 && k <= MAX_K &&
+    return b <= (1ull << 19) && n_rows >= 1 && n_rows < (1ull << 31) - 1 && dim >= 1 && dim <= 8192 && k >= 1 && k <= MAX_K &&
            (dtype == CGV_DTYPE_F32 || dtype == CGV_DTYPE_BF16 || dtype == CGV_DTYPE_FP16);
 }
 
 int check_loss(const void* q, uint64_t qs, const void* r, uint64_t rs, int dtype, uint64_t b, uint64_t n, uint32_t dim, const int64_t* ids, uint32_t k,
                float scale, float tscale, const void* saved) {
     if (dtype != CGV_DTYPE_F32 && dtype != CGV_DTYPE_BF16 && dtype != CGV_DTYPE_FP16) return fail(CGV_ERR_INVALID_ARG, "dtype must be f32, bf16 or fp16");
-    if (!sizes_ok(b, n, dim, k, dtype)) return fail(CGV_ERR_INVALID_ARG, "b must be at most 2^24, n_rows in 1..2^31 - 1, dim in 1..=8192, k in 1..=256");
+    if (!sizes_ok(b, n, dim, k, dtype)) return fail(CGV_ERR_INVALID_ARG, "b must be at most 2^19, n_rows in 1..2^31 - 1, dim in 1..=8192, k in 1..=256");
     if (qs < dim || rs < dim) return fail(CGV_ERR_INVALID_ARG, "a stride is smaller than dim");
     if (!(fabsf(scale) < INFINITY) || !(fabsf(tscale) < INFINITY)) return fail(CGV_ERR_NONFINITE, "scale is not finite");
     if (!r || (b && (!q || !ids || !saved))) return fail(CGV_ERR_INVALID_ARG, "NULL argument");

@@ -131,7 +131,7 @@ def lookup_rows_grad(dout, ids, n_rows, scale=1.0):
 def _loss(queries, rows, ids, scores, scale, teacher_scale):
     L = lib()
     b, d = queries.shape
-    n, k = rows.shape[0], ids.shape[1]
+    n, k = rows.shape[0], 1 if scores is None else ids.shape[1]      # the targets of a cross entropy: lists of one
     code, dev = _CODES[rows.dtype], rows.device
     loss = torch.empty((b,), dtype=torch.float32, device=dev)
     saved = torch.empty((b * (k + 2),), dtype=torch.float64, device=dev)
@@ -156,7 +156,7 @@ class _CorpusLoss(torch.autograd.Function):
         L = lib()
         queries, rows, ids, scores, saved = ctx.saved_tensors
         b, d = queries.shape
-        n, k = rows.shape[0], ids.shape[1]
+        n, k = rows.shape[0], 1 if scores is None else ids.shape[1]
         code, dev = _CODES[rows.dtype], rows.device
         dq = torch.empty((b, d), dtype=queries.dtype, device=dev) if ctx.needs_input_grad[0] else None
         dr = torch.empty((n, d), dtype=rows.dtype, device=dev) if ctx.needs_input_grad[1] else None
@@ -193,7 +193,7 @@ def corpus_cross_entropy(queries, rows, targets, scale=1.0):
     targets = _ids(targets, "targets", queries.device if isinstance(queries, torch.Tensor) else None)
     if targets.dim() != 1 or targets.shape[0] != queries.shape[0]:
         raise _bad(f"targets {tuple(targets.shape)} do not fit queries {tuple(queries.shape)}", CGV_ERR_DIM_MISMATCH)
-    return _corpus_loss(queries, rows, targets[:, None], None, scale, 1.0)
+    return _corpus_loss(queries, rows, targets, None, scale, 1.0)
 
 
 def corpus_distillation(queries, rows, teacher_ids, teacher_scores, scale=1.0, teacher_scale=1.0):
