@@ -238,12 +238,12 @@ struct Half {
     }
 };
 
-// queries q0 .. q1 - 1 into their places (LDS, or the image of it in memory), by a workgroup: largest magnitudes first (as bits: NaN
+// all queries into their places in LDS, by a workgroup: largest magnitudes first (as bits: NaN
 // and Inf win), then the parts. A thread has four elements on their way at a time
 template <class P, uint32_t THREADS>
-__device__ inline void stage_queries(const ScoreArgs& a, uint32_t q0, uint32_t q1, char* xs, uint32_t rows, int* expo, uint32_t* top) {
-    const uint32_t kp = a.L.kc * CHUNK, total = (q1 - q0) * kp;
-    for (uint32_t q = threadIdx.x; q < q1 - q0; q += THREADS) top[q] = 0;
+__device__ inline void stage_queries(const ScoreArgs& a, char* xs, uint32_t rows, int* expo, uint32_t* top) {
+    const uint32_t kp = a.L.kc * CHUNK, total = a.m * kp;
+    for (uint32_t q = threadIdx.x; q < a.m; q += THREADS) top[q] = 0;
     __syncthreads();
     constexpr uint32_t BATCH = 4;
     for (int pass = 0; pass < 2; ++pass) {
@@ -252,7 +252,7 @@ __device__ inline void stage_queries(const ScoreArgs& a, uint32_t q0, uint32_t q
 #pragma unroll
             for (uint32_t j = 0; j < BATCH; ++j) {
                 const uint32_t i = i0 + j * THREADS + threadIdx.x, q = i / kp, e = i - q * kp;
-                v[j] = i < total && e < a.L.dim ? load_query(a.queries, a.qdt, (uint64_t)(q0 + q) * a.L.dim + e) : 0.0f;
+                v[j] = i < total && e < a.L.dim ? load_query(a.queries, a.qdt, (uint64_t)q * a.L.dim + e) : 0.0f;
             }
 #pragma unroll
             for (uint32_t j = 0; j < BATCH; ++j) {
@@ -266,8 +266,8 @@ __device__ inline void stage_queries(const ScoreArgs& a, uint32_t q0, uint32_t q
                     const uint32_t t = top[q];
                     const bool bad = t >= 0x7f800000u;
                     const int ex = bad ? 0 : P::unit(__uint_as_float(t));
-                    P::stage(xs, rows, q0 + q, e, bad ? 0.0f : ldexpf(v[j], ex));
-                    if (e == 0) expo[q0 + q] = bad ? INT_MIN : P::SCORE_SHIFT - ex;
+                    P::stage(xs, rows, q, e, bad ? 0.0f : ldexpf(v[j], ex));
+                    if (e == 0) expo[q] = bad ? INT_MIN : P::SCORE_SHIFT - ex;
                 }
             }
         }
@@ -275,12 +275,31 @@ __device__ inline void stage_queries(const ScoreArgs& a, uint32_t q0, uint32_t q
     }
 }
 
-// a workgroup per query: the image of what the kernel below wants in LDS
+// a workgroup per query: the image of what the kernel below wants in LDS. A query stays in registers between the two steps
 template <class P>
-__global__ __launch_bounds__(256) void q4_image_kernel(ScoreArgs a, char* image) {
-    __shared__ uint32_t top;
-    const uint32_t rows = a.m * P::ROWS;
-    stage_queries<P, 256>(a, blockIdx.x, blockIdx.x + 1, image, rows, (int*)(image + (uint64_t)(a.L.kc * CHUNK / 32) * rows * P::ROW_BYTES), &top);
+__global__ __launch_bounds__(1024) void q4_image_kernel(ScoreArgs a, char* image) {
+    __shared__ uint32_t tops[16];
+    const uint32_t rows = a.m * P::ROWS, kp = a.L.kc * CHUNK, q = blockIdx.x;
+    float v[8];                                        // dim is at most 8192
+    uint32_t bits = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+        const uint32_t e = j * 1024 + threadIdx.x;
+        v[j] = e < a.L.dim ? load_query(a.queries, a.qdt, (uint64_t)q * a.L.dim + e) : 0.0f;
+        bits = max(bits, __float_as_uint(fabsf(v[j])));
+    }
+    for (int o = 32; o; o >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, o));
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = bits;
+    __syncthreads();
+    for (int x = 0; x < 16; ++x) bits = max(bits, tops[x]);
+    const bool bad = bits >= 0x7f800000u;
+    const int ex = bad ? 0 : P::unit(__uint_as_float(bits));
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+        const uint32_t e = j * 1024 + threadIdx.x;
+        if (e < kp) P::stage(image, rows, q, e, bad ? 0.0f : ldexpf(v[j], ex));
+    }
+    if (threadIdx.x == 0) ((int*)(image + (uint64_t)(kp / 32) * rows * P::ROW_BYTES))[q] = bad ? INT_MIN : P::SCORE_SHIFT - ex;
 }
 
 // MT operands of queries, NT tiles at a time
@@ -326,7 +345,7 @@ __global__ __launch_bounds__(64 * WAVES) void q4_scores_kernel(ScoreArgs a) {
         for (uint32_t i = threadIdx.x; i < pieces; i += 64 * WAVES) ((uint4*)xs)[i] = src[i];
         for (uint32_t i = threadIdx.x; i < a.m; i += 64 * WAVES) expo[i] = ((const int*)(src + pieces))[i];
     } else {
-        stage_queries<P, 64 * WAVES>(a, 0, a.m, xs, rows, expo, (uint32_t*)expo + a.m);
+        stage_queries<P, 64 * WAVES>(a, xs, rows, expo, (uint32_t*)expo + a.m);
     }
     __syncthreads();
 
@@ -550,7 +569,7 @@ int scores_by(const cgv_q4_index* h, const void* q, int qdt, uint32_t m, float* 
         ScoreArgs a{(const u32x4*)h->codes, h->scales, (const char*)q + (uint64_t)i * h->L.dim * esize(qdt), out + (uint64_t)i * h->n, h->n, h->L,
                     std::min(most, m - i), qdt, nullptr};
         if ((uint64_t)a.m * h->L.kc * CHUNK > STAGE_IN_PLACE) {
-            hipLaunchKernelGGL((q4_image_kernel<P>), dim3(a.m), dim3(256), 0, s, a, ws);
+            hipLaunchKernelGGL((q4_image_kernel<P>), dim3(a.m), dim3(1024), 0, s, a, ws);
             OPCHK(hipGetLastError());
             a.image = ws;
         }

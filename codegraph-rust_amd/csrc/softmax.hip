@@ -204,15 +204,27 @@ __global__ __launch_bounds__(256) void forward_prep_kernel(Problem P, uint32_t* 
     double* sv = P.saved + (uint64_t)i * (P.k + 2);
     const uint32_t j0 = list * 16 + wave;
     if (j0 < P.k) {
-        uint32_t id[4];
+        uint64_t at[4];                                // an entry without a row reads row 0, and nobody its score
         double s[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) id[x] = j0 + 4 * x < P.k ? pick(l.id, j0 + 4 * x) : NONE;
-        for (uint32_t e = lane; e < P.dim; e += 64) {
-            const double q = load_elem<DT>(P.queries, (uint64_t)i * P.q_stride + e);
+        for (int x = 0; x < 4; ++x) {
+            const uint32_t id = j0 + 4 * x < P.k ? pick(l.id, j0 + 4 * x) : NONE;
+            at[x] = id == NONE ? 0 : (uint64_t)id * P.r_stride;
+        }
+        for (uint32_t e0 = 0; e0 < P.dim; e0 += 256) { // 20 loads on their way at a time
+            float q[4], r[4][4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-                if (id[x] != NONE) s[x] = fma(q, (double)load_elem<DT>(P.rows, (uint64_t)id[x] * P.r_stride + e), s[x]);
+            for (int y = 0; y < 4; ++y) {
+                const uint32_t e = e0 + y * 64 + lane, ec = min(e, P.dim - 1);
+                q[y] = load_elem<DT>(P.queries, (uint64_t)i * P.q_stride + ec);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) r[y][x] = load_elem<DT>(P.rows, at[x] + ec);
+                if (e >= P.dim) q[y] = r[y][0] = r[y][1] = r[y][2] = r[y][3] = 0.0f;
+            }
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) s[x] = fma((double)q[y], (double)r[y][x], s[x]);
         }
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
