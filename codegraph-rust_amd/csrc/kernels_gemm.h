@@ -66,9 +66,11 @@ struct Args {
     // epilogues
     float scale2;                                 // LSE, G: scores in units of log 2 = accumulator * scale2
     uint32_t m_valid, n_valid;                    // rows / columns of the result that exist
+    uint32_t n_pad;                               // LSE, G: columns that have a place in part / out, n_valid rounded up to 64
     uint64_t row0;                                // LSE, G: corpus row of m = 0
     const uint32_t* anchor;                       // LSE: [n] corpus row left out of the sum, 0xffffffff for none
-    float2* part;                                 // LSE: [splits * WM][part_ld] (maximum, sum)
+    float2* part;                                 // LSE: [slots][part_ld] (maximum, sum), slots at least splits * WM
+    uint32_t slots;
     uint32_t part_ld;
     const float* coef;                            // G: [n] factor
     const float2* lse2;                           // G: [n] log2 of the softmax sum, its f32 and what that leaves
@@ -528,7 +530,7 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
                             const uint32_t n = p * OUT + lane / LPR, chunk = (uint32_t)(lane % LPR) ^ row_swz(n);
                             const uint4 v = *(const uint4*)(xp + n * 128 + chunk * 16);
                             const uint32_t q = n0 + nb * 32 + n;
-                            if (q < g.part_ld)
+                            if (q < g.n_pad)
                                 *(uint4*)(g.out + plane * g.out_plane + q * g.out_pitch + (uint64_t)(m0 + mp * 32) * 2 + lane % LPR * 16) = v;
                         }
                         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -625,7 +627,12 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
             const float nm = fmaxf(run_m[nb], om), base = nm == -INFINITY ? 0.0f : nm;
             const float s = run_s[nb] * __builtin_amdgcn_exp2f(run_m[nb] - base) + os * __builtin_amdgcn_exp2f(om - base);
             const uint32_t q = n0 + nb * 32 + (lane & 31);
-            if (lane < 32 && q < g.part_ld) g.part[(uint64_t)(split * S::WM + wm) * g.part_ld + q] = make_float2(nm, s);
+            const uint32_t own = split * S::WM + wm;
+            if (lane < 32 && q < g.n_pad) {
+                g.part[(uint64_t)own * g.part_ld + q] = make_float2(nm, s);
+                for (uint32_t x = own + g.splits * S::WM; x < g.slots; x += g.splits * S::WM)      // other columns have more
+                    g.part[(uint64_t)x * g.part_ld + q] = make_float2(-INFINITY, 0.0f);
+            }
         }
     }
     if (EPI == EPI_G) {
@@ -663,6 +670,16 @@ template <int DT, class S, bool TA, bool TB, int EPI>
 static __global__ __launch_bounds__(S::THREADS) void gemm_kernel(const Args g) {
 #if defined(__HIP_DEVICE_COMPILE__)
     work<DT, S, TA, TB, EPI>(g, blockIdx.x);
+#endif
+}
+
+// columns of two widths: `a` with tiles of shape S, `b` with tiles of shape T
+template <int DT, class S, class T, bool TA, bool TB, int EPI>
+static __global__ __launch_bounds__(S::THREADS) void mixed_kernel(const Args a, const Args b) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    static_assert(S::THREADS == T::THREADS, "one workgroup size");
+    if (blockIdx.x < a.blocks) work<DT, S, TA, TB, EPI>(a, blockIdx.x);
+    else work<DT, T, TA, TB, EPI>(b, blockIdx.x - a.blocks);
 #endif
 }
 

@@ -385,10 +385,13 @@ typedef Shape<256, 256, 2, 4> S256;
 uint64_t up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
 struct Plan {
-    uint32_t b, bp, dim, dp, k, planes, bm, bn, wm, tn;   // tiles of the scores: corpus rows, queries; wave rows of a tile; tiles of the batch
+    uint32_t b, bp, dim, dp, k, planes, bm;               // bm: corpus rows of a tile of the scores
+    uint32_t bn, columns, bn2, off;                       // the batch: `columns` tiles of bn queries, and from query `off` on one of bn2 (0: none)
     bool copy;                     // corpus rows go through a padded copy
     uint64_t n, piece_f, piece_b;  // corpus rows of a piece, forward and backward
-    uint32_t parts_per_piece, dq_splits;
+    uint32_t parts;                // (maximum, sum) pairs of a query, all pieces together
+    struct Shares { uint32_t s1, s2; };                   // shares of the long axis, for the columns of bn and for that of bn2
+    uint32_t dqn, dq_columns, dq_splits;                  // dQ: tiles of dqn queries, shares of the corpus
     Plan(uint64_t b_, uint64_t n_, uint32_t dim_, uint32_t k_, int dtype) : b((uint32_t)b_), dim(dim_), k(k_), n(n_) {
         bp = (uint32_t)up(std::max<uint64_t>(b_, 1), 64);
         dp = (uint32_t)up(dim_, 64);
@@ -397,28 +400,59 @@ struct Plan {
         // the tile width whose padded batch takes the least time. Narrower tiles read LDS more often per product: 768 queries over 200 k x 768
         // (bf16, loss and both gradients) take 1.29 ms with tiles of 256, 1.35 with 192, 1.48 with 128, 1.91 with 64. Against that stands the
         // padding: 576 queries take 0.99 ms with 192, 1.06 with 256, 1.14 with 128
-        static const uint32_t width[4] = {256, 192, 128, 64};
-        static const double worth[4] = {1.0, 0.95, 0.87, 0.68};
+        // The scores' last column may be narrower than the others (loss of 320 queries as 192 + 128: 130 us, as 2 x 192: 163 us). Not so dQ's:
+        // columns with different shares of the corpus do not read it together (300 queries x 300 k x 1000: 339 us, with equal columns 304 us)
         double least = 1e30;
         for (int i = 0; i < 4; ++i) {
-            const double t = up(bp, width[i]) / worth[i];
-            if (t < least) least = t, bn = width[i];
+            const double t = (bp + WIDTH[i] - 1) / WIDTH[i] * cost(WIDTH[i]);
+            if (t < least) least = t, bn = WIDTH[i], bn2 = 0;
         }
+        dqn = bn;
+        for (int i = 0; i < 2; ++i)
+            for (int j = i + 1; j < 3; ++j) {
+                const uint32_t w = WIDTH[i];
+                if (bp <= WIDTH[j]) continue;
+                const double t = (bp - WIDTH[j] + w - 1) / w * cost(w) + cost(WIDTH[j]);
+                if (t < 0.97 * least) least = t, bn = w, bn2 = WIDTH[j];
+            }
         bm = 256;
         // few tiles: small ones on more CUs, with more stages on the way. Loss and gradients of 256 queries x 768 with small and with large tiles,
         // bf16: 127 and 134 us at 20 k rows, 156 and 148 at 25 k; f32: 317 and 401 us at 20 k, 481 and 512 at 30 k
-        if ((n_ + 255) / 256 * ((bp + bn - 1) / bn) < (planes == 3 ? CUS / 2 : CUS * 3 / 8)) bm = bn = 64;
-        wm = bm == 64 ? S64x64::WM : bn == 256 ? S256::WM : S64::WM;
-        tn = (bp + bn - 1) / bn;
+        if ((n_ + 255) / 256 * ((bp - bn2 + bn - 1) / bn + (bn2 > 0)) < (planes == 3 ? CUS / 2 : CUS * 3 / 8)) bm = bn = dqn = 64, bn2 = 0;
+        columns = (bp - bn2 + bn - 1) / bn;
+        off = bn2 ? columns * bn : bp;
         const uint64_t rows = up(n_, 256);
         const uint64_t by_copy = copy ? std::max<uint64_t>(256, PIECE_BYTES / ((uint64_t)dp * 2 * planes) / 256 * 256) : rows;
         const uint64_t by_g = std::max<uint64_t>(PIECE_ROWS, PIECE_BYTES / ((uint64_t)bp * 2 * planes) / 256 * 256);
         piece_f = std::min(rows, by_copy);
         piece_b = std::min(rows, std::min(by_copy, by_g));
         if (piece_b < rows && piece_b > 256 * CUS / 4) piece_b = piece_b / (256 * CUS / 4) * (256 * CUS / 4);
-        parts_per_piece = std::max<uint32_t>(1, CUS / tn) * wm;
-        const uint32_t dq_tiles = ((dp + bm - 1) / bm) * tn;
-        dq_splits = std::max<uint32_t>(1, std::min<uint32_t>((uint32_t)(piece_b / BK), CUS / dq_tiles));
+        const uint64_t last = n - (pieces_f() - 1) * piece_f;
+        parts = (uint32_t)((pieces_f() - 1) * slots(score_shares((uint32_t)(piece_f / bm))) + slots(score_shares((uint32_t)((last + bm - 1) / bm))));
+        dq_columns = (bp + dqn - 1) / dqn;
+        dq_splits = std::max<uint32_t>(1, std::min<uint32_t>((uint32_t)(piece_b / BK), CUS / ((dp + bm - 1) / bm * dq_columns)));
+    }
+    static constexpr uint32_t WIDTH[4] = {256, 192, 128, 64};
+    static double cost(uint32_t w) { return w / (w == 256 ? 1.0 : w == 192 ? 0.95 : w == 128 ? 0.87 : 0.68); }
+    static uint32_t wave_rows(uint32_t bm, uint32_t bn) { return bm == 64 ? S64x64::WM : bn == 256 ? S256::WM : S64::WM; }
+    uint32_t slots(Shares s) const { return std::max(s.s1 * wave_rows(bm, bn), bn2 ? s.s2 * wave_rows(bm, bn2) : 0u); }
+    // shares of `tm` rows of tiles that occupy the card and end together, no more than the same time needs
+    Shares score_shares(uint32_t tm) const {
+        Shares s{std::max<uint32_t>(1, std::min(tm, CUS / columns)), 0};
+        if (bn2) {
+            double least = 1e30;
+            s = {1, 1};
+            for (uint32_t s1 = 1; s1 * columns < CUS; ++s1) {
+                const uint32_t s2 = CUS - s1 * columns;
+                const double t = std::max((tm + s1 - 1) / s1 * cost(bn), (tm + s2 - 1) / s2 * cost(bn2));
+                if (t < least) least = t, s = {std::min(tm, s1), std::min(tm, s2)};
+            }
+            const uint32_t each = (tm + s.s2 - 1) / s.s2;
+            s.s2 = (tm + each - 1) / each;
+        }
+        const uint32_t each = (tm + s.s1 - 1) / s.s1;
+        s.s1 = (tm + each - 1) / each;
+        return s;
     }
     uint64_t pieces_f() const { return (n + piece_f - 1) / piece_f; }
     uint64_t q_bytes() const { return up((uint64_t)planes * bp * dp * 2, 256); }
@@ -426,7 +460,7 @@ struct Plan {
     // forward workspace
     uint64_t f_anchor() const { return q_bytes(); }
     uint64_t f_part() const { return f_anchor() + up((uint64_t)bp * 4, 256); }
-    uint64_t f_rows() const { return f_part() + up(pieces_f() * parts_per_piece * bp * 8, 256); }
+    uint64_t f_rows() const { return f_part() + up((uint64_t)parts * bp * 8, 256); }
     uint64_t f_bytes() const { return f_rows() + r_bytes(piece_f); }
     // backward workspace
     uint64_t b_coef() const { return q_bytes(); }                       // lse2 (two f32), coef, has: [bp] each; mul: [2]
@@ -470,13 +504,52 @@ int launch_gradients(const Args& q, const Args& r, int device, hipStream_t s) {
     OPCHK(hipGetLastError());
     return CGV_OK;
 }
+template <int DT, class S, class T, bool TA, bool TB, int EPI>
+int launch_mixed(const Args& a, const Args& b, int device, hipStream_t s) {
+    constexpr bool xpose = EPI == EPI_G;
+    constexpr int bytes = std::max(S::lds_bytes(xpose), T::lds_bytes(xpose));
+    void (*kern)(const Args, const Args) = mixed_kernel<DT, S, T, TA, TB, EPI>;
+    static LdsLimit limit;
+    OPCHK(limit.raise((const void*)kern, device, bytes));
+    hipLaunchKernelGGL(kern, dim3(a.blocks + b.blocks), dim3(S::THREADS), bytes, s, a, b);
+    OPCHK(hipGetLastError());
+    return CGV_OK;
+}
 template <int DT, bool TA, bool TB, int EPI>
-int launch_by_queries(const Plan& pl, const Args& a, int device, hipStream_t s) {
-    if (pl.bm == 64) return launch_gemm<DT, Small<DT>, TA, TB, EPI>(a, device, s);
-    const uint32_t bn = pl.bn;
+int launch_by_width(const Args& a, uint32_t bm, uint32_t bn, int device, hipStream_t s) {
+    if (bm == 64) return launch_gemm<DT, Small<DT>, TA, TB, EPI>(a, device, s);
+    if (bn == 64) return launch_gemm<DT, S64, TA, TB, EPI>(a, device, s);
+    if (bn == 128) return launch_gemm<DT, S128, TA, TB, EPI>(a, device, s);
     if (bn == 192) return launch_gemm<DT, S192, TA, TB, EPI>(a, device, s);
-    return bn == 64 ? launch_gemm<DT, S64, TA, TB, EPI>(a, device, s) : bn == 128 ? launch_gemm<DT, S128, TA, TB, EPI>(a, device, s)
-                                                              : launch_gemm<DT, S256, TA, TB, EPI>(a, device, s);
+    return launch_gemm<DT, S256, TA, TB, EPI>(a, device, s);
+}
+// scores: the arguments `a` of all columns, and their shares
+template <int DT, int EPI>
+int launch_scores(const Plan& pl, Args a, Plan::Shares sh, int device, hipStream_t s) {
+    a.tn = pl.columns;
+    a.splits = sh.s1;
+    a.blocks = a.tn * a.splits;
+    if (!pl.bn2) return launch_by_width<DT, false, false, EPI>(a, pl.bm, pl.bn, device, s);
+    Args b = a;                        // the last column
+    b.tn = 1;
+    b.splits = b.blocks = sh.s2;
+    b.b.p += pl.off * b.b.pitch;
+    b.b.limit -= pl.off;
+    b.n_valid -= pl.off;
+    b.n_pad -= pl.off;
+    if (EPI == EPI_LSE) {
+        b.anchor += pl.off;
+        b.part += pl.off;
+    } else {
+        b.coef += pl.off;
+        b.lse2 += pl.off;
+        b.ent_id += (uint64_t)pl.off * b.ent_k;
+        b.ent_val += (uint64_t)pl.off * b.ent_k;
+        b.out += pl.off * b.out_pitch;
+    }
+    a.n_valid = a.n_pad = pl.off;
+    if (pl.bn2 == 192) return launch_mixed<DT, S256, S192, false, false, EPI>(a, b, device, s);
+    return pl.bn == 256 ? launch_mixed<DT, S256, S128, false, false, EPI>(a, b, device, s) : launch_mixed<DT, S192, S128, false, false, EPI>(a, b, device, s);
 }
 
 // scores of the corpus rows [n0, n0 + c) against all queries
@@ -488,15 +561,10 @@ Args score_args(const Plan& pl, const Problem& P, int dtype, const char* rows, u
     a.ksteps = pl.dp / BK;
     a.kvalid = pl.copy ? pl.dp : pl.dim;
     a.tm = (c + pl.bm - 1) / pl.bm;
-    a.tn = pl.tn;
-    const uint32_t most = std::max<uint32_t>(1, CUS / pl.tn);
-    const uint32_t each = (a.tm + most - 1) / most;
-    a.splits = (a.tm + each - 1) / each;
-    a.blocks = a.tn * a.splits;
     a.scale2 = (float)(P.scale * LOG2E);
     a.m_valid = c;
     a.n_valid = pl.b;
-    a.part_ld = pl.bp;
+    a.n_pad = a.part_ld = pl.bp;
     return a;
 }
 
@@ -536,8 +604,10 @@ int forward(const Plan& pl, Problem P, int dtype, float* loss, char* ws, hipStre
         a.row0 = n0;
         a.anchor = anchor;
         a.part = part + (uint64_t)parts * pl.bp;
-        parts += a.splits * pl.wm;
-        const int rc = launch_by_queries<DT, false, false, EPI_LSE>(pl, a, P.device, s);
+        const Plan::Shares sh = pl.score_shares(a.tm);
+        a.slots = pl.slots(sh);
+        parts += a.slots;
+        const int rc = launch_scores<DT, EPI_LSE>(pl, a, sh, P.device, s);
         if (rc) return rc;
     }
     hipLaunchKernelGGL(loss_kernel, dim3((pl.b + 3) / 4), dim3(256), 0, s, P, (const float2*)part, parts, loss);
@@ -556,7 +626,6 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
     float* ent_val = (float*)(ent_id + (uint64_t)pl.b * pl.k);
     char* G = ws + pl.b_g();
     float* part = (float*)(ws + pl.b_part());
-    const uint32_t splits = pl.dq_splits;
     const uint64_t g_pitch = pl.piece_b * 2, g_plane = (uint64_t)pl.bp * g_pitch;
     const Piece first = piece_of(pl, P, 0, pl.piece_b, ws + pl.b_rows());
     hipLaunchKernelGGL((backward_prep_kernel<DT>), dim3(pl.bp + copy_blocks(first)), dim3(256), 0, s, P, dloss, coef, lse2, has, ent_id, ent_val, mul, first);
@@ -587,7 +656,7 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
         a.out = G;
         a.out_pitch = g_pitch;
         a.out_plane = g_plane;
-        if ((rc = launch_by_queries<DT, false, false, EPI_G>(pl, a, P.device, s))) return rc;
+        if ((rc = launch_scores<DT, EPI_G>(pl, a, pl.score_shares(a.tm), P.device, s))) return rc;
         // the corpus' gradient: large tiles if they are enough to occupy half the card; in small ones both gradients share a launch
         const bool big = dr && (uint64_t)((pl.dim + 255) / 256) * ((c + 255) / 256) >= CUS / 2, together = dq && dr && !big && pl.bm == 64;
         Args d{}, e{};
@@ -598,8 +667,8 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             d.ksteps = (c + BK - 1) / BK;
             d.kvalid = c;
             d.tm = (pl.dp + pl.bm - 1) / pl.bm;
-            d.tn = pl.tn;
-            d.splits = splits;
+            d.tn = pl.dq_columns;
+            d.splits = pl.dq_splits;
             d.blocks = d.tm * d.tn * d.splits;
             d.m_valid = pl.dp;
             d.n_valid = pl.b;
@@ -630,11 +699,11 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             if ((rc = launch_gradients<DT>(d, e, P.device, s))) return rc;
             continue;
         }
-        if (dq && (rc = launch_by_queries<DT, true, false, EPI_DQ>(pl, d, P.device, s))) return rc;
+        if (dq && (rc = launch_by_width<DT, true, false, EPI_DQ>(d, pl.bm, pl.dqn, P.device, s))) return rc;
         if (dr && (rc = big ? launch_gemm<DT, S256, true, true, EPI_DR>(e, P.device, s) : launch_gemm<DT, Small<DT>, true, true, EPI_DR>(e, P.device, s))) return rc;
     }
     if (dq) {
-        hipLaunchKernelGGL((finish_dq_kernel<DT>), dim3(pl.b, (pl.dim + 255) / 256), dim3(256), 0, s, (const float*)part, splits, (uint64_t)pl.bp * pl.dp,
+        hipLaunchKernelGGL((finish_dq_kernel<DT>), dim3(pl.b, (pl.dim + 255) / 256), dim3(256), 0, s, (const float*)part, pl.dq_splits, (uint64_t)pl.bp * pl.dp,
                            pl.dim, pl.dp, (const uint32_t*)has, (const float*)mul, dq);
         OPCHK(hipGetLastError());
     }

@@ -136,6 +136,24 @@ def test_corpus_in_pieces(b, n, d, k, dt):
 
 
 @pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("b,n,d,k", [(300, 20_000, 72, 2), (430, 17_001, 96, 3), (640, 12_000, 63, 1), (700, 20_000, 40, 20), (3000, 6000, 64, 1),
+                                     (65_950, 300, 16, 1)])
+def test_batches_in_columns_of_two_widths(b, n, d, k, dt):
+    """Batches whose last column of tiles is narrower than the others, up to more columns than the card has CUs."""
+    m = pkg()
+    q, r, ids, sc, g = _problem(b, n, d, k, dt, b + 1)
+    ids[b - 1] = n - 1
+    ids[b - 2] = -1
+    q.requires_grad_()
+    r.requires_grad_()
+    ref = _reference(q.detach(), r.detach(), ids, sc, g, 8.0, 3.0)
+    loss = m.corpus_distillation(q, r, ids, sc, scale=8.0, teacher_scale=3.0)
+    dq, dr = torch.autograd.grad(loss, (q, r), g)
+    _check(loss.detach(), dq, dr, ref, d, n, 8.0, dt, g)
+    assert bool((dq[b - 2] == 0).all())
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
 def test_one_gradient_at_a_time(dt):
     m = pkg()
     q, r, ids, sc, g = _problem(70, 900, 128, 3, dt, 5)
