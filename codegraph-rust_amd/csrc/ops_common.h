@@ -80,6 +80,14 @@ struct LdsLimit {
     }
 };
 
+// a grid of any number of workgroups: a launch holds less than 2^32 threads in each direction, so the second one takes over
+constexpr uint64_t MOST_BLOCKS = 65535ull << 20;
+inline dim3 wide_grid(uint64_t blocks) {
+    const uint64_t x = std::min<uint64_t>(blocks, 1u << 20);
+    return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+__device__ inline uint64_t wide_block() { return (uint64_t)blockIdx.y * gridDim.x + blockIdx.x; }   // may be beyond the last one
+
 // 16-bit value -> f32 by storage type (CGV_DTYPE_BF16 / CGV_DTYPE_FP16)
 template <int DT>
 __device__ inline float half_to_f32(uint16_t v) {

@@ -10,6 +10,7 @@
 
 #include <mutex>
 #include <type_traits>
+#include <vector>
 
 #include "../../include/cgvec_q4.h"
 #include "ops_common.h"
@@ -416,6 +417,8 @@ struct cgv_q4_index {
     size_t stage_bytes = 0;
     uint32_t* bad = nullptr;
     hipStream_t stream = nullptr;
+    bool captured = false;          // a graph may hold the addresses of codes and scales
+    std::vector<void*> retired;     // such buffers that a larger corpus has left: kept for the graph's replays
     mutable std::mutex mu;
 };
 
@@ -436,6 +439,7 @@ int grow(cgv_q4_index* h, uint64_t rows, bool exact) {
     if (rows <= h->cap) return CGV_OK;
     uint64_t want = exact ? rows : std::max<uint64_t>(rows, h->cap + h->cap / 2);
     want = (std::max<uint64_t>(want, 1024) + 15) / 16 * 16;
+    if (h->captured) h->retired.reserve(h->retired.size() + 2);
     uint32_t* c = nullptr;
     uint16_t* s = nullptr;
     const uint64_t cb = h->L.tile_codes(want / 16), sb = h->L.tile_scales(want / 16) * 2;
@@ -452,8 +456,10 @@ int grow(cgv_q4_index* h, uint64_t rows, bool exact) {
         if (s) (void)hipFree(s);
         return fail(e == hipErrorOutOfMemory ? CGV_ERR_OOM : CGV_ERR_HIP, std::string("growing the 4-bit corpus: ") + hipGetErrorString(e));
     }
-    if (h->codes) (void)hipFree(h->codes);
-    if (h->scales) (void)hipFree(h->scales);
+    for (void* p : {(void*)h->codes, (void*)h->scales}) {
+        if (p && h->captured) h->retired.push_back(p);      // room for both was made beforehand
+        else if (p) (void)hipFree(p);
+    }
     h->codes = c;
     h->scales = s;
     h->cap = want;
@@ -518,7 +524,7 @@ template <class P, int SDT, int GPC, int MT, int NT, bool ONCE = false>
 int launch_scores(const cgv_q4_index* h, const ScoreArgs& a, hipStream_t s) {
     constexpr int WAVES = 8;
     const size_t lds = a.m * query_bytes<P>(h);
-    const uint64_t units = ((h->n + 15) / 16 + NT - 1) / NT;
+    const uint64_t units = ((a.n + 15) / 16 + NT - 1) / NT;
     const uint64_t per_cu = std::min<uint64_t>(2, LDS_MAX / lds);     // workgroups of a CU
     const unsigned blocks = (unsigned)std::min<uint64_t>((units + WAVES - 1) / WAVES, 256 * per_cu);
     void (*kern)(ScoreArgs) = q4_scores_kernel<P, SDT, GPC, MT, NT, ONCE, WAVES>;
@@ -536,8 +542,8 @@ int launch_by_queries(const cgv_q4_index* h, const ScoreArgs& a, hipStream_t s) 
     // Codes that the 256 MiB last-level cache cannot hold until the next call are read past it (1M x 768: 78 -> 69 us), smaller ones
     // stay there (250 k x 768, the same corpus again: 25 -> 21 us)
     if (a.m <= P::QPT) {
-        if (h->n < 16ull * 4 * 4096) return launch_scores<P, SDT, GPC, 1, 1>(h, a, s);
-        return h->L.tile_codes((h->n + 15) / 16) > (256ull << 20) ? launch_scores<P, SDT, GPC, 1, 2, true>(h, a, s)
+        if (a.n < 16ull * 4 * 4096) return launch_scores<P, SDT, GPC, 1, 1>(h, a, s);
+        return h->L.tile_codes((a.n + 15) / 16) > (256ull << 20) ? launch_scores<P, SDT, GPC, 1, 2, true>(h, a, s)
                                                                    : launch_scores<P, SDT, GPC, 1, 2>(h, a, s);
     }
     return a.m <= 2 * P::QPT ? launch_scores<P, SDT, GPC, 2, 2>(h, a, s)
@@ -563,10 +569,10 @@ size_t image_bytes(const cgv_q4_index* h, uint32_t m) {
 }
 
 template <class P>
-int scores_by(const cgv_q4_index* h, const void* q, int qdt, uint32_t m, float* out, char* ws, hipStream_t s) {
+int scores_by(const cgv_q4_index* h, const void* q, int qdt, uint32_t m, uint64_t n, float* out, char* ws, hipStream_t s) {
     const uint32_t most = queries_per_launch<P>(h);
     for (uint32_t i = 0; i < m; i += most) {
-        ScoreArgs a{(const u32x4*)h->codes, h->scales, (const char*)q + (uint64_t)i * h->L.dim * esize(qdt), out + (uint64_t)i * h->n, h->n, h->L,
+        ScoreArgs a{(const u32x4*)h->codes, h->scales, (const char*)q + (uint64_t)i * h->L.dim * esize(qdt), out + (uint64_t)i * n, n, h->L,
                     std::min(most, m - i), qdt, nullptr};
         if ((uint64_t)a.m * h->L.kc * CHUNK > STAGE_IN_PLACE) {
             hipLaunchKernelGGL((q4_image_kernel<P>), dim3(a.m), dim3(1024), 0, s, a, ws);
@@ -583,8 +589,8 @@ size_t scores_workspace(const cgv_q4_index* h, int qdt, uint32_t m) {
     return qdt == CGV_DTYPE_F32 ? image_bytes<Fixed>(h, m) : image_bytes<Half>(h, m);
 }
 
-int scores_on(const cgv_q4_index* h, const void* q, int qdt, uint32_t m, float* out, char* ws, hipStream_t s) {
-    return qdt == CGV_DTYPE_F32 ? scores_by<Fixed>(h, q, qdt, m, out, ws, s) : scores_by<Half>(h, q, qdt, m, out, ws, s);
+int scores_on(const cgv_q4_index* h, const void* q, int qdt, uint32_t m, uint64_t n, float* out, char* ws, hipStream_t s) {
+    return qdt == CGV_DTYPE_F32 ? scores_by<Fixed>(h, q, qdt, m, n, out, ws, s) : scores_by<Half>(h, q, qdt, m, n, out, ws, s);
 }
 
 }  // namespace
@@ -631,6 +637,7 @@ int cgv_q4_destroy(cgv_q4_index* h) {
     void* bufs[] = {h->codes, h->scales, h->stage, h->bad};
     for (void* p : bufs)
         if (p) (void)hipFree(p);   // waits for the device: scores in flight on any stream have ended
+    for (void* p : h->retired) (void)hipFree(p);
     if (h->stream) (void)hipStreamDestroy(h->stream);
     delete h;
     return CGV_OK;
@@ -758,17 +765,18 @@ int cgv_q4_get_row_f32(cgv_q4_index* h, uint64_t id, float* out_host) {
     });
 }
 
-int cgv_q4_scores_f32(cgv_q4_index* h, const float* queries_host, uint32_t m, float* out_host) {
+int cgv_q4_scores_f32(cgv_q4_index* h, const float* queries_host, uint32_t m, uint64_t n_rows, float* out_host) {
     return guarded([&]() -> int {
         if (!h) return fail(CGV_ERR_INVALID_ARG, "handle is NULL");
         std::lock_guard<std::mutex> lk(h->mu);
-        if (m == 0 || h->n == 0) return CGV_OK;
+        if (n_rows > h->n) return fail(CGV_ERR_OUT_OF_RANGE, "n_rows is beyond the last row");
+        if (m == 0 || n_rows == 0) return CGV_OK;
         if (!queries_host || !out_host) return fail(CGV_ERR_INVALID_ARG, "NULL argument");
         DeviceScope dev(h->device);
         OPCHK(dev.enter());
         // queries in pieces whose scores fit the staging buffer
-        const uint64_t per = std::max<uint64_t>(1, std::min<uint64_t>(m, (512ull << 20) / (h->n * 4)));
-        const size_t qb = ((size_t)per * h->L.dim * 4 + 255) / 256 * 256, sb = (per * h->n * 4 + 255) / 256 * 256;
+        const uint64_t per = std::max<uint64_t>(1, std::min<uint64_t>(m, (512ull << 20) / (n_rows * 4)));
+        const size_t qb = ((size_t)per * h->L.dim * 4 + 255) / 256 * 256, sb = (per * n_rows * 4 + 255) / 256 * 256;
         int rc = ensure_stage(h, qb + sb + scores_workspace(h, CGV_DTYPE_F32, (uint32_t)per));
         if (rc) return rc;
         float* dq = (float*)h->stage;
@@ -776,8 +784,8 @@ int cgv_q4_scores_f32(cgv_q4_index* h, const float* queries_host, uint32_t m, fl
         for (uint64_t a = 0; a < m; a += per) {
             const uint32_t c = (uint32_t)std::min<uint64_t>(per, m - a);
             OPCHK(hipMemcpyAsync(dq, queries_host + a * h->L.dim, (size_t)c * h->L.dim * 4, hipMemcpyHostToDevice, h->stream));
-            if ((rc = scores_on(h, dq, CGV_DTYPE_F32, c, ds, (char*)h->stage + qb + sb, h->stream))) return rc;
-            OPCHK(hipMemcpyAsync(out_host + a * h->n, ds, (size_t)c * h->n * 4, hipMemcpyDeviceToHost, h->stream));
+            if ((rc = scores_on(h, dq, CGV_DTYPE_F32, c, n_rows, ds, (char*)h->stage + qb + sb, h->stream))) return rc;
+            OPCHK(hipMemcpyAsync(out_host + a * n_rows, ds, (size_t)c * n_rows * 4, hipMemcpyDeviceToHost, h->stream));
             OPCHK(hipStreamSynchronize(h->stream));
         }
         return CGV_OK;
@@ -786,21 +794,27 @@ int cgv_q4_scores_f32(cgv_q4_index* h, const float* queries_host, uint32_t m, fl
 
 size_t cgv_q4_scores_workspace(const cgv_q4_index* h, int query_dtype, uint32_t m) { return h && m ? scores_workspace(h, query_dtype, m) : 0; }
 
-int cgv_q4_scores_dev(cgv_q4_index* h, const void* queries_dev, int query_dtype, uint32_t m, float* out_dev, void* workspace_dev,
+int cgv_q4_scores_dev(cgv_q4_index* h, const void* queries_dev, int query_dtype, uint32_t m, uint64_t n_rows, float* out_dev, void* workspace_dev,
                       size_t workspace_bytes, void* stream) {
     return guarded([&]() -> int {
         if (!h) return fail(CGV_ERR_INVALID_ARG, "handle is NULL");
         if (query_dtype != CGV_DTYPE_F32 && query_dtype != CGV_DTYPE_BF16 && query_dtype != CGV_DTYPE_FP16)
             return fail(CGV_ERR_INVALID_ARG, "dtype must be f32, bf16 or fp16");
         std::lock_guard<std::mutex> lk(h->mu);
-        if (m == 0 || h->n == 0) return CGV_OK;
+        if (n_rows > h->n) return fail(CGV_ERR_OUT_OF_RANGE, "n_rows is beyond the last row");
+        if (m == 0 || n_rows == 0) return CGV_OK;
         if (!queries_dev || !out_dev) return fail(CGV_ERR_INVALID_ARG, "NULL argument");
         const size_t need = scores_workspace(h, query_dtype, m);
         if (workspace_bytes < need || (need && !workspace_dev)) return fail(CGV_ERR_INVALID_ARG, "the workspace is smaller than cgv_q4_scores_workspace says");
         if (need && (uintptr_t)workspace_dev % 256) return fail(CGV_ERR_INVALID_ARG, "the workspace must be aligned to 256 bytes");
         DeviceScope dev(h->device);
         OPCHK(dev.enter());
-        return scores_on(h, queries_dev, query_dtype, m, out_dev, (char*)workspace_dev, (hipStream_t)stream);
+        if (!h->captured) {
+            hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+            OPCHK(hipStreamIsCapturing((hipStream_t)stream, &st));
+            h->captured = st != hipStreamCaptureStatusNone;
+        }
+        return scores_on(h, queries_dev, query_dtype, m, n_rows, out_dev, (char*)workspace_dev, (hipStream_t)stream);
     });
 }
 

@@ -130,13 +130,13 @@ struct Piece {              // corpus rows [n0, n0 + c) on their way into the pa
 };
 // a workgroup of 256 threads, each with eight elements of a row
 template <int DT>
-__device__ inline void copy_piece_block(const Piece& P, uint32_t block) {
+__device__ inline void copy_piece_block(const Piece& P, uint64_t block) {
     const void* rows = P.rows;
     const uint64_t stride = P.stride, n0 = P.n0, plane = P.plane;
     const uint32_t c = P.c, dim = P.dim, dp = P.dp;
     uint16_t* dst = P.dst;
     const uint32_t per = dp / 8;
-    const uint64_t t = (uint64_t)block * 256 + threadIdx.x;
+    const uint64_t t = block * 256 + threadIdx.x;
     const uint64_t row = t / per;
     if (row >= c) return;
     const uint32_t e = (uint32_t)(t - row * per) * 8;
@@ -187,8 +187,9 @@ struct Problem {
 template <int DT>
 __global__ __launch_bounds__(256) void forward_prep_kernel(Problem P, uint32_t* __restrict__ anchor, Piece first) {
     const uint32_t lists = (P.k + 15) / 16;            // workgroups of a query
-    if (blockIdx.x >= P.bp * lists) return copy_piece_block<DT>(first, blockIdx.x - P.bp * lists);
-    const uint32_t i = blockIdx.x / lists, list = blockIdx.x % lists, wave = threadIdx.x >> 6;
+    const uint64_t block = wide_block(), listing = (uint64_t)P.bp * lists;
+    if (block >= listing) return copy_piece_block<DT>(first, block - listing);
+    const uint32_t i = (uint32_t)(block / lists), list = (uint32_t)(block % lists), wave = threadIdx.x >> 6;
     const int lane = threadIdx.x & 63;
     const uint64_t plane = (uint64_t)P.bp * P.dp;
     uint16_t* dst = P.qws + (uint64_t)i * P.dp;
@@ -277,10 +278,11 @@ template <int DT>
 __global__ __launch_bounds__(256) void backward_prep_kernel(Problem P, const float* __restrict__ dloss, float* __restrict__ coef, float2* __restrict__ lse2,
                                                             uint32_t* __restrict__ has, uint32_t* __restrict__ ent_id, float* __restrict__ ent_val,
                                                             float* __restrict__ mul, Piece first_piece) {
-    if (blockIdx.x >= P.bp) return copy_piece_block<DT>(first_piece, blockIdx.x - P.bp);
+    const uint64_t block = wide_block();
+    if (block >= P.bp) return copy_piece_block<DT>(first_piece, block - P.bp);
     __shared__ uint32_t ids[MAX_K];
     __shared__ double ps[MAX_K];
-    const uint32_t i = blockIdx.x, wave = threadIdx.x >> 6;
+    const uint32_t i = (uint32_t)block, wave = threadIdx.x >> 6;
     const int lane = threadIdx.x & 63;
     const uint64_t plane = (uint64_t)P.bp * P.dp;
     uint16_t* dst = P.qws + (uint64_t)i * P.dp;
@@ -346,24 +348,27 @@ __global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ c
 
 // dQ: the shares' partial sums, added in a fixed order and rounded once. 64 threads a stretch of 256 elements, four groups of shares
 template <int DT>
-__global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict__ part, uint32_t splits, uint64_t share, uint32_t dim, uint32_t dp,
+__global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict__ part, uint32_t splits, uint64_t share, uint32_t b, uint32_t dim, uint32_t dp,
                                                         const uint32_t* __restrict__ has, const float* __restrict__ mul, void* __restrict__ dq) {
     __shared__ float4 sum[4][64];
-    const uint32_t i = blockIdx.x, t = threadIdx.x & 63, group = threadIdx.x >> 6, e = blockIdx.y * 256 + t * 4;
+    const uint32_t stretches = (dim + 255) / 256;
+    const uint64_t i = wide_block() / stretches;
+    const uint32_t first = (uint32_t)(wide_block() % stretches) * 256, t = threadIdx.x & 63, group = threadIdx.x >> 6, e = first + t * 4;
+    if (i >= b) return;
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (e < dp)
 #pragma unroll 4
         for (uint32_t x = group; x < splits; x += 4) {
-            const float4 v = *(const float4*)(part + x * share + (uint64_t)i * dp + e);
+            const float4 v = *(const float4*)(part + x * share + i * dp + e);
             s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
         }
     sum[group][t] = s;
     __syncthreads();
-    const uint32_t o = threadIdx.x, at = blockIdx.y * 256 + o;
+    const uint32_t o = threadIdx.x, at = first + o;
     if (at >= dim) return;
     float v = 0.0f;
     for (int x = 0; x < 4; ++x) v += ((const float*)sum[x])[o];
-    store_elem<DT>(dq, (uint64_t)i * dim + at, has[i] ? v * mul[1] : 0.0f);
+    store_elem<DT>(dq, i * dim + at, has[i] ? v * mul[1] : 0.0f);
 }
 
 template <int DT>
@@ -586,7 +591,7 @@ int forward(const Plan& pl, Problem P, int dtype, float* loss, char* ws, hipStre
     uint32_t* anchor = (uint32_t*)(ws + pl.f_anchor());
     float2* part = (float2*)(ws + pl.f_part());
     const Piece first = piece_of(pl, P, 0, pl.piece_f, ws + pl.f_rows());
-    hipLaunchKernelGGL((forward_prep_kernel<DT>), dim3(pl.bp * ((pl.k + 15) / 16) + copy_blocks(first)), dim3(256), 0, s, P, anchor, first);
+    hipLaunchKernelGGL((forward_prep_kernel<DT>), wide_grid((uint64_t)pl.bp * ((pl.k + 15) / 16) + copy_blocks(first)), dim3(256), 0, s, P, anchor, first);
     OPCHK(hipGetLastError());
     uint32_t parts = 0;
     for (uint64_t n0 = 0; n0 < pl.n; n0 += pl.piece_f) {
@@ -628,7 +633,7 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
     float* part = (float*)(ws + pl.b_part());
     const uint64_t g_pitch = pl.piece_b * 2, g_plane = (uint64_t)pl.bp * g_pitch;
     const Piece first = piece_of(pl, P, 0, pl.piece_b, ws + pl.b_rows());
-    hipLaunchKernelGGL((backward_prep_kernel<DT>), dim3(pl.bp + copy_blocks(first)), dim3(256), 0, s, P, dloss, coef, lse2, has, ent_id, ent_val, mul, first);
+    hipLaunchKernelGGL((backward_prep_kernel<DT>), wide_grid((uint64_t)pl.bp + copy_blocks(first)), dim3(256), 0, s, P, dloss, coef, lse2, has, ent_id, ent_val, mul, first);
     OPCHK(hipGetLastError());
     if (DT == cgv::DT_FP16) {
         hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1024), 0, s, (const float*)coef, pl.b, mul);
@@ -703,22 +708,22 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
         if (dr && (rc = big ? launch_gemm<DT, S256, true, true, EPI_DR>(e, P.device, s) : launch_gemm<DT, Small<DT>, true, true, EPI_DR>(e, P.device, s))) return rc;
     }
     if (dq) {
-        hipLaunchKernelGGL((finish_dq_kernel<DT>), dim3(pl.b, (pl.dim + 255) / 256), dim3(256), 0, s, (const float*)part, pl.dq_splits, (uint64_t)pl.bp * pl.dp,
-                           pl.dim, pl.dp, (const uint32_t*)has, (const float*)mul, dq);
+        hipLaunchKernelGGL((finish_dq_kernel<DT>), wide_grid((uint64_t)pl.b * ((pl.dim + 255) / 256)), dim3(256), 0, s, (const float*)part, pl.dq_splits, (uint64_t)pl.bp * pl.dp,
+                           pl.b, pl.dim, pl.dp, (const uint32_t*)has, (const float*)mul, dq);
         OPCHK(hipGetLastError());
     }
     return CGV_OK;
 }
 
 bool sizes_ok(uint64_t b, uint64_t n_rows, uint32_t dim, uint32_t k, int dtype) {
-    return b <= (1ull << 19) && n_rows >= 1 && n_rows < (1ull << 31) - 1 && dim >= 1 && dim <= 8192 && k >= 1 && k <= MAX_K &&
+    return b <= (1ull << 24) && n_rows >= 1 && n_rows < (1ull << 31) - 1 && dim >= 1 && dim <= 8192 && k >= 1 && k <= MAX_K &&
            (dtype == CGV_DTYPE_F32 || dtype == CGV_DTYPE_BF16 || dtype == CGV_DTYPE_FP16);
 }
 
 int check_loss(const void* q, uint64_t qs, const void* r, uint64_t rs, int dtype, uint64_t b, uint64_t n, uint32_t dim, const int64_t* ids, uint32_t k,
                float scale, float tscale, const void* saved) {
     if (dtype != CGV_DTYPE_F32 && dtype != CGV_DTYPE_BF16 && dtype != CGV_DTYPE_FP16) return fail(CGV_ERR_INVALID_ARG, "dtype must be f32, bf16 or fp16");
-    if (!sizes_ok(b, n, dim, k, dtype)) return fail(CGV_ERR_INVALID_ARG, "b must be at most 2^19, n_rows in 1..2^31 - 1, dim in 1..=8192, k in 1..=256");
+    if (!sizes_ok(b, n, dim, k, dtype)) return fail(CGV_ERR_INVALID_ARG, "b must be at most 2^24, n_rows in 1..2^31 - 1, dim in 1..=8192, k in 1..=256");
     if (qs < dim || rs < dim) return fail(CGV_ERR_INVALID_ARG, "a stride is smaller than dim");
     if (!(fabsf(scale) < INFINITY) || !(fabsf(tscale) < INFINITY)) return fail(CGV_ERR_NONFINITE, "scale is not finite");
     if (!r || (b && (!q || !ids || !saved))) return fail(CGV_ERR_INVALID_ARG, "NULL argument");

@@ -23,8 +23,8 @@ def lib():
         L.cgv_q4_add_codes.argtypes = [vp, vp, vp, u64]
         L.cgv_q4_add_codes_dev.argtypes = [vp, vp, vp, u64, vp]
         L.cgv_q4_get_row_f32.argtypes = [vp, u64, vp]
-        L.cgv_q4_scores_f32.argtypes = [vp, vp, u32, vp]
-        L.cgv_q4_scores_dev.argtypes = [vp, vp, i32, u32, vp, vp, C.c_size_t, vp]
+        L.cgv_q4_scores_f32.argtypes = [vp, vp, u32, u64, vp]
+        L.cgv_q4_scores_dev.argtypes = [vp, vp, i32, u32, u64, vp, vp, C.c_size_t, vp]
         L.cgv_q4_scores_workspace.argtypes = [vp, i32, u32]
         L.cgv_q4_scores_workspace.restype = C.c_size_t
         for n in ("cgv_q4_create", "cgv_q4_destroy", "cgv_q4_reserve", "cgv_q4_add_f32", "cgv_q4_add_f32_dev", "cgv_q4_add_codes",
@@ -146,10 +146,13 @@ class Int4ScanIndex:
             if q.dim() != 2 or q.shape[1] != self.dim:
                 raise CgvError(CGV_ERR_DIM_MISMATCH, f"query dim {tuple(queries.shape)} != {self.dim}")
             L, m = lib(), q.shape[0]
-            out = torch.empty((m, L.cgv_q4_count(self._h)), dtype=torch.float32, device=q.device)
+            if m >= 1 << 32:
+                raise CgvError(CGV_ERR_INVALID_ARG, "more than 2^32 - 1 queries")
+            n = L.cgv_q4_count(self._h)
+            out = torch.empty((m, n), dtype=torch.float32, device=q.device)
             nb = L.cgv_q4_scores_workspace(self._h, code, m)
             ws = torch.empty((nb,), dtype=torch.uint8, device=q.device) if nb else None
-            _check(L.cgv_q4_scores_dev(self._h, q.data_ptr(), code, m, out.data_ptr(), ws.data_ptr() if nb else None, nb, self._stream()))
+            _check(L.cgv_q4_scores_dev(self._h, q.data_ptr(), code, m, n, out.data_ptr(), ws.data_ptr() if nb else None, nb, self._stream()))
             return out[0] if one else out
         if _is_torch(queries):
             queries = queries.detach().float().numpy()
@@ -159,5 +162,5 @@ class Int4ScanIndex:
         if q.ndim != 2 or q.shape[1] != self.dim:
             raise CgvError(CGV_ERR_DIM_MISMATCH, f"query dim {q.shape} != {self.dim}")
         out = np.empty((q.shape[0], len(self)), dtype=np.float32)
-        _check(lib().cgv_q4_scores_f32(self._h, q.ctypes.data_as(C.c_void_p), q.shape[0], out.ctypes.data_as(C.c_void_p)))
+        _check(lib().cgv_q4_scores_f32(self._h, q.ctypes.data_as(C.c_void_p), q.shape[0], out.shape[1], out.ctypes.data_as(C.c_void_p)))
         return out[0] if one else out

@@ -11,8 +11,9 @@
  * Same status / error convention as cgvec.h. No CPU fallback: creating a handle without a GPU fails.
  *
  * Threading: calls on one handle may come from several threads; those that add rows run alone. cgv_q4_scores_dev only enqueues.
- * A HIP graph that captured cgv_q4_scores_dev keeps the addresses of that moment: rows added after the capture may move the
- * corpus (cgv_q4_reserve beforehand keeps it in place), and a replay scores the rows that were there at the capture. */
+ * A HIP graph that captured cgv_q4_scores_dev keeps the addresses of that moment, and a replay scores the rows that were there at
+ * the capture: where rows added later move the corpus, the handle keeps what it left until it is destroyed (cgv_q4_reserve
+ * beforehand keeps the corpus in place). */
 #ifndef CGVEC_Q4_H
 #define CGVEC_Q4_H
 
@@ -48,15 +49,16 @@ int cgv_q4_add_codes_dev(cgv_q4_index* h, const uint8_t* codes_dev, const uint16
 /* Row `id` as f32 values (HOST). CGV_ERR_OUT_OF_RANGE beyond the last row. */
 int cgv_q4_get_row_f32(cgv_q4_index* h, uint64_t id, float* out_host);
 
-/* Scores of m queries against all rows: out [m][count] f32. A query with a NaN or Inf gets NaN for every row.
+/* Scores of m queries against the first n_rows rows: out [m][n_rows] f32; more than cgv_q4_count: CGV_ERR_OUT_OF_RANGE (rows that
+ * another thread adds between the two calls do not matter). A query with a NaN or Inf gets NaN for every row.
  * _f32: HOST queries [m][dim] and output, returns when done. _dev: DEVICE queries of type query_dtype (CGV_DTYPE_F32 / BF16 /
- * FP16), contiguous [m][dim]; enqueued on `stream`, no synchronisation, nothing allocated. m == 0 or an empty index: nothing is
+ * FP16), contiguous [m][dim]; enqueued on `stream`, no synchronisation, nothing allocated. m == 0 or n_rows == 0: nothing is
  * written. The workspace (DEVICE, cgv_q4_scores_workspace bytes, 0 for one query of ordinary size; aligned to 256) belongs to one
  * call until its work on the stream is done. */
-int cgv_q4_scores_f32(cgv_q4_index* h, const float* queries_host, uint32_t m, float* out_host);
+int cgv_q4_scores_f32(cgv_q4_index* h, const float* queries_host, uint32_t m, uint64_t n_rows, float* out_host);
 size_t cgv_q4_scores_workspace(const cgv_q4_index* h, int query_dtype, uint32_t m);
-int cgv_q4_scores_dev(cgv_q4_index* h, const void* queries_dev, int query_dtype, uint32_t m, float* out_dev, void* workspace_dev,
-                      size_t workspace_bytes, void* stream);
+int cgv_q4_scores_dev(cgv_q4_index* h, const void* queries_dev, int query_dtype, uint32_t m, uint64_t n_rows, float* out_dev,
+                      void* workspace_dev, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -153,6 +153,23 @@ def test_batches_in_columns_of_two_widths(b, n, d, k, dt):
     assert bool((dq[b - 2] == 0).all())
 
 
+def test_a_million_queries_with_long_lists():
+    """More than 2^32 threads' worth of lists."""
+    m = pkg()
+    b, n, d, k = 2 ** 20 + 7, 20, 8, 256
+    q, r, ids, sc, g = _problem(b, n, d, k, "bf16", 5)
+    ids[b - 1, 1:] = -1
+    ids[b - 2] = -1
+    q.requires_grad_()
+    r.requires_grad_()
+    ref = _reference(q.detach(), r.detach(), ids, sc, g, 8.0, 3.0)
+    loss = m.corpus_distillation(q, r, ids, sc, scale=8.0, teacher_scale=3.0)
+    dq, dr = torch.autograd.grad(loss, (q, r), g)
+    _check(loss.detach(), dq, dr, ref, d, n, 8.0, "bf16", g)
+    del ref, q, r, ids, sc, g, loss, dq, dr
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("dt", list(TYPES))
 def test_one_gradient_at_a_time(dt):
     m = pkg()

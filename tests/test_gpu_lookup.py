@@ -228,3 +228,26 @@ def test_rows_behind_the_hits_of_a_search():
         assert torch.equal(out[:, :7].cpu(), torch.from_numpy(rows)[ids[:, :7].cpu()]) and bool((out[:, 7:] == 0).all())
     finally:
         ix.close()
+
+
+def test_more_elements_than_a_direction_of_a_launch():
+    """More than 2^32 threads' worth of single elements: rows of three 16-bit elements cannot be read in wider vectors."""
+    m = pkg()
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    k, n = 1_431_655_800, 1000
+    table = _table(gen, n, 3, "bf16")
+    ids = torch.arange(k, device="cuda").remainder_(n + 1)            # n itself: no row
+    out = m.lookup_rows(table, ids, scale=2.0)
+    at = torch.cat([torch.randint(0, k, (100_000,), generator=gen, device="cuda"), torch.arange(k - 1000, k, device="cuda")])
+    want = torch.where((ids[at] < n)[:, None], table[ids[at].clamp_max(n - 1)] * 2.0, torch.zeros((), dtype=table.dtype, device="cuda"))
+    assert torch.equal(out[at], want)
+    del out, ids
+    for few in (40, 600):                                             # one launch, and sorted
+        some = torch.cat([torch.randint(0, k, (few - 2,), generator=gen, device="cuda"), torch.tensor([0, k - 1], device="cuda")])
+        dout = _table(gen, few, 3, "bf16")
+        g = m.lookup_rows_grad(dout, some, k)
+        assert some.unique().numel() == few and torch.equal(g[some], dout)
+        g[some] = 0
+        assert not bool(g.view(torch.int16)[:1 << 28].any()) and not bool(g.view(torch.int16)[-(1 << 28):].any())
+        del g
+    torch.cuda.empty_cache()

@@ -277,3 +277,81 @@ def test_two_threads_score_one_index():
         assert not bad
     finally:
         ix.close()
+
+
+def test_replays_after_the_corpus_has_moved():
+    import torch
+    m = pkg()
+    rng = np.random.default_rng(13)
+    rows = _rows(rng, 70_000, 200)
+    ix = m.Int4ScanIndex(200)
+    try:
+        ix.add(rows[:40])
+        x = torch.from_numpy(_rows(rng, 2, 200)).cuda()
+        g = torch.cuda.CUDAGraph()
+        ix.scores(x)
+        with torch.cuda.graph(g):
+            out = ix.scores(x)
+        at = 40
+        for n in (3000, 20_000, 46_960):                   # each beyond what the buffers hold
+            ix.add(rows[at:at + n])
+            at += n
+            x.copy_(torch.from_numpy(_rows(rng, 2, 200)))
+            out.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            now = ix.scores(x)
+            assert now.shape == (2, at) and torch.equal(out, now[:, :40])
+    finally:
+        ix.close()
+
+
+def test_scores_of_the_first_rows():
+    import ctypes as C
+    m = pkg()
+    rng = np.random.default_rng(14)
+    ix = m.Int4ScanIndex(96, group=32)
+    try:
+        ix.add(_rows(rng, 1000, 96))
+        x = _rows(rng, 3, 96)
+        want = ix.scores(x)
+        L, p = m.q4scan.lib(), lambda a: a.ctypes.data_as(C.c_void_p)
+        for n in (0, 1, 15, 16, 17, 999, 1000):
+            out = np.full((3, n + 1), 7.0, np.float32)
+            assert L.cgv_q4_scores_f32(ix._h, p(x), 3, n, p(out)) == 0
+            assert np.array_equal(out.ravel()[:3 * n].reshape(3, n), want[:, :n]) and np.all(out.ravel()[3 * n:] == 7.0)
+        out = np.zeros((3, 1001), np.float32)
+        assert L.cgv_q4_scores_f32(ix._h, p(x), 3, 1001, p(out)) == m.cgvec.CGV_ERR_OUT_OF_RANGE
+        assert L.cgv_q4_scores_dev(ix._h, p(x), 0, 3, 1001, p(out), None, 0, None) == m.cgvec.CGV_ERR_OUT_OF_RANGE
+    finally:
+        ix.close()
+
+
+def test_scoring_while_another_thread_adds():
+    import threading
+    import torch
+    m = pkg()
+    rng = np.random.default_rng(15)
+    rows = _rows(rng, 60_000, 64)
+    x = torch.from_numpy(_rows(rng, 2, 64)).cuda()
+    ix = m.Int4ScanIndex(64)
+    got = []
+    try:
+        ix.add(rows[:100])
+
+        def add():
+            for a in range(100, 60_000, 5990):
+                ix.add(rows[a:a + 5990])
+        t = threading.Thread(target=add)
+        t.start()
+        while True:
+            last = not t.is_alive()
+            got.append(ix.scores(x))
+            if last:
+                break
+        t.join()
+        torch.cuda.synchronize()
+        assert got[-1].shape == (2, 60_000)
+        assert all(torch.equal(s, got[-1][:, :s.shape[1]]) for s in got)
+    finally:
+        ix.close()

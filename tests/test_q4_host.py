@@ -33,7 +33,7 @@ def test_null_handles():
     assert L.cgv_q4_add_f32(None, p, 1) == bad and L.cgv_q4_add_f32_dev(None, p, 1, None) == bad
     assert L.cgv_q4_add_codes(None, p, p, 1) == bad and L.cgv_q4_add_codes_dev(None, p, p, 1, None) == bad
     assert L.cgv_q4_get_row_f32(None, 0, p) == bad
-    assert L.cgv_q4_scores_f32(None, p, 1, p) == bad and L.cgv_q4_scores_dev(None, p, 0, 1, p, None, 0, None) == bad
+    assert L.cgv_q4_scores_f32(None, p, 1, 1, p) == bad and L.cgv_q4_scores_dev(None, p, 0, 1, 1, p, None, 0, None) == bad
     assert L.cgv_q4_scores_workspace(None, 0, 5) == 0
 
 
