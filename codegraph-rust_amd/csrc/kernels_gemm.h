@@ -96,7 +96,12 @@ struct Shape {
         const int n = (160 * 1024 - (xpose ? NW * XPOSE : 0)) / STAGE;
         return n < 6 ? n : 6;
     }
-    static constexpr int lds_bytes(bool xpose) { return stages(xpose) * STAGE + (xpose ? NW * XPOSE : 0); }
+    // where only two fit, the operand that comes from HBM has three places and loads two stages ahead; the other, which the workgroups
+    // share through L2, has two. Results then leave through the long operand's free place
+    static constexpr bool UNEVEN = STAGE * 3 > 160 * 1024;
+    static constexpr int lds_bytes(bool xpose, bool long_a) {
+        return UNEVEN ? 2 * STAGE + (long_a ? A_BYTES : B_BYTES) : stages(xpose) * STAGE + (xpose ? NW * XPOSE : 0);
+    }
 };
 
 // swizzle of a row's eight 16-byte pieces: 16 consecutive rows put the same piece at 16 different places of the 256 bytes that the
@@ -131,13 +136,21 @@ struct Loader {
             }
         }
     }
-    __device__ void issue(const char* base, uint32_t soff, char* lds, int wave) const {
+    __device__ void issue_one(int i, const char* base, uint32_t soff, char* lds, int wave) const {
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(lds + (wave * I + i) * 1024), 16, voff[i], soff, 0, 0);
+    }
+    __device__ void issue(const char* base, uint32_t soff, char* lds, int wave) const {
 #pragma unroll
-        for (int i = 0; i < I; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(lds + (wave * I + i) * 1024), 16, voff[i], soff, 0, 0);
+        for (int i = 0; i < I; ++i) issue_one(i, base, soff, lds, wave);
     }
 };
+
+// Four rows of a column form's piece, turned. `restrict` here is for the compiler's waits alone: in front of a transposing read about which
+// it knows nothing it waits for every load into LDS on its way (dQ of 1024 x 125 k x 768: A us with those waits, B without them). That the
+// piece has landed is what the stage's own wait and barrier see to
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+__device__ __forceinline__ s16x4 read_turned(lds_s16x4* __restrict__ p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p); }
 
 // fragment of 32 rows (or columns) starting at `at` of a stage, 16 elements of K from kk * 16
 template <bool T, int W>
@@ -150,8 +163,7 @@ __device__ inline s16x8 fragment(const char* lds, uint32_t at, int kk, int lane)
     const uint32_t k = (uint32_t)kk * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2);
     const uint32_t seg = at / 16 + ((lane >> 4) & 1);
     const char* p = lds + k * RB + ((seg ^ seg_swz<W>(k)) << 5) + (lane & 3) * 8;
-    typedef __attribute__((address_space(3))) s16x4 lds4;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * RB));
+    const s16x4 lo = read_turned((lds_s16x4*)p), hi = read_turned((lds_s16x4*)(p + 4 * RB));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
@@ -170,7 +182,8 @@ __device__ inline uint32_t unit_of(uint32_t id, uint32_t blocks) {
 template <int DT, class S, bool TA, bool TB, int EPI>
 __device__ __forceinline__ void work(const Args& g, uint32_t block) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    constexpr int NST = S::stages(EPI == EPI_G || EPI == EPI_DR);
+    constexpr bool XPOSE = EPI == EPI_G || EPI == EPI_DR, UNEVEN = S::UNEVEN, LONG_A = EPI != EPI_DR;
+    constexpr int NST = UNEVEN ? 2 : S::stages(XPOSE), NSA = UNEVEN && LONG_A ? 3 : NST, NSB = UNEVEN && !LONG_A ? 3 : NST;   // places of A and B
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % S::WM, wn = wave / S::WM;
     const uint32_t unit = unit_of(block, g.blocks);
@@ -264,13 +277,44 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
         pa = uniform(pa);
         pb = uniform(pb);
     };
-    auto issue = [&](int slot) {
-        char* l = smem + slot * S::STAGE;
+    char *const smem_a = smem, *const smem_b = smem + NSA * S::PL * S::A_BYTES;
+    auto issue_a = [&](const Loader<TA, S::BM, S::NW>& l, const char* base, uint32_t off, int slot) {
 #pragma unroll
-        for (int p = 0; p < S::PL; ++p) {
-            la.issue(pa + p * g.a.plane, sa, l + p * S::A_BYTES, wave);
-            lb.issue(pb + p * g.b.plane, sb, l + S::PL * S::A_BYTES + p * S::B_BYTES, wave);
+        for (int p = 0; p < S::PL; ++p) l.issue(base + p * g.a.plane, off, smem_a + (slot * S::PL + p) * S::A_BYTES, wave);
+    };
+    auto issue_b = [&](const Loader<TB, S::BN, S::NW>& l, const char* base, uint32_t off, int slot) {
+#pragma unroll
+        for (int p = 0; p < S::PL; ++p) l.issue(base + p * g.b.plane, off, smem_b + (slot * S::PL + p) * S::B_BYTES, wave);
+    };
+    // UNEVEN: the short operand's stage before the prepared one, still to be loaded (a short B is the same query tile all the time)
+    Loader<TA, S::BM, S::NW> wla;
+    const char* wp = nullptr;
+    uint32_t ws = 0;
+    auto keep = [&]() {
+        if constexpr (UNEVEN) {
+            if (LONG_A) wp = pb, ws = sb;
+            else wla = la, wp = pa, ws = sa;
         }
+    };
+    constexpr int IA = Loader<TA, S::BM, S::NW>::I, IB = Loader<TB, S::BN, S::NW>::I, SHORT = LONG_A ? IB : IA;
+    // load q of those that follow when the places (a, b) become free: of the prepared stage, UNEVEN: the short operand's kept stage first
+    auto issue_one = [&](int q, int a, int b) {
+        if constexpr (UNEVEN) {
+            if (q < SHORT) {
+                if (LONG_A) lb.issue_one(q, wp, ws, smem_b + b * S::B_BYTES, wave);
+                else wla.issue_one(q, wp, ws, smem_a + a * S::A_BYTES, wave);
+            } else {
+                if (LONG_A) la.issue_one(q - SHORT, pa, sa, smem_a + a * S::A_BYTES, wave);
+                else lb.issue_one(q - SHORT, pb, sb, smem_b + b * S::B_BYTES, wave);
+            }
+        } else {
+            if (q < IA) la.issue_one(q, pa, sa, smem_a + a * S::A_BYTES, wave);
+            else lb.issue_one(q - IA, pb, sb, smem_b + b * S::B_BYTES, wave);
+        }
+    };
+    auto issue = [&](int a, int b) {
+        issue_a(la, pa, sa, a);
+        issue_b(lb, pb, sb, b);
     };
 
     float run_m[S::NB], run_s[S::NB];                 // LSE: per query of the lane, over the corpus rows of the lane
@@ -283,14 +327,30 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
     constexpr int SETS = SMALL ? 4 : 1, FA = S::PL * S::MB, FB = S::PL * S::NB;
     s16x8 fa0[SETS][FA], fb0[SETS][FB], fa1[SETS][FA], fb1[SETS][FB];
     f32x16 acc[S::MB][S::NB], low[S::PL == 3 ? S::MB : 1][S::PL == 3 ? S::NB : 1];   // three planes: the five small products have their own sum
-    auto read = [&](s16x8(&fa)[FA], s16x8(&fb)[FB], int buf, int kk) {
-        const char *as = smem + buf * S::STAGE, *bs = as + S::PL * S::A_BYTES;
+    auto read = [&](s16x8(&fa)[FA], s16x8(&fb)[FB], int a, int b, int kk) {
 #pragma unroll
         for (int p = 0; p < S::PL; ++p) {
 #pragma unroll
-            for (int nb = 0; nb < S::NB; ++nb) fb[p * S::NB + nb] = fragment<TB, S::BN>(bs + p * S::B_BYTES, (uint32_t)(wn * S::TN + nb * 32), kk, lane);
+            for (int nb = 0; nb < S::NB; ++nb)
+                fb[p * S::NB + nb] = fragment<TB, S::BN>(smem_b + (b * S::PL + p) * S::B_BYTES, (uint32_t)(wn * S::TN + nb * 32), kk, lane);
 #pragma unroll
-            for (int mb = 0; mb < S::MB; ++mb) fa[p * S::MB + mb] = fragment<TA, S::BM>(as + p * S::A_BYTES, (uint32_t)(wm * S::TM + mb * 32), kk, lane);
+            for (int mb = 0; mb < S::MB; ++mb)
+                fa[p * S::MB + mb] = fragment<TA, S::BM>(smem_a + (a * S::PL + p) * S::A_BYTES, (uint32_t)(wm * S::TM + mb * 32), kk, lane);
+        }
+    };
+    // the fragments that are read in gap x of a phase, the first in gap `from`
+    auto read_at = [&](int x, int from, s16x8(&fa)[FA], s16x8(&fb)[FB], int a, int b, int kk) {
+        constexpr int N = FA + FB, P = S::MB * S::NB;
+#pragma unroll
+        for (int f = 0; f < N; ++f) {
+            if (x != from + f * (P - 1 - from) / N) continue;
+            if (f == 0 || (f > 1 && f <= FB)) {
+                const int nb = f ? f - 1 : 0;
+                fb[nb] = fragment<TB, S::BN>(smem_b + b * S::B_BYTES, (uint32_t)(wn * S::TN + nb * 32), kk, lane);
+            } else {
+                const int mb = f == 1 ? 0 : f - FB;
+                fa[mb] = fragment<TA, S::BM>(smem_a + a * S::A_BYTES, (uint32_t)(wm * S::TM + mb * 32), kk, lane);
+            }
         }
     };
     auto products = [&](s16x8(&fa)[FA], s16x8(&fb)[FB]) {
@@ -312,7 +372,10 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
                 for (int nb = 0; nb < S::NB; ++nb) acc[mb][nb] = mma<DT>(fa[mb], fb[nb], acc[mb][nb]);
         }
     };
-    constexpr int LOADS = S::PL * (decltype(la)::I + decltype(lb)::I), WAIT = (NST - 2) * LOADS;   // of a stage; of the stages behind the next one
+    constexpr bool PLACED = !SMALL && S::NW == 8;
+    constexpr int LOADS = S::PL * (IA + IB);                                  // of a stage
+    constexpr int FIRST = UNEVEN ? SHORT : (LOADS + 2) / 3;                   // of those that follow right behind the stage's change
+    constexpr int WAIT = UNEVEN ? IA + IB - SHORT : (NST - 2) * LOADS;        // of what lies behind the next stage
     auto stage_ready = [&]() {
         // this wave's part of the next stage has landed, its reads of this one are done
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(WAIT) : "memory");
@@ -337,34 +400,121 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
     };
 
     if (!ksteps) tiles = EPI == EPI_DQ ? tiles : 0;
-    int buf = 0;                                      // slot of the stage at work; the one before it is where the next load goes
+    int buf = 0, bufb = 0;                            // places of the stage at work; when it is done the next loads go there
+    auto after = [](int x, int n) { return n == 2 ? x ^ 1 : x + 1 == n ? 0 : x + 1; };
     auto read_stage = [&](s16x8(&fa)[SETS][FA], s16x8(&fb)[SETS][FB], int slot) {
 #pragma unroll
-        for (int kk = 0; kk < SETS; ++kk) read(fa[kk], fb[kk], slot, kk);
+        for (int kk = 0; kk < SETS; ++kk) read(fa[kk], fb[kk], slot, slot, kk);
     };
     // small wave tiles: a stage's products while the next stage's fragments are read
     auto step = [&](s16x8(&ca)[SETS][FA], s16x8(&cb)[SETS][FB], s16x8(&na)[SETS][FA], s16x8(&nb)[SETS][FB]) {
         __builtin_amdgcn_sched_barrier(0);
         prepare();
         stage_ready();
-        const int next = buf + 1 == NST ? 0 : buf + 1;
+        const int next = after(buf, NST);
         read_stage(na, nb, next);
-        issue(buf);
+        issue(buf, buf);
         buf = next;
 #pragma unroll
         for (int kk = 0; kk < SETS; ++kk) products(ca[kk], cb[kk]);
         __builtin_amdgcn_sched_barrier(0);
     };
     if (tiles && ksteps) {
-        for (int x = 0; x < NST - 1; ++x) {
+        if constexpr (UNEVEN) {
             prepare();
-            issue(x);
+            issue_a(la, pa, sa, 0);
+            issue_b(lb, pb, sb, 0);
+            prepare();
+            if (LONG_A) issue_a(la, pa, sa, 1);
+            else issue_b(lb, pb, sb, 1);
+            keep();
+            prepare();
+            stage_ready();
+            for (int q = 0; q < SHORT; ++q) issue_one(q, NSA - 1, NSB - 1);
+        } else {
+            for (int x = 0; x < NST - 1; ++x) {
+                prepare();
+                issue(x, x);
+            }
+            prepare();
+            stage_ready();
+            if (PLACED)
+                for (int q = 0; q < FIRST; ++q) issue_one(q, NST - 1, NST - 1);
+            else
+                issue(NST - 1, NST - 1);
         }
-        prepare();
-        stage_ready();
-        issue(NST - 1);
         read_stage(fa0, fb0, 0);
     }
+    // Large wave tiles: products one by one, and between them what is issued beside them. The compiler moves matrix instructions as it likes,
+    // so that empty asm statements tie each to its place: behind one that has its result, before one that has an operand of the next
+    auto phase = [&](s16x8(&fa)[FA], s16x8(&fb)[FB], auto&& gap) {
+        constexpr auto col = [](int x) { return x / S::NB % 2 ? S::NB - 1 - x % S::NB : x % S::NB; };   // neighbours share an operand
+#pragma unroll
+        for (int x = 0; x < S::MB * S::NB; ++x) {
+            f32x16& c = acc[x / S::NB][col(x)];
+            c = mma<DT>(fa[x / S::NB], fb[col(x)], c);
+            asm volatile("" : "+v"(c)::"memory");
+            gap(x);
+            if (x + 1 < S::MB * S::NB) {
+                if ((x + 1) / S::NB != x / S::NB) asm volatile("" : "+v"(fa[(x + 1) / S::NB])::"memory");
+                else asm volatile("" : "+v"(fb[col(x + 1)])::"memory");
+            }
+        }
+    };
+    // loads q .. q + n - 1 spread over the gaps of a phase, behind the fragments' reads
+    auto loads_at = [&](int x, int q, int n, int a, int b) {
+        constexpr int P = S::MB * S::NB, from = P >= 8 ? 3 : P >= 6 ? 2 : 1;
+#pragma unroll
+        for (int d = 0; d < n; ++d)
+            if (x == from + d * (P - from) / n) issue_one(q + d, a, b);
+    };
+    auto placed_step = [&]() {
+        constexpr int P0 = (LOADS - FIRST + 1) / 2, P1 = LOADS - FIRST - P0;
+        const int fra = buf ? buf - 1 : NSA - 1, frb = bufb ? bufb - 1 : NSB - 1;        // places that the stage before has left
+        phase(fa0[0], fb0[0], [&](int x) {
+            read_at(x, 0, fa1[0], fb1[0], buf, bufb, 1);
+            loads_at(x, FIRST, P0, fra, frb);
+        });
+        phase(fa1[0], fb1[0], [&](int x) {
+            read_at(x, 0, fa0[0], fb0[0], buf, bufb, 2);
+            loads_at(x, FIRST + P0, P1, fra, frb);
+        });
+        phase(fa0[0], fb0[0], [&](int x) {
+            read_at(x, 0, fa1[0], fb1[0], buf, bufb, 3);
+        });
+        keep();
+        prepare();
+        const int a = after(buf, NSA), b = after(bufb, NSB);
+        // the stage changes behind the first product of its last 16 elements, whose fragments have been read
+        phase(fa1[0], fb1[0], [&](int x) {
+            if (x == 0) stage_ready();
+            read_at(x, 1, fa0[0], fb0[0], a, b, 0);
+            loads_at(x, 0, FIRST, buf, bufb);
+        });
+        buf = a;
+        bufb = b;
+    };
+    // four waves, one a SIMD: the same in the compiler's order, which suits them better (64 queries x 200 k x 768, loss: 82 us, placed 120)
+    auto ordered_step = [&]() {
+        __builtin_amdgcn_sched_barrier(0);
+        read(fa1[0], fb1[0], buf, bufb, 1);
+        products(fa0[0], fb0[0]);
+        interleave(0);
+        read(fa0[0], fb0[0], buf, bufb, 2);
+        products(fa1[0], fb1[0]);
+        interleave(0);
+        read(fa1[0], fb1[0], buf, bufb, 3);
+        products(fa0[0], fb0[0]);
+        interleave(0);
+        prepare();
+        stage_ready();
+        const int next = after(buf, NST);
+        read(fa0[0], fb0[0], next, next, 0);
+        issue(buf, bufb);
+        buf = bufb = next;
+        products(fa1[0], fb1[0]);
+        interleave(LOADS);
+    };
     uint32_t nmt = mt, nnt = nt;
     for (uint32_t i = 0; i < tiles; ++i) {
         // (mt, nt) belong to the load side, which may already be in the next tile
@@ -403,26 +553,8 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
             }
         } else {
             for (uint32_t s = 0; s < stages; ++s) {
-                // fragments of the next 16 elements of K are on their way from LDS while the products of these run; the stage changes
-                // behind the reads of its last 16, whose products stand ready on the other side of the barrier
-                __builtin_amdgcn_sched_barrier(0);
-                read(fa1[0], fb1[0], buf, 1);
-                products(fa0[0], fb0[0]);
-                interleave(0);
-                read(fa0[0], fb0[0], buf, 2);
-                products(fa1[0], fb1[0]);
-                interleave(0);
-                read(fa1[0], fb1[0], buf, 3);
-                products(fa0[0], fb0[0]);
-                interleave(0);
-                prepare();
-                stage_ready();
-                const int next = NST == 2 ? buf ^ 1 : buf + 1 == NST ? 0 : buf + 1;
-                read(fa0[0], fb0[0], next, 0);
-                issue(buf);
-                buf = next;
-                products(fa1[0], fb1[0]);
-                interleave(LOADS);
+                if constexpr (PLACED) placed_step();
+                else ordered_step();
             }
             if constexpr (S::PL == 3) {
 #pragma unroll
@@ -433,6 +565,9 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
         }
 
         // ---- epilogue of the tile
+        // a wave's own piece of LDS for results on their way out
+        char* const xp = (UNEVEN ? LONG_A ? smem_a + (buf ? buf - 1 : NSA - 1) * S::A_BYTES : smem_b + (bufb ? bufb - 1 : NSB - 1) * S::B_BYTES
+                                 : smem + NST * S::STAGE) + wave * S::XPOSE;
         constexpr int PAIR = S::MB < 2 ? 1 : 2, LPR = PAIR * 4, OUT = 64 / LPR;   // G, DR: blocks of 32 that leave together; lanes of a row, rows of an instruction
         const uint32_t m0 = my_mt * S::BM + wm * S::TM, n0 = my_nt * S::BN + wn * S::TN;
         const uint32_t half4 = (uint32_t)(lane >> 5) * 4;
@@ -487,7 +622,6 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
                 }
             }
         } else if (EPI == EPI_G) {
-            char* xp = smem + NST * S::STAGE + wave * S::XPOSE;
 #pragma unroll
             for (int nb = 0; nb < S::NB; ++nb) {
                 const uint32_t q = n0 + nb * 32 + (lane & 31);
@@ -561,7 +695,6 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
             }
         } else {   // EPI_DR
             const float u = *g.unscale;
-            char* xp = smem + NST * S::STAGE + wave * S::XPOSE;
 #pragma unroll
             for (int nb = 0; nb < S::NB; ++nb) {
                 if (DT != cgv::DT_F32 && g.vec_out) {
@@ -616,6 +749,10 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
                         }
                 }
             }
+        }
+        if constexpr (UNEVEN && XPOSE) {
+            __builtin_amdgcn_s_barrier();                                 // every wave's results have left their places
+            asm volatile("" ::: "memory");
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in LDS behind the workgroup's end
