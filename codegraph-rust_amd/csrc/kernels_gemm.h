@@ -90,18 +90,12 @@ struct Shape {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM_ * WN_, THREADS = 64 * NW;
     static constexpr int TM = BM / WM, TN = BN / WN, MB = TM / 32, NB = TN / 32;
     static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, STAGE = PL * (A_BYTES + B_BYTES);
-    static constexpr int XPOSE = 4096;            // per wave: a 32 x 64 piece of 16-bit results on its way out
     // stages in LDS: as many as fit, six at most; all but one of them are loading or waiting
-    static constexpr int stages(bool xpose) {
-        const int n = (160 * 1024 - (xpose ? NW * XPOSE : 0)) / STAGE;
-        return n < 6 ? n : 6;
-    }
+    static constexpr int STAGES = 160 * 1024 / STAGE < 6 ? 160 * 1024 / STAGE : 6;
     // where only two fit, the operand that comes from HBM has three places and loads two stages ahead; the other, which the workgroups
-    // share through L2, has two. Results then leave through the long operand's free place
-    static constexpr bool UNEVEN = STAGE * 3 > 160 * 1024;
-    static constexpr int lds_bytes(bool xpose, bool long_a) {
-        return UNEVEN ? 2 * STAGE + (long_a ? A_BYTES : B_BYTES) : stages(xpose) * STAGE + (xpose ? NW * XPOSE : 0);
-    }
+    // share through L2, has two
+    static constexpr bool UNEVEN = STAGES == 2;
+    static constexpr int lds_bytes(bool long_a) { return STAGES * STAGE + (UNEVEN ? long_a ? A_BYTES : B_BYTES : 0); }
 };
 
 // swizzle of a row's eight 16-byte pieces: 16 consecutive rows put the same piece at 16 different places of the 256 bytes that the
@@ -167,6 +161,32 @@ __device__ inline s16x8 fragment(const char* lds, uint32_t at, int kk, int lane)
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// two f32 -> two 16-bit values in a word (f32: the largest plane)
+template <int DT>
+__device__ inline uint32_t pair(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    if constexpr (DT == cgv::DT_FP16) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+    } else {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+    }
+}
+// A lane's rows (x & 3) + 8 (x >> 2) + 4 (lane >> 5), x < 8, of its column in 16 bits -> the column's rows 8 (lane >> 5) + 0 .. 7, which are
+// neighbours in memory: the lanes l and l + 32 trade halves. f32: the largest plane, and v keeps what it leaves
+template <int DT>
+__device__ inline uint4 sixteen(float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = pair<DT>(v[2 * i], v[2 * i + 1]);
+        if (DT == cgv::DT_F32) v[2 * i] -= __uint_as_float(w[i] << 16), v[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+    }
+    const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+    return make_uint4(x[0], y[0], x[1], y[1]);
+}
+
 __device__ inline const char* uniform(const char* p) {
     const uint64_t v = (uint64_t)p;
     return (const char*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
@@ -182,8 +202,8 @@ __device__ inline uint32_t unit_of(uint32_t id, uint32_t blocks) {
 template <int DT, class S, bool TA, bool TB, int EPI>
 __device__ __forceinline__ void work(const Args& g, uint32_t block) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    constexpr bool XPOSE = EPI == EPI_G || EPI == EPI_DR, UNEVEN = S::UNEVEN, LONG_A = EPI != EPI_DR;
-    constexpr int NST = UNEVEN ? 2 : S::stages(XPOSE), NSA = UNEVEN && LONG_A ? 3 : NST, NSB = UNEVEN && !LONG_A ? 3 : NST;   // places of A and B
+    constexpr bool UNEVEN = S::UNEVEN, LONG_A = EPI != EPI_DR;
+    constexpr int NST = S::STAGES, NSA = UNEVEN && LONG_A ? 3 : NST, NSB = UNEVEN && !LONG_A ? 3 : NST;   // places of A and B
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % S::WM, wn = wave / S::WM;
     const uint32_t unit = unit_of(block, g.blocks);
@@ -317,6 +337,14 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
         issue_b(lb, pb, sb, b);
     };
 
+    float g_coef[S::NB];                              // G: of the lane's queries
+    float2 g_lse[S::NB];
+    if (EPI == EPI_G)
+        for (int nb = 0; nb < S::NB; ++nb) {
+            const uint32_t q = nt * S::BN + wn * S::TN + nb * 32 + (lane & 31);
+            g_coef[nb] = q < g.n_valid ? g.coef[q] * *g.unscale : 0.0f;
+            g_lse[nb] = q < g.n_valid ? g.lse2[q] : make_float2(0.0f, 0.0f);
+        }
     float run_m[S::NB], run_s[S::NB];                 // LSE: per query of the lane, over the corpus rows of the lane
     if (EPI == EPI_LSE)
         for (int nb = 0; nb < S::NB; ++nb) run_m[nb] = -INFINITY, run_s[nb] = 0.0f;
@@ -565,10 +593,6 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
         }
 
         // ---- epilogue of the tile
-        // a wave's own piece of LDS for results on their way out
-        char* const xp = (UNEVEN ? LONG_A ? smem_a + (buf ? buf - 1 : NSA - 1) * S::A_BYTES : smem_b + (bufb ? bufb - 1 : NSB - 1) * S::B_BYTES
-                                 : smem + NST * S::STAGE) + wave * S::XPOSE;
-        constexpr int PAIR = S::MB < 2 ? 1 : 2, LPR = PAIR * 4, OUT = 64 / LPR;   // G, DR: blocks of 32 that leave together; lanes of a row, rows of an instruction
         const uint32_t m0 = my_mt * S::BM + wm * S::TM, n0 = my_nt * S::BN + wn * S::TN;
         const uint32_t half4 = (uint32_t)(lane >> 5) * 4;
         if (EPI == EPI_LSE) {
@@ -622,56 +646,34 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
                 }
             }
         } else if (EPI == EPI_G) {
+            auto store = [&](auto at_edge) {
 #pragma unroll
-            for (int nb = 0; nb < S::NB; ++nb) {
-                const uint32_t q = n0 + nb * 32 + (lane & 31);
-                const float c = q < g.n_valid ? g.coef[q] * *g.unscale : 0.0f;
-                const float2 l2 = q < g.n_valid ? g.lse2[q] : make_float2(0.0f, 0.0f);
+                for (int nb = 0; nb < S::NB; ++nb) {
+                    const uint32_t q = n0 + nb * 32 + (lane & 31);
+                    char* const o = g.out + q * g.out_pitch + (uint64_t)(m0 + (lane >> 5) * 8) * 2;
 #pragma unroll
-                for (int mp = 0; mp < S::MB; mp += PAIR) {      // 64 (32) corpus rows x 32 queries at a time, through the wave's own LDS
+                    for (int mb = 0; mb < S::MB; ++mb)
 #pragma unroll
-                    for (int mi = 0; mi < PAIR; ++mi)
+                        for (int p = 0; p < 2; ++p) {
+                            float v[8];
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const uint32_t m = m0 + (mp + mi) * 32 + (r & 3) + 8 * (r >> 2) + half4;
-                            const float v = c * __builtin_amdgcn_exp2f(fmaf(acc[mp + mi][nb][r], g.scale2, -l2.x) - l2.y);
-                            acc[mp + mi][nb][r] = c == 0.0f || m >= g.m_valid ? 0.0f : v;
-                        }
-#pragma unroll
-                    for (uint32_t plane = 0; plane < (DT == cgv::DT_F32 ? 3u : 1u); ++plane) {
-#pragma unroll
-                        for (int mi = 0; mi < PAIR; ++mi)
-#pragma unroll
-                            for (int r4 = 0; r4 < 4; ++r4) {
-                                uint16_t h[4];
-#pragma unroll
-                                for (int x = 0; x < 4; ++x) {
-                                    const float v = acc[mp + mi][nb][r4 * 4 + x];
-                                    if (DT == cgv::DT_FP16) {
-                                        h[x] = cgv::f32_to_f16_rne(v);
-                                    } else {
-                                        h[x] = cgv::f32_to_bf16_rne(v);
-                                        if (DT == cgv::DT_F32) acc[mp + mi][nb][r4 * 4 + x] = v - cgv::bf16_to_f32(h[x]);   // what the next plane holds
-                                    }
-                                }
-                                const uint32_t n = lane & 31, chunk = (uint32_t)(mi * 4 + r4) ^ row_swz(n);
-                                *(uint2*)(xp + n * 128 + chunk * 16 + half4 * 2) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+                            for (int x = 0; x < 8; ++x) {
+                                const float t = fmaf(acc[mb][nb][p * 8 + x], g.scale2, -g_lse[nb].x);
+                                // the second part of the logarithm is below the roundings of 16 bits
+                                v[x] = g_coef[nb] * __builtin_amdgcn_exp2f(DT == cgv::DT_F32 ? t - g_lse[nb].y : t);
+                                const uint32_t m = m0 + mb * 32 + p * 16 + (x & 3) + 8 * (x >> 2) + half4;
+                                if (g_coef[nb] == 0.0f || (decltype(at_edge)::value && m >= g.m_valid)) v[x] = 0.0f;
                             }
-                        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                        for (int p = 0; p < 32 / OUT; ++p) {
-                            const uint32_t n = p * OUT + lane / LPR, chunk = (uint32_t)(lane % LPR) ^ row_swz(n);
-                            const uint4 v = *(const uint4*)(xp + n * 128 + chunk * 16);
-                            const uint32_t q = n0 + nb * 32 + n;
-                            if (q < g.n_pad)
-                                *(uint4*)(g.out + plane * g.out_plane + q * g.out_pitch + (uint64_t)(m0 + mp * 32) * 2 + lane % LPR * 16) = v;
+                            for (uint32_t plane = 0; plane < (DT == cgv::DT_F32 ? 3u : 1u); ++plane) {
+                                const uint4 w = sixteen<DT>(v);
+                                if (q < g.n_pad) *(uint4*)(o + plane * g.out_plane + (mb * 32 + p * 16) * 2) = w;
+                            }
                         }
-                        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                        __builtin_amdgcn_wave_barrier();
-                    }
                 }
-            }
+            };
+            if (m0 + S::TM > g.m_valid) store(std::true_type());
+            else store(std::false_type());
         } else if (EPI == EPI_DQ) {
             float* out = (float*)(g.out + split * g.out_plane);
 #pragma unroll
@@ -697,36 +699,21 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
             const float u = *g.unscale;
 #pragma unroll
             for (int nb = 0; nb < S::NB; ++nb) {
+                const uint32_t row = n0 + nb * 32 + (lane & 31);
                 if (DT != cgv::DT_F32 && g.vec_out) {
+                    char* const o = g.out + row * g.out_pitch;
 #pragma unroll
-                    for (int mp = 0; mp < S::MB; mp += PAIR) {
+                    for (int mb = 0; mb < S::MB; ++mb)
 #pragma unroll
-                        for (int mi = 0; mi < PAIR; ++mi)
+                        for (int p = 0; p < 2; ++p) {
+                            float v[8];
 #pragma unroll
-                            for (int r4 = 0; r4 < 4; ++r4) {
-                                uint16_t h[4];
-#pragma unroll
-                                for (int x = 0; x < 4; ++x) {
-                                    const float v = acc[mp + mi][nb][r4 * 4 + x] * u;
-                                    h[x] = DT == cgv::DT_FP16 ? cgv::f32_to_f16_rne(v) : cgv::f32_to_bf16_rne(v);
-                                }
-                                const uint32_t n = lane & 31, chunk = (uint32_t)(mi * 4 + r4) ^ row_swz(n);
-                                *(uint2*)(xp + n * 128 + chunk * 16 + half4 * 2) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
-                            }
-                        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                        for (int p = 0; p < 32 / OUT; ++p) {
-                            const uint32_t n = p * OUT + lane / LPR, chunk = (uint32_t)(lane % LPR) ^ row_swz(n);
-                            const uint4 v = *(const uint4*)(xp + n * 128 + chunk * 16);
-                            const uint32_t row = n0 + nb * 32 + n, m = m0 + mp * 32 + lane % LPR * 8;
-                            if (row < g.n_valid && m < g.m_valid) *(uint4*)(g.out + row * g.out_pitch + m * 2) = v;   // m_valid: a multiple of 8
+                            for (int x = 0; x < 8; ++x) v[x] = acc[mb][nb][p * 8 + x] * u;
+                            const uint4 w = sixteen<DT>(v);
+                            const uint32_t m = m0 + mb * 32 + p * 16 + (lane >> 5) * 8;
+                            if (row < g.n_valid && m < g.m_valid) *(uint4*)(o + m * 2) = w;      // m_valid: a multiple of 8
                         }
-                        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                        __builtin_amdgcn_wave_barrier();
-                    }
                 } else {
-                    const uint32_t row = n0 + nb * 32 + (lane & 31);
 #pragma unroll
                     for (int mb = 0; mb < S::MB; ++mb)
 #pragma unroll
@@ -749,10 +736,6 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
                         }
                 }
             }
-        }
-        if constexpr (UNEVEN && XPOSE) {
-            __builtin_amdgcn_s_barrier();                                 // every wave's results have left their places
-            asm volatile("" ::: "memory");
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in LDS behind the workgroup's end

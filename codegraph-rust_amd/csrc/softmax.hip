@@ -489,7 +489,7 @@ void set_segments(Args& a, int dtype, bool small) {
 
 template <int DT, class S, bool TA, bool TB, int EPI>
 int launch_gemm(const Args& a, int device, hipStream_t s) {
-    constexpr int bytes = S::lds_bytes(EPI == EPI_G || EPI == EPI_DR, EPI != EPI_DR);
+    constexpr int bytes = S::lds_bytes(EPI != EPI_DR);
     if (a.blocks == 0) return CGV_OK;
     void (*kern)(const Args) = gemm_kernel<DT, S, TA, TB, EPI>;
     static LdsLimit limit;
@@ -501,7 +501,7 @@ int launch_gemm(const Args& a, int device, hipStream_t s) {
 template <int DT>
 int launch_gradients(const Args& q, const Args& r, int device, hipStream_t s) {
     typedef Small<DT> S;
-    constexpr int bytes = S::lds_bytes(true, true);
+    constexpr int bytes = S::lds_bytes(true);
     void (*kern)(const Args, const Args) = gradients_kernel<DT, S>;
     static LdsLimit limit;
     OPCHK(limit.raise((const void*)kern, device, bytes));
@@ -511,8 +511,7 @@ int launch_gradients(const Args& q, const Args& r, int device, hipStream_t s) {
 }
 template <int DT, class S, class T, bool TA, bool TB, int EPI>
 int launch_mixed(const Args& a, const Args& b, int device, hipStream_t s) {
-    constexpr bool xpose = EPI == EPI_G;
-    constexpr int bytes = std::max(S::lds_bytes(xpose, true), T::lds_bytes(xpose, true));
+    constexpr int bytes = std::max(S::lds_bytes(true), T::lds_bytes(true));
     void (*kern)(const Args, const Args) = mixed_kernel<DT, S, T, TA, TB, EPI>;
     static LdsLimit limit;
     OPCHK(limit.raise((const void*)kern, device, bytes));
