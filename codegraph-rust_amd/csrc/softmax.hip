@@ -403,8 +403,8 @@ struct Plan {
         planes = dtype == CGV_DTYPE_F32 ? 3 : 1;
         copy = dtype == CGV_DTYPE_F32 || dim % 8 != 0;
         // the tile width whose padded batch takes the least time. Narrower tiles read LDS more often per product: 768 queries over 200 k x 768
-        // (bf16, loss and both gradients) take 1.29 ms with tiles of 256, 1.35 with 192, 1.48 with 128, 1.91 with 64. Against that stands the
-        // padding: 576 queries take 0.99 ms with 192, 1.06 with 256, 1.14 with 128
+        // (bf16, loss and both gradients) take 1.19 ms with tiles of 256, 1.22 with 192, 1.28 with 128, 1.63 with 64. Against that stands the
+        // padding: 576 queries take 0.84 ms with 192, 0.93 with 256, 0.92 with 128
         // The scores' last column may be narrower than the others (loss of 320 queries as 192 + 128: 130 us, as 2 x 192: 163 us). Not so dQ's:
         // columns with different shares of the corpus do not read it together (300 queries x 300 k x 1000: 339 us, with equal columns 304 us)
         double least = 1e30;
@@ -422,7 +422,7 @@ struct Plan {
             }
         bm = 256;
         // few tiles: small ones on more CUs, with more stages on the way. Loss and gradients of 256 queries x 768 with small and with large tiles,
-        // bf16: 127 and 134 us at 20 k rows, 156 and 148 at 25 k; f32: 317 and 401 us at 20 k, 481 and 512 at 30 k
+        // bf16: 107 and 122 us at 20 k rows, 157 and 148 at 25 k; f32: 316 and 371 us at 20 k, 473 and 484 at 30 k
         if ((n_ + 255) / 256 * ((bp - bn2 + bn - 1) / bn + (bn2 > 0)) < (planes == 3 ? CUS / 2 : CUS * 3 / 8)) bm = bn = dqn = 64, bn2 = 0;
         columns = (bp - bn2 + bn - 1) / bn;
         off = bn2 ? columns * bn : bp;
@@ -438,7 +438,7 @@ struct Plan {
         dq_splits = std::max<uint32_t>(1, std::min<uint32_t>((uint32_t)(piece_b / BK), CUS / ((dp + bm - 1) / bm * dq_columns)));
     }
     static constexpr uint32_t WIDTH[4] = {256, 192, 128, 64};
-    static double cost(uint32_t w) { return w / (w == 256 ? 1.0 : w == 192 ? 0.95 : w == 128 ? 0.87 : 0.68); }
+    static double cost(uint32_t w) { return w / (w == 256 ? 1.0 : w == 192 ? 0.98 : w == 128 ? 0.93 : 0.73); }
     static uint32_t wave_rows(uint32_t bm, uint32_t bn) { return bm == 64 ? S64x64::WM : bn == 256 ? S256::WM : S64::WM; }
     uint32_t slots(Shares s) const { return std::max(s.s1 * wave_rows(bm, bn), bn2 ? s.s2 * wave_rows(bm, bn2) : 0u); }
     // shares of `tm` rows of tiles that occupy the card and end together, no more than the same time needs
@@ -661,7 +661,8 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
         a.out_pitch = g_pitch;
         a.out_plane = g_plane;
         if ((rc = launch_scores<DT, EPI_G>(pl, a, pl.score_shares(a.tm), P.device, s))) return rc;
-        // the corpus' gradient: large tiles if they are enough to occupy half the card; in small ones both gradients share a launch
+        // the corpus' gradient: large tiles if they are enough to occupy half the card (256 queries x 20 k x 768 bf16, both gradients: 72 us, in
+        // small ones 81); in small ones both gradients share a launch
         const bool big = dr && (uint64_t)((pl.dim + 255) / 256) * ((c + 255) / 256) >= CUS / 2, together = dq && dr && !big && pl.bm == 64;
         Args d{}, e{};
         if (dq) {
