@@ -12,7 +12,7 @@ static __global__ void f64_to_f32_kernel(const double* __restrict__ in, uint64_t
 
 extern "C" {
 
-uint32_t cgv_version(void) { return (0u << 16) | 9u; }  // 0.9: + sample-repair stats (0.8: scalar-arm normalise, small-batch stats, phase times, synthetic inputs)
+uint32_t cgv_version(void) { return (0u << 16) | 10u; }  // 0.10: + cgvec_q4.h, cgvec_train.h (0.9: sample-repair stats; 0.8: scalar-arm normalise, small-batch stats, phase times, synthetic inputs)
 
 // internal: lets the host mirror (host/store.cpp) share this library's thread-local error message
 int cgv_set_error_(int code, const char* msg) {

@@ -1,4 +1,4 @@
-// kernels_gemm.h - the matrix products behind the softmax losses (softmax.hip): one persistent MFMA kernel, three products, four
+// kernels_gemm.h - the matrix products behind the softmax losses (softmax.hip): one persistent MFMA loop, three products, four
 // epilogues. Written from the formulas: with S = c Q R^T, G = dL/dS * c,
 //     scores   M = corpus rows, N = queries,     K = elements   -> running maximum and sum of exp per query, or a piece of G
 //     dQ       M = elements,    N = queries,     K = corpus     -> f32 partial sums, one slot per share of the corpus
@@ -13,8 +13,17 @@
 // [query][corpus], dQ and dR.
 //
 // f32 inputs are three bf16 planes x = h + m + l (8 bits each, exact); a product is the six plane products of weight 2^0 .. 2^-16
-// (the three left out are below 2^-24 of it), added from the smallest up in the same f32 accumulators: six passes of bf16 MFMA run
-// at 2.5 / 6 = 0.42 PFLOP/s, the f32 MFMA at 0.16.
+// (the three left out are below 2^-24 of it), added in f32 from the smallest up, or the five small ones in a sum of their own: six passes
+// of bf16 MFMA run at 2.5 / 6 = 0.42 PFLOP/s, the f32 MFMA at 0.16.
+//
+// Workgroup tiles of 256 corpus rows x 256 queries, eight waves of 128 x 64: 128 accumulators leave room for two waves a SIMD and two sets
+// of fragments. Stages of 64 elements of K (128 bytes of a row: shorter pieces load at less than half the rate) go from memory to LDS
+// directly; a wave issues its loads one at a time between matrix instructions, as a burst behind the barrier they held the wave up
+// (scores of 1024 x 125 k x 768 bf16: 216 us, spread 177). One barrier a stage. Bound by the matrix cores at the clock that they
+// leave (bf16, same sizes, 197 GFLOP each): scores 177 us with their exponentials, dQ 173 us, dR 202 us and G 205 us with 190 and 256 MB of
+// results; matrix pipes busy 0.66, 0.71 and 0.58 of the time (scores, dQ, dR) at 1.5 .. 1.6 GHz. What is left of the scores' time are the
+// exponentials, a sixth of it, which nothing runs beside: both waves of a SIMD reach them at the same barrier, and two workgroups of
+// 128 x 128 on a CU, which would not, load twice as much (scores 252 us, dQ 253 us).
 #pragma once
 #include <type_traits>
 
@@ -112,6 +121,7 @@ __device__ inline uint32_t seg_swz(uint32_t k) {
 template <bool T, int W, int NW>
 struct Loader {
     static constexpr int I = W / 8 / NW;          // 1-KiB instructions of a wave
+    static_assert(!T || 1024 % (W * 2) == 0, "columns form: an instruction loads whole k-rows");
     uint32_t voff[I];
     // first = first row / column of the tile; elems: elements of K that exist from the stage's first on, 64 but for the last stage.
     // Rows form: the missing ones are read as the row's last eight (the other operand holds zeros there); columns form: as the last k-row

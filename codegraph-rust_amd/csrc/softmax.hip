@@ -4,12 +4,16 @@
 //           sum of exp per query; loss.
 // backward  per piece of the corpus: G = c (exp(s - lse) - p) in 16 bits (three planes for f32), dQ += G R in f32 partial sums,
 //           dR = G^T Q; then dQ's partial sums are added and rounded.
+// Four products of 2 b n dim operations (the scores twice: keeping them would be the matrix that is not to be stored). 1024 queries x
+// 1M x 768 bf16, loss and both gradients: 5.79 ms = 1.09 PFLOP/s; 256 x 1M x 1536 fp16, loss alone: 0.79 ms = 1.0 PFLOP/s, 3.9 TB/s.
 //
 // Two things keep a small loss and a small gradient exact where exp(s - lse) is close to 1. The heaviest listed row (the anchor) is
 // left out of the sum over the corpus: tail = lse - s_anchor = log(1 + sum of the others' exp(s - s_anchor)) then comes from log1p
 // and not from the difference of two large numbers, and the anchor's 1 - exp(s - lse) is -expm1(-tail). And the listed rows' entries
 // of G, softmax minus weight, are computed in f32 from the saved scores and put into G as differences, before any rounding.
 //
+// For 16-bit inputs G is rounded to their type, which is what the matrix cores multiply their rows with: bf16 gradients are off by 0.0023
+// of their norm against 64 bits, 0.0017 of it from the rounding of the result itself.
 // fp16: G is scaled by a power of two that brings the largest |dloss * scale| to 2^13 .. 2^14 (softmax values of 1e-9 are then still
 // above the type's smallest step); the products' results are scaled back in f32.
 #include <type_traits>

@@ -1,5 +1,6 @@
 """ctypes binding of include/cgvec_train.h with torch's autograd: rows of a table by id, and the losses that train what an index
-serves. CUDA tensors only (there is no CPU fallback); every call enqueues on torch's current stream of the tensors' device."""
+serves. CUDA tensors only (there is no CPU fallback); every call enqueues on torch's current stream of the tensors' device and can be captured
+into a graph. (A backward pass is captured without eager autograd graphs of the same leaves alive, as torch asks for.)"""
 import ctypes as C
 
 import torch
