@@ -19,9 +19,9 @@
 // Workgroup tiles of 256 corpus rows x 256 queries, eight waves of 128 x 64: 128 accumulators leave room for two waves a SIMD and two sets
 // of fragments. Stages of 64 elements of K (128 bytes of a row: shorter pieces load at less than half the rate) go from memory to LDS
 // directly; a wave issues its loads one at a time between matrix instructions, as a burst behind the barrier they held the wave up
-// (scores of 1024 x 125 k x 768 bf16: 216 us, spread 177). One barrier a stage. Bound by the matrix cores at the clock that they
-// leave (bf16, same sizes, 197 GFLOP each): scores 177 us with their exponentials, dQ 173 us, dR 202 us and G 205 us with 190 and 256 MB of
-// results; matrix pipes busy 0.66, 0.71 and 0.58 of the time (scores, dQ, dR) at 1.5 .. 1.6 GHz. What is left of the scores' time are the
+// (scores of 1024 x 125 k x 768 bf16: 198 us, spread 177). One barrier a stage. Bound by the matrix cores at the clock that they
+// leave (bf16, same sizes, 197 GFLOP each): scores 173 us with their exponentials, dQ 171 us, dR 186 us and G 203 us with 192 and 256 MB of
+// results; matrix pipes busy 0.65, 0.71, 0.55 and 0.54 of the time at 1.5 .. 1.8 GHz. What is left of the scores' time are the
 // exponentials, a sixth of it, which nothing runs beside: both waves of a SIMD reach them at the same barrier, and two workgroups of
 // 128 x 128 on a CU, which would not, load twice as much (scores 252 us, dQ 253 us).
 #pragma once
@@ -414,9 +414,16 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
     constexpr int LOADS = S::PL * (IA + IB);                                  // of a stage
     constexpr int FIRST = UNEVEN ? SHORT : (LOADS + 2) / 3;                   // of those that follow right behind the stage's change
     constexpr int WAIT = UNEVEN ? IA + IB - SHORT : (NST - 2) * LOADS;        // of what lies behind the next stage
+    // dR: the results of a whole wave tile are at least STORED stores (16 bytes a lane is the widest there is). They count like loads and in
+    // turn with them; the first stage behind them needs only what was issued before them, and so does not wait for them (1024 x 125 k x
+    // 768 bf16: 235 -> 219 us; G, with the same, gains nothing)
+    constexpr int STORED = EPI == EPI_DR && DT != cgv::DT_F32 && UNEVEN ? 2 * S::MB * S::NB : 0;
+    bool stored = false;
     auto stage_ready = [&]() {
         // this wave's part of the next stage has landed, its reads of this one are done
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(WAIT) : "memory");
+        if (STORED && stored) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(WAIT + STORED) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(WAIT) : "memory");
+        stored = false;
         __builtin_amdgcn_s_barrier();                                 // everybody's: the next stage can be read, this one overwritten
         asm volatile("" ::: "memory");
     };
@@ -707,6 +714,7 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
             }
         } else {   // EPI_DR
             const float u = *g.unscale;
+            stored = g.vec_out && m0 + S::TM <= g.m_valid && n0 + S::TN <= g.n_valid;
 #pragma unroll
             for (int nb = 0; nb < S::NB; ++nb) {
                 const uint32_t row = n0 + nb * 32 + (lane & 31);
