@@ -96,6 +96,7 @@ struct Args {
 template <int BM_, int BN_, int WM_, int WN_, int PL_ = 1>
 struct Shape {
     static constexpr int PL = PL_;
+    static constexpr bool ONCE = false;           // A is read past the caches
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM_ * WN_, THREADS = 64 * NW;
     static constexpr int TM = BM / WM, TN = BN / WN, MB = TM / 32, NB = TN / 32;
     static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, STAGE = PL * (A_BYTES + B_BYTES);
@@ -105,6 +106,11 @@ struct Shape {
     // share through L2, has two
     static constexpr bool UNEVEN = STAGES == 2;
     static constexpr int lds_bytes(bool long_a) { return STAGES * STAGE + (UNEVEN ? long_a ? A_BYTES : B_BYTES : 0); }
+};
+
+template <class S>
+struct Once : S {
+    static constexpr bool ONCE = true;
 };
 
 // swizzle of a row's eight 16-byte pieces: 16 consecutive rows put the same piece at 16 different places of the 256 bytes that the
@@ -140,13 +146,15 @@ struct Loader {
             }
         }
     }
+    template <int AUX>
     __device__ void issue_one(int i, const char* base, uint32_t soff, char* lds, int wave) const {
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(lds + (wave * I + i) * 1024), 16, voff[i], soff, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(lds + (wave * I + i) * 1024), 16, voff[i], soff, 0, AUX);
     }
+    template <int AUX>
     __device__ void issue(const char* base, uint32_t soff, char* lds, int wave) const {
 #pragma unroll
-        for (int i = 0; i < I; ++i) issue_one(i, base, soff, lds, wave);
+        for (int i = 0; i < I; ++i) issue_one<AUX>(i, base, soff, lds, wave);
     }
 };
 
@@ -308,13 +316,14 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
         pb = uniform(pb);
     };
     char *const smem_a = smem, *const smem_b = smem + NSA * S::PL * S::A_BYTES;
+    constexpr int AUX = S::ONCE ? 2 : 0;              // of A's loads: nontemporal
     auto issue_a = [&](const Loader<TA, S::BM, S::NW>& l, const char* base, uint32_t off, int slot) {
 #pragma unroll
-        for (int p = 0; p < S::PL; ++p) l.issue(base + p * g.a.plane, off, smem_a + (slot * S::PL + p) * S::A_BYTES, wave);
+        for (int p = 0; p < S::PL; ++p) l.template issue<AUX>(base + p * g.a.plane, off, smem_a + (slot * S::PL + p) * S::A_BYTES, wave);
     };
     auto issue_b = [&](const Loader<TB, S::BN, S::NW>& l, const char* base, uint32_t off, int slot) {
 #pragma unroll
-        for (int p = 0; p < S::PL; ++p) l.issue(base + p * g.b.plane, off, smem_b + (slot * S::PL + p) * S::B_BYTES, wave);
+        for (int p = 0; p < S::PL; ++p) l.template issue<0>(base + p * g.b.plane, off, smem_b + (slot * S::PL + p) * S::B_BYTES, wave);
     };
     // UNEVEN: the short operand's stage before the prepared one, still to be loaded (a short B is the same query tile all the time)
     Loader<TA, S::BM, S::NW> wla;
@@ -331,15 +340,15 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
     auto issue_one = [&](int q, int a, int b) {
         if constexpr (UNEVEN) {
             if (q < SHORT) {
-                if (LONG_A) lb.issue_one(q, wp, ws, smem_b + b * S::B_BYTES, wave);
-                else wla.issue_one(q, wp, ws, smem_a + a * S::A_BYTES, wave);
+                if (LONG_A) lb.template issue_one<0>(q, wp, ws, smem_b + b * S::B_BYTES, wave);
+                else wla.template issue_one<AUX>(q, wp, ws, smem_a + a * S::A_BYTES, wave);
             } else {
-                if (LONG_A) la.issue_one(q - SHORT, pa, sa, smem_a + a * S::A_BYTES, wave);
-                else lb.issue_one(q - SHORT, pb, sb, smem_b + b * S::B_BYTES, wave);
+                if (LONG_A) la.template issue_one<AUX>(q - SHORT, pa, sa, smem_a + a * S::A_BYTES, wave);
+                else lb.template issue_one<0>(q - SHORT, pb, sb, smem_b + b * S::B_BYTES, wave);
             }
         } else {
-            if (q < IA) la.issue_one(q, pa, sa, smem_a + a * S::A_BYTES, wave);
-            else lb.issue_one(q - IA, pb, sb, smem_b + b * S::B_BYTES, wave);
+            if (q < IA) la.template issue_one<AUX>(q, pa, sa, smem_a + a * S::A_BYTES, wave);
+            else lb.template issue_one<0>(q - IA, pb, sb, smem_b + b * S::B_BYTES, wave);
         }
     };
     auto issue = [&](int a, int b) {

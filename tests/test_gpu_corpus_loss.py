@@ -153,6 +153,18 @@ def test_batches_in_columns_of_two_widths(b, n, d, k, dt):
     assert bool((dq[b - 2] == 0).all())
 
 
+@pytest.mark.parametrize("b,n,d,dt", [(3, 700_001, 200, "bf16"), (100, 300_000, 456, "fp16"), (190, 130_001, 1040, "bf16"), (250, 270_000, 520, "fp16")])
+def test_a_corpus_that_no_cache_holds(b, n, d, dt):
+    """One column of tiles over more than 256 MiB of rows."""
+    m = pkg()
+    q, r, ids, sc, g = _problem(b, n, d, 2, dt, 9)
+    ids[b - 1] = n - 1
+    ref = _reference(q, r, ids, sc, g, 8.0, 3.0)
+    loss = m.corpus_distillation(q, r, ids, sc, scale=8.0, teacher_scale=3.0)
+    _check(loss, None, None, ref, d, n, 8.0, dt, g)
+    assert torch.equal(loss, m.corpus_distillation(q, r, ids, sc, scale=8.0, teacher_scale=3.0))
+
+
 def test_a_million_queries_with_long_lists():
     """More than 2^32 threads' worth of lists."""
     m = pkg()
