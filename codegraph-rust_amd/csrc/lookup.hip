@@ -4,8 +4,9 @@
 // row and adds up its summands, so that each row is written exactly once and no atomics touch a float; for that the positions
 // are sorted by id first (stable, so that a row's summands come in the order of the input).
 //   few ids (<= DIRECT_IDS): a workgroup owns some table rows, looks through all ids itself, and there is one launch;
-//   more: radix sort of (id, position), 11 bits at most a pass; a run's ends are noted per row; rows whose run is longer than
-//   LONG positions are first summed in pieces of LONG by separate waves (a frequent token would otherwise keep one thread busy).
+//   more: (id, position) sorted, by one workgroup up to SMALL_SORT of them, else by radix, 11 bits at most a pass; a run's ends are
+//   noted per row; rows whose run is longer than `longer` positions are first summed in pieces of that many by separate waves (a
+//   frequent token would otherwise keep one thread busy).
 // Bound by the bytes of the incoming rows and of the whole table gradient. 65 536 ids, 100 k x 768 f32: forward 61 us (402 MB, 6.6 TB/s), rows
 // of the gradient 100 us (508 MB, 5.1 TB/s), pieces of long runs 18 us, sorting 33 us; 10 240 rows of 768 bf16: 8 us.
 #include <type_traits>
@@ -17,7 +18,11 @@ using namespace cgv_ops;
 
 namespace {
 
-constexpr uint32_t DIRECT_IDS = 512;
+// Without sorting a row's summands come one after another. 10 k x 384 fp16, ids at random / all the same: 250 ids 10 / 99 us, sorted 22 / 21;
+// 500 ids 10 / 195, sorted 21 / 22
+constexpr uint32_t DIRECT_IDS = 256;
+// One workgroup's sort against the radix passes, six launches: 1000 ids 23 and 30 us, 2000 ids 30 and 31, 4000 ids 46 and 33
+constexpr uint32_t SMALL_SORT = 2048;
 constexpr uint32_t SORT_THREADS = 256, SORT_STEPS = 4, SORT_BLOCK = SORT_THREADS * SORT_STEPS;   // elements of a workgroup
 constexpr uint32_t MAX_DIGIT = 11;
 constexpr uint32_t FLIGHT = 4;
@@ -261,6 +266,38 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(SortPass p) 
     }
 }
 
+// up to SMALL_SORT ids: one workgroup sorts (key, position) in its LDS, in the order of a bitonic network - positions differ, so the order is
+// the stable one -, and the others clear the rows' run ends
+__global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restrict__ ids, uint32_t n, uint32_t n_rows, uint32_t* __restrict__ keys,
+                                                          uint32_t* __restrict__ pos, uint64_t* __restrict__ runs) {
+    if (blockIdx.x) {
+        for (uint64_t i = (uint64_t)(blockIdx.x - 1) * 1024 + threadIdx.x; i < n_rows; i += (uint64_t)(gridDim.x - 1) * 1024) runs[i] = 0;
+        return;
+    }
+    __shared__ uint64_t a[SMALL_SORT];
+    uint32_t size = 2;
+    while (size < n) size *= 2;
+    for (uint32_t i = threadIdx.x; i < size; i += 1024) {
+        const int64_t id = i < n ? ids[i] : -1;
+        const uint32_t key = id >= 0 && id < (int64_t)n_rows ? (uint32_t)id : n_rows;      // strangers go behind the last row
+        a[i] = i < n ? (uint64_t)key << 32 | i : ~0ull;
+    }
+    for (uint32_t k = 2; k <= size; k *= 2)
+        for (uint32_t j = k / 2; j; j /= 2) {
+            __syncthreads();
+            for (uint32_t t = threadIdx.x; t < size / 2; t += 1024) {
+                const uint32_t lo = t / j * 2 * j + t % j, hi = lo + j;
+                const uint64_t x = a[lo], y = a[hi];
+                if ((x > y) == ((lo & k) == 0)) a[lo] = y, a[hi] = x;
+            }
+        }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += 1024) {
+        keys[i] = (uint32_t)(a[i] >> 32);
+        pos[i] = (uint32_t)a[i];
+    }
+}
+
 // runs[r] = where the positions of row r begin (low word) and end (high word)
 __global__ __launch_bounds__(256) void runs_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t n_rows, uint32_t* __restrict__ runs) {
     const uint32_t i = blockIdx.x * 256 + threadIdx.x;
@@ -288,7 +325,7 @@ __device__ inline void sum_positions(Vec<DT, V>& acc, const void* dout, const ui
     }
 }
 
-// piece c of LONG sorted positions: a run longer than LONG crosses an end of every piece it touches, so a piece has at most two
+// piece c of `longer` sorted positions: a longer run crosses an end of every piece it touches, so a piece has at most two
 // such runs - the one of its first position (slot 2 c) and the one of its last (slot 2 c + 1)
 template <int DT, int V>
 __global__ __launch_bounds__(64) void pieces_kernel(const void* __restrict__ dout, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
@@ -440,7 +477,13 @@ int launch_grad(const void* dout, const int64_t* ids, uint64_t n_ids, uint64_t n
         return CGV_OK;
     }
     uint64_t* runs = (uint64_t*)(ws + pl.off_runs);
-    for (uint32_t i = 0; i < pl.passes; ++i) {
+    const uint32_t last = n_ids <= SMALL_SORT ? 0 : (pl.passes - 1) & 1;
+    if (n_ids <= SMALL_SORT) {
+        hipLaunchKernelGGL(sort_small_kernel, dim3(1 + (unsigned)std::min<uint64_t>((n_rows + 4095) / 4096, 1024)), dim3(1024), 0, s, ids, (uint32_t)n_ids,
+                           (uint32_t)n_rows, (uint32_t*)(ws + pl.off_keys[0]), (uint32_t*)(ws + pl.off_pos[0]), runs);
+        OPCHK(hipGetLastError());
+    }
+    for (uint32_t i = 0; i < pl.passes && n_ids > SMALL_SORT; ++i) {
         SortPass p{};
         p.ids = i == 0 ? ids : nullptr;
         p.keys = (const uint32_t*)(ws + pl.off_keys[(i + 1) & 1]);
@@ -462,7 +505,6 @@ int launch_grad(const void* dout, const int64_t* ids, uint64_t n_ids, uint64_t n
         hipLaunchKernelGGL(sort_scatter_kernel, dim3(pl.blocks), dim3(SORT_THREADS), 0, s, p);
         OPCHK(hipGetLastError());
     }
-    const uint32_t last = (pl.passes - 1) & 1;
     const uint32_t* keys = (const uint32_t*)(ws + pl.off_keys[last]);
     const uint32_t* pos = (const uint32_t*)(ws + pl.off_pos[last]);
     float* partial = (float*)(ws + pl.off_partial);
