@@ -83,6 +83,7 @@ struct Args {
     uint32_t part_ld;
     const float* coef;                            // G: [n] factor
     const float2* lse2;                           // G: [n] log2 of the softmax sum, its f32 and what that leaves
+    uint32_t twin;                                // G: from this column on, what 16 bits leave of the entries of the column `twin` before; 0: none
     const uint32_t* ent_id;                       // G: [n][ent_k] corpus rows whose entries are given, 0xffffffff for none
     const float* ent_val;                         // G: [n][ent_k] those entries
     uint32_t ent_k;
@@ -191,6 +192,9 @@ __device__ inline uint32_t pair(float a, float b) {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
     }
 }
+// what 16 bits leave of a value
+template <int DT>
+__device__ inline float rest16(float v) { return v - cgv_ops::half_to_f32<DT>(cgv_ops::f32_to_half<DT>(v)); }
 // A lane's rows (x & 3) + 8 (x >> 2) + 4 (lane >> 5), x < 8, of its column in 16 bits -> the column's rows 8 (lane >> 5) + 0 .. 7, which are
 // neighbours in memory: the lanes l and l + 32 trade halves. f32: the largest plane, and v keeps what it leaves
 template <int DT>
@@ -689,6 +693,7 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
                                 v[x] = g_coef[nb] * __builtin_amdgcn_exp2f(DT == cgv::DT_F32 ? t - g_lse[nb].y : t);
                                 const uint32_t m = m0 + mb * 32 + p * 16 + (x & 3) + 8 * (x >> 2) + half4;
                                 if (g_coef[nb] == 0.0f || (decltype(at_edge)::value && m >= g.m_valid)) v[x] = 0.0f;
+                                if (DT != cgv::DT_F32 && g.twin && q >= g.twin) v[x] = rest16<DT>(v[x]);
                             }
 #pragma unroll
                             for (uint32_t plane = 0; plane < (DT == cgv::DT_F32 ? 3u : 1u); ++plane) {
@@ -805,7 +810,7 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
                     split3(v, p);
                     for (int i = 0; i < 3; ++i) o[i * (g.out_plane / 2)] = p[i];
                 } else {
-                    *o = cgv_ops::f32_to_half<DT>(v);
+                    *o = cgv_ops::f32_to_half<DT>(g.twin && n0 + t / g.ent_k >= g.twin ? rest16<DT>(v) : v);
                 }
             }
         }

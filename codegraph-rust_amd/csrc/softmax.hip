@@ -13,7 +13,9 @@
 // of G, softmax minus weight, are computed in f32 from the saved scores and put into G as differences, before any rounding.
 //
 // For 16-bit inputs G is rounded to their type, which is what the matrix cores multiply their rows with: bf16 gradients are off by 0.0023
-// of their norm against 64 bits, 0.0017 of it from the rounding of the result itself.
+// of their norm against 64 bits, 0.0017 of it from the rounding of the result itself. Over many queries these roundings average out. Up to
+// TWINS queries leave half of a tile's columns empty: there what the rounding leaves of G is stored and multiplied too (3 queries x 326 x
+// 123 bf16: 0.0029 without, 0.0018 with).
 // fp16: G is scaled by a power of two that brings the largest |dloss * scale| to 2^13 .. 2^14 (softmax values of 1e-9 are then still
 // above the type's smallest step); the products' results are scaled back in f32.
 #include <type_traits>
@@ -28,7 +30,7 @@ using namespace cgv_gemm;
 namespace {
 
 constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
-constexpr uint32_t MAX_K = 256, NONE = 0xffffffffu;
+constexpr uint32_t MAX_K = 256, NONE = 0xffffffffu, TWINS = 32;
 constexpr uint32_t CUS = 256;                                  // workgroups of one per CU that fill the card
 // of G, and of copied corpus rows. Each piece costs a round over dQ's partial sums (1024 x 500 k x 768, gradient: 3.05 ms with 128 MiB, 2.99 with
 // 512, 2.97 with 1024); the corpus' gradient needs some 256 tiles a piece, however many queries there are
@@ -186,6 +188,7 @@ struct Problem {
     float scale, tscale;
     uint16_t* qws;            // [planes][bp][dp]
     int device;
+    uint32_t twin;            // backward: query i also stands at twin + i; 0: it does not
 };
 
 // (the first piece of the corpus is copied by further workgroups of the same launch)
@@ -287,14 +290,15 @@ __global__ __launch_bounds__(256) void backward_prep_kernel(Problem P, const flo
     if (block >= P.bp) return copy_piece_block<DT>(first_piece, block - P.bp);
     __shared__ uint32_t ids[MAX_K];
     __shared__ double ps[MAX_K];
-    const uint32_t i = (uint32_t)block, wave = threadIdx.x >> 6;
+    const uint32_t place = (uint32_t)block, i = P.twin && place >= P.twin ? place - P.twin : place, wave = threadIdx.x >> 6;
     const int lane = threadIdx.x & 63;
     const uint64_t plane = (uint64_t)P.bp * P.dp;
-    uint16_t* dst = P.qws + (uint64_t)i * P.dp;
-    if (i == 0 && threadIdx.x < 2) mul[threadIdx.x] = 1.0f;
+    uint16_t* dst = P.qws + (uint64_t)place * P.dp;
+    if (place == 0 && threadIdx.x < 2) mul[threadIdx.x] = 1.0f;
     if (i >= P.b) {
         copy_row<DT>(nullptr, 0, P.dim, P.dp, dst, plane, threadIdx.x, 256);
-        if (threadIdx.x == 0) coef[i] = 0.0f, lse2[i] = make_float2(0.0f, 0.0f), has[i] = 0;
+        if (threadIdx.x == 0) coef[place] = 0.0f, lse2[place] = make_float2(0.0f, 0.0f), has[place] = 0;
+        if (P.twin && threadIdx.x < P.k) ent_id[(uint64_t)place * P.k + threadIdx.x] = NONE;
         return;
     }
     const List l = read_list(P.ids, P.tscores, i, P.k, P.n_rows, P.tscale, lane);
@@ -302,10 +306,10 @@ __global__ __launch_bounds__(256) void backward_prep_kernel(Problem P, const flo
     const double* sv = P.saved + (uint64_t)i * (P.k + 2);
     const float c = l.has ? dloss[i] * P.scale : 0.0f;
     if (threadIdx.x == 0) {
-        coef[i] = c;
+        coef[place] = c;
         const double l2 = l.has ? sv[0] * LOG2E : 0.0;
-        lse2[i] = make_float2((float)l2, (float)(l2 - (double)(float)l2));
-        has[i] = l.has;
+        lse2[place] = make_float2((float)l2, (float)(l2 - (double)(float)l2));
+        has[place] = l.has;
     }
     if (wave == 0)
         for (int x = 0; x < 4; ++x) {
@@ -328,8 +332,8 @@ __global__ __launch_bounds__(256) void backward_prep_kernel(Problem P, const flo
     }
     double v = 0.0;
     if (first) v = id == aid ? expm1(-sv[1]) + other : exp(sv[2 + j] - sv[0]) - same;
-    ent_id[(uint64_t)i * P.k + j] = first ? id : NONE;
-    ent_val[(uint64_t)i * P.k + j] = (float)(v * c);
+    ent_id[(uint64_t)place * P.k + j] = first ? id : NONE;
+    ent_val[(uint64_t)place * P.k + j] = (float)(v * c);
 }
 
 // fp16: the power of two that brings the largest factor to 2^13 .. 2^14, and its inverse
@@ -353,7 +357,8 @@ __global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ c
 
 // dQ: the shares' partial sums, added in a fixed order and rounded once. 64 threads a stretch of 256 elements, four groups of shares
 template <int DT>
-__global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict__ part, uint32_t splits, uint64_t share, uint32_t b, uint32_t dim, uint32_t dp,
+__global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict__ part, uint32_t splits, uint64_t share, uint32_t b, uint32_t twin,
+                                                        uint32_t dim, uint32_t dp,
                                                         const uint32_t* __restrict__ has, const float* __restrict__ mul, void* __restrict__ dq) {
     __shared__ float4 sum[4][64];
     const uint32_t stretches = (dim + 255) / 256;
@@ -366,6 +371,10 @@ __global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict_
         for (uint32_t x = group; x < splits; x += 4) {
             const float4 v = *(const float4*)(part + x * share + i * dp + e);
             s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+            if (twin) {
+                const float4 w = *(const float4*)(part + x * share + (i + twin) * dp + e);
+                s = make_float4(s.x + w.x, s.y + w.y, s.z + w.z, s.w + w.w);
+            }
         }
     sum[group][t] = s;
     __syncthreads();
@@ -475,7 +484,8 @@ struct Plan {
     // backward workspace
     uint64_t b_coef() const { return q_bytes(); }                       // lse2 (two f32), coef, has: [bp] each; mul: [2]
     uint64_t b_ent() const { return b_coef() + up((uint64_t)bp * 16 + 8, 256); }
-    uint64_t b_g() const { return b_ent() + up((uint64_t)b * k * 8, 256); }
+    uint32_t twin() const { return planes == 1 && b <= TWINS ? TWINS : 0; }
+    uint64_t b_g() const { return b_ent() + up((uint64_t)bp * k * 8, 256); }
     uint64_t b_part() const { return b_g() + up((uint64_t)planes * bp * piece_b * 2, 256); }
     uint64_t b_rows() const { return b_part() + up((uint64_t)dq_splits * bp * dp * 4, 256); }
     uint64_t b_bytes() const { return b_rows() + r_bytes(piece_b); }
@@ -642,7 +652,8 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
     uint32_t* has = (uint32_t*)(coef + pl.bp);
     float* mul = (float*)(has + pl.bp);
     uint32_t* ent_id = (uint32_t*)(ws + pl.b_ent());
-    float* ent_val = (float*)(ent_id + (uint64_t)pl.b * pl.k);
+    float* ent_val = (float*)(ent_id + (uint64_t)pl.bp * pl.k);
+    P.twin = pl.twin();
     char* G = ws + pl.b_g();
     float* part = (float*)(ws + pl.b_part());
     const uint64_t g_pitch = pl.piece_b * 2, g_plane = (uint64_t)pl.bp * g_pitch;
@@ -668,6 +679,8 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
         a.coef = coef;
         a.lse2 = lse2;
         a.unscale = mul;
+        if (P.twin) a.n_valid = pl.bp;
+        a.twin = P.twin;
         a.row0 = n0;
         a.ent_id = ent_id;
         a.ent_val = ent_val;
@@ -691,7 +704,7 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             d.splits = pl.dq_splits;
             d.blocks = d.tm * d.tn * d.splits;
             d.m_valid = pl.dp;
-            d.n_valid = pl.b;
+            d.n_valid = P.twin ? pl.bp : pl.b;
             d.part_ld = pl.dp;
             d.out = (char*)part;
             d.out_plane = (uint64_t)pl.bp * pl.dp * 4;
@@ -724,7 +737,7 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
     }
     if (dq) {
         hipLaunchKernelGGL((finish_dq_kernel<DT>), wide_grid((uint64_t)pl.b * ((pl.dim + 255) / 256)), dim3(256), 0, s, (const float*)part, pl.dq_splits, (uint64_t)pl.bp * pl.dp,
-                           pl.b, pl.dim, pl.dp, (const uint32_t*)has, (const float*)mul, dq);
+                           pl.b, P.twin, pl.dim, pl.dp, (const uint32_t*)has, (const float*)mul, dq);
         OPCHK(hipGetLastError());
     }
     return CGV_OK;
@@ -777,7 +790,7 @@ int cgv_corpus_loss_dev(int device_id, const void* queries_dev, uint64_t query_s
         DeviceScope dev(device_id);
         OPCHK(dev.enter());
         const Problem P{queries_dev, rows_dev, query_stride, row_stride, n_rows, ids_dev, teacher_scores_dev, saved_dev,
-                        pl.b, pl.bp, dim, pl.dp, k, scale, teacher_scale, nullptr, device_id};
+                        pl.b, pl.bp, dim, pl.dp, k, scale, teacher_scale, nullptr, device_id, 0};
         return by_dtype(dtype, [&](auto t) { return forward<decltype(t)::value>(pl, P, dtype, loss_dev, (char*)workspace_dev, (hipStream_t)stream); });
     });
 }
@@ -800,7 +813,7 @@ int cgv_corpus_loss_grad_dev(int device_id, const void* queries_dev, uint64_t qu
         OPCHK(dev.enter());
         const hipStream_t s = (hipStream_t)stream;
         const Problem P{queries_dev, rows_dev, query_stride, row_stride, n_rows, ids_dev, teacher_scores_dev, const_cast<double*>(saved_dev),
-                        pl.b, pl.bp, dim, pl.dp, k, scale, teacher_scale, nullptr, device_id};
+                        pl.b, pl.bp, dim, pl.dp, k, scale, teacher_scale, nullptr, device_id, 0};
         return by_dtype(dtype, [&](auto t) -> int {
             constexpr int DT = decltype(t)::value;
             if (b == 0) {

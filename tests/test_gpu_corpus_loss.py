@@ -58,7 +58,7 @@ def _reference(q, r, ids, sc, g, scale, tscale):
                 norm=q.norm(dim=1) * r.norm(dim=1).max(), q=q, r=r, w=w)
 
 
-def _check(got_loss, got_dq, got_dr, ref, d, n, scale, dt, g):
+def _check(got_loss, got_dq, got_dr, ref, d, n, scale, dt, g, u=None):
     # A score is a sum of d products in f32: partial sums stay below |q| |r|, each addition rounds by at most 2^-24 of one, signs
     # at random: 4 sqrt(d) of them (and the product's own, and the factor's). log-sum-exp: the exponentials' arguments are rounded
     # once more (2^-24 of the score), exp2 itself is good to 2^-22, their sum has errors like 4 sqrt(n) * 2^-24.
@@ -67,7 +67,7 @@ def _check(got_loss, got_dq, got_dr, ref, d, n, scale, dt, g):
     lim = rel + U * (ref["loss"].abs() + 8)
     err = (got_loss.double() - ref["loss"]).abs()
     assert bool((err <= lim).all()), ("loss", float((err / lim).max()))
-    u = max(_half_step(dt), 2.0 ** -22)           # G is rounded to the type (f32: three planes, 2^-24 of a product left out twice)
+    u = u or max(_half_step(dt), 2.0 ** -22)      # G is rounded to the type (f32: three planes, 2^-24 of a product left out twice)
     per = rel.max() + u + U * (4 * math.sqrt(max(n, got_loss.numel())) + 8)
     # fp16: entries of G below 2^-14 of the scaled range lose digits: an absolute 2^-38 of the largest factor
     # every type: a softmax value below 2^-126, the smallest normal f32, is zero - its entry of G is off by 2^-126 |dloss * scale|
@@ -151,6 +151,26 @@ def test_batches_in_columns_of_two_widths(b, n, d, k, dt):
     dq, dr = torch.autograd.grad(loss, (q, r), g)
     _check(loss.detach(), dq, dr, ref, d, n, 8.0, dt, g)
     assert bool((dq[b - 2] == 0).all())
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("b,n,d,k", [(1, 1, 8, 1), (1, 40, 17, 3), (3, 326, 123, 1), (8, 5000, 96, 256), (31, 20_000, 64, 2), (32, 60_000, 200, 5)])
+def test_few_queries_lose_nothing_to_16_bits(b, n, d, k, dt):
+    """Up to 32 queries: G is kept in two 16-bit parts, off by half a step of half a step; only the results' own rounding is left."""
+    m = pkg()
+    q, r, ids, sc, g = _problem(b, n, d, k, dt, b + n)
+    if b > 3:
+        ids[2] = -1
+    if k > 2:
+        ids[0, 2] = ids[0, 1]
+    for h in (g, torch.where(torch.arange(b, device="cuda") % 2 == 0, g, g * 2.0 ** -6)):
+        q.requires_grad_(), r.requires_grad_()
+        ref = _reference(q.detach(), r.detach(), ids, sc, h, 8.0, 3.0)
+        loss = m.corpus_distillation(q, r, ids, sc, scale=8.0, teacher_scale=3.0)
+        dq, dr = torch.autograd.grad(loss, (q, r), h)
+        _check(loss.detach(), dq, dr, ref, d, n, 8.0, dt, h, u=_half_step(dt) ** 2)
+        (only,) = torch.autograd.grad(m.corpus_distillation(q, r.detach(), ids, sc, scale=8.0, teacher_scale=3.0), (q,), h)
+        assert torch.equal(only, dq)
 
 
 @pytest.mark.parametrize("b,n,d,dt", [(3, 700_001, 200, "bf16"), (100, 300_000, 456, "fp16"), (190, 130_001, 1040, "bf16"), (250, 270_000, 520, "fp16")])
