@@ -12,8 +12,9 @@
 // and not from the difference of two large numbers, and the anchor's 1 - exp(s - lse) is -expm1(-tail). And the listed rows' entries
 // of G, softmax minus weight, are computed in f32 from the saved scores and put into G as differences, before any rounding.
 //
-// For 16-bit inputs G is rounded to their type, which is what the matrix cores multiply their rows with: bf16 gradients are off by 0.0023
-// of their norm against 64 bits, 0.0017 of it from the rounding of the result itself. Over many queries these roundings average out. Up to
+// For 16-bit inputs G is rounded to their type, which is what the matrix cores multiply their rows with: the corpus' bf16 gradient is off by
+// 0.0023 of its norm against 64 bits, 0.0017 of it from the rounding of the result itself. Over many queries these roundings average out; the
+// listed entries' are made good in dQ. Up to
 // TWINS queries leave half of a tile's columns empty: there what the rounding leaves of G is stored and multiplied too (3 queries x 326 x
 // 123 bf16: 0.0029 without, 0.0018 with).
 // fp16: G is scaled by a power of two that brings the largest |dloss * scale| to 2^13 .. 2^14 (softmax values of 1e-9 are then still
@@ -355,11 +356,21 @@ __global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ c
     }
 }
 
+// 16-bit inputs, more than TWINS queries: the listed entries of G are its largest, and often all alike, so that their roundings do not average
+// out. What 16 bits leave of them is added to dQ here (812 queries x 115 k x 64 fp16, lists of two: 0.00032 of its norm against 64 bits
+// without, 0.00021 with, which is the result's own rounding)
+struct Listed {
+    const uint32_t* id;
+    const float* val;
+    uint32_t k;               // entries of a query, 0: not needed
+    const void* rows;
+    uint64_t stride;
+};
 // dQ: the shares' partial sums, added in a fixed order and rounded once. 64 threads a stretch of 256 elements, four groups of shares
 template <int DT>
 __global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict__ part, uint32_t splits, uint64_t share, uint32_t b, uint32_t twin,
                                                         uint32_t dim, uint32_t dp,
-                                                        const uint32_t* __restrict__ has, const float* __restrict__ mul, void* __restrict__ dq) {
+                                                        const uint32_t* __restrict__ has, const float* __restrict__ mul, void* __restrict__ dq, Listed l) {
     __shared__ float4 sum[4][64];
     const uint32_t stretches = (dim + 255) / 256;
     const uint64_t i = wide_block() / stretches;
@@ -382,6 +393,14 @@ __global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict_
     if (at >= dim) return;
     float v = 0.0f;
     for (int x = 0; x < 4; ++x) v += ((const float*)sum[x])[o];
+    if (DT != cgv::DT_F32 && l.k) {
+#pragma unroll 4
+        for (uint32_t j = 0; j < l.k; ++j) {
+            const uint32_t id = l.id[i * l.k + j];
+            const float rest = rest16<DT>(l.val[i * l.k + j] * mul[0]), r = load_elem<DT>(l.rows, (id == NONE ? 0 : (uint64_t)id) * l.stride + at);
+            if (id != NONE) v = fmaf(rest, r, v);
+        }
+    }
     store_elem<DT>(dq, i * dim + at, has[i] ? v * mul[1] : 0.0f);
 }
 
@@ -737,7 +756,7 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
     }
     if (dq) {
         hipLaunchKernelGGL((finish_dq_kernel<DT>), wide_grid((uint64_t)pl.b * ((pl.dim + 255) / 256)), dim3(256), 0, s, (const float*)part, pl.dq_splits, (uint64_t)pl.bp * pl.dp,
-                           pl.b, P.twin, pl.dim, pl.dp, (const uint32_t*)has, (const float*)mul, dq);
+                           pl.b, P.twin, pl.dim, pl.dp, (const uint32_t*)has, (const float*)mul, dq, Listed{ent_id, ent_val, P.twin ? 0 : pl.k, P.rows, P.r_stride});
         OPCHK(hipGetLastError());
     }
     return CGV_OK;
