@@ -76,7 +76,7 @@ struct Args {
     float scale2;                                 // LSE, G: scores in units of log 2 = accumulator * scale2
     uint32_t m_valid, n_valid;                    // rows / columns of the result that exist
     uint32_t n_pad;                               // LSE, G: columns that have a place in part / out, n_valid rounded up to 64
-    uint64_t row0;                                // LSE, G: corpus row of m = 0
+    uint64_t row0;                                // LSE, G: corpus row of m = 0; DR: of n = 0
     const uint32_t* anchor;                       // LSE: [n] corpus row left out of the sum, 0xffffffff for none
     float2* part;                                 // LSE: [slots][part_ld] (maximum, sum), slots at least splits * WM
     uint32_t slots;
@@ -84,13 +84,13 @@ struct Args {
     const float* coef;                            // G: [n] factor
     const float2* lse2;                           // G: [n] log2 of the softmax sum, its f32 and what that leaves
     uint32_t twin;                                // G: from this column on, what 16 bits leave of the entries of the column `twin` before; 0: none
-    const uint32_t* ent_id;                       // G: [n][ent_k] corpus rows whose entries are given, 0xffffffff for none
+    const uint32_t* ent_id;                       // G, DR: [n][ent_k] corpus rows whose entries are given, 0xffffffff for none
     const float* ent_val;                         // G: [n][ent_k] those entries
-    uint32_t ent_k;
+    uint32_t ent_k, ent_n;                        // DR, small tiles: ent_n of them, all queries together, whose rounding is made good; 0: none
     char* out;                                    // G, DR, DQ
     uint64_t out_pitch, out_plane;                // bytes
     uint32_t accumulate, vec_out;                 // DQ: add to what is there; DR: 16-byte stores possible
-    const float* unscale;                         // G: [1] factor of the entries; DR: [1] factor of the result
+    const float* unscale;                         // G: [1] factor of the entries; DR: [1] factor of the result, before it that of the entries
 };
 
 // PL planes of an operand in a stage: 3 for f32 where tiles are small - each plane is then loaded once and not once per product
@@ -729,6 +729,39 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
         } else {   // EPI_DR
             const float u = *g.unscale;
             stored = g.vec_out && m0 + S::TM <= g.m_valid && n0 + S::TN <= g.n_valid;
+            if (DT != cgv::DT_F32 && S::MB == 1 && g.ent_n) {
+                // what 16 bits leave of the listed entries of G, in the order of the list: eight times 64 of them looked through at a time
+                constexpr uint32_t AT_ONCE = 8;
+                for (uint32_t e0 = 0; e0 < g.ent_n; e0 += 64 * AT_ONCE) {
+                    uint32_t at[AT_ONCE];
+#pragma unroll
+                    for (uint32_t x = 0; x < AT_ONCE; ++x) {
+                        const uint32_t e = e0 + x * 64 + lane;
+                        at[x] = e < g.ent_n ? g.ent_id[e] - (uint32_t)(g.row0 + n0) : 0xffffffffu;       // column of the wave tile, or beyond it
+                    }
+#pragma unroll
+                    for (uint32_t x = 0; x < AT_ONCE; ++x)
+                        for (uint64_t hits = __ballot(at[x] < (uint32_t)S::TN); hits; hits &= hits - 1) {
+                            const int l = __ffsll((unsigned long long)hits) - 1;
+                            const uint32_t e = e0 + x * 64 + l, c = __builtin_amdgcn_readlane(at[x], l);
+                            const float rest = rest16<DT>(g.ent_val[e] * g.unscale[-1]), mine = (uint32_t)(lane & 31) == (c & 31u) ? rest : 0.0f;
+                            const char* row = g.a.p + (uint64_t)(e / g.ent_k) * g.a.pitch;
+#pragma unroll
+                            for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+                                for (int r4 = 0; r4 < 4; ++r4) {
+                                    const uint2 w = *(const uint2*)(row + min(m0 + mb * 32 + r4 * 8 + half4, g.a.limit - 4) * 2);
+                                    const float q[4] = {cgv_ops::half_to_f32<DT>((uint16_t)w.x), cgv_ops::half_to_f32<DT>((uint16_t)(w.x >> 16)),
+                                                        cgv_ops::half_to_f32<DT>((uint16_t)w.y), cgv_ops::half_to_f32<DT>((uint16_t)(w.y >> 16))};
+#pragma unroll
+                                    for (int nb = 0; nb < S::NB; ++nb)
+                                        if (nb == (int)(c / 32))
+#pragma unroll
+                                            for (int y = 0; y < 4; ++y) acc[mb][nb][r4 * 4 + y] = fmaf(mine, q[y], acc[mb][nb][r4 * 4 + y]);
+                                }
+                        }
+                }
+            }
 #pragma unroll
             for (int nb = 0; nb < S::NB; ++nb) {
                 const uint32_t row = n0 + nb * 32 + (lane & 31);

@@ -14,7 +14,7 @@
 //
 // For 16-bit inputs G is rounded to their type, which is what the matrix cores multiply their rows with: the corpus' bf16 gradient is off by
 // 0.0023 of its norm against 64 bits, 0.0017 of it from the rounding of the result itself. Over many queries these roundings average out; the
-// listed entries' are made good in dQ. Up to
+// listed entries' are made good in dQ, and in small problems in dR. Up to
 // TWINS queries leave half of a tile's columns empty: there what the rounding leaves of G is stored and multiplied too (3 queries x 326 x
 // 123 bf16: 0.0029 without, 0.0018 with).
 // fp16: G is scaled by a power of two that brings the largest |dloss * scale| to 2^13 .. 2^14 (softmax values of 1e-9 are then still
@@ -32,6 +32,10 @@ namespace {
 
 constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
 constexpr uint32_t MAX_K = 256, NONE = 0xffffffffu, TWINS = 32;
+// listed entries, all queries together, that every small tile of the corpus' gradient looks through to make their rounding good: in small
+// problems there are too few for their roundings to average out (69 queries x 5054 x 64 fp16: 1.97 times the error of rounding the result
+// alone, with it 1.01 times); in large tiles the look through costs registers that the products need
+constexpr uint32_t LOOKED_THROUGH = 1024;
 constexpr uint32_t CUS = 256;                                  // workgroups of one per CU that fill the card
 // of G, and of copied corpus rows. Each piece costs a round over dQ's partial sums (1024 x 500 k x 768, gradient: 3.05 ms with 128 MiB, 2.99 with
 // 512, 2.97 with 1024); the corpus' gradient needs some 256 tiles a piece, however many queries there are
@@ -746,6 +750,11 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             e.out_pitch = (uint64_t)pl.dim * esize(dtype);
             e.vec_out = e.out_pitch % 16 == 0 && (uintptr_t)dr % 16 == 0;
             e.unscale = mul + 1;
+            e.row0 = n0;
+            e.ent_id = ent_id;
+            e.ent_val = ent_val;
+            e.ent_k = pl.k;
+            e.ent_n = big || P.twin || DT == cgv::DT_F32 || (uint64_t)pl.b * pl.k > LOOKED_THROUGH ? 0 : pl.b * pl.k;
         }
         if (together) {
             if ((rc = launch_gradients<DT>(d, e, P.device, s))) return rc;

@@ -154,10 +154,10 @@ def test_batches_in_columns_of_two_widths(b, n, d, k, dt):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp16"])
-@pytest.mark.parametrize("b,n,d,k", [(33, 500, 64, 1), (70, 3000, 123, 2), (812, 20_000, 64, 2), (200, 30_000, 72, 30)])
+@pytest.mark.parametrize("b,n,d,k", [(33, 500, 64, 1), (70, 3000, 123, 2), (1000, 700, 40, 1), (100, 2000, 8, 10), (812, 20_000, 64, 2), (200, 30_000, 72, 30)])
 def test_listed_entries_lose_nothing_to_16_bits(b, n, d, k, dt):
-    """The queries' gradient: only what the rows outside the list add is rounded to 16 bits on its way. dloss is the same for all queries, so
-    that the listed entries and their roundings are nearly alike."""
+    """The queries' gradient, in small problems the corpus' too: only what the rows outside the list add is rounded to 16 bits on its way. dloss is
+    the same for all queries, so that the listed entries and their roundings are nearly alike."""
     m = pkg()
     q, r, ids, sc, _ = _problem(b, n, d, k, dt, b + n)
     ids[5] = -1
@@ -176,6 +176,13 @@ def test_listed_entries_lose_nothing_to_16_bits(b, n, d, k, dt):
     lim = lim + (2.0 ** -37 if dt == "fp16" else 2.0 ** -126) * 8.2 * ref["r"].abs().sum(dim=0)[None] + (2.0 ** -24 if dt == "fp16" else 2.0 ** -126)
     err = (dq.double() - ref["dq"]).abs()
     assert bool((err <= lim).all()), float((err / lim).max())
+    if b * k <= 1024 and n <= 5000:                          # small problems: the corpus' gradient as well
+        r.requires_grad_()
+        (dr,) = torch.autograd.grad(m.corpus_distillation(q, r, ids, sc, scale=8.0, teacher_scale=1.0), (r,), g)
+        lim = (P * g[:, None].double() * 8.0).t() @ ref["q"].abs() * u + ref["mr"] * per + ref["dr"].abs() * u * 1.001
+        lim = lim + (2.0 ** -37 if dt == "fp16" else 2.0 ** -126) * 8.2 * ref["q"].abs().sum(dim=0)[None] + (2.0 ** -24 if dt == "fp16" else 2.0 ** -126)
+        err = (dr.double() - ref["dr"]).abs()
+        assert bool((err <= lim).all()), float((err / lim).max())
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp16"])
