@@ -52,7 +52,7 @@ def _check_grad(got, dout, ids, n, scale, dt):
 
 
 @pytest.mark.parametrize("dt", list(TYPES))
-@pytest.mark.parametrize("n,d,k", [(1, 1, 1), (3, 8, 5), (100, 7, 64), (1000, 64, 513), (511, 100, 1000), (70, 384, 512), (5000, 768, 2049),
+@pytest.mark.parametrize("n,d,k", [(1, 1, 1), (3, 8, 5), (40, 16, 256), (40, 16, 257), (3, 8, 2048), (90_000, 24, 2047), (100, 7, 64), (1000, 64, 513), (511, 100, 1000), (70, 384, 512), (5000, 768, 2049),
                                    (300_000, 16, 70_000), (40, 1536, 9000), (2, 32, 30_000), (9, 8192, 40)])
 def test_forward_and_gradient(n, d, k, dt):
     m = pkg()
