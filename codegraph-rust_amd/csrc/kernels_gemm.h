@@ -73,7 +73,7 @@ struct Args {
     uint32_t tm, tn;                              // tiles of M and N
     uint32_t splits, blocks;                      // shares of the long axis; workgroups
     // epilogues
-    float scale2;                                 // LSE, G: scores in units of log 2 = accumulator * scale2
+    float scale2;                                 // LSE, G: scores in units of log 2 = accumulator * scale2, not zero
     uint32_t m_valid, n_valid;                    // rows / columns of the result that exist
     uint32_t n_pad;                               // LSE, G: columns that have a place in part / out, n_valid rounded up to 64
     uint64_t row0;                                // LSE, G: corpus row of m = 0; DR: of n = 0
@@ -368,9 +368,13 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
             g_coef[nb] = q < g.n_valid ? g.coef[q] * *g.unscale : 0.0f;
             g_lse[nb] = q < g.n_valid ? g.lse2[q] : make_float2(0.0f, 0.0f);
         }
-    float run_m[S::NB], run_s[S::NB];                 // LSE: per query of the lane, over the corpus rows of the lane
+    // LSE: per query of the lane, over the corpus rows of the lane: maximum, sum, and what the sum's additions lost. Where scores are alike all
+    // additions round the same way, and a query's share may be the whole corpus: a chain of single exponentials was off by 1.4e-3 of the sum (33 000
+    // queries, 300 k equal rows). So a tile's are added up apart (16 a block, then the blocks), and adding a tile to the rest loses nothing. The
+    // maximum is rounded up to an integer: moving to a new one multiplies by a power of two, which is exact however often it happens
+    float run_m[S::NB], run_s[S::NB], run_r[S::NB];
     if (EPI == EPI_LSE)
-        for (int nb = 0; nb < S::NB; ++nb) run_m[nb] = -INFINITY, run_s[nb] = 0.0f;
+        for (int nb = 0; nb < S::NB; ++nb) run_m[nb] = -INFINITY, run_s[nb] = run_r[nb] = 0.0f;
 
     // A small wave tile has few products per read: it keeps the fragments of two whole stages and reads the next one while it
     // multiplies this one; a large one keeps those of two times 16 elements of K
@@ -633,47 +637,42 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
                 // corpus row that this query leaves out, as a row of the wave's part of the tile
                 const uint32_t skip = q < g.n_valid ? g.anchor[q] - (uint32_t)(g.row0 + m0) : 0xffffffffu;
                 const bool any = __ballot(skip < (uint32_t)S::TM) != 0;
-                if (edge || any) {                     // rows beyond the corpus, the row left out
-                    float mx = -INFINITY;
+                if (edge || any) {                     // rows beyond the corpus, the row left out: a score of -inf (scale2 is not zero)
+                    const float none = g.scale2 > 0.0f ? -INFINITY : INFINITY;
 #pragma unroll
                     for (int mb = 0; mb < S::MB; ++mb)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const uint32_t m = mb * 32 + (r & 3) + 8 * (r >> 2) + half4;
-                            const float t = m == skip || m0 + m >= g.m_valid ? -INFINITY : acc[mb][nb][r] * g.scale2;
-                            acc[mb][nb][r] = t;
-                            mx = fmaxf(mx, t);
+                            if (m == skip || m0 + m >= g.m_valid) acc[mb][nb][r] = none;
                         }
-                    const float nm = fmaxf(run_m[nb], mx), base = nm == -INFINITY ? 0.0f : nm;
-                    float s = run_s[nb] * __builtin_amdgcn_exp2f(run_m[nb] - base);
-#pragma unroll
-                    for (int mb = 0; mb < S::MB; ++mb)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(acc[mb][nb][r] - base);
-                    run_m[nb] = nm;
-                    run_s[nb] = s;
-                } else {
-                    float ext = acc[0][nb][0];
-                    if (g.scale2 >= 0.0f) {
-#pragma unroll
-                        for (int mb = 0; mb < S::MB; ++mb)
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) ext = fmaxf(ext, acc[mb][nb][r]);
-                    } else {
-#pragma unroll
-                        for (int mb = 0; mb < S::MB; ++mb)
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) ext = fminf(ext, acc[mb][nb][r]);
-                    }
-                    const float nm = fmaxf(run_m[nb], ext * g.scale2), base = nm == -INFINITY ? 0.0f : nm;
-                    float s = run_s[nb] * __builtin_amdgcn_exp2f(run_m[nb] - base);
-#pragma unroll
-                    for (int mb = 0; mb < S::MB; ++mb)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[mb][nb][r], g.scale2, -base));
-                    run_m[nb] = nm;
-                    run_s[nb] = s;
                 }
+                float ext = acc[0][nb][0];
+                if (g.scale2 >= 0.0f) {
+#pragma unroll
+                    for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) ext = fmaxf(ext, acc[mb][nb][r]);
+                } else {
+#pragma unroll
+                    for (int mb = 0; mb < S::MB; ++mb)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) ext = fminf(ext, acc[mb][nb][r]);
+                }
+                const float nm = fmaxf(run_m[nb], ceilf(ext * g.scale2)), base = nm == -INFINITY ? 0.0f : nm;
+                const float f = __builtin_amdgcn_exp2f(run_m[nb] - base), before = run_s[nb] * f;
+                float sum[S::MB];                      // of the tile: a lane's 16 rows of a block
+#pragma unroll
+                for (int mb = 0; mb < S::MB; ++mb) {
+                    sum[mb] = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sum[mb] += __builtin_amdgcn_exp2f(fmaf(acc[mb][nb][r], g.scale2, -base));
+                    if (mb) sum[0] += sum[mb];
+                }
+                const float s = before + sum[0], b = s - before;
+                run_m[nb] = nm;
+                run_s[nb] = s;
+                run_r[nb] = fmaf(run_r[nb], f, (before - (s - b)) + (sum[0] - b));
             }
         } else if (EPI == EPI_G) {
             auto store = [&](auto at_edge) {
@@ -808,9 +807,9 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
         const uint32_t n0 = nt * S::BN + wn * S::TN;
 #pragma unroll
         for (int nb = 0; nb < S::NB; ++nb) {
-            const float om = __shfl_xor(run_m[nb], 32), os = __shfl_xor(run_s[nb], 32);
+            const float mine = run_s[nb] + run_r[nb], om = __shfl_xor(run_m[nb], 32), os = __shfl_xor(mine, 32);
             const float nm = fmaxf(run_m[nb], om), base = nm == -INFINITY ? 0.0f : nm;
-            const float s = run_s[nb] * __builtin_amdgcn_exp2f(run_m[nb] - base) + os * __builtin_amdgcn_exp2f(om - base);
+            const float s = mine * __builtin_amdgcn_exp2f(run_m[nb] - base) + os * __builtin_amdgcn_exp2f(om - base);
             const uint32_t q = n0 + nb * 32 + (lane & 31);
             const uint32_t own = split * S::WM + wm;
             if (lane < 32 && q < g.n_pad) {

@@ -19,6 +19,8 @@
 // 123 bf16: 0.0029 without, 0.0018 with).
 // fp16: G is scaled by a power of two that brings the largest |dloss * scale| to 2^13 .. 2^14 (softmax values of 1e-9 are then still
 // above the type's smallest step); the products' results are scaled back in f32.
+#include <float.h>
+
 #include <type_traits>
 
 #include "../../include/cgvec_train.h"
@@ -262,17 +264,18 @@ __global__ __launch_bounds__(256) void loss_kernel(Problem P, const float2* __re
         if (lane == 0) loss[i] = 0.0f, sv[0] = 0.0, sv[1] = 0.0;
         return;
     }
-    float m = -INFINITY, s = 0.0f;
+    float m = -INFINITY;
+    double s = 0.0;           // maxima are integers (or infinite): the factors are exact
     for (uint32_t p = lane; p < parts; p += 64) {
         const float2 v = part[(uint64_t)p * P.bp + i];
         const float nm = fmaxf(m, v.x), base = nm == -INFINITY ? 0.0f : nm;
-        s = s * exp2f(m - base) + v.y * exp2f(v.x - base);
+        s = s * (double)exp2f(m - base) + (double)v.y * (double)exp2f(v.x - base);
         m = nm;
     }
     const float top = wave_max(m), base = top == -INFINITY ? 0.0f : top;
-    s = wave_sum(s * exp2f(m - base));
+    s = wave_sum(s * (double)exp2f(m - base));
     const double sa = sv[2 + l.anchor];
-    const double rest = (double)base * LN2 - sa + log((double)s);       // log of (the others' sum / the anchor's term)
+    const double rest = (double)base * LN2 - sa + log(s);       // log of (the others' sum / the anchor's term)
     const double tail = rest > 40.0 ? rest : log1p(exp(rest));
     double sum = 0.0;
 #pragma unroll
@@ -614,6 +617,7 @@ Args score_args(const Plan& pl, const Problem& P, int dtype, const char* rows, u
     a.kvalid = pl.copy ? pl.dp : pl.dim;
     a.tm = (c + pl.bm - 1) / pl.bm;
     a.scale2 = (float)(P.scale * LOG2E);
+    if (a.scale2 == 0.0f) a.scale2 = FLT_MIN;     // -inf times it is to stay -inf
     a.m_valid = c;
     a.n_valid = pl.b;
     a.n_pad = a.part_ld = pl.bp;
