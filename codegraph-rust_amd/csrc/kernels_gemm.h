@@ -90,7 +90,7 @@ struct Args {
     char* out;                                    // G, DR, DQ
     uint64_t out_pitch, out_plane;                // bytes
     uint32_t accumulate, vec_out;                 // DQ: add to what is there; DR: 16-byte stores possible
-    const float* unscale;                         // G: [1] factor of the entries; DR: [1] factor of the result, before it that of the entries
+    const float* unscale;                         // DR: [1] factor of the result; NULL: 1
 };
 
 // PL planes of an operand in a stage: 3 for f32 where tiles are small - each plane is then loaded once and not once per product
@@ -365,7 +365,7 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
     if (EPI == EPI_G)
         for (int nb = 0; nb < S::NB; ++nb) {
             const uint32_t q = nt * S::BN + wn * S::TN + nb * 32 + (lane & 31);
-            g_coef[nb] = q < g.n_valid ? g.coef[q] * *g.unscale : 0.0f;
+            g_coef[nb] = q < g.n_valid ? g.coef[q] : 0.0f;
             g_lse[nb] = q < g.n_valid ? g.lse2[q] : make_float2(0.0f, 0.0f);
         }
     // LSE: per query of the lane, over the corpus rows of the lane: maximum, sum, and what the sum's additions lost. Where scores are alike all
@@ -726,7 +726,7 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
                     }
             }
         } else {   // EPI_DR
-            const float u = *g.unscale;
+            const float u = g.unscale ? *g.unscale : 1.0f;
             stored = g.vec_out && m0 + S::TM <= g.m_valid && n0 + S::TN <= g.n_valid;
             if (DT != cgv::DT_F32 && S::MB == 1 && g.ent_n) {
                 // what 16 bits leave of the listed entries of G, in the order of the list: eight times 64 of them looked through at a time
@@ -743,7 +743,7 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
                         for (uint64_t hits = __ballot(at[x] < (uint32_t)S::TN); hits; hits &= hits - 1) {
                             const int l = __ffsll((unsigned long long)hits) - 1;
                             const uint32_t e = e0 + x * 64 + l, c = __builtin_amdgcn_readlane(at[x], l);
-                            const float rest = rest16<DT>(g.ent_val[e] * g.unscale[-1]), mine = (uint32_t)(lane & 31) == (c & 31u) ? rest : 0.0f;
+                            const float rest = rest16<DT>(g.ent_val[e]), mine = (uint32_t)(lane & 31) == (c & 31u) ? rest : 0.0f;
                             const char* row = g.a.p + (uint64_t)(e / g.ent_k) * g.a.pitch;
 #pragma unroll
                             for (int mb = 0; mb < S::MB; ++mb)
@@ -822,7 +822,6 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
     if (EPI == EPI_G) {
         // the listed rows' entries, computed apart, take the place of what this workgroup has stored for them: every wave's stores are done
         __syncthreads();
-        const float u = *g.unscale;
         const uint32_t n0 = nt * S::BN, queries = min((uint32_t)S::BN, g.n_valid - n0);
         const uint32_t* ids = g.ent_id + (uint64_t)n0 * g.ent_k;
         const float* vals = g.ent_val + (uint64_t)n0 * g.ent_k;
@@ -836,7 +835,7 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
                 if (m >= g.m_valid || (uint32_t)m / S::BM % g.splits != split) continue;
                 const uint32_t t = t0 + x * S::THREADS;
                 uint16_t* o = (uint16_t*)(g.out + (n0 + t / g.ent_k) * g.out_pitch) + m;
-                const float v = vals[t] * u;
+                const float v = vals[t];
                 if (DT == cgv::DT_F32) {
                     uint16_t p[3];
                     split3(v, p);

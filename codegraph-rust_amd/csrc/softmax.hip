@@ -17,9 +17,12 @@
 // listed entries' are made good in dQ, and in small problems in dR. Up to
 // TWINS queries leave half of a tile's columns empty: there what the rounding leaves of G is stored and multiplied too (3 queries x 326 x
 // 123 bf16: 0.0029 without, 0.0018 with).
-// fp16: G is scaled by a power of two that brings the largest |dloss * scale| to 2^13 .. 2^14 (softmax values of 1e-9 are then still
-// above the type's smallest step); the products' results are scaled back in f32.
+// fp16: each query's entries of G are scaled by a power of two of its own, which brings its largest to 2^13 .. 2^14 (what is 2^-27 of that still has
+// all its digits); dQ is scaled back in f32. Factors of other queries do not matter then - with one power for all, a query of a
+// millionth of the largest factor lost half of its dQ. dR sums over queries: it takes them from a copy that is scaled the other way round, so
+// that all products carry the same power, the largest that keeps every query in range.
 #include <float.h>
+#include <limits.h>
 
 #include <type_traits>
 
@@ -122,18 +125,24 @@ __device__ inline T pick(const T (&v)[4], uint32_t j) {     // entry j of the li
     return __shfl(x, (int)(j & 63u));
 }
 
-// a row of the padded copy: 16-bit types as they are, f32 as three planes; zeros beyond dim, and altogether if !src
+// a row of the padded copy: 16-bit types as they are, f32 as three planes; zeros beyond dim, and altogether if !src. fp16: the largest finite
+// magnitude that the thread has seen
 template <int DT>
-__device__ inline void copy_row(const void* src, uint64_t at, uint32_t dim, uint32_t dp, uint16_t* dst, uint64_t plane, uint32_t t0, uint32_t step) {
+__device__ inline float copy_row(const void* src, uint64_t at, uint32_t dim, uint32_t dp, uint16_t* dst, uint64_t plane, uint32_t t0, uint32_t step) {
+    float most = 0.0f;
     for (uint32_t e = t0; e < dp; e += step) {
         if (DT == cgv::DT_F32) {
             uint16_t p[3] = {0, 0, 0};
             if (src && e < dim) split3(((const float*)src)[at + e], p);
             for (int x = 0; x < 3; ++x) dst[x * plane + e] = p[x];
         } else {
-            dst[e] = src && e < dim ? ((const uint16_t*)src)[at + e] : (uint16_t)0;
+            const uint16_t v = src && e < dim ? ((const uint16_t*)src)[at + e] : (uint16_t)0;
+            dst[e] = v;
+            const float a = DT == cgv::DT_FP16 ? fabsf(half_to_f32<DT>(v)) : 0.0f;
+            if (a < INFINITY) most = fmaxf(most, a);
         }
     }
+    return most;
 }
 
 struct Piece {              // corpus rows [n0, n0 + c) on their way into the padded copy
@@ -289,48 +298,54 @@ __global__ __launch_bounds__(256) void loss_kernel(Problem P, const float2* __re
     }
 }
 
+// fp16: the power of two for a query's entries of G, of which the largest is |c| * most: to 2^13 .. 2^14, as far as c itself stays in range
+__device__ inline int g_power(float c, double most) {
+    const double x = fabs((double)c * most);
+    return x > 0.0 && x < (double)INFINITY ? max(min(min(13 - ilogb(x), 110 - ilogbf(c)), 120), -126) : 0;
+}
+
+// per place of a query, [bp] each
+struct Places {
+    float2* lse2;             // log2 of the softmax sum: its f32 and what that leaves
+    float* coef;              // factor of G, times 2^power
+    uint32_t* has;            // has a list
+    int *power, *room;        // fp16; room: what power and the power of the query's copy for dR can add up to, INT_MAX: anything
+};
+
 // factor and log2 of the softmax sum per query; entries of G on the listed rows; the padded copy of the queries
 template <int DT>
-__global__ __launch_bounds__(256) void backward_prep_kernel(Problem P, const float* __restrict__ dloss, float* __restrict__ coef, float2* __restrict__ lse2,
-                                                            uint32_t* __restrict__ has, uint32_t* __restrict__ ent_id, float* __restrict__ ent_val,
-                                                            float* __restrict__ mul, Piece first_piece) {
+__global__ __launch_bounds__(256) void backward_prep_kernel(Problem P, const float* __restrict__ dloss, Places at, uint32_t* __restrict__ ent_id,
+                                                            float* __restrict__ ent_val, Piece first_piece) {
     const uint64_t block = wide_block();
     if (block >= P.bp) return copy_piece_block<DT>(first_piece, block - P.bp);
     __shared__ uint32_t ids[MAX_K];
-    __shared__ double ps[MAX_K];
+    __shared__ double ps[MAX_K], vs[4];
+    __shared__ float qs[4];
     const uint32_t place = (uint32_t)block, i = P.twin && place >= P.twin ? place - P.twin : place, wave = threadIdx.x >> 6;
     const int lane = threadIdx.x & 63;
     const uint64_t plane = (uint64_t)P.bp * P.dp;
     uint16_t* dst = P.qws + (uint64_t)place * P.dp;
-    if (place == 0 && threadIdx.x < 2) mul[threadIdx.x] = 1.0f;
     if (i >= P.b) {
         copy_row<DT>(nullptr, 0, P.dim, P.dp, dst, plane, threadIdx.x, 256);
-        if (threadIdx.x == 0) coef[place] = 0.0f, lse2[place] = make_float2(0.0f, 0.0f), has[place] = 0;
+        if (threadIdx.x == 0) at.coef[place] = 0.0f, at.lse2[place] = make_float2(0.0f, 0.0f), at.has[place] = 0, at.power[place] = 0, at.room[place] = INT_MAX;
         if (P.twin && threadIdx.x < P.k) ent_id[(uint64_t)place * P.k + threadIdx.x] = NONE;
         return;
     }
     const List l = read_list(P.ids, P.tscores, i, P.k, P.n_rows, P.tscale, lane);
-    copy_row<DT>(l.has ? P.queries : nullptr, (uint64_t)i * P.q_stride, P.dim, P.dp, dst, plane, threadIdx.x, 256);
+    float most_q = copy_row<DT>(l.has ? P.queries : nullptr, (uint64_t)i * P.q_stride, P.dim, P.dp, dst, plane, threadIdx.x, 256);
     const double* sv = P.saved + (uint64_t)i * (P.k + 2);
     const float c = l.has ? dloss[i] * P.scale : 0.0f;
-    if (threadIdx.x == 0) {
-        coef[place] = c;
-        const double l2 = l.has ? sv[0] * LOG2E : 0.0;
-        lse2[place] = make_float2((float)l2, (float)(l2 - (double)(float)l2));
-        has[place] = l.has;
-    }
     if (wave == 0)
         for (int x = 0; x < 4; ++x) {
             ids[x * 64 + lane] = l.id[x];
             ps[x * 64 + lane] = l.p[x];
         }
     __syncthreads();
-    if (threadIdx.x >= P.k) return;
-    const uint32_t j = threadIdx.x, id = ids[j];
+    const uint32_t j = threadIdx.x, id = j < P.k ? ids[j] : NONE;
     const uint32_t aid = l.has ? ids[l.anchor] : NONE;
     bool first = id != NONE;
     double same = 0.0, other = 0.0;
-    for (uint32_t x = 0; x < P.k; ++x) {
+    for (uint32_t x = 0; first && x < P.k; ++x) {
         if (ids[x] == id) {
             if (x < j) first = false;
             same += ps[x];
@@ -340,26 +355,59 @@ __global__ __launch_bounds__(256) void backward_prep_kernel(Problem P, const flo
     }
     double v = 0.0;
     if (first) v = id == aid ? expm1(-sv[1]) + other : exp(sv[2 + j] - sv[0]) - same;
+    int power = 0;
+    if constexpr (DT == cgv::DT_FP16) {
+        // rows outside the list have a softmax value of 1 - exp(-tail) at most, the heaviest listed row having the rest
+        double most = fabs(v);
+        for (int o = 32; o; o >>= 1) most = fmax(most, __shfl_xor(most, o));
+        most_q = wave_max(most_q);
+        if (lane == 0) vs[wave] = most, qs[wave] = most_q;
+        __syncthreads();
+        most = fmax(fmax(fmax(vs[0], vs[1]), fmax(vs[2], vs[3])), l.has ? -expm1(-sv[1]) : 0.0);
+        most_q = fmaxf(fmaxf(qs[0], qs[1]), fmaxf(qs[2], qs[3]));
+        power = g_power(c, most);
+        const double x = fabs((double)c * most);
+        if (threadIdx.x == 0) {
+            at.power[place] = power;
+            at.room[place] = x > 0.0 && x < (double)INFINITY && most_q > 0.0f ? power + 15 - ilogbf(most_q) : INT_MAX;
+        }
+    }
+    if (threadIdx.x == 0) {
+        at.coef[place] = ldexpf(c, power);
+        const double l2 = l.has ? sv[0] * LOG2E : 0.0;
+        at.lse2[place] = make_float2((float)l2, (float)(l2 - (double)(float)l2));
+        at.has[place] = l.has;
+    }
+    if (j >= P.k) return;
     ent_id[(uint64_t)place * P.k + j] = first ? id : NONE;
-    ent_val[(uint64_t)place * P.k + j] = (float)(v * c);
+    ent_val[(uint64_t)place * P.k + j] = (float)ldexp(v * c, power);
 }
 
-// fp16: the power of two that brings the largest factor to 2^13 .. 2^14, and its inverse
-__global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ coef, uint32_t b, float* __restrict__ mul) {
-    __shared__ float w[16];
-    float mx = 0.0f;
-    for (uint32_t i = threadIdx.x; i < b; i += 1024) {
-        const float a = fabsf(coef[i]);
-        if (a < INFINITY) mx = fmaxf(mx, a);
-    }
-    mx = wave_max(mx);
-    if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = mx;
+// fp16: the queries' copy for dR, and the factor that takes the common power back. Few workgroups, each of which looks for that power itself
+__global__ __launch_bounds__(256) void scaled_queries_kernel(Problem P, Places at, uint16_t* __restrict__ dst, float* __restrict__ unscale) {
+    __shared__ int low[4];
+    int common = INT_MAX;
+    for (uint32_t i = threadIdx.x; i < P.bp; i += 256) common = min(common, at.room[i]);
+    for (int o = 32; o; o >>= 1) common = min(common, __shfl_xor(common, o));
+    if ((threadIdx.x & 63) == 0) low[threadIdx.x >> 6] = common;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int x = 1; x < 16; ++x) mx = fmaxf(mx, w[x]);
-        const int e = mx > 0.0f ? min(max(13 - ilogbf(mx), -100), 100) : 0;
-        mul[0] = ldexpf(1.0f, e);
-        mul[1] = ldexpf(1.0f, -e);
+    common = min(min(low[0], low[1]), min(low[2], low[3]));
+    common = common == INT_MAX ? 0 : min(common, 120);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *unscale = ldexpf(1.0f, -common);
+    const uint32_t per = P.dp / 8;
+    const uint64_t total = (uint64_t)P.bp * per;
+    for (uint64_t t = (uint64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (uint64_t)gridDim.x * 256) {
+        const uint32_t place = (uint32_t)(t / per);
+        // a query without a gradient, or with one that is not finite, stays as it is
+        const int shift = at.room[place] == INT_MAX ? 0 : common - at.power[place];
+        const uint4 in = ((const uint4*)P.qws)[t];
+        const uint32_t w[4] = {in.x, in.y, in.z, in.w};
+        uint32_t o[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            o[x] = f32_to_half<cgv::DT_FP16>(ldexpf(half_to_f32<cgv::DT_FP16>((uint16_t)w[x]), shift)) |
+                   (uint32_t)f32_to_half<cgv::DT_FP16>(ldexpf(half_to_f32<cgv::DT_FP16>((uint16_t)(w[x] >> 16)), shift)) << 16;
+        ((uint4*)dst)[t] = make_uint4(o[0], o[1], o[2], o[3]);
     }
 }
 
@@ -377,7 +425,7 @@ struct Listed {
 template <int DT>
 __global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict__ part, uint32_t splits, uint64_t share, uint32_t b, uint32_t twin,
                                                         uint32_t dim, uint32_t dp,
-                                                        const uint32_t* __restrict__ has, const float* __restrict__ mul, void* __restrict__ dq, Listed l) {
+                                                        const uint32_t* __restrict__ has, const int* __restrict__ power, void* __restrict__ dq, Listed l) {
     __shared__ float4 sum[4][64];
     const uint32_t stretches = (dim + 255) / 256;
     const uint64_t i = wide_block() / stretches;
@@ -404,11 +452,12 @@ __global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict_
 #pragma unroll 4
         for (uint32_t j = 0; j < l.k; ++j) {
             const uint32_t id = l.id[i * l.k + j];
-            const float rest = rest16<DT>(l.val[i * l.k + j] * mul[0]), r = load_elem<DT>(l.rows, (id == NONE ? 0 : (uint64_t)id) * l.stride + at);
+            const float rest = rest16<DT>(l.val[i * l.k + j]), r = load_elem<DT>(l.rows, (id == NONE ? 0 : (uint64_t)id) * l.stride + at);
             if (id != NONE) v = fmaf(rest, r, v);
         }
     }
-    store_elem<DT>(dq, i * dim + at, has[i] ? v * mul[1] : 0.0f);
+    if (DT == cgv::DT_FP16) v = ldexpf(v, -power[i]);
+    store_elem<DT>(dq, i * dim + at, has[i] ? v : 0.0f);
 }
 
 template <int DT>
@@ -433,6 +482,7 @@ struct Plan {
     uint32_t b, bp, dim, dp, k, planes, bm;               // bm: corpus rows of a tile of the scores
     uint32_t bn, columns, bn2, off;                       // the batch: `columns` tiles of bn queries, and from query `off` on one of bn2 (0: none)
     bool copy;                     // corpus rows go through a padded copy
+    bool scaled;                   // fp16: dR takes the queries from a copy of their own
     uint64_t n, piece_f, piece_b;  // corpus rows of a piece, forward and backward
     uint32_t parts;                // (maximum, sum) pairs of a query, all pieces together
     struct Shares { uint32_t s1, s2; };                   // shares of the long axis, for the columns of bn and for that of bn2
@@ -442,6 +492,7 @@ struct Plan {
         dp = (uint32_t)up(dim_, 64);
         planes = dtype == CGV_DTYPE_F32 ? 3 : 1;
         copy = dtype == CGV_DTYPE_F32 || dim % 8 != 0;
+        scaled = dtype == CGV_DTYPE_FP16;
         // the tile width whose padded batch takes the least time. Narrower tiles read LDS more often per product: 768 queries over 200 k x 768
         // (bf16, loss and both gradients) take 1.19 ms with tiles of 256, 1.22 with 192, 1.28 with 128, 1.63 with 64. Against that stands the
         // padding: 576 queries take 0.84 ms with 192, 0.93 with 256, 0.92 with 128
@@ -508,13 +559,14 @@ struct Plan {
     uint64_t f_rows() const { return f_part() + up((uint64_t)parts * bp * 8, 256); }
     uint64_t f_bytes() const { return f_rows() + r_bytes(piece_f); }
     // backward workspace
-    uint64_t b_coef() const { return q_bytes(); }                       // lse2 (two f32), coef, has: [bp] each; mul: [2]
-    uint64_t b_ent() const { return b_coef() + up((uint64_t)bp * 16 + 8, 256); }
+    uint64_t b_places() const { return q_bytes(); }                     // Places, and the factor of dR
+    uint64_t b_ent() const { return b_places() + up((uint64_t)bp * 24 + 4, 256); }
     uint32_t twin() const { return planes == 1 && b <= TWINS ? TWINS : 0; }
     uint64_t b_g() const { return b_ent() + up((uint64_t)bp * k * 8, 256); }
     uint64_t b_part() const { return b_g() + up((uint64_t)planes * bp * piece_b * 2, 256); }
     uint64_t b_rows() const { return b_part() + up((uint64_t)dq_splits * bp * dp * 4, 256); }
-    uint64_t b_bytes() const { return b_rows() + r_bytes(piece_b); }
+    uint64_t b_scaled() const { return b_rows() + r_bytes(piece_b); }
+    uint64_t b_bytes() const { return b_scaled() + (scaled ? q_bytes() : 0); }
 };
 
 void set_segments(Args& a, int dtype, bool small) {
@@ -674,10 +726,13 @@ int forward(const Plan& pl, Problem P, int dtype, float* loss, char* ws, hipStre
 template <int DT>
 int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq, void* dr, char* ws, hipStream_t s) {
     P.qws = (uint16_t*)ws;
-    float2* lse2 = (float2*)(ws + pl.b_coef());
-    float* coef = (float*)(lse2 + pl.bp);
-    uint32_t* has = (uint32_t*)(coef + pl.bp);
-    float* mul = (float*)(has + pl.bp);
+    Places at;
+    at.lse2 = (float2*)(ws + pl.b_places());
+    at.coef = (float*)(at.lse2 + pl.bp);
+    at.has = (uint32_t*)(at.coef + pl.bp);
+    at.power = (int*)(at.has + pl.bp);
+    at.room = at.power + pl.bp;
+    float* unscale = (float*)(at.room + pl.bp);
     uint32_t* ent_id = (uint32_t*)(ws + pl.b_ent());
     float* ent_val = (float*)(ent_id + (uint64_t)pl.bp * pl.k);
     P.twin = pl.twin();
@@ -685,10 +740,11 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
     float* part = (float*)(ws + pl.b_part());
     const uint64_t g_pitch = pl.piece_b * 2, g_plane = (uint64_t)pl.bp * g_pitch;
     const Piece first = piece_of(pl, P, 0, pl.piece_b, ws + pl.b_rows());
-    hipLaunchKernelGGL((backward_prep_kernel<DT>), wide_grid((uint64_t)pl.bp + copy_blocks(first)), dim3(256), 0, s, P, dloss, coef, lse2, has, ent_id, ent_val, mul, first);
+    hipLaunchKernelGGL((backward_prep_kernel<DT>), wide_grid((uint64_t)pl.bp + copy_blocks(first)), dim3(256), 0, s, P, dloss, at, ent_id, ent_val, first);
     OPCHK(hipGetLastError());
-    if (DT == cgv::DT_FP16) {
-        hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1024), 0, s, (const float*)coef, pl.b, mul);
+    if (DT == cgv::DT_FP16 && dr) {
+        const uint64_t blocks = ((uint64_t)pl.bp * (pl.dp / 8) + 255) / 256;
+        hipLaunchKernelGGL(scaled_queries_kernel, dim3((unsigned)std::min<uint64_t>(blocks, CUS)), dim3(256), 0, s, P, at, (uint16_t*)(ws + pl.b_scaled()), unscale);
         OPCHK(hipGetLastError());
     }
     for (uint64_t n0 = 0; n0 < pl.n; n0 += pl.piece_b) {
@@ -703,9 +759,8 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             plane = pl.piece_b * pitch;
         }
         Args a = score_args(pl, P, dtype, rows, pitch, plane, c);
-        a.coef = coef;
-        a.lse2 = lse2;
-        a.unscale = mul;
+        a.coef = at.coef;
+        a.lse2 = at.lse2;
         if (P.twin) a.n_valid = pl.bp;
         a.twin = P.twin;
         a.row0 = n0;
@@ -738,7 +793,7 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             d.accumulate = n0 > 0;
         }
         if (dr) {
-            e.a = {(const char*)P.qws, (uint64_t)pl.dp * 2, (uint64_t)pl.bp * pl.dp * 2, pl.dp};
+            e.a = {DT == cgv::DT_FP16 ? ws + pl.b_scaled() : (const char*)P.qws, (uint64_t)pl.dp * 2, (uint64_t)pl.bp * pl.dp * 2, pl.dp};
             e.b = {G, g_pitch, g_plane, (uint32_t)pl.piece_b};
             e.ksteps = pl.bp / BK;
             e.kvalid = pl.bp;
@@ -753,7 +808,7 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             e.out = (char*)dr + n0 * pl.dim * esize(dtype);
             e.out_pitch = (uint64_t)pl.dim * esize(dtype);
             e.vec_out = e.out_pitch % 16 == 0 && (uintptr_t)dr % 16 == 0;
-            e.unscale = mul + 1;
+            e.unscale = DT == cgv::DT_FP16 ? unscale : nullptr;
             e.row0 = n0;
             e.ent_id = ent_id;
             e.ent_val = ent_val;
@@ -769,7 +824,7 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
     }
     if (dq) {
         hipLaunchKernelGGL((finish_dq_kernel<DT>), wide_grid((uint64_t)pl.b * ((pl.dim + 255) / 256)), dim3(256), 0, s, (const float*)part, pl.dq_splits, (uint64_t)pl.bp * pl.dp,
-                           pl.b, P.twin, pl.dim, pl.dp, (const uint32_t*)has, (const float*)mul, dq, Listed{ent_id, ent_val, P.twin ? 0 : pl.k, P.rows, P.r_stride});
+                           pl.b, P.twin, pl.dim, pl.dp, (const uint32_t*)at.has, (const int*)at.power, dq, Listed{ent_id, ent_val, P.twin ? 0 : pl.k, P.rows, P.r_stride});
         OPCHK(hipGetLastError());
     }
     return CGV_OK;

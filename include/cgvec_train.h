@@ -49,7 +49,8 @@ int cgv_lookup_grad_dev(int device_id, const void* dout_dev, int dtype, const in
  * teacher_scores [b][k] f32, loss [b] f32. saved [b * (k + 2)] f64 carries what the gradient needs (the softmax sums, the scores of
  * the listed rows). b in 0..=2^24, k in 1..=256, n_rows in 1..2^31 - 1, dim in 1..=8192.
  * The gradient's workspace holds the scores' gradient of one piece of the corpus in 16 bits (f32: three times that): 512 MiB, or
- * 16384 rows of the corpus for very many queries; f32 rows, and rows whose dim is no multiple of 8, also a copy of the piece. */
+ * 16384 rows of the corpus for very many queries; f32 rows, and rows whose dim is no multiple of 8, also a copy of the piece; fp16
+ * queries a second copy. */
 size_t cgv_corpus_loss_workspace(uint64_t b, uint64_t n_rows, uint32_t dim, uint32_t k, int dtype);
 int cgv_corpus_loss_dev(int device_id, const void* queries_dev, uint64_t query_stride, const void* rows_dev, uint64_t row_stride, int dtype,
                         uint64_t b, uint64_t n_rows, uint32_t dim, const int64_t* ids_dev, const float* teacher_scores_dev, uint32_t k,
