@@ -36,7 +36,9 @@ struct Layout {
     }
 };
 
-constexpr uint32_t BAD_NONFINITE = 1, BAD_RANGE = 2;
+constexpr uint32_t BAD_NONFINITE = 1, BAD_RANGE = 2, HAS_LARGE = 4;
+// below this no group's sum times its scale, nor the sum of a row's 256 groups, leaves f32's range on its way (codes times queries: 2^25 a group)
+constexpr float LARGE_SCALE = 0x1p94f;
 
 __device__ inline uint32_t pair_bits(uint32_t c0, uint32_t c1, uint32_t p) { return c0 << (4 * p) | c1 << (16 + 4 * p); }
 
@@ -49,6 +51,7 @@ __global__ __launch_bounds__(256) void q4_quantise_kernel(const float* __restric
     const uint64_t i = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (i >= n) return;
     const float* x = rows + i * L.dim;
+    bool large = false;
     for (uint32_t k = 0; k < L.kc; ++k) {
         const uint32_t e = k * CHUNK + lane * 2;
         const float v0 = e < L.dim ? x[e] : 0.0f, v1 = e + 1 < L.dim ? x[e + 1] : 0.0f;
@@ -58,6 +61,7 @@ __global__ __launch_bounds__(256) void q4_quantise_kernel(const float* __restric
         const uint16_t sb = f32_to_half<SDT>(a / 7.0f);
         const float s = half_to_f32<SDT>(sb);
         if (!(s < INFINITY)) atomicOr(bad, BAD_RANGE);
+        large |= s >= LARGE_SCALE;
         const uint32_t g = e / L.group;
         if (lane % (L.group / 2) == 0) scales[L.scale(row0 + i, g)] = g < L.ng ? sb : (uint16_t)0;
         const int q0 = s > 0.0f ? (int)fminf(fmaxf(rintf(v0 / s), -8.0f), 7.0f) : 0;
@@ -67,6 +71,7 @@ __global__ __launch_bounds__(256) void q4_quantise_kernel(const float* __restric
         w |= __shfl_xor(w, 2);
         if ((lane & 3) == 0) codes[L.dword(row0 + i, e)] = w;
     }
+    if (__any(large) && lane == 0) atomicOr(bad, HAS_LARGE);
 }
 
 template <int SDT>
@@ -85,11 +90,15 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(const uint8_t* __restrict_
         w |= __shfl_xor(w, 2);
         if ((lane & 3) == 0) codes[L.dword(row0 + i, e)] = w;
     }
+    bool large = false;
     for (uint32_t g = lane; g < L.kc * L.gpc; g += 64) {
         const uint16_t s = g < L.ng ? src_scales[i * L.ng + g] : (uint16_t)0;
-        if (!(fabsf(half_to_f32<SDT>(s)) < INFINITY)) atomicOr(bad, BAD_NONFINITE);
+        const float v = fabsf(half_to_f32<SDT>(s));
+        if (!(v < INFINITY)) atomicOr(bad, BAD_NONFINITE);
+        large |= v >= LARGE_SCALE;
         scales[L.scale(row0 + i, g)] = s;
     }
+    if (__any(large) && lane == 0) atomicOr(bad, HAS_LARGE);
 }
 
 template <int SDT>
@@ -406,6 +415,28 @@ __global__ __launch_bounds__(64 * WAVES) void q4_scores_kernel(ScoreArgs a) {
     }
 }
 
+// Rows with scales of 2^94 and more (bf16): group sums are formed at the size that the queries have on the matrix cores, and can leave f32's
+// range where the score itself does not. Such results are Inf or NaN; a thread each computes them again in 64 bits. A launch of its own, and
+// only for an index that has such rows: nothing else pays for it
+__global__ __launch_bounds__(256) void q4_again_kernel(ScoreArgs a) {
+    const uint64_t t = wide_block() * 256 + threadIdx.x;
+    if (t >= a.m * a.n || fabsf(a.out[t]) < INFINITY) return;
+    const uint64_t q = t / a.n, row = t - q * a.n;
+    double sum = 0.0;
+    bool bad = false;
+    for (uint32_t e = 0; e < a.L.dim; e += 8) {
+        const uint32_t w = ((const uint32_t*)a.codes)[a.L.dword(row, e)];
+        double part = 0.0;
+        for (uint32_t j = 0; j < 8 && e + j < a.L.dim; ++j) {
+            const float x = load_query(a.queries, a.qdt, q * a.L.dim + e + j);
+            bad |= !(fabsf(x) < INFINITY);
+            part = fma((double)x, (double)((int)((w >> (4 * (j >> 1) + 16 * (j & 1u))) & 15u) - 8), part);
+        }
+        sum = fma((double)half_to_f32<cgv::DT_BF16>(a.scales[a.L.scale(row, e / a.L.group)]), part, sum);
+    }
+    a.out[t] = bad ? NAN : (float)sum;
+}
+
 }  // namespace
 
 struct cgv_q4_index {
@@ -418,6 +449,7 @@ struct cgv_q4_index {
     size_t stage_bytes = 0;
     uint32_t* bad = nullptr;
     hipStream_t stream = nullptr;
+    bool large = false;             // rows with scales of LARGE_SCALE or more (bf16)
     bool captured = false;          // a graph may hold the addresses of codes and scales
     std::vector<void*> retired;     // such buffers that a larger corpus has left: kept for the graph's replays
     mutable std::mutex mu;
@@ -483,6 +515,7 @@ int commit(cgv_q4_index* h, uint64_t n, hipStream_t s) {
     if (bad & BAD_NONFINITE) return fail(CGV_ERR_NONFINITE, "NaN or Inf in the rows or scales: not applied");
     if (bad & BAD_RANGE) return fail(CGV_ERR_INVALID_ARG, "a group's scale is beyond the scale type: not applied");
     h->n += n;
+    h->large |= (bad & HAS_LARGE) != 0;
     return CGV_OK;
 }
 
@@ -582,6 +615,10 @@ int scores_by(const cgv_q4_index* h, const void* q, int qdt, uint32_t m, uint64_
         }
         const int rc = h->sdt == CGV_DTYPE_FP16 ? launch_by_group<P, cgv::DT_FP16>(h, a, s) : launch_by_group<P, cgv::DT_BF16>(h, a, s);
         if (rc) return rc;
+        if (h->large) {
+            hipLaunchKernelGGL(q4_again_kernel, wide_grid((a.m * a.n + 255) / 256), dim3(256), 0, s, a);
+            OPCHK(hipGetLastError());
+        }
     }
     return CGV_OK;
 }

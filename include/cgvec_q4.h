@@ -5,7 +5,8 @@
  *   score[m][r]                 = sum over k of query[m][k] * value[r][k]
  *
  * It stands beside the int8 scan (cgvec_i8.h): half its bytes per element, scales that follow each group of a row instead of the
- * fixed range [-1, 1], and queries that are NOT quantised (f32, bf16 or fp16, used at their full precision; sums in f32). The
+ * fixed range [-1, 1], and queries that are NOT quantised (f32: 24 bits of an element, or an absolute 2^-39 of the query's largest; fp16
+ * and bf16: all bits of an element down to 2^-28 of the largest; sums in f32). The
  * reference quantises to 4 bits (optimization.rs:248-262) but scans 8-bit data only (:76-82).
  * A single query is bound by the bytes of the corpus: dim / 2 + 2 * ceil(dim / group) per row.
  * Same status / error convention as cgvec.h. No CPU fallback: creating a handle without a GPU fails.
@@ -50,7 +51,8 @@ int cgv_q4_add_codes_dev(cgv_q4_index* h, const uint8_t* codes_dev, const uint16
 int cgv_q4_get_row_f32(cgv_q4_index* h, uint64_t id, float* out_host);
 
 /* Scores of m queries against the first n_rows rows: out [m][n_rows] f32; more than cgv_q4_count: CGV_ERR_OUT_OF_RANGE (rows that
- * another thread adds between the two calls do not matter). A query with a NaN or Inf gets NaN for every row.
+ * another thread adds between the two calls do not matter). A query with a NaN or Inf gets NaN for every row. A score is Inf only
+ * if it is itself beyond f32 (rows with bf16 scales of 2^94 and more cost a launch more: their sums may need 64 bits).
  * _f32: HOST queries [m][dim] and output, returns when done. _dev: DEVICE queries of type query_dtype (CGV_DTYPE_F32 / BF16 /
  * FP16), contiguous [m][dim]; enqueued on `stream`, no synchronisation, nothing allocated. m == 0 or n_rows == 0: nothing is
  * written. The workspace (DEVICE, cgv_q4_scores_workspace bytes, 0 for one query of ordinary size; aligned to 256) belongs to one
