@@ -197,6 +197,13 @@ def raw_stream(device_index):
     return torch._C._cuda_getCurrentRawStream(device_index)
 
 
+def refuse_tangent(t, name):
+    """An operator without a forward-mode derivative says so: a dual tensor's values alone would drop its tangent."""
+    import torch
+    if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        raise CgvError(CGV_ERR_INVALID_ARG, f"{name} carries a forward-mode tangent: only reverse mode is supported")
+
+
 def _is_torch(x):
     return type(x).__module__.startswith("torch")
 

@@ -3,7 +3,7 @@ import ctypes as C
 
 import numpy as np
 
-from .cgvec import CGV_ERR_DIM_MISMATCH, CGV_ERR_INVALID_ARG, DTYPES, CgvError, _check, _is_torch, lib as _base_lib, raw_stream
+from .cgvec import CGV_ERR_DIM_MISMATCH, CGV_ERR_INVALID_ARG, DTYPES, CgvError, _check, _is_torch, lib as _base_lib, raw_stream, refuse_tangent
 
 _decl = False
 
@@ -134,7 +134,10 @@ class Int4ScanIndex:
 
     def scores(self, queries):
         """Dot products with every row, f32: [dim] -> [n], [m, dim] -> [m, n]. Host arrays in, numpy out; a CUDA tensor (f32,
-        bf16 or fp16) in, a CUDA tensor out, enqueued on torch's current stream."""
+        bf16 or fp16) in, a CUDA tensor out, enqueued on torch's current stream. Not differentiable: the result never requires a
+        gradient, also where the queries do."""
+        if _is_torch(queries):
+            refuse_tangent(queries, "queries")
         if _is_torch(queries) and queries.is_cuda:
             import torch
             code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}.get(queries.dtype)

@@ -6,7 +6,7 @@ import ctypes as C
 import torch
 from torch.autograd.function import once_differentiable
 
-from .cgvec import CGV_ERR_DIM_MISMATCH, CGV_ERR_INVALID_ARG, CgvError, _check, lib as _base_lib, raw_stream as _stream
+from .cgvec import CGV_ERR_DIM_MISMATCH, CGV_ERR_INVALID_ARG, CgvError, _check, lib as _base_lib, raw_stream as _stream, refuse_tangent
 
 _decl = False
 _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -50,6 +50,7 @@ def _matrix(t, name):
         raise _bad(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
     if not 1 <= t.shape[1] <= 8192:
         raise _bad(f"{name}: dim must be in 1..=8192, got {t.shape[1]}")
+    refuse_tangent(t, name)
     if not t.is_contiguous() and (t.shape[0] <= 1 or t.stride(1) != 1 or t.stride(0) < t.shape[1]):
         t = t.contiguous()
     return t
@@ -90,6 +91,7 @@ class _LookupRows(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
+        refuse_tangent(dout, "dout")
         (ids,) = ctx.saved_tensors
         return _lookup_grad(dout.contiguous(), ids, ctx.n, ctx.scale), None, None
 
@@ -121,6 +123,7 @@ def lookup_rows_grad(dout, ids, n_rows, scale=1.0):
         raise _bad("dout must be a CUDA tensor (there is no CPU fallback)")
     if dout.dtype not in _CODES:
         raise _bad(f"dout must be float32, bfloat16 or float16, not {dout.dtype}")
+    refuse_tangent(dout, "dout")
     ids = _ids(ids, "ids", dout.device)
     if dout.dim() < 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
         raise _bad(f"dout {tuple(dout.shape)} does not fit ids {tuple(ids.shape)}", CGV_ERR_DIM_MISMATCH)
@@ -154,6 +157,7 @@ class _CorpusLoss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
+        refuse_tangent(dloss, "dloss")
         L = lib()
         queries, rows, ids, scores, saved = ctx.saved_tensors
         b, d = queries.shape
@@ -208,6 +212,7 @@ def corpus_distillation(queries, rows, teacher_ids, teacher_scores, scale=1.0, t
     if ids.dim() != 2 or ids.shape[0] != queries.shape[0] or ids.shape != teacher_scores.shape:
         raise _bad(f"teacher_ids {tuple(ids.shape)} and teacher_scores {tuple(teacher_scores.shape)} do not fit queries {tuple(queries.shape)}",
                    CGV_ERR_DIM_MISMATCH)
+    refuse_tangent(teacher_scores, "teacher_scores")
     if not 1 <= ids.shape[1] <= 256:
         raise _bad(f"teacher lists must have 1..256 entries, got {ids.shape[1]}")
     return _corpus_loss(queries, rows, ids, teacher_scores.detach().to(torch.float32).contiguous(), scale, teacher_scale)
