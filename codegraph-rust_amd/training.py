@@ -194,7 +194,11 @@ def _corpus_loss(queries, rows, ids, scores, scale, teacher_scale):
 def corpus_cross_entropy(queries, rows, targets, scale=1.0):
     """Softmax cross entropy of queries [b, dim] over ALL rows [n, dim] of a corpus: loss[i] = log(sum over j of
     exp(scale * <q_i, r_j>)) - scale * <q_i, r_targets[i]>, f32 [b]. A target outside [0, n) (-1) takes the query out: loss 0, no
-    gradient. The b x n scores are never stored. Differentiable in queries and rows; gradients have their types."""
+    gradient. The b x n scores are never stored. Differentiable in queries and rows; gradients have their types. For 16-bit types the
+    scores' gradient is rounded to the type before it is multiplied (more than 32 queries; its listed entries are made good in the
+    queries' gradient): include/cgvec_train.h has the bounds; f32 inputs keep f32's digits throughout.
+    16-bit rows whose dim is a multiple of 8 are read in place if they start on 16-byte addresses, a multiple of 8 elements (at most 2^22)
+    apart; other such rows are copied whole on every call."""
     targets = _ids(targets, "targets", queries.device if isinstance(queries, torch.Tensor) else None)
     if targets.dim() != 1 or targets.shape[0] != queries.shape[0]:
         raise _bad(f"targets {tuple(targets.shape)} do not fit queries {tuple(queries.shape)}", CGV_ERR_DIM_MISMATCH)
@@ -205,7 +209,8 @@ def corpus_distillation(queries, rows, teacher_ids, teacher_scores, scale=1.0, t
     """KL divergence, f32 [b], of softmax(scale * queries @ rows.T) over the WHOLE corpus from the teacher's distribution on its
     list: softmax(teacher_scale * teacher_scores[i]) over the rows teacher_ids[i] ([b, k] each, k <= 256) - the ids and scores
     that a search returns, its padding (-1, -inf) included: entries with an id outside [0, n) or a score of -inf have no weight, a
-    query without entries no loss and no gradient. Differentiable in queries and rows; teacher_scores get no gradient."""
+    query without entries no loss and no gradient. Differentiable in queries and rows; teacher_scores get no gradient.
+    Roundings and copies as in corpus_cross_entropy."""
     ids = _ids(teacher_ids, "teacher_ids", queries.device if isinstance(queries, torch.Tensor) else None)
     if not isinstance(teacher_scores, torch.Tensor) or teacher_scores.device != ids.device or not teacher_scores.dtype.is_floating_point:
         raise _bad(f"teacher_scores must be a floating-point tensor on {ids.device}")

@@ -2,8 +2,8 @@
  * softmax losses of queries against ALL rows of a corpus with theirs.
  *
  * All buffers are DEVICE memory of `device_id`, rows are contiguous in their elements, dtype is CGV_DTYPE_F32, CGV_DTYPE_BF16 or
- * CGV_DTYPE_FP16; sums are f32, each output is rounded once. Every call only enqueues on `stream` (a hipStream_t; NULL is HIP's
- * default stream): it allocates nothing, waits for nothing, can be captured into a HIP graph, and the thread's current device is
+ * CGV_DTYPE_FP16; sums are f32, each output is rounded once (what the losses' gradients round on their way stands with them). Every
+ * call only enqueues on `stream` (a hipStream_t; NULL is HIP's default stream): it allocates nothing, waits for nothing, can be captured into a HIP graph, and the thread's current device is
  * left as it was. Results do not depend on the order in which workgroups run: the same call gives the same bits.
  * A workspace belongs to ONE call at a time: calls that may overlap (two streams, two captured graphs) need one each. Its size
  * comes from the *_workspace function beside the call; it needs no initial contents, an alignment of 256 bytes, and may be reused
@@ -28,7 +28,8 @@ int cgv_lookup_rows_dev(int device_id, const void* table_dev, int dtype, uint64_
 
 /* The table's gradient: dtable[r] = scale * (sum of dout[i] over the i with ids[i] == r, in f32), rounded to dtype. EVERY row of
  * dtable [n_rows][dim] is written; rows that no id names become zero; ids outside [0, n_rows) take no part.
- * Ids are sorted (a stable radix sort), a row's summands are added in a fixed order. */
+ * A row's summands are added in the order of the input, those of an id with many of them in pieces: more than 256 ids are sorted
+ * first, stably - up to 2048 by one workgroup, else by radix. */
 size_t cgv_lookup_grad_workspace(uint64_t n_ids, uint64_t n_rows, uint32_t dim);
 int cgv_lookup_grad_dev(int device_id, const void* dout_dev, int dtype, const int64_t* ids_dev, uint64_t n_ids, uint64_t n_rows,
                         uint32_t dim, float scale, void* dtable_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
@@ -41,7 +42,8 @@ int cgv_lookup_grad_dev(int device_id, const void* dout_dev, int dtype, const in
  * of the student's scores from the teacher's on its list - what a search returns goes in as it is: entries whose id is outside
  * [0, n_rows) or whose score is -Inf have weight 0 (its padding is both). An id may be listed twice: its weights add up.
  * A query without an entry of positive weight takes no part: loss 0, no gradient, its values are not read into any other result.
- * NaN or Inf in a query, in a corpus row or in a teacher's score makes the losses they enter NaN (or Inf).
+ * NaN or Inf in a query, in a corpus row or in a teacher's score makes the losses they enter NaN (or Inf; a corpus row whose Inf gives a
+ * query of 16 bits a score of -Inf has no weight there).
  *
  * The b x n_rows scores are never stored: the corpus is scored in tiles and only a running maximum and sum per query are kept; the
  * gradient scores it again, piece by piece.
@@ -59,7 +61,12 @@ int cgv_corpus_loss_dev(int device_id, const void* queries_dev, uint64_t query_s
 
 /* Gradients of sum over i of dloss[i] * loss[i] in the queries and in the corpus rows (either may be NULL: it is not computed), from
  * the same arguments and the `saved` of the forward call: dqueries [b][dim] and drows [n_rows][dim], contiguous, of type dtype;
- * every row of them is written. */
+ * every row of them is written.
+ * The scores' gradient G, softmax minus weight times dloss and scale, is what both products read. f32: it keeps 24 bits. 16-bit types: up to
+ * 32 queries it keeps two parts of the type; above, an entry is rounded to the type once (fp16: at a power of two of its query's own),
+ * half a step at most. What that leaves of the listed rows' entries, the largest, is added to dqueries, and to drows where b * k <= 1024
+ * and ceil(dim / 256) * ceil(n_rows / 256) < 128 (n_rows: of a piece); other drows are off by up to half a step of each entry besides
+ * their own rounding (1024 x 125 k x 768 bf16: 0.0023 of the norm, 0.0017 of it their own rounding). */
 size_t cgv_corpus_loss_grad_workspace(uint64_t b, uint64_t n_rows, uint32_t dim, uint32_t k, int dtype);
 int cgv_corpus_loss_grad_dev(int device_id, const void* queries_dev, uint64_t query_stride, const void* rows_dev, uint64_t row_stride,
                              int dtype, uint64_t b, uint64_t n_rows, uint32_t dim, const int64_t* ids_dev, const float* teacher_scores_dev,
