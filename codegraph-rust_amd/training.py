@@ -40,12 +40,16 @@ def _bad(msg, code=CGV_ERR_INVALID_ARG):
     return CgvError(code, msg)
 
 
-def _matrix(t, name):
-    """A CUDA matrix of a supported type whose rows are contiguous."""
+def _need_matrix(t, name):
     if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
         raise _bad(f"{name} must be a CUDA tensor (there is no CPU fallback)")
     if t.dim() != 2:
         raise _bad(f"{name} must be a matrix, got shape {tuple(t.shape)}", CGV_ERR_DIM_MISMATCH)
+
+
+def _matrix(t, name):
+    """A CUDA matrix of a supported type whose rows are contiguous."""
+    _need_matrix(t, name)
     if t.dtype not in _CODES:
         raise _bad(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
     if not 1 <= t.shape[1] <= 8192:
@@ -199,7 +203,8 @@ def corpus_cross_entropy(queries, rows, targets, scale=1.0):
     queries' gradient): include/cgvec_train.h has the bounds; f32 inputs keep f32's digits throughout.
     16-bit rows whose dim is a multiple of 8 are read in place if they start on 16-byte addresses, a multiple of 8 elements (at most 2^22)
     apart; other such rows are copied whole on every call."""
-    targets = _ids(targets, "targets", queries.device if isinstance(queries, torch.Tensor) else None)
+    _need_matrix(queries, "queries")
+    targets = _ids(targets, "targets", queries.device)
     if targets.dim() != 1 or targets.shape[0] != queries.shape[0]:
         raise _bad(f"targets {tuple(targets.shape)} do not fit queries {tuple(queries.shape)}", CGV_ERR_DIM_MISMATCH)
     return _corpus_loss(queries, rows, targets, None, scale, 1.0)
@@ -211,7 +216,8 @@ def corpus_distillation(queries, rows, teacher_ids, teacher_scores, scale=1.0, t
     that a search returns, its padding (-1, -inf) included: entries with an id outside [0, n) or a score of -inf have no weight, a
     query without entries no loss and no gradient. Differentiable in queries and rows; teacher_scores get no gradient.
     Roundings and copies as in corpus_cross_entropy."""
-    ids = _ids(teacher_ids, "teacher_ids", queries.device if isinstance(queries, torch.Tensor) else None)
+    _need_matrix(queries, "queries")
+    ids = _ids(teacher_ids, "teacher_ids", queries.device)
     if not isinstance(teacher_scores, torch.Tensor) or teacher_scores.device != ids.device or not teacher_scores.dtype.is_floating_point:
         raise _bad(f"teacher_scores must be a floating-point tensor on {ids.device}")
     if ids.dim() != 2 or ids.shape[0] != queries.shape[0] or ids.shape != teacher_scores.shape:
