@@ -87,6 +87,8 @@ struct Args {
     const uint32_t* ent_id;                       // G, DR: [n][ent_k] corpus rows whose entries are given, 0xffffffff for none
     const float* ent_val;                         // G: [n][ent_k] those entries
     uint32_t ent_k, ent_n;                        // DR, small tiles: ent_n of them, all queries together, whose rounding is made good; 0: none
+    const uint32_t *ent_start, *ent_pos;          // DR, or by corpus row: where those of each 32 rows start, [ent_groups + 1], and their places; NULL: none
+    uint32_t ent_groups;
     char* out;                                    // G, DR, DQ
     uint64_t out_pitch, out_plane;                // bytes
     uint32_t accumulate, vec_out;                 // DQ: add to what is there; DR: 16-byte stores possible
@@ -588,6 +590,13 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
             nnt = t / g.tm;
         }
         const uint32_t my_mt = nmt, my_nt = nnt, stages = g.nseg * ksteps;
+        uint32_t l0 = 0, l1 = 0;                      // DR: listed entries of the wave's corpus rows, asked for long before they are needed
+        if (EPI == EPI_DR && DT != cgv::DT_F32 && g.ent_start) {
+            const auto* start = (const __attribute__((address_space(4))) uint32_t*)g.ent_start;
+            const uint32_t at = (uint32_t)(g.row0 / 32) + (my_nt * S::BN + wn * S::TN) / 32;
+            l0 = start[min(at, g.ent_groups)];
+            l1 = start[min(at + S::TN / 32, g.ent_groups)];
+        }
 #pragma unroll
         for (int mb = 0; mb < S::MB; ++mb)
 #pragma unroll
@@ -759,6 +768,36 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
                                             for (int y = 0; y < 4; ++y) acc[mb][nb][r4 * 4 + y] = fmaf(mine, q[y], acc[mb][nb][r4 * 4 + y]);
                                 }
                         }
+                }
+            }
+            if constexpr (DT != cgv::DT_F32) {
+                // the same with entries sorted by corpus row: 16 of them are K of one more product, queries' rows times what is left of each in its column
+                for (uint32_t l = l0; l < l1; l += 16) {
+                    uint32_t query = 0, word = 0xffff0000u;           // of entry l + (lane & 15): its query; column of the wave tile, and what is left
+                    if (l + (lane & 15) < l1) {
+                        const uint32_t e = g.ent_pos[l + (lane & 15)], c = g.ent_id[e] - (uint32_t)(g.row0 + n0);
+                        query = e / g.ent_k;
+                        if (c < (uint32_t)S::TN) word = c << 16 | cgv_ops::f32_to_half<DT>(rest16<DT>(g.ent_val[e]));
+                    }
+                    s16x8 fb[S::NB];
+                    uint64_t from[8];
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        const int of = (lane >> 5) * 8 + x;
+                        const uint32_t w = __shfl(word, of);
+                        from[x] = (uint64_t)__shfl(query, of) * g.a.pitch;
+#pragma unroll
+                        for (int nb = 0; nb < S::NB; ++nb) fb[nb][x] = (short)(w >> 16 == (uint32_t)(nb * 32 + (lane & 31)) ? w & 0xffffu : 0u);
+                    }
+#pragma unroll
+                    for (int mb = 0; mb < S::MB; ++mb) {
+                        const char* q = g.a.p + min(m0 + mb * 32 + (lane & 31), g.a.limit - 1) * 2;
+                        s16x8 fa;
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) fa[x] = *(const short*)(q + from[x]);
+#pragma unroll
+                        for (int nb = 0; nb < S::NB; ++nb) acc[mb][nb] = mma<DT>(fa, fb[nb], acc[mb][nb]);
+                    }
                 }
             }
 #pragma unroll

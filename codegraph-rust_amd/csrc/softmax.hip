@@ -12,9 +12,8 @@
 // and not from the difference of two large numbers, and the anchor's 1 - exp(s - lse) is -expm1(-tail). And the listed rows' entries
 // of G, softmax minus weight, are computed in f32 from the saved scores and put into G as differences, before any rounding.
 //
-// For 16-bit inputs G is rounded to their type, which is what the matrix cores multiply their rows with: the corpus' bf16 gradient is off by
-// 0.0023 of its norm against 64 bits, 0.0017 of it from the rounding of the result itself. Over many queries these roundings average out; the
-// listed entries' are made good in dQ, and in small problems in dR. Up to
+// For 16-bit inputs G is rounded to their type, which is what the matrix cores multiply their rows with. Over many entries these roundings
+// average out; the listed entries', the largest and often alone in their rows, are made good in dQ and dR. Up to
 // TWINS queries leave half of a tile's columns empty: there what the rounding leaves of G is stored and multiplied too (3 queries x 326 x
 // 123 bf16: 0.0029 without, 0.0018 with).
 // fp16: each query's entries of G are scaled by a power of two of its own, which brings its largest to 2^13 .. 2^14 (what is 2^-27 of that still has
@@ -29,6 +28,7 @@
 #include "../../include/cgvec_train.h"
 #include "kernels_gemm.h"
 #include "ops_common.h"
+#include "sort_ids.h"
 
 using namespace cgv_ops;
 using namespace cgv_gemm;
@@ -37,10 +37,12 @@ namespace {
 
 constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
 constexpr uint32_t MAX_K = 256, NONE = 0xffffffffu, TWINS = 32;
-// listed entries, all queries together, that every small tile of the corpus' gradient looks through to make their rounding good: in small
-// problems there are too few for their roundings to average out (69 queries x 5054 x 64 fp16: 1.97 times the error of rounding the result
-// alone, with it 1.01 times); in large tiles the look through costs registers that the products need
+// The listed entries are the largest of a row of the corpus' gradient, and often alone in it: what 16 bits leave of them is added there too
+// (1024 queries x 125 k x 768 bf16, lists of ten: 0.0023 of the norm off without, 0.0017 with, which is the result's own rounding). Up to
+// this many of them, all queries together, every small tile looks through (two launches less); more, and large tiles, have them sorted by row
 constexpr uint32_t LOOKED_THROUGH = 1024;
+// not where lists cover more than one in this many corpus rows: a row is listed so often there that its roundings average out
+constexpr uint32_t LISTED_ONE_IN = 256;
 constexpr uint32_t CUS = 256;                                  // workgroups of one per CU that fill the card
 // of G, and of copied corpus rows. Each piece costs a round over dQ's partial sums (1024 x 500 k x 768, gradient: 3.05 ms with 128 MiB, 2.99 with
 // 512, 2.97 with 1024); the corpus' gradient needs some 256 tiles a piece, however many queries there are
@@ -460,6 +462,20 @@ __global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict_
     store_elem<DT>(dq, i * dim + at, has[i] ? v : 0.0f);
 }
 
+// where the sorted entries of each 32 corpus rows start; entries without a row are behind the last
+__global__ __launch_bounds__(256) void starts_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint64_t n_rows, uint32_t groups, uint32_t* __restrict__ start) {
+    const uint64_t g = wide_block() * 256 + threadIdx.x;
+    if (g > groups) return;
+    const uint64_t row = min(g * 32, n_rows);
+    uint32_t lo = 0, hi = n;
+    while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (keys[mid] < row) lo = mid + 1;
+        else hi = mid;
+    }
+    start[g] = lo;
+}
+
 template <int DT>
 __global__ void zero_kernel(void* p, uint64_t total) {
     for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) store_elem<DT>(p, i, 0.0f);
@@ -487,6 +503,8 @@ struct Plan {
     uint32_t parts;                // (maximum, sum) pairs of a query, all pieces together
     struct Shares { uint32_t s1, s2; };                   // shares of the long axis, for the columns of bn and for that of bn2
     uint32_t dqn, dq_columns, dq_splits;                  // dQ: tiles of dqn queries, shares of the corpus
+    SortPlan sort{0, 0};                                  // dR: of the listed entries, if they are sorted
+    uint32_t groups;                                      // dR: of 32 corpus rows
     Plan(uint64_t b_, uint64_t n_, uint32_t dim_, uint32_t k_, int dtype) : b((uint32_t)b_), dim(dim_), k(k_), n(n_) {
         bp = (uint32_t)up(std::max<uint64_t>(b_, 1), 64);
         dp = (uint32_t)up(dim_, 64);
@@ -527,7 +545,14 @@ struct Plan {
         parts = (uint32_t)((pieces_f() - 1) * slots(score_shares((uint32_t)(piece_f / bm))) + slots(score_shares((uint32_t)((last + bm - 1) / bm))));
         dq_columns = (bp + dqn - 1) / dqn;
         dq_splits = std::max<uint32_t>(1, std::min<uint32_t>((uint32_t)(piece_b / BK), CUS / ((dp + bm - 1) / bm * dq_columns)));
+        const uint64_t entries = b_ * k_;
+        if (planes == 1 && !twin() && entries < 1ull << 31 && n >= (uint64_t)LISTED_ONE_IN * k_ && (entries > LOOKED_THROUGH || large_dr(std::min(n, piece_b))))
+            sort = SortPlan(entries, n);
+        groups = (uint32_t)((n + 31) / 32);
     }
+    // the corpus' gradient of a piece of c rows: large tiles if they are enough to occupy half the card (256 queries x 20 k x 768 bf16, both
+    // gradients: 72 us, in small ones 81)
+    bool large_dr(uint64_t c) const { return (uint64_t)((dim + 255) / 256) * ((c + 255) / 256) >= CUS / 2; }
     static constexpr uint32_t WIDTH[4] = {256, 192, 128, 64};
     static double cost(uint32_t w) { return w / (w == 256 ? 1.0 : w == 192 ? 0.98 : w == 128 ? 0.93 : 0.73); }
     static uint32_t wave_rows(uint32_t bm, uint32_t bn) { return bm == 64 ? S64x64::WM : bn == 256 ? S256::WM : S64::WM; }
@@ -566,7 +591,9 @@ struct Plan {
     uint64_t b_part() const { return b_g() + up((uint64_t)planes * bp * piece_b * 2, 256); }
     uint64_t b_rows() const { return b_part() + up((uint64_t)dq_splits * bp * dp * 4, 256); }
     uint64_t b_scaled() const { return b_rows() + r_bytes(piece_b); }
-    uint64_t b_bytes() const { return b_scaled() + (scaled ? q_bytes() : 0); }
+    uint64_t b_sort() const { return b_scaled() + (scaled ? q_bytes() : 0); }
+    uint64_t b_start() const { return b_sort() + sort.bytes; }
+    uint64_t b_bytes() const { return b_start() + (sort.passes ? up((uint64_t)(groups + 1) * 4, 256) : 0); }
 };
 
 void set_segments(Args& a, int dtype, bool small) {
@@ -747,6 +774,14 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
         hipLaunchKernelGGL(scaled_queries_kernel, dim3((unsigned)std::min<uint64_t>(blocks, CUS)), dim3(256), 0, s, P, at, (uint16_t*)(ws + pl.b_scaled()), unscale);
         OPCHK(hipGetLastError());
     }
+    const uint32_t *keys, *pos = nullptr;
+    uint32_t* start = nullptr;
+    if (dr && pl.sort.passes) {
+        if (const int rc = sort_ids(pl.sort, P.ids, (uint64_t)pl.b * pl.k, pl.n, ws + pl.b_sort(), nullptr, &keys, &pos, s)) return rc;
+        start = (uint32_t*)(ws + pl.b_start());
+        hipLaunchKernelGGL(starts_kernel, wide_grid(((uint64_t)pl.groups + 256) / 256), dim3(256), 0, s, keys, pl.b * pl.k, pl.n, pl.groups, start);
+        OPCHK(hipGetLastError());
+    }
     for (uint64_t n0 = 0; n0 < pl.n; n0 += pl.piece_b) {
         const uint32_t c = (uint32_t)std::min<uint64_t>(pl.piece_b, pl.n - n0);
         const char* rows = (const char*)P.rows + n0 * P.r_stride * 2;
@@ -771,9 +806,7 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
         a.out_pitch = g_pitch;
         a.out_plane = g_plane;
         if ((rc = launch_scores<DT, EPI_G>(pl, a, pl.score_shares(a.tm), P.device, s))) return rc;
-        // the corpus' gradient: large tiles if they are enough to occupy half the card (256 queries x 20 k x 768 bf16, both gradients: 72 us, in
-        // small ones 81); in small ones both gradients share a launch
-        const bool big = dr && (uint64_t)((pl.dim + 255) / 256) * ((c + 255) / 256) >= CUS / 2, together = dq && dr && !big && pl.bm == 64;
+        const bool big = dr && pl.large_dr(c), together = dq && dr && !big && pl.bm == 64;      // small tiles: both gradients share a launch
         Args d{}, e{};
         if (dq) {
             d.a = {rows, pitch, plane, pl.copy ? pl.dp : pl.dim};
@@ -813,7 +846,10 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             e.ent_id = ent_id;
             e.ent_val = ent_val;
             e.ent_k = pl.k;
-            e.ent_n = big || P.twin || DT == cgv::DT_F32 || (uint64_t)pl.b * pl.k > LOOKED_THROUGH ? 0 : pl.b * pl.k;
+            e.ent_n = big || start || P.twin || DT == cgv::DT_F32 || (uint64_t)pl.b * pl.k > LOOKED_THROUGH ? 0 : pl.b * pl.k;
+            e.ent_start = start;
+            e.ent_pos = pos;
+            e.ent_groups = pl.groups;
         }
         if (together) {
             if ((rc = launch_gradients<DT>(d, e, P.device, s))) return rc;

@@ -199,8 +199,8 @@ def corpus_cross_entropy(queries, rows, targets, scale=1.0):
     """Softmax cross entropy of queries [b, dim] over ALL rows [n, dim] of a corpus: loss[i] = log(sum over j of
     exp(scale * <q_i, r_j>)) - scale * <q_i, r_targets[i]>, f32 [b]. A target outside [0, n) (-1) takes the query out: loss 0, no
     gradient. The b x n scores are never stored. Differentiable in queries and rows; gradients have their types. For 16-bit types the
-    scores' gradient is rounded to the type before it is multiplied (more than 32 queries; its listed entries are made good in the
-    queries' gradient): include/cgvec_train.h has the bounds; f32 inputs keep f32's digits throughout.
+    scores' gradient is rounded to the type before it is multiplied (more than 32 queries; its listed entries, the largest, are made
+    good): include/cgvec_train.h has the bounds; f32 inputs keep f32's digits throughout.
     16-bit rows whose dim is a multiple of 8 are read in place if they start on 16-byte addresses, a multiple of 8 elements (at most 2^22)
     apart; other such rows are copied whole on every call."""
     _need_matrix(queries, "queries")
