@@ -87,7 +87,7 @@ struct Args {
     const uint32_t* ent_id;                       // G, DR: [n][ent_k] corpus rows whose entries are given, 0xffffffff for none
     const float* ent_val;                         // G: [n][ent_k] those entries
     uint32_t ent_k, ent_n;                        // DR, small tiles: ent_n of them, all queries together, whose rounding is made good; 0: none
-    const uint32_t *ent_start, *ent_pos;          // DR, or by corpus row: where those of each 32 rows start, [ent_groups + 1], and their places; NULL: none
+    const uint32_t *ent_start, *ent_pos;          // DR, or by corpus row: where those of each 32 rows from row0 on start, [ent_groups + 1], and their places; NULL: none
     uint32_t ent_groups;
     char* out;                                    // G, DR, DQ
     uint64_t out_pitch, out_plane;                // bytes
@@ -593,7 +593,7 @@ __device__ __forceinline__ void work(const Args& g, uint32_t block) {
         uint32_t l0 = 0, l1 = 0;                      // DR: listed entries of the wave's corpus rows, asked for long before they are needed
         if (EPI == EPI_DR && DT != cgv::DT_F32 && g.ent_start) {
             const auto* start = (const __attribute__((address_space(4))) uint32_t*)g.ent_start;
-            const uint32_t at = (uint32_t)(g.row0 / 32) + (my_nt * S::BN + wn * S::TN) / 32;
+            const uint32_t at = (my_nt * S::BN + wn * S::TN) / 32;
             l0 = start[min(at, g.ent_groups)];
             l1 = start[min(at + S::TN / 32, g.ent_groups)];
         }

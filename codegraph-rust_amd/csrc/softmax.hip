@@ -462,11 +462,12 @@ __global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict_
     store_elem<DT>(dq, i * dim + at, has[i] ? v : 0.0f);
 }
 
-// where the sorted entries of each 32 corpus rows start; entries without a row are behind the last
-__global__ __launch_bounds__(256) void starts_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint64_t n_rows, uint32_t groups, uint32_t* __restrict__ start) {
-    const uint64_t g = wide_block() * 256 + threadIdx.x;
+// where the sorted entries of each 32 of the corpus rows [row0, end) start
+__global__ __launch_bounds__(256) void starts_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t row0, uint32_t end, uint32_t groups,
+                                                     uint32_t* __restrict__ start) {
+    const uint32_t g = blockIdx.x * 256 + threadIdx.x;
     if (g > groups) return;
-    const uint64_t row = min(g * 32, n_rows);
+    const uint32_t row = g == groups ? end : row0 + g * 32;
     uint32_t lo = 0, hi = n;
     while (lo < hi) {
         const uint32_t mid = lo + (hi - lo) / 2;
@@ -504,7 +505,6 @@ struct Plan {
     struct Shares { uint32_t s1, s2; };                   // shares of the long axis, for the columns of bn and for that of bn2
     uint32_t dqn, dq_columns, dq_splits;                  // dQ: tiles of dqn queries, shares of the corpus
     SortPlan sort{0, 0};                                  // dR: of the listed entries, if they are sorted
-    uint32_t groups;                                      // dR: of 32 corpus rows
     Plan(uint64_t b_, uint64_t n_, uint32_t dim_, uint32_t k_, int dtype) : b((uint32_t)b_), dim(dim_), k(k_), n(n_) {
         bp = (uint32_t)up(std::max<uint64_t>(b_, 1), 64);
         dp = (uint32_t)up(dim_, 64);
@@ -548,7 +548,6 @@ struct Plan {
         const uint64_t entries = b_ * k_;
         if (planes == 1 && !twin() && entries < 1ull << 31 && n >= (uint64_t)LISTED_ONE_IN * k_ && (entries > LOOKED_THROUGH || large_dr(std::min(n, piece_b))))
             sort = SortPlan(entries, n);
-        groups = (uint32_t)((n + 31) / 32);
     }
     // the corpus' gradient of a piece of c rows: large tiles if they are enough to occupy half the card (256 queries x 20 k x 768 bf16, both
     // gradients: 72 us, in small ones 81)
@@ -593,7 +592,7 @@ struct Plan {
     uint64_t b_scaled() const { return b_rows() + r_bytes(piece_b); }
     uint64_t b_sort() const { return b_scaled() + (scaled ? q_bytes() : 0); }
     uint64_t b_start() const { return b_sort() + sort.bytes; }
-    uint64_t b_bytes() const { return b_start() + (sort.passes ? up((uint64_t)(groups + 1) * 4, 256) : 0); }
+    uint64_t b_bytes() const { return b_start() + (sort.passes ? up((piece_b / 32 + 1) * 4, 256) : 0); }
 };
 
 void set_segments(Args& a, int dtype, bool small) {
@@ -779,8 +778,6 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
     if (dr && pl.sort.passes) {
         if (const int rc = sort_ids(pl.sort, P.ids, (uint64_t)pl.b * pl.k, pl.n, ws + pl.b_sort(), nullptr, &keys, &pos, s)) return rc;
         start = (uint32_t*)(ws + pl.b_start());
-        hipLaunchKernelGGL(starts_kernel, wide_grid(((uint64_t)pl.groups + 256) / 256), dim3(256), 0, s, keys, pl.b * pl.k, pl.n, pl.groups, start);
-        OPCHK(hipGetLastError());
     }
     for (uint64_t n0 = 0; n0 < pl.n; n0 += pl.piece_b) {
         const uint32_t c = (uint32_t)std::min<uint64_t>(pl.piece_b, pl.n - n0);
@@ -825,6 +822,14 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             d.out_plane = (uint64_t)pl.bp * pl.dp * 4;
             d.accumulate = n0 > 0;
         }
+        if (start) {
+            const uint32_t groups = (c + 31) / 32;
+            hipLaunchKernelGGL(starts_kernel, dim3(groups / 256 + 1), dim3(256), 0, s, keys, pl.b * pl.k, (uint32_t)n0, (uint32_t)n0 + c, groups, start);
+            OPCHK(hipGetLastError());
+            e.ent_start = start;
+            e.ent_pos = pos;
+            e.ent_groups = groups;
+        }
         if (dr) {
             e.a = {DT == cgv::DT_FP16 ? ws + pl.b_scaled() : (const char*)P.qws, (uint64_t)pl.dp * 2, (uint64_t)pl.bp * pl.dp * 2, pl.dp};
             e.b = {G, g_pitch, g_plane, (uint32_t)pl.piece_b};
@@ -847,9 +852,6 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             e.ent_val = ent_val;
             e.ent_k = pl.k;
             e.ent_n = big || start || P.twin || DT == cgv::DT_F32 || (uint64_t)pl.b * pl.k > LOOKED_THROUGH ? 0 : pl.b * pl.k;
-            e.ent_start = start;
-            e.ent_pos = pos;
-            e.ent_groups = pl.groups;
         }
         if (together) {
             if ((rc = launch_gradients<DT>(d, e, P.device, s))) return rc;

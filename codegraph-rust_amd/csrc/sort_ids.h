@@ -178,8 +178,8 @@ struct SortPlan {             // where things lie in a workspace; n = 0: nothing
             off_keys[i] = bytes, bytes += up256(n * 4);
             off_pos[i] = bytes, bytes += up256(n * 4);
         }
-        off_hist = bytes, bytes += up256(((uint64_t)blocks << bits) * 4);
-        off_total = bytes, bytes += up256(4ull << bits);
+        off_hist = bytes, bytes += up256(((uint64_t)blocks << MAX_DIGIT) * 4);      // the same for every n_rows
+        off_total = bytes, bytes += up256(4ull << MAX_DIGIT);
     }
 };
 
