@@ -20,8 +20,8 @@
 // of fragments. Stages of 64 elements of K (128 bytes of a row: shorter pieces load at less than half the rate) go from memory to LDS
 // directly; a wave issues its loads one at a time between matrix instructions, as a burst behind the barrier they held the wave up
 // (scores of 1024 x 125 k x 768 bf16: 198 us, spread 177). One barrier a stage. Bound by the matrix cores at the clock that they
-// leave (bf16, same sizes, 197 GFLOP each): scores 173 us with their exponentials, dQ 171 us, dR 186 us and G 203 us with 192 and 256 MB of
-// results; matrix pipes busy 0.65, 0.71, 0.62 and 0.53 of the time at 1.5 .. 1.8 GHz. What is left of the scores' time are the
+// leave (bf16, same sizes, 197 GFLOP each): scores 170 us with their exponentials, dQ 163 us, dR 186 us (200 with the listed entries of 1024 lists
+// of ten) and G 199 us with 192 and 256 MB of results; matrix pipes busy 0.65, 0.70, 0.62 (0.56) and 0.54 of the time at 1.5 .. 1.8 GHz. What is left of the scores' time are the
 // exponentials, a sixth of it, which nothing runs beside: both waves of a SIMD reach them at the same barrier, and two workgroups of
 // 128 x 128 on a CU, which would not, load twice as much (scores 252 us, dQ 253 us).
 #pragma once

@@ -5,7 +5,7 @@
 // backward  per piece of the corpus: G = c (exp(s - lse) - p) in 16 bits (three planes for f32), dQ += G R in f32 partial sums,
 //           dR = G^T Q; then dQ's partial sums are added and rounded.
 // Four products of 2 b n dim operations (the scores twice: keeping them would be the matrix that is not to be stored). 1024 queries x
-// 1M x 768 bf16, loss and both gradients: 5.79 ms = 1.09 PFLOP/s; 256 x 1M x 1536 fp16, loss alone: 0.79 ms = 1.0 PFLOP/s, 3.9 TB/s.
+// 1M x 768 bf16, loss and both gradients: 5.90 ms = 1.07 PFLOP/s; 256 x 1M x 1536 fp16, loss alone: 0.79 ms = 1.0 PFLOP/s, 3.9 TB/s.
 //
 // Two things keep a small loss and a small gradient exact where exp(s - lse) is close to 1. The heaviest listed row (the anchor) is
 // left out of the sum over the corpus: tail = lse - s_anchor = log(1 + sum of the others' exp(s - s_anchor)) then comes from log1p
