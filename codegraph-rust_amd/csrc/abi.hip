@@ -142,7 +142,9 @@ int cgv_create(uint32_t dim, int metric, int dtype, int device_id, cgv_index** o
     if (e == hipSuccess) e = hipMalloc((void**)&h->max_norm_dev, 4);
     if (e == hipSuccess) e = hipHostMalloc((void**)&h->h_flags, (F_COUNT + 3) * 4);
     if (e == hipSuccess) e = hipMalloc((void**)&h->resmax_dev, 8);
-    if (e == hipSuccess) e = hipMemset(h->resmax_dev, 0, 8);
+    // cleared on the handle's own stream and waited for: a plain hipMemset runs on the default stream, behind whatever the caller has there, and
+    // the handle's streams do not wait for that one - it would clear what the first add or search has already written
+    if (e == hipSuccess) e = hipMemsetAsync(h->resmax_dev, 0, 8, h->own_stream);
     for (SearchCtx& c : h->ctx) {
         if (e == hipSuccess) e = hipStreamCreateWithFlags(&c.stream, hipStreamNonBlocking);
         if (e == hipSuccess) e = hipEventCreateWithFlags(&c.dep, hipEventDisableTiming);
@@ -156,11 +158,12 @@ int cgv_create(uint32_t dim, int metric, int dtype, int device_id, cgv_index** o
         if (e == hipSuccess) e = hipHostGetDevicePointer((void**)&c.h_flags_dev, c.h_flags, 0);
         if (e == hipSuccess) e = hipHostMalloc((void**)&c.h_stage, SMALL_Q_BYTES + SMALL_OUT_BYTES, hipHostMallocMapped);
         if (e == hipSuccess) e = hipHostGetDevicePointer((void**)&c.h_stage_dev, c.h_stage, 0);
-        if (e == hipSuccess) e = hipMemset(c.flags, 0, CTX_FLAG_WORDS * 4);
+        if (e == hipSuccess) e = hipMemsetAsync(c.flags, 0, CTX_FLAG_WORDS * 4, h->own_stream);
         if (e == hipSuccess) c.flags_clean = true;
     }
-    if (e == hipSuccess) e = hipMemset(h->flags, 0, F_COUNT * 4);
-    if (e == hipSuccess) e = hipMemset(h->max_norm_dev, 0, 4);
+    if (e == hipSuccess) e = hipMemsetAsync(h->flags, 0, F_COUNT * 4, h->own_stream);
+    if (e == hipSuccess) e = hipMemsetAsync(h->max_norm_dev, 0, 4, h->own_stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(h->own_stream);
     if (e != hipSuccess) {
         std::string m = hipGetErrorString(e);
         cgv_destroy(h);
