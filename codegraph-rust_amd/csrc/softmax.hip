@@ -39,10 +39,13 @@ constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
 constexpr uint32_t MAX_K = 256, NONE = 0xffffffffu, TWINS = 32;
 // The listed entries are the largest of a row of the corpus' gradient, and often alone in it: what 16 bits leave of them is added there too
 // (1024 queries x 125 k x 768 bf16, lists of ten: 0.0023 of the norm off without, 0.0017 with, which is the result's own rounding). Up to
-// this many of them, all queries together, every small tile looks through (two launches less); more, and large tiles, have them sorted by row
-constexpr uint32_t LOOKED_THROUGH = 1024;
-// not where lists cover more than one in this many corpus rows: a row is listed so often there that its roundings average out
-constexpr uint32_t LISTED_ONE_IN = 256;
+// this many of them, all queries together, every small tile looks through; in large problems they are sorted by groups of rows, up to seven small
+// launches, and make up one more product of their tiles. That takes a twentieth of the time or less from so many products of elements on and
+// with lists so short beside the corpus; elsewhere the entries' rounding stays (0.0023 as well). 1024 x 65 536 x 768, half as many products, and
+// lists of 16: loss and gradients 464 us without, 511 with; lists of 64, one row in 1024: 529 and 601, of 256: 781 and 967; 600 x 4000 x 256
+// and lists of two: 60 and 84
+constexpr uint32_t LOOKED_THROUGH = 1024, LISTED_ONE_IN = 1024, GROUP_BITS = 5;
+constexpr double SORTED_FROM = 0x1p36;
 constexpr uint32_t CUS = 256;                                  // workgroups of one per CU that fill the card
 // of G, and of copied corpus rows. Each piece costs a round over dQ's partial sums (1024 x 500 k x 768, gradient: 3.05 ms with 128 MiB, 2.99 with
 // 512, 2.97 with 1024); the corpus' gradient needs some 256 tiles a piece, however many queries there are
@@ -462,16 +465,14 @@ __global__ __launch_bounds__(256) void finish_dq_kernel(const float* __restrict_
     store_elem<DT>(dq, i * dim + at, has[i] ? v : 0.0f);
 }
 
-// where the sorted entries of each 32 of the corpus rows [row0, end) start
-__global__ __launch_bounds__(256) void starts_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t row0, uint32_t end, uint32_t groups,
-                                                     uint32_t* __restrict__ start) {
+// where the sorted entries of each group of corpus rows start, from group `first` on
+__global__ __launch_bounds__(256) void starts_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t first, uint32_t groups, uint32_t* __restrict__ start) {
     const uint32_t g = blockIdx.x * 256 + threadIdx.x;
     if (g > groups) return;
-    const uint32_t row = g == groups ? end : row0 + g * 32;
     uint32_t lo = 0, hi = n;
     while (lo < hi) {
         const uint32_t mid = lo + (hi - lo) / 2;
-        if (keys[mid] < row) lo = mid + 1;
+        if (keys[mid] < first + g) lo = mid + 1;
         else hi = mid;
     }
     start[g] = lo;
@@ -546,8 +547,8 @@ struct Plan {
         dq_columns = (bp + dqn - 1) / dqn;
         dq_splits = std::max<uint32_t>(1, std::min<uint32_t>((uint32_t)(piece_b / BK), CUS / ((dp + bm - 1) / bm * dq_columns)));
         const uint64_t entries = b_ * k_;
-        if (planes == 1 && !twin() && entries < 1ull << 31 && n >= (uint64_t)LISTED_ONE_IN * k_ && (entries > LOOKED_THROUGH || large_dr(std::min(n, piece_b))))
-            sort = SortPlan(entries, n);
+        if (planes == 1 && !twin() && entries < 1ull << 31 && n >= (uint64_t)LISTED_ONE_IN * k_ && (double)b_ * n * dim >= SORTED_FROM)
+            sort = SortPlan(entries, n, GROUP_BITS);
     }
     // the corpus' gradient of a piece of c rows: large tiles if they are enough to occupy half the card (256 queries x 20 k x 768 bf16, both
     // gradients: 72 us, in small ones 81)
@@ -592,7 +593,7 @@ struct Plan {
     uint64_t b_scaled() const { return b_rows() + r_bytes(piece_b); }
     uint64_t b_sort() const { return b_scaled() + (scaled ? q_bytes() : 0); }
     uint64_t b_start() const { return b_sort() + sort.bytes; }
-    uint64_t b_bytes() const { return b_start() + (sort.passes ? up((piece_b / 32 + 1) * 4, 256) : 0); }
+    uint64_t b_bytes() const { return b_start() + (sort.passes ? up(((piece_b >> GROUP_BITS) + 1) * 4, 256) : 0); }
 };
 
 void set_segments(Args& a, int dtype, bool small) {
@@ -695,7 +696,7 @@ Args score_args(const Plan& pl, const Problem& P, int dtype, const char* rows, u
     a.kvalid = pl.copy ? pl.dp : pl.dim;
     a.tm = (c + pl.bm - 1) / pl.bm;
     a.scale2 = (float)(P.scale * LOG2E);
-    if (a.scale2 == 0.0f) a.scale2 = FLT_MIN;     // -inf times it is to stay -inf
+    if (a.scale2 == 0.0f) a.scale2 = FLT_TRUE_MIN;     // -inf times it is to stay -inf
     a.m_valid = c;
     a.n_valid = pl.b;
     a.n_pad = a.part_ld = pl.bp;
@@ -823,8 +824,8 @@ int backward(const Plan& pl, Problem P, int dtype, const float* dloss, void* dq,
             d.accumulate = n0 > 0;
         }
         if (start) {
-            const uint32_t groups = (c + 31) / 32;
-            hipLaunchKernelGGL(starts_kernel, dim3(groups / 256 + 1), dim3(256), 0, s, keys, pl.b * pl.k, (uint32_t)n0, (uint32_t)n0 + c, groups, start);
+            const uint32_t groups = (c + (1u << GROUP_BITS) - 1) >> GROUP_BITS;
+            hipLaunchKernelGGL(starts_kernel, dim3(groups / 256 + 1), dim3(256), 0, s, keys, pl.b * pl.k, (uint32_t)(n0 >> GROUP_BITS), groups, start);
             OPCHK(hipGetLastError());
             e.ent_start = start;
             e.ent_pos = pos;

@@ -1,5 +1,5 @@
-// sort_ids.h - (id, position) sorted by id, stably: what lookup.hip sums a table's gradient by, and softmax.hip finds the listed rows by.
-// By one workgroup up to SMALL_SORT ids; more by radix, 11 bits at most a pass, three launches each. Ids outside [0, n_rows) come last.
+// sort_ids.h - (id, position) sorted by id, stably: what lookup.hip sums a table's gradient by, and softmax.hip finds the listed rows by (there
+// by groups of ids: 2^down ids have one key). By one workgroup up to SMALL_SORT ids; more by radix, 11 bits at most a pass, three launches each. Ids outside [0, n_rows) come last.
 #pragma once
 #include "ops_common.h"
 
@@ -11,17 +11,18 @@ constexpr uint32_t SMALL_SORT = 2048;
 constexpr uint32_t SORT_THREADS = 256, SORT_STEPS = 4, SORT_BLOCK = SORT_THREADS * SORT_STEPS;   // elements of a workgroup
 constexpr uint32_t MAX_DIGIT = 11;
 
+// strangers go behind the last row
+__device__ inline uint32_t key_of(int64_t id, uint32_t n_rows, uint32_t down) {
+    return id >= 0 && id < (int64_t)n_rows ? (uint32_t)id >> down : (n_rows + (1u << down) - 1) >> down;
+}
+
 struct SortPass {
     const int64_t* ids;             // first pass: keys come from here
     const uint32_t *keys, *pos;     // later passes
     uint32_t *keys_out, *pos_out;
     uint32_t *hist, *total;         // [bins][blocks], [bins]
-    uint32_t n, n_rows, blocks, shift, bits;
-    __device__ uint32_t key(uint32_t i) const {
-        if (!ids) return keys[i];
-        const int64_t id = ids[i];
-        return id >= 0 && id < (int64_t)n_rows ? (uint32_t)id : n_rows;   // strangers go behind the last row
-    }
+    uint32_t n, n_rows, down, blocks, shift, bits;
+    __device__ uint32_t key(uint32_t i) const { return ids ? key_of(ids[i], n_rows, down) : keys[i]; }
     __device__ uint32_t digit(uint32_t k) const { return (k >> shift) & ((1u << bits) - 1u); }
 };
 
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(SortPass p) 
 
 // up to SMALL_SORT ids: one workgroup sorts (key, position) in its LDS, in the order of a bitonic network - positions differ, so the order is
 // the stable one -, and the others clear the rows' run ends
-__global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restrict__ ids, uint32_t n, uint32_t n_rows, uint32_t* __restrict__ keys,
+__global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restrict__ ids, uint32_t n, uint32_t n_rows, uint32_t down, uint32_t* __restrict__ keys,
                                                           uint32_t* __restrict__ pos, uint64_t* __restrict__ runs) {
     if (blockIdx.x) {
         for (uint64_t i = (uint64_t)(blockIdx.x - 1) * 1024 + threadIdx.x; i < n_rows; i += (uint64_t)(gridDim.x - 1) * 1024) runs[i] = 0;
@@ -140,8 +141,7 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restr
     uint32_t size = 2;
     while (size < n) size *= 2;
     for (uint32_t i = threadIdx.x; i < size; i += 1024) {
-        const int64_t id = i < n ? ids[i] : -1;
-        const uint32_t key = id >= 0 && id < (int64_t)n_rows ? (uint32_t)id : n_rows;      // strangers go behind the last row
+        const uint32_t key = key_of(i < n ? ids[i] : -1, n_rows, down);
         a[i] = i < n ? (uint64_t)key << 32 | i : ~0ull;
     }
     for (uint32_t k = 2; k <= size; k *= 2)
@@ -165,12 +165,13 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restr
 inline uint64_t up256(uint64_t b) { return (b + 255) / 256 * 256; }
 
 struct SortPlan {             // where things lie in a workspace; n = 0: nothing to sort
-    uint32_t passes = 0, bits = 0, blocks = 0;
+    uint32_t passes = 0, bits = 0, blocks = 0, down;
     uint64_t off_keys[2], off_pos[2], off_hist, off_total, bytes = 0;
-    SortPlan(uint64_t n, uint64_t n_rows) {
+    SortPlan(uint64_t n, uint64_t n_rows, uint32_t down_ = 0) : down(down_) {
         if (!n) return;
+        const uint64_t stranger = (n_rows + (1ull << down) - 1) >> down;      // the largest key
         uint32_t need = 1;
-        while (need < 32 && (n_rows >> need)) ++need;      // bits of n_rows itself: the key of ids that name no row
+        while (need < 32 && (stranger >> need)) ++need;
         passes = (need + MAX_DIGIT - 1) / MAX_DIGIT;
         bits = (need + passes - 1) / passes;
         blocks = (uint32_t)((n + SORT_BLOCK - 1) / SORT_BLOCK);
@@ -190,7 +191,7 @@ inline int sort_ids(const SortPlan& pl, const int64_t* ids, uint64_t n, uint64_t
     const uint64_t clearing = runs ? (n_rows + 4095) / 4096 : 0;
     if (n <= SMALL_SORT) {
         hipLaunchKernelGGL(sort_small_kernel, dim3(1 + (unsigned)std::min<uint64_t>(clearing, 1024)), dim3(1024), 0, s, ids, (uint32_t)n,
-                           (uint32_t)n_rows, (uint32_t*)(ws + pl.off_keys[0]), (uint32_t*)(ws + pl.off_pos[0]), runs);
+                           (uint32_t)n_rows, pl.down, (uint32_t*)(ws + pl.off_keys[0]), (uint32_t*)(ws + pl.off_pos[0]), runs);
         OPCHK(hipGetLastError());
     }
     for (uint32_t i = 0; i < pl.passes && n > SMALL_SORT; ++i) {
@@ -204,6 +205,7 @@ inline int sort_ids(const SortPlan& pl, const int64_t* ids, uint64_t n, uint64_t
         p.total = (uint32_t*)(ws + pl.off_total);
         p.n = (uint32_t)n;
         p.n_rows = (uint32_t)n_rows;
+        p.down = pl.down;
         p.blocks = pl.blocks;
         p.shift = i * pl.bits;
         p.bits = pl.bits;

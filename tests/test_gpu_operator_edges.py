@@ -78,10 +78,10 @@ def test_a_corpus_row_with_nan_or_inf(b, n, d, dt):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp16"])
-@pytest.mark.parametrize("b,n,d,k,made_good", [(512, 4000, 64, 2, True), (513, 4000, 64, 2, True), (70, 3000, 123, 14, True), (70, 3000, 123, 15, False),
-                                               (70, 15 * 256, 123, 15, True), (500, 10_000, 512, 2, True), (500, 20_000, 512, 2, True), (40, 30_000, 1024, 25, True),
-                                               (40, 33_333, 1016, 1, True), (1000, 6000, 768, 23, True), (1000, 5800, 768, 23, False), (900, 70_001, 136, 40, True),
-                                               (2000, 300_007, 64, 3, True), (5000, 30_011, 72, 100, True), (33, 256, 8192, 1, True)])
+@pytest.mark.parametrize("b,n,d,k,made_good", [(512, 4000, 64, 2, True), (513, 4000, 64, 2, False), (70, 3000, 123, 14, True), (70, 3000, 123, 15, False),
+                                               (500, 10_000, 512, 2, True), (500, 20_000, 512, 2, False), (40, 30_000, 1024, 25, False),
+                                               (1024, 65_000, 1024, 2, False), (1024, 70_001, 1024, 2, True), (1030, 90_112, 768, 88, True), (1030, 90_111, 768, 88, False),
+                                               (2100, 300_007, 112, 3, True), (66_000, 2000, 528, 1, True), (40, 900_000, 2000, 1, True)])
 def test_the_corpus_gradient_on_both_sides_of_its_rule(b, n, d, k, made_good, dt):
     """Where the listed entries' rounding is made good only the results' own and the unlisted entries' remain; elsewhere each entry is off by half a
     step of its type at most, which is all that is promised."""
