@@ -206,3 +206,38 @@ def test_host_rows_that_come_in_pieces():
         assert np.array_equal(ix.scores(x.cpu().numpy()), want.cpu().numpy())
     finally:
         ix.close()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_sorted_entries_repeat_and_replay(dt):
+    """The corpus' gradient of a large problem: the same bits every time, captured on two graphs with lists that change between replays."""
+    m = pkg()
+    b, n, d, k = 1024, 70_001, 1024, 3
+    q, r, ids, sc, g = _problem(b, n, d, k, dt, 21)
+    q.requires_grad_(), r.requires_grad_()
+
+    def step():
+        loss = m.corpus_distillation(q, r, ids, sc, scale=8.0)
+        return (loss.detach(), *torch.autograd.grad(loss, (q, r), g))
+
+    want = step()
+    assert all(torch.equal(x, y) for x, y in zip(step(), want))
+    graphs = []
+    for _ in range(2):
+        cg = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(cg):
+            res = step()
+        graphs.append((cg, res))
+    gen = torch.Generator(device="cuda").manual_seed(22)
+    for _ in range(3):
+        ids.copy_(torch.randint(-2, n + 2, (b, k), generator=gen, device="cuda"))
+        ids[::5] = ids[0, 0]
+        for _, res in graphs:
+            [x.zero_() for x in res]
+        want = step()
+        torch.cuda.synchronize()
+        for cg, _ in graphs:
+            cg.replay()
+        torch.cuda.synchronize()
+        for _, res in graphs:
+            assert all(torch.equal(x, y) for x, y in zip(res, want))
